@@ -3,7 +3,7 @@
 The kernels live in ``libdoe_mi355x.so`` (built from ``doe_amd/csrc`` by
 ``doe_amd.build``); this package is the ctypes host layer over it.
 """
-from . import q4k
+from . import mx4, q4k
 from ._lib import DoeError, DoeLibraryMissing, LIB_PATH
 from .device import DeviceBuffer, Event, Graph, Stream, device_info, init, synchronize
 from . import ops
@@ -18,6 +18,7 @@ __all__ = [
     "Stream",
     "device_info",
     "init",
+    "mx4",
     "synchronize",
     "ops",
     "q4k",

@@ -93,6 +93,19 @@ SIGNATURES: dict[str, list] = {
     "doe_q4k_gemv_fused": [_vp, _vp, _vp, _i64, _i64, _vp, _f32, _i32, _vp, _i32, _vp],
     "doe_q4k_gemv_qkv_rope_kv": [_vp, _vp, _vp, _i64, _vp, _f32, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
                                  _vp],
+    "doe_mx4_page_bytes": [_i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_mx4_kv_write": [_vp, _vp, _vp, _i32, _i64, _vp, _i64, _vp],
+    "doe_mx4_kv_read": [_vp, _vp, _vp, _i64, _vp, _i64, _vp],
+    "doe_attn_mx4_decode_workspace": [_i64, _i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_attn_mx4_decode": [_vp, _vp, _i32, _vp, _i32, _i64, _f32, _f32, _i64, _vp, _i64, _vp],
+    "doe_attn_mx4_prompt_workspace": [_i64, _i64, _i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_attn_mx4_prompt": [_vp, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _i64, _f32, _f32, _i64, _vp, _i64, _vp],
+    "doe_kv_pages_workspace": [_i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_kv_pages_extend": [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp],
+    "doe_kv_pages_fork": [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp],
+    "doe_kv_pages_free": [_vp, _vp, _i64, _vp, _vp],
+    "doe_kv_pages_compact": [_vp, _vp, _vp, _i64, _vp],
+    "doe_kv_pages_copy": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp],
     "doe_rmsnorm": [_vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp],
     "doe_rope": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
     "doe_rope_partial": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp],

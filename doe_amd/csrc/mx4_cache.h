@@ -1,0 +1,84 @@
+// mx4_cache.h -- the pages of the KV cache held in 4 bits, for the kernels that
+// write and read them (mx4_cache.hip, attn_mx4.hip, attn_mx4_prompt.hip).
+//
+// A value is an E2M1 code (sign, two exponent bits, one mantissa bit: 0, 0.5,
+// 1, 1.5, 2, 3, 4, 6) times 2^(scale - 127), one scale byte for 32 dims of a
+// row.  The page layout is given in doe_mi355x.h; V is held in the order in
+// which a lane of the P V product takes it: columns of D / 16 dims, and of 32
+// positions the eight that a lane group holds side by side, so a lane's bytes
+// of a block are one run and no byte is shared between positions.
+#pragma once
+
+#include "common.h"
+
+namespace doe {
+
+constexpr int kMx4Block = 32;           // positions of a V block, and dims of a scale
+constexpr int kMx4MinExp = -23;         // every value exact in f16: 0.5 x 2^-23 is its
+constexpr int kMx4MaxExp = 13;          // least, 6 x 2^13 within its range
+constexpr int kMx4NanScale = 255;
+
+// A cache as the kernels take it.
+struct Mx4View {
+    uint8_t *pool;
+    const int32_t *table, *lens;
+    int num_pages, page_shift, kv_heads, batch, table_stride;
+};
+
+// Byte offsets within the slab of one head of a page of 1 << shift positions.
+template <int D>
+struct Mx4Slab {
+    static __device__ __forceinline__ int64_t bytes(int shift) { return (int64_t)(D + D / 16) << shift; }
+    static __device__ __forceinline__ int k_code(int x) { return x * (D / 2); }
+    static __device__ __forceinline__ int k_scale(int shift, int x) { return (D << shift) + x * (D / 32); }
+    // column c of position x: D / 32 bytes
+    static __device__ __forceinline__ int v_code(int shift, int x, int c) {
+        return ((D / 2) << shift) + ((((x >> 5) * 4 + ((x >> 2) & 3)) * 16 + c) * 8 + ((x >> 4) & 1) * 4 + (x & 3)) * (D / 32);
+    }
+    static __device__ __forceinline__ int v_scale(int shift, int x, int group) {
+        return ((D + D / 32) << shift) + (((x >> 5) * 4 + ((x >> 2) & 3)) * (D / 32) + group) * 8 + ((x >> 4) & 1) * 4 + (x & 3);
+    }
+};
+
+// Positions of sequence b that the cache can hold and has in use.
+__device__ __forceinline__ int mx4_len(const Mx4View &c, int b) {
+    const int64_t room = (int64_t)c.table_stride << c.page_shift;
+    const int n = c.lens[b];
+    return n < 0 ? 0 : (n > room ? (int)room : n);
+}
+
+// The sequence b and position of row `row` of a call (row_starts null: row b of
+// sequence b); false where it has none: rows before and behind the
+// sequences', positions before 0.
+__device__ __forceinline__ bool mx4_row(const Mx4View &c, const int32_t *row_starts, int64_t row, int &b, int &pos) {
+    int lo = 0;
+    int64_t first = row, next = row + 1;
+    if (row_starts) {
+        int hi = c.batch;  // the last b with row_starts[b] <= row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (row_starts[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        first = row_starts[lo];
+        next = row_starts[lo + 1];
+        if (row < first || row >= next) return false;
+    } else {
+        lo = (int)row;
+    }
+    b = lo;
+    const int64_t p = (int64_t)mx4_len(c, b) - (next - first) + (row - first);
+    pos = (int)p;
+    return p >= 0;
+}
+
+// The page of position pos of sequence b; -1 where the table names none of the pool.
+__device__ __forceinline__ int mx4_page(const Mx4View &c, int b, int pos) {
+    const int page = c.table[(int64_t)b * c.table_stride + (pos >> c.page_shift)];
+    return page >= 0 && page < c.num_pages ? page : -1;
+}
+
+// Checks a cache and turns it into the kernels' form; returns a DOE status.
+int mx4_view(const doe_mx4_cache *cache, Mx4View *view);
+
+}  // namespace doe

@@ -1,0 +1,293 @@
+// mx4_cache.hip -- K / V rows into the paged cache held in 4 bits, and back.
+//
+// Quantisation of a block of 32 values x: a = max |x|, e = floor(log2 a) - 2,
+// one more where a / 2^floor(log2 a) >= 1.75 (a then rounds to the next power of
+// two among the codes), held within [-23, 13] so that every value is exact in
+// f16; codes are the nearest E2M1 value of x 2^-e (exact in f32), ties to the
+// even code, at most 6.  v_cvt_scalef32_pk_fp4_f32 rounds so: checked against
+// comparisons over all codes' borders and their neighbours.  A block with an
+// infinity or a NaN keeps scale byte 255 (codes 0) and reads as NaN throughout.
+#include "mx4_cache.h"
+
+namespace {
+
+using doe::Mx4Slab;
+using doe::Mx4View;
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+struct RowArgs {
+    Mx4View c;
+    const void *k, *v;
+    float *k_out, *v_out;
+    const int32_t *row_starts;
+    int64_t rows, row_stride;
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+// Bits of the largest magnitude over each 8 lanes, an infinity's or NaN's above
+// all others (as numbers a maximum would drop a NaN).
+__device__ __forceinline__ uint32_t max8(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lane ^ 2
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // the other four of eight
+}
+
+// The 4-bit codes of four values of a block that eight lanes hold (16 bits),
+// and the block's scale byte.
+__device__ __forceinline__ uint32_t quantise(const float4 x, int &scale) {
+    const uint32_t m = 0x7fffffffu;
+    const uint32_t top = max8(max(max(__float_as_uint(x.x) & m, __float_as_uint(x.y) & m),
+                                  max(__float_as_uint(x.z) & m, __float_as_uint(x.w) & m)));
+    int e = (int)((top + 0x200000u) >> 23) - 129;
+    e = e < doe::kMx4MinExp ? doe::kMx4MinExp : (e > doe::kMx4MaxExp ? doe::kMx4MaxExp : e);
+    scale = top < 0x7f800000u ? e + 127 : doe::kMx4NanScale;
+    const float s = __uint_as_float((uint32_t)(e + 127) << 23);
+    // (values beyond 6 x 2^13 only where e was held at 13)
+    const float lim = 6.0f * s;
+    auto in = [&](float v) { return fminf(fmaxf(v, -lim), lim); };
+    uint32_t q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, in(x.x), in(x.y), s, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, in(x.z), in(x.w), s, 1) & 0xffffu;
+    return scale == doe::kMx4NanScale ? 0u : q;
+}
+
+constexpr int kRowsPerWg = 16;
+
+// One row's place, found once for a workgroup's rows.
+struct Place {
+    int64_t page;  // page * kv_heads, -1: none
+    int x;
+};
+
+// A workgroup takes kRowsPerWg rows; a thread four dims of K and V of a row's head.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
+    __shared__ Place place[kRowsPerWg];
+    const int64_t row0 = (int64_t)blockIdx.x * kRowsPerWg;
+    if (threadIdx.x < kRowsPerWg) {
+        const int64_t row = row0 + threadIdx.x;
+        Place p{-1, 0};
+        int b, pos;
+        if (row < a.rows && doe::mx4_row(a.c, a.row_starts, row, b, pos)) {
+            const int page = doe::mx4_page(a.c, b, pos);
+            if (page >= 0) p = Place{(int64_t)page * a.c.kv_heads, pos & ((1 << a.c.page_shift) - 1)};
+        }
+        place[threadIdx.x] = p;
+    }
+    __syncthreads();
+    using S = Mx4Slab<D>;
+    constexpr int QUADS = D / 4;
+    const int shift = a.c.page_shift, per_row = a.c.kv_heads * QUADS;
+    for (int i = threadIdx.x; i < kRowsPerWg * per_row; i += 256) {
+        const int r = i / per_row, in_row = i - r * per_row, head = in_row / QUADS, d = (in_row - head * QUADS) * 4;
+        const Place p = place[r];
+        if (p.page < 0) continue;
+        const int64_t at = (row0 + r) * a.row_stride + (int64_t)head * D + d;
+        float4 k, v;
+        if constexpr (F16) {
+            const h4 kh = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.k) + at);
+            const h4 vh = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.v) + at);
+            k = make_float4((float)kh[0], (float)kh[1], (float)kh[2], (float)kh[3]);
+            v = make_float4((float)vh[0], (float)vh[1], (float)vh[2], (float)vh[3]);
+        } else {
+            k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.k) + at);
+            v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.v) + at);
+        }
+        int ks, vs;
+        const uint32_t kc = quantise(k, ks), vc = quantise(v, vs);
+        uint8_t *slab = a.c.pool + (p.page + head) * S::bytes(shift);
+        *reinterpret_cast<uint16_t *>(slab + S::k_code(p.x) + d / 2) = (uint16_t)kc;
+        if constexpr (D == 160) {  // columns of five bytes
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                slab[S::v_code(shift, p.x, (d + 2 * e) / 10) + (d + 2 * e) % 10 / 2] = (uint8_t)(vc >> (8 * e));
+        } else {
+            *reinterpret_cast<uint16_t *>(slab + S::v_code(shift, p.x, d / (D / 16)) + d % (D / 16) / 2) = (uint16_t)vc;
+        }
+        if ((d & 31) == 0) {
+            slab[S::k_scale(shift, p.x) + d / 32] = (uint8_t)ks;
+            slab[S::v_scale(shift, p.x, d / 32)] = (uint8_t)vs;
+        }
+    }
+}
+
+__device__ __forceinline__ float4 values(uint32_t codes, int scale) {
+    const float s = __uint_as_float(scale == doe::kMx4NanScale ? 0x7fc00000u : (uint32_t)scale << 23);
+    const h2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 0), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 1);
+    return make_float4((float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void mx4_read_kernel(RowArgs a) {
+    __shared__ Place place[kRowsPerWg];
+    __shared__ bool mine[kRowsPerWg];
+    const int64_t row0 = (int64_t)blockIdx.x * kRowsPerWg;
+    if (threadIdx.x < kRowsPerWg) {
+        const int64_t row = row0 + threadIdx.x;
+        Place p{-1, 0};
+        int b, pos;
+        if (row < a.rows && doe::mx4_row(a.c, a.row_starts, row, b, pos)) {
+            const int page = doe::mx4_page(a.c, b, pos);
+            if (page >= 0) p = Place{(int64_t)page * a.c.kv_heads, pos & ((1 << a.c.page_shift) - 1)};
+        }
+        place[threadIdx.x] = p;
+        // rows of no sequence stay as they were
+        mine[threadIdx.x] = row < a.rows && (!a.row_starts || (row >= a.row_starts[0] && row < a.row_starts[a.c.batch]));
+    }
+    __syncthreads();
+    using S = Mx4Slab<D>;
+    constexpr int QUADS = D / 4;
+    const int shift = a.c.page_shift, per_row = a.c.kv_heads * QUADS;
+    for (int i = threadIdx.x; i < kRowsPerWg * per_row; i += 256) {
+        const int r = i / per_row, in_row = i - r * per_row, head = in_row / QUADS, d = (in_row - head * QUADS) * 4;
+        const Place p = place[r];
+        if (!mine[r]) continue;
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+        if (p.page >= 0) {
+            const uint8_t *slab = a.c.pool + (p.page + head) * S::bytes(shift);
+            const uint32_t kc = *reinterpret_cast<const uint16_t *>(slab + S::k_code(p.x) + d / 2);
+            uint32_t vc;
+            if constexpr (D == 160) {
+                vc = slab[S::v_code(shift, p.x, d / 10) + d % 10 / 2] |
+                     (uint32_t)slab[S::v_code(shift, p.x, (d + 2) / 10) + (d + 2) % 10 / 2] << 8;
+            } else {
+                vc = *reinterpret_cast<const uint16_t *>(slab + S::v_code(shift, p.x, d / (D / 16)) + d % (D / 16) / 2);
+            }
+            k = values(kc, slab[S::k_scale(shift, p.x) + d / 32]);
+            v = values(vc, slab[S::v_scale(shift, p.x, d / 32)]);
+        }
+        const int64_t at = (row0 + r) * a.row_stride + (int64_t)head * D + d;
+        *reinterpret_cast<float4 *>(a.k_out + at) = k;
+        *reinterpret_cast<float4 *>(a.v_out + at) = v;
+    }
+}
+
+int row_checks(const Mx4View &c, int64_t head_dim, int64_t rows, int64_t row_stride, const int32_t *row_starts,
+               const void *k, const void *v, int size) {
+    DOE_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31), DOE_E_INVALID, "rows %lld", (long long)rows);
+    DOE_REQUIRE(row_starts || rows == c.batch, DOE_E_INVALID, "without row_starts a call takes one row a sequence (%lld rows, batch %d)",
+                (long long)rows, c.batch);
+    DOE_REQUIRE(row_stride >= c.kv_heads * head_dim && row_stride * size % 16 == 0, DOE_E_INVALID,
+                "row stride %lld below a row of %lld, or not a multiple of 16 bytes", (long long)row_stride,
+                (long long)(c.kv_heads * head_dim));
+    DOE_REQUIRE(rows == 0 || (k && v), DOE_E_INVALID, "null pointer");
+    DOE_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0, DOE_E_INVALID, "k and v must be 16-byte aligned");
+    return DOE_OK;
+}
+
+template <int D>
+void launch_write(bool f16, dim3 grid, hipStream_t st, const RowArgs &a) {
+    if (f16) hipLaunchKernelGGL((mx4_write_kernel<D, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mx4_write_kernel<D, false>), grid, dim3(256), 0, st, a);
+}
+
+}  // namespace
+
+namespace doe {
+
+int mx4_view(const doe_mx4_cache *cache, Mx4View *view) {
+    DOE_REQUIRE(cache, DOE_E_INVALID, "null cache");
+    const doe_mx4_cache &c = *cache;
+    DOE_REQUIRE(c.head_dim == 64 || c.head_dim == 128 || c.head_dim == 160 || c.head_dim == 256 || c.head_dim == 512,
+                DOE_E_UNSUPPORTED, "head_dim %lld unsupported (64, 128, 160, 256, 512)", (long long)c.head_dim);
+    int shift = 0;
+    while (shift < 9 && ((int64_t)1 << shift) != c.page_size) ++shift;
+    DOE_REQUIRE(shift >= 5 && shift <= 8, DOE_E_UNSUPPORTED, "page_size %lld unsupported (32, 64, 128, 256)",
+                (long long)c.page_size);
+    DOE_REQUIRE(c.num_kv_heads > 0 && c.num_kv_heads <= 1024, DOE_E_INVALID, "num_kv_heads %lld outside 1..1024",
+                (long long)c.num_kv_heads);
+    DOE_REQUIRE(c.num_pages > 0 && c.num_pages < ((int64_t)1 << 31), DOE_E_INVALID, "num_pages %lld", (long long)c.num_pages);
+    DOE_REQUIRE(c.batch >= 0 && c.batch <= 65535, DOE_E_INVALID, "batch %lld outside 0..65535", (long long)c.batch);
+    DOE_REQUIRE(c.table_stride > 0 && c.table_stride * c.page_size < ((int64_t)1 << 30), DOE_E_INVALID,
+                "table_stride %lld: a sequence holds fewer than 2^30 positions", (long long)c.table_stride);
+    DOE_REQUIRE(c.pool && c.page_table && c.kv_lens, DOE_E_INVALID, "null pointer");
+    DOE_REQUIRE(((uintptr_t)c.pool & 15) == 0, DOE_E_INVALID, "the pool must be 16-byte aligned");
+    view->pool = static_cast<uint8_t *>(c.pool);
+    view->table = c.page_table;
+    view->lens = c.kv_lens;
+    view->num_pages = (int)c.num_pages;
+    view->page_shift = shift;
+    view->kv_heads = (int)c.num_kv_heads;
+    view->batch = (int)c.batch;
+    view->table_stride = (int)c.table_stride;
+    return DOE_OK;
+}
+
+}  // namespace doe
+
+extern "C" {
+
+int doe_mx4_page_bytes(int64_t page_size, int64_t num_kv_heads, int64_t head_dim, int64_t *bytes) {
+    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
+    int32_t some = 0;
+    doe_mx4_cache c{};
+    c.pool = reinterpret_cast<void *>(16);
+    c.page_table = c.kv_lens = &some;
+    c.num_pages = c.table_stride = 1;
+    c.page_size = page_size;
+    c.num_kv_heads = num_kv_heads;
+    c.head_dim = head_dim;
+    Mx4View v;
+    const int rc = doe::mx4_view(&c, &v);
+    if (rc) return rc;
+    *bytes = page_size * num_kv_heads * (head_dim + head_dim / 16);
+    return DOE_OK;
+}
+
+int doe_mx4_kv_write(const doe_mx4_cache *cache, const void *k, const void *v, int in_f16, int64_t row_stride,
+                     const int32_t *row_starts, int64_t rows, doe_stream_t stream) {
+    RowArgs a{};
+    int rc = doe::mx4_view(cache, &a.c);
+    if (rc) return rc;
+    if ((rc = row_checks(a.c, cache->head_dim, rows, row_stride, row_starts, k, v, in_f16 ? 2 : 4))) return rc;
+    if ((rc = doe::require_init())) return rc;
+    if (rows == 0 || a.c.batch == 0) return DOE_OK;
+    a.k = k;
+    a.v = v;
+    a.row_starts = row_starts;
+    a.rows = rows;
+    a.row_stride = row_stride;
+    const dim3 grid((unsigned)((rows + kRowsPerWg - 1) / kRowsPerWg));
+    const hipStream_t st = (hipStream_t)stream;
+    switch (cache->head_dim) {
+        case 64: launch_write<64>(in_f16, grid, st, a); break;
+        case 128: launch_write<128>(in_f16, grid, st, a); break;
+        case 160: launch_write<160>(in_f16, grid, st, a); break;
+        case 256: launch_write<256>(in_f16, grid, st, a); break;
+        default: launch_write<512>(in_f16, grid, st, a); break;
+    }
+    DOE_LAUNCH_CHECK("mx4_write_kernel");
+    return DOE_OK;
+}
+
+int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_stride, const int32_t *row_starts,
+                    int64_t rows, doe_stream_t stream) {
+    RowArgs a{};
+    int rc = doe::mx4_view(cache, &a.c);
+    if (rc) return rc;
+    if ((rc = row_checks(a.c, cache->head_dim, rows, row_stride, row_starts, k, v, 4))) return rc;
+    if ((rc = doe::require_init())) return rc;
+    if (rows == 0 || a.c.batch == 0) return DOE_OK;
+    a.k_out = k;
+    a.v_out = v;
+    a.row_starts = row_starts;
+    a.rows = rows;
+    a.row_stride = row_stride;
+    const dim3 grid((unsigned)((rows + kRowsPerWg - 1) / kRowsPerWg));
+    const hipStream_t st = (hipStream_t)stream;
+    switch (cache->head_dim) {
+        case 64: hipLaunchKernelGGL(mx4_read_kernel<64>, grid, dim3(256), 0, st, a); break;
+        case 128: hipLaunchKernelGGL(mx4_read_kernel<128>, grid, dim3(256), 0, st, a); break;
+        case 160: hipLaunchKernelGGL(mx4_read_kernel<160>, grid, dim3(256), 0, st, a); break;
+        case 256: hipLaunchKernelGGL(mx4_read_kernel<256>, grid, dim3(256), 0, st, a); break;
+        default: hipLaunchKernelGGL(mx4_read_kernel<512>, grid, dim3(256), 0, st, a); break;
+    }
+    DOE_LAUNCH_CHECK("mx4_read_kernel");
+    return DOE_OK;
+}
+
+}  // extern "C"

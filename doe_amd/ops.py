@@ -15,6 +15,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
+from . import mx4 as _mx4
 from . import q4k as _q4k
 from . import q8_0 as _q8_0
 from .device import DeviceBuffer, _stream_ptr
@@ -720,6 +721,201 @@ def lm_head_sample(weight_f16: DeviceBuffer, activation: DeviceBuffer, n: int, k
     return int(cnt.value)
 
 
+class _Mx4CacheArgs(C.Structure):
+    """doe_mx4_cache, field for field."""
+    _fields_ = [("pool", C.c_void_p), ("page_table", C.c_void_p), ("kv_lens", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("num_pages", "page_size", "num_kv_heads", "head_dim", "batch", "table_stride")]
+
+
+class _KvPagesArgs(C.Structure):
+    """doe_kv_pages, field for field."""
+    _fields_ = [("pools", C.c_void_p), ("layers", C.c_int64), ("layer_stride", C.c_int64), ("page_bytes", C.c_int64),
+                ("page_table", C.c_void_p), ("kv_lens", C.c_void_p), ("page_refs", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("max_seqs", "table_stride", "num_pages", "page_size")]
+
+
+def _opt(buf: DeviceBuffer | None) -> C.c_void_p:
+    return C.c_void_p(None if buf is None else buf.ptr)
+
+
+class Mx4Cache:
+    """One layer's KV cache held in 4 bits: a pool of pages with the page table
+    and lengths of ``batch`` sequences (device int32).  Keeps its buffers
+    alive; build one per layer and use it for every call."""
+
+    def __init__(self, pool: DeviceBuffer, page_table: DeviceBuffer, kv_lens: DeviceBuffer, *, num_pages: int,
+                 page_size: int, num_kv_heads: int, head_dim: int, batch: int, table_stride: int):
+        self.page_bytes = _mx4.page_bytes(page_size, num_kv_heads, head_dim)
+        _need(pool, num_pages * self.page_bytes, "pool")
+        _need(page_table, batch * table_stride * 4, "page_table")
+        _need(kv_lens, batch * 4, "kv_lens")
+        self.buffers = (pool, page_table, kv_lens)
+        self.num_kv_heads, self.head_dim, self.batch = num_kv_heads, head_dim, batch
+        self.args = _Mx4CacheArgs(pool.ptr, page_table.ptr, kv_lens.ptr, num_pages, page_size, num_kv_heads, head_dim,
+                                  batch, table_stride)
+
+
+class KvPages:
+    """The pages of a paged KV cache: the page table and lengths of
+    ``max_seqs`` sequences, the count of sequences that hold each page, and the
+    pools of ``layers`` layers ([layers][num_pages][page_bytes] unless
+    ``layer_stride`` says otherwise).  Without pools only the bookkeeping is
+    done."""
+
+    def __init__(self, page_table: DeviceBuffer, kv_lens: DeviceBuffer, page_refs: DeviceBuffer, *, max_seqs: int,
+                 table_stride: int, num_pages: int, page_size: int, pools: DeviceBuffer | None = None, layers: int = 0,
+                 page_bytes: int = 0, layer_stride: int | None = None):
+        _need(page_table, max_seqs * table_stride * 4, "page_table")
+        _need(kv_lens, max_seqs * 4, "kv_lens")
+        _need(page_refs, num_pages * 4, "page_refs")
+        stride = num_pages * page_bytes if layer_stride is None else layer_stride
+        if layers:
+            if pools is None:
+                raise ValueError(f"{layers} layers without pools")
+            _need(pools, (layers - 1) * stride + num_pages * page_bytes, "pools")
+        self.buffers = (page_table, kv_lens, page_refs, pools)
+        self.args = _KvPagesArgs(pools.ptr if pools is not None else None, layers, stride, page_bytes, page_table.ptr,
+                                 kv_lens.ptr, page_refs.ptr, max_seqs, table_stride, num_pages, page_size)
+
+
+def _mx4_rows(cache: Mx4Cache, rows: int, row_starts: DeviceBuffer | None) -> None:
+    if row_starts is not None:
+        _need(row_starts, (cache.batch + 1) * 4, "row_starts")
+    elif rows != cache.batch:
+        raise ValueError(f"{rows} rows without row_starts, expected one for each of {cache.batch} sequences")
+
+
+def mx4_kv_write(cache: Mx4Cache, k: DeviceBuffer, v: DeviceBuffer, rows: int, *, row_starts: DeviceBuffer | None = None,
+                 row_stride: int | None = None, in_f16: bool = False, stream=None) -> None:
+    """K / V rows [num_kv_heads][head_dim] (f32, or f16) into the cache: one row
+    a sequence, or with ``row_starts`` (device int32 [batch + 1]) the rows of
+    ragged prompts, the last of a sequence at kv_len - 1."""
+    hd = cache.num_kv_heads * cache.head_dim
+    stride = hd if row_stride is None else row_stride
+    _mx4_rows(cache, rows, row_starts)
+    if rows:
+        size = ((rows - 1) * stride + hd) * (2 if in_f16 else 4)
+        _need(k, size, "k")
+        _need(v, size, "v")
+    _lib.call("doe_mx4_kv_write", C.byref(cache.args), _p(k), _p(v), int(in_f16), stride, _opt(row_starts), rows,
+              _stream_ptr(stream))
+
+
+def mx4_kv_read(cache: Mx4Cache, k: DeviceBuffer, v: DeviceBuffer, rows: int, *, row_starts: DeviceBuffer | None = None,
+                row_stride: int | None = None, stream=None) -> None:
+    """The values (f32) of the rows that ``mx4_kv_write`` would write."""
+    hd = cache.num_kv_heads * cache.head_dim
+    stride = hd if row_stride is None else row_stride
+    _mx4_rows(cache, rows, row_starts)
+    if rows:
+        _need(k, ((rows - 1) * stride + hd) * 4, "k")
+        _need(v, ((rows - 1) * stride + hd) * 4, "v")
+    _lib.call("doe_mx4_kv_read", C.byref(cache.args), _p(k), _p(v), stride, _opt(row_starts), rows, _stream_ptr(stream))
+
+
+def attention_mx4_workspace(batch: int, num_heads: int, num_kv_heads: int, head_dim: int, rows: int | None = None) -> int:
+    """Workspace bytes of ``attention_mx4``, or with ``rows`` of ``attention_mx4_prompt``."""
+    n = C.c_int64()
+    if rows is None:
+        _lib.call("doe_attn_mx4_decode_workspace", batch, num_heads, num_kv_heads, head_dim, C.byref(n))
+    else:
+        _lib.call("doe_attn_mx4_prompt_workspace", batch, rows, num_heads, num_kv_heads, head_dim, C.byref(n))
+    return n.value
+
+
+def attention_mx4(cache: Mx4Cache, q: DeviceBuffer, output: DeviceBuffer, *, num_heads: int, scale: float,
+                  workspace: DeviceBuffer, q_f16: bool = False, out_f16: bool = False, softcap: float = 0.0,
+                  sliding_window: int = 0, stream=None) -> None:
+    """``attention`` over the 4-bit cache, one query token a sequence: q and
+    output [batch][num_heads][head_dim], the query of a sequence at its last
+    position.  ``workspace`` is the call's own while it runs (its size:
+    ``attention_mx4_workspace``)."""
+    n = cache.batch * num_heads * cache.head_dim
+    _need(q, n * (2 if q_f16 else 4), "q")
+    _need(output, n * (2 if out_f16 else 4), "output")
+    _lib.call("doe_attn_mx4_decode", C.byref(cache.args), _p(q), int(q_f16), _p(output), int(out_f16), num_heads, scale,
+              softcap, sliding_window, _p(workspace), workspace.nbytes, _stream_ptr(stream))
+
+
+def attention_mx4_prompt(cache: Mx4Cache, q: DeviceBuffer, output: DeviceBuffer, rows: int, *, num_heads: int,
+                         scale: float, workspace: DeviceBuffer, row_starts: DeviceBuffer | None = None,
+                         q_f16: bool = False, out_f16: bool = False, q_row_stride: int | None = None,
+                         out_row_stride: int | None = None, softcap: float = 0.0, sliding_window: int = 0,
+                         stream=None) -> None:
+    """Causal ``attention`` of prompt rows over the 4-bit cache (the rows of
+    ``mx4_kv_write``; a sequence's n rows at its last n positions)."""
+    hd = num_heads * cache.head_dim
+    qs = hd if q_row_stride is None else q_row_stride
+    os_ = hd if out_row_stride is None else out_row_stride
+    _mx4_rows(cache, rows, row_starts)
+    if rows:
+        _need(q, ((rows - 1) * qs + hd) * (2 if q_f16 else 4), "q")
+        _need(output, ((rows - 1) * os_ + hd) * (2 if out_f16 else 4), "output")
+    _lib.call("doe_attn_mx4_prompt", C.byref(cache.args), _p(q), int(q_f16), qs, _p(output), int(out_f16), os_,
+              _opt(row_starts), rows, num_heads, scale, softcap, sliding_window, _p(workspace), workspace.nbytes,
+              _stream_ptr(stream))
+
+
+def kv_pages_workspace(num_pages: int, max_seqs: int = 0, n: int = 0) -> int:
+    """Workspace bytes of the ``kv_pages_`` calls over lists of ``n``."""
+    size = C.c_int64()
+    _lib.call("doe_kv_pages_workspace", num_pages, max_seqs, n, C.byref(size))
+    return size.value
+
+
+def kv_pages_extend(pages: KvPages, seqs: DeviceBuffer, add: DeviceBuffer, n: int, *, status: DeviceBuffer,
+                    workspace: DeviceBuffer, stream=None) -> None:
+    """``add[i]`` more positions for sequence ``seqs[i]``, with fresh pages.
+    ``status`` (device int32): 0 done, > 0 pages missing, -1 lists not in
+    order; nothing changes unless it is 0."""
+    _need(seqs, n * 4, "seqs")
+    _need(add, n * 4, "add")
+    _need(status, 4, "status")
+    _lib.call("doe_kv_pages_extend", C.byref(pages.args), _p(seqs), _p(add), n, _p(status), _p(workspace),
+              workspace.nbytes, _stream_ptr(stream))
+
+
+def kv_pages_fork(pages: KvPages, parents: DeviceBuffer, children: DeviceBuffer, n: int, *, status: DeviceBuffer,
+                  workspace: DeviceBuffer, stream=None) -> None:
+    """Free slot ``children[i]`` becomes a copy of ``parents[i]``: whole pages
+    shared, a partly filled last one copied in every layer."""
+    _need(parents, n * 4, "parents")
+    _need(children, n * 4, "children")
+    _need(status, 4, "status")
+    _lib.call("doe_kv_pages_fork", C.byref(pages.args), _p(parents), _p(children), n, _p(status), _p(workspace),
+              workspace.nbytes, _stream_ptr(stream))
+
+
+def kv_pages_free(pages: KvPages, seqs: DeviceBuffer, n: int, *, status: DeviceBuffer,
+                  workspace: DeviceBuffer | None = None, stream=None) -> None:
+    """Ends sequences: their pages and slots are free.  (No workspace is
+    needed; one is taken so that the calls look alike.)"""
+    _need(seqs, n * 4, "seqs")
+    _need(status, 4, "status")
+    _lib.call("doe_kv_pages_free", C.byref(pages.args), _p(seqs), n, _p(status), _stream_ptr(stream))
+
+
+def kv_pages_compact(pages: KvPages, *, status: DeviceBuffer, workspace: DeviceBuffer, stream=None) -> None:
+    """Moves the pages in use to the lowest ids, in every layer."""
+    _need(status, 4, "status")
+    _lib.call("doe_kv_pages_compact", C.byref(pages.args), _p(status), _p(workspace), workspace.nbytes,
+              _stream_ptr(stream))
+
+
+def kv_pages_copy(pools: DeviceBuffer, sources: DeviceBuffer, destinations: DeviceBuffer, n: int, *, layers: int,
+                  num_pages: int, page_bytes: int, status: DeviceBuffer, workspace: DeviceBuffer,
+                  layer_stride: int | None = None, stream=None) -> None:
+    """Page ``destinations[i]`` = page ``sources[i]`` in every layer."""
+    step = num_pages * page_bytes if layer_stride is None else layer_stride
+    if layers:
+        _need(pools, (layers - 1) * step + num_pages * page_bytes, "pools")
+    _need(sources, n * 4, "sources")
+    _need(destinations, n * 4, "destinations")
+    _need(status, 4, "status")
+    _lib.call("doe_kv_pages_copy", _p(pools), layers, step, page_bytes, num_pages, _p(sources), _p(destinations), n,
+              _p(status), _p(workspace), workspace.nbytes, _stream_ptr(stream))
+
+
 def tune(key: str, value: int) -> None:
     """Overrides a launch-shape choice (``doe_tune_set``); 0 restores automatic."""
     _lib.call("doe_tune_set", key.encode(), int(value))
@@ -727,11 +923,13 @@ def tune(key: str, value: int) -> None:
 
 OPS = {
     "attention": attention,
+    "attention_mx4": attention_mx4,
     "attention_prefill": attention_prefill,
     "dequant": dequant_q4k,
     "embed": embed,
     "gelu_gated": gelu_gated,
     "kv_write": kv_write,
+    "mx4_kv_write": mx4_kv_write,
     "lm_head": lm_head,
     "matmul_q4k": matmul_q4k,
     "matmul_q4k_gemm": matmul_q4k_gemm,

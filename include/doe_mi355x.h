@@ -475,6 +475,142 @@ int doe_attn_decode_partials(const void *q, int q_f16, const uint16_t *k_cache,
                              int64_t partials_capacity, int64_t max_splits, int32_t *splits,
                              doe_stream_t stream);
 
+/* ---- paged KV cache held in 4 bits ------------------------------------------
+ * A quarter of the f16 cache's bytes (17 / 64): K and V rows as microscaled
+ * 4-bit floats in pages of page_size positions, one pool of pages a layer,
+ * any number of sequences.  No reference counterpart: its caches are f16
+ * (attention_head256_f16kv.wgsl:14-63, whose paged layout these pages follow
+ * in spirit: a table of page ids, positions in order).
+ *
+ * A value is an E2M1 code (sign, two exponent bits, one mantissa bit: 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6) times 2^(scale - 127), one scale byte for 32 dims of a
+ * row.  Writing: e = floor(log2 max |x|) - 2, one more from 1.75 times that
+ * power on, held within [-23, 13] (scale bytes 104..140: every value is exact
+ * in f16; larger ones are held as 6 x 2^13 = 49152); codes are the nearest,
+ * ties to the even code.  A block with an infinity or a NaN has scale 255, and
+ * reads as NaN.  Other scale bytes are never written; attention reads them
+ * as far as f16 does.
+ *
+ * A page is num_kv_heads slabs of page_size * (D + D / 16) bytes (D =
+ * head_dim), each:
+ *   K codes   [page_size][D / 2]                     the even dim in the low bits
+ *   V codes   [page_size / 32][4][16][8][D / 32]
+ *   K scales  [page_size][D / 32]
+ *   V scales  [page_size / 32][4][D / 32][8]
+ * where position x of a 32 has its V in quarter (x / 4) % 4 at place
+ * 4 (x / 16) + x % 4 of eight, in 16 columns of D / 16 dims: the order in
+ * which the attention's matrix operands take it, no byte shared by positions.
+ *
+ *   pool        [num_pages][page bytes], 16-byte aligned
+ *   page_table  device int32 [batch][table_stride]: page of positions
+ *               [page_size i, page_size (i + 1)) of a sequence.  An entry
+ *               outside the pool holds nothing: not written, read as zeros,
+ *               not attended.
+ *   kv_lens     device int32 [batch]: positions in use, read by the kernels
+ *               (a captured graph replays with a growing cache); more than
+ *               table_stride * page_size count as that many.
+ * head_dim 64, 128, 160, 256, 512; page_size 32, 64, 128, 256. */
+typedef struct doe_mx4_cache {
+    void *pool;
+    const int32_t *page_table;
+    const int32_t *kv_lens;
+    int64_t num_pages, page_size, num_kv_heads, head_dim, batch, table_stride;
+} doe_mx4_cache;
+
+int doe_mx4_page_bytes(int64_t page_size, int64_t num_kv_heads, int64_t head_dim, int64_t *bytes);
+/* Rows [num_kv_heads][head_dim] of K and V (f32, or f16 with in_f16), row_stride
+ * elements apart, into the cache.  row_starts, device int32 [batch + 1]: rows
+ * [row_starts[b], row_starts[b + 1]) are sequence b's, the last at position
+ * kv_lens[b] - 1, the others before it in order (kv_lens already counts them);
+ * NULL: rows == batch, one row a sequence.  Rows of no sequence and positions
+ * below 0 are skipped.  A page that a call writes must not be held by two of
+ * its sequences (doe_kv_pages_fork gives each its own last page). */
+int doe_mx4_kv_write(const doe_mx4_cache *cache, const void *k, const void *v, int in_f16, int64_t row_stride,
+                     const int32_t *row_starts, int64_t rows, doe_stream_t stream);
+/* The values of the rows that doe_mx4_kv_write would write, as f32.  Rows at
+ * positions that the cache does not hold are zeros, rows of no sequence stay
+ * as they were. */
+int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_stride, const int32_t *row_starts,
+                    int64_t rows, doe_stream_t stream);
+
+/* GQA attention over that cache, one query token a sequence (doe_attn_decode's
+ * rules): q and out [batch][num_heads][head_dim], f16 (q_f16 / out_f16) or
+ * f32; the query of sequence b is at position kv_lens[b] - 1; sliding_window
+ * > 0 keeps the last sliding_window positions; softcap > 0 applies tanh(s /
+ * cap) * cap; a sequence without keys gives zeros.  num_heads any multiple of
+ * num_kv_heads.  f32-accurate (2-4e-7 from float64 with f32 queries and
+ * output).  The work is divided over the device by the lengths that the
+ * kernel reads, so ragged batches fill it evenly.
+ * The workspace (16-byte aligned, doe_attn_mx4_decode_workspace bytes) is the
+ * caller's: calls that may overlap, and captured graphs that may be replayed
+ * side by side, each take their own.  Nothing is kept in it between calls. */
+int doe_attn_mx4_decode_workspace(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                  int64_t *bytes);
+int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, void *out, int out_f16, int64_t num_heads,
+                        float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
+                        doe_stream_t stream);
+/* The prompt form: rows of q and out as in doe_mx4_kv_write (row_starts,
+ * rows; q_row_stride and out_row_stride elements apart), row i of the n of a
+ * sequence at position kv_lens[b] - n + i, causal.  Rows of no sequence are
+ * left as they were; a row at a position below 0 gives zeros.  f32 queries are
+ * carried as f16 hi + lo and probabilities as f16 hi + lo (2-4e-7 from
+ * float64); with q_f16 and out_f16 the probabilities are f16 (below the
+ * output's own rounding).  A short prompt over a long cache splits its keys
+ * over the device and joins them through the workspace. */
+int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
+                                  int64_t head_dim, int64_t *bytes);
+int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,
+                        int out_f16, int64_t out_row_stride, const int32_t *row_starts, int64_t rows, int64_t num_heads,
+                        float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
+                        doe_stream_t stream);
+
+/* ---- pages of a KV cache -------------------------------------------------------
+ * The bookkeeping of a paged cache on the device, of any page format (the 4-bit
+ * cache above, or the f16 pages of doe_attention_dispatch): sequences 0 ..
+ * max_seqs - 1 with rows of page_table and kv_lens (0: the slot is free), and
+ * for each page how many sequences hold it (page_refs, 0: free).  Pages are
+ * taken lowest id first.  Data moves in every layer: layer l's page p is the
+ * page_bytes at pools + l * layer_stride + p * page_bytes (layers 0: only the
+ * bookkeeping; doe_kv_pages_extend and _free move none).
+ * *status (device int32): 0 done; > 0 so many pages are missing; -1 the call's
+ * lists are not in order (a sequence outside [0, max_seqs), named twice, a
+ * child in use or also a parent, a negative count, a table row too short).
+ * A call whose status is not 0 changes nothing -- but doe_kv_pages_free, which
+ * skips entries outside [0, max_seqs) and counts one named twice once.
+ * Asynchronous and capturable; the workspace (16-byte aligned,
+ * doe_kv_pages_workspace bytes; n 0 for compact, max_seqs 0 for copy) is the
+ * caller's, as above. */
+typedef struct doe_kv_pages {
+    void *pools;
+    int64_t layers, layer_stride, page_bytes;
+    int32_t *page_table;
+    int32_t *kv_lens;
+    int32_t *page_refs;
+    int64_t max_seqs, table_stride, num_pages, page_size;
+} doe_kv_pages;
+
+int doe_kv_pages_workspace(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *bytes);
+/* kv_lens[seqs[i]] += add[i] for n sequences, with fresh pages for the positions
+ * past those that they hold. */
+int doe_kv_pages_extend(const doe_kv_pages *pages, const int32_t *seqs, const int32_t *add, int64_t n, int32_t *status,
+                        void *workspace, int64_t workspace_bytes, doe_stream_t stream);
+/* Sequence children[i] (a free slot) becomes a copy of parents[i]: it shares the
+ * parent's whole pages and gets a copy of a last, partly filled one. */
+int doe_kv_pages_fork(const doe_kv_pages *pages, const int32_t *parents, const int32_t *children, int64_t n,
+                      int32_t *status, void *workspace, int64_t workspace_bytes, doe_stream_t stream);
+/* Ends n sequences: their pages are given back, their slots are free. */
+int doe_kv_pages_free(const doe_kv_pages *pages, const int32_t *seqs, int64_t n, int32_t *status, doe_stream_t stream);
+/* Moves the pages in use to the lowest ids (those already there stay), data,
+ * table entries and counts: afterwards the first ones of the pool are in use
+ * and the rest is free. */
+int doe_kv_pages_compact(const doe_kv_pages *pages, int32_t *status, void *workspace, int64_t workspace_bytes,
+                         doe_stream_t stream);
+/* Page destinations[i] = page sources[i] in every layer; status -1 where an id
+ * is outside the pool, a destination comes twice or is also a source. */
+int doe_kv_pages_copy(void *pools, int64_t layers, int64_t layer_stride, int64_t page_bytes, int64_t num_pages,
+                      const int32_t *sources, const int32_t *destinations, int64_t n, int32_t *status, void *workspace,
+                      int64_t workspace_bytes, doe_stream_t stream);
+
 /* ---- normalisation, position and elementwise ops ---------------------------
  * RMSNorm per row: out = x * 1/sqrt(mean(x^2) + eps) * (w or 1 + w).
  * Replaces the `rmsnorm` op (emit_csl_exec_v1.zig:128; rmsnorm.wgsl:1-93,
