@@ -1,15 +1,29 @@
-// attn_mx4.hip -- GQA attention over the paged KV cache held in 4 bits: one
-// query token a sequence (doe_attn_mx4_decode) and prompt rows
-// (doe_attn_mx4_prompt).
+// attn_mx4.hip -- GQA attention of single tokens over the paged KV cache held in 4
+// bits (doe_attn_mx4_decode): o = softmax(cap(q . k scale)) v for one query a
+// sequence, whose length the kernel reads.
 //
-// o = sum_p softmax_p(cap(q . k_p scale)) v_p over the positions p that a row
-// sees: p <= pos, p < kv_len, with a window p > pos - window.
-//
-// One workgroup a row and head: 256 positions at a time, a thread one score;
-// then the running maximum and sum, and a thread one or two dims of P V.
+// A row is a sequence and up to eight query heads of one KV head.  Rows are
+// cut in blocks of 32 positions; all rows' blocks, one after another, are
+// divided evenly among the workgroups, whatever the lengths.  A row that falls
+// into several workgroups leaves its parts (o, m, l) in the caller's workspace
+// and a second kernel joins them.
+//   * S^T = K Q^T on v_mfma_f32_16x16x32_f16: 16 positions x 16 query rows, of
+//     which 0..7 are the heads' f16 hi parts and 8..15 their lo parts (one
+//     exchange of lane halves adds them: f32 quality for no more matrix work).
+//     A lane reads D / 4 dims of a position in one piece and turns each dword of
+//     codes into an operand with four v_cvt_scalef32_pk_f16_fp4, the block's
+//     power of two applied by the same instruction.
+//   * S^T's sums are P^T's operand order as they stand.  P goes to f16 as hi (rows
+//     0..7) + lo (8..15), so it too is carried with 22 bits for nothing.
+//   * O^T = V^T P^T: the page layout gives a lane its eight positions x D / 16 dims
+//     in one piece; pairs of positions are brought together by v_perm.
+//   * The running max is raised only when a score exceeds it by 2^8, P lies
+//     2^7 above it, so that f16's small values lose nothing.
+// No wave waits for another until a row's end.
 #include "mx4_cache.h"
 
 #include <math.h>
+#include <algorithm>
 
 namespace {
 
@@ -17,145 +31,537 @@ using doe::Mx4Slab;
 using doe::Mx4View;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-struct Args {
+constexpr int kWaves = 4, kHeads = 8;
+constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P above the running max, and how far that may lag
+
+struct TokenArgs {
     Mx4View c;
     const void *q;
     void *out;
-    const int32_t *row_starts;
-    int64_t rows, q_stride, out_stride;
-    int q_f16, out_f16, num_heads, window;
+    int q_f16, out_f16, num_heads, group, heads, groups;  // query heads of a KV head, of a row, rows of a KV head
+    int window, per_row, by_row, min_share;
     float scale, softcap;
+    float *part;    // [workgroup][2][kHeads][D], then [workgroup][2][kHeads][2]
+    int2 *joined;   // rows to join: first and last workgroup
 };
 
-__device__ __forceinline__ float scale_of(int s) {
-    return __uint_as_float(s == doe::kMx4NanScale ? 0x7fc00000u : (uint32_t)s << 23);
+// Workgroups that fill the device: as many waves as the registers allow.
+template <int D>
+constexpr int workgroups() { return D <= 128 ? 1024 : (D <= 256 ? 512 : 256); }
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+// The same query row's value in the other half (hi / lo) of its sixteen.
+__device__ __forceinline__ float other_half(float v) { return dpp<0x128>(v); }
+
+// Blocks of sequence b's rows: positions [lo, hi), at least one block.
+__device__ __forceinline__ int blocks_of(const TokenArgs &a, int b, int &lo, int &hi) {
+    hi = doe::mx4_len(a.c, b);
+    lo = a.window > 0 && hi > a.window ? hi - a.window : 0;
+    const int n = (hi + 31) / 32 - lo / 32;
+    return n < 1 ? 1 : n;
+}
+
+// A lane's bytes of a block.
+template <int D>
+struct Block {
+    uint32_t k[2][D / 32], v[D / 16];
+    uint32_t ks[2];                     // scale bytes of its dims, for the two 16-position tiles
+    uint32_t vs[D == 160 ? 4 : 2];      // of its eight positions (160: of both groups its dims may lie in)
+};
+
+// n dwords at p (aligned to 4 bytes, 8 or 16 where n is a multiple of 2 or 4 and so the layout).
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *p) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(p + 4 * i);
+            dst[i] = v[0], dst[i + 1] = v[1], dst[i + 2] = v[2], dst[i + 3] = v[3];
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const u32x2 v = *reinterpret_cast<const u32x2 *>(p + 4 * i);
+            dst[i] = v[0], dst[i + 1] = v[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) dst[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
+    }
+}
+
+// Lane (c16, g4) of the block at position x of a page.
+template <int D>
+__device__ __forceinline__ void load_block(Block<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
+    using S = Mx4Slab<D>;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        load_words<D / 32>(b.k[t], slab + S::k_code(x + 16 * t + c16) + g4 * (D / 8));
+        const uint8_t *ks = slab + S::k_scale(shift, x + 16 * t + c16);
+        if constexpr (D == 64) b.ks[t] = ks[g4 >> 1];
+        else if constexpr (D == 128) b.ks[t] = ks[g4];
+        else if constexpr (D == 160) b.ks[t] = ks[g4] | (uint32_t)ks[g4 + 1] << 8;
+        else if constexpr (D == 256) b.ks[t] = *reinterpret_cast<const uint16_t *>(ks + 2 * g4);
+        else b.ks[t] = *reinterpret_cast<const uint32_t *>(ks + 4 * g4);
+    }
+    load_words<D / 16>(b.v, slab + S::v_code(shift, x, 0) + (g4 * 16 + c16) * (D / 4));
+    const int group = c16 * (D / 16) / 32;
+    const uint8_t *vs = slab + S::v_scale(shift, x, 0) + g4 * (D / 32) * 8;
+    load_words<2>(b.vs, vs + group * 8);
+    if constexpr (D == 160) load_words<2>(b.vs + 2, vs + min(group + 1, 4) * 8);
+}
+
+__device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
+    return __uint_as_float((word >> (8 * byte) & 255u) << 23);
+}
+template <int BYTE>
+__device__ __forceinline__ h2 pair(uint32_t word, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, s, BYTE);
+}
+__device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
+    switch (byte & 3) {
+        case 0: return pair<0>(word, s);
+        case 1: return pair<1>(word, s);
+        case 2: return pair<2>(word, s);
+        default: return pair<3>(word, s);
+    }
+}
+
+// A row's running state in a wave: O^T tile T, dims (4 g4 + i) D / 16 + T of
+// query row c16.
+template <int D>
+struct State {
+    f32x4 o[D / 16];
+    float m, l;
+};
+
+template <int D>
+__device__ __forceinline__ void attend(const TokenArgs &a, State<D> &st, const h8 *qf, const Block<D> &b, float rowf,
+                                       int p0, int lo, int hi, int c16, int g4) {
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            float f;
+            if constexpr (D == 160) f = byte_scale(g4 + i >= 4 ? b.ks[t] >> 8 : b.ks[t], 0);
+            else f = byte_scale(b.ks[t], D >= 128 ? i / 4 : 0);
+            const uint32_t w = b.k[t][i];
+            const h2 k0 = pair<0>(w, f), k1 = pair<1>(w, f), k2 = pair<2>(w, f), k3 = pair<3>(w, f);
+            const h8 kf = {k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]};
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i], s[t], 0, 0, 0);
+        }
+    }
+    // lane: query row c16, positions p0 + 16 t + 4 g4 + i at 4 t + i
+    float x[8];
+    const float kLog2e = 1.4426950408889634f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = s[j >> 2][j & 3];
+        x[j] = (v + other_half(v)) * rowf;
+    }
+    if (a.softcap > 0.0f) {
+        const float f = a.softcap * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = tanhf(x[j]) * f;
+    }
+    const bool whole = p0 >= lo && p0 + 32 <= hi;
+    if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int p = p0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
+            x[j] = p >= lo && p < hi ? x[j] : -INFINITY;
+        }
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(top > st.m + kLazy)) {  // (m = -inf: any score)
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = top > st.m + kLazy ? top : st.m;
+        const float corr = mn == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
+        st.m = mn;
+        st.l *= corr;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.o[t][i] *= corr;
+    }
+    const float mref = st.m == -INFINITY ? 0.0f : st.m - kBias;
+    h8 pf;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float p = __builtin_amdgcn_exp2f(x[j] - mref);
+        st.l += p;
+        const _Float16 ph = (_Float16)p;
+        pf[j] = c16 < 8 ? ph : (_Float16)(p - (float)ph);
+    }
+    // V: position j of the lane's eight at bytes j D / 32 ..; scale 0 where masked (0 times a NaN is one)
+    float vs[8], vs2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        vs[j] = byte_scale(b.vs[j >> 2], j & 3);
+        if constexpr (D == 160) vs2[j] = byte_scale(b.vs[2 + (j >> 2)], j & 3);
+    }
+    if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int p = p0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
+            const bool in = p >= lo && p < hi;
+            vs[j] = in ? vs[j] : 0.0f;
+            if constexpr (D == 160) vs2[j] = in ? vs2[j] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {  // dims 2 i and 2 i + 1 of the lane's
+        h2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = j * (D / 32) + i;
+            float f = vs[j];
+            if constexpr (D == 160) f = 5 * c16 % 16 + i >= 16 ? vs2[j] : f;
+            v[j] = pair_at(b.v[at >> 2], f, at);
+        }
+        const h8 v0 = {v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
+        const h8 v1 = {v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
+        st.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf, st.o[2 * i], 0, 0, 0);
+        st.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf, st.o[2 * i + 1], 0, 0, 0);
+    }
+}
+
+// Query operands of a row in a wave: lane (c16, g4) the dims g4 D / 4 + 8 i ..
+// of head c16 % 8, scaled by a power of two (max near 2^14), hi or lo part;
+// rowf takes the scale out of a score again.
+template <int D>
+__device__ __forceinline__ void load_query(const TokenArgs &a, h8 *qf, float &rowf, int b, int head0, int heads, int c16, int g4) {
+    const int head = c16 & 7;
+    const bool real = head < heads;
+    const int64_t at = ((int64_t)b * a.num_heads + head0 + (real ? head : 0)) * D + g4 * (D / 4);
+    float f[D / 4];
+    if (a.q_f16) {
+#pragma unroll
+        for (int i = 0; i < D / 4; i += 8) {
+            const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + at + i);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; i += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + i);
+            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+        }
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) amax = fmaxf(amax, fabsf(f[i]));
+    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    int sg = 0;
+    if (amax > 0.0f && amax <= 3.0e38f) {
+        sg = 14 - __builtin_amdgcn_frexp_expf(amax);
+        sg = sg < -100 ? -100 : (sg > 100 ? 100 : sg);
+    }
+    const float sc = real ? __builtin_amdgcn_ldexpf(1.0f, sg) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = f[8 * i + e] * sc;
+            const _Float16 h = (_Float16)v;
+            qf[i][e] = c16 < 8 ? h : (_Float16)(v - (float)h);
+        }
+    rowf = a.scale * __builtin_amdgcn_ldexpf(1.0f, -sg);
+    rowf = a.softcap > 0.0f ? rowf / a.softcap : rowf * 1.4426950408889634f;
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void attn_mx4_rows_kernel(Args a) {
-    using S = Mx4Slab<D>;
-    __shared__ float qs[D], p_[256], red[4];
-    __shared__ int page_[256];
-    const int tid = threadIdx.x, head = blockIdx.x % a.num_heads;
-    const int64_t row = blockIdx.x / a.num_heads;
-    int b, pos;
-    const bool seen = doe::mx4_row(a.c, a.row_starts, row, b, pos);
-    if (a.row_starts && (row < a.row_starts[0] || row >= a.row_starts[a.c.batch])) return;
-    const int kvh = head / (a.num_heads / a.c.kv_heads), shift = a.c.page_shift;
-    int hi = 0, lo = 0;
-    if (seen) {
-        hi = min(pos + 1, doe::mx4_len(a.c, b));
-        if (a.window > 0) lo = max(0, pos - a.window + 1);
+struct TokenLds {
+    static constexpr int kRow = D + 4;
+    float o[kWaves][kHeads][kRow];
+    float2 ml[kWaves][kHeads];
+};
+
+template <int D>
+__global__ __launch_bounds__(64 * kWaves) void attn_mx4_token_kernel(TokenArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
+    TokenLds<D> &sm = *reinterpret_cast<TokenLds<D> *>(lds_raw);
+    __shared__ int sums[kWaves], start[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4, shift = a.c.page_shift;
+    const int rows_of = a.c.kv_heads * a.groups;  // rows of a sequence
+    // this workgroup's blocks [at, end) of all, the first of them in sequence b
+    int64_t at, end, share, base = 0;  // base: the first block of sequence b
+    int b = 0;
+    if (a.per_row) {
+        b = (int)blockIdx.x / rows_of;
+        int lo, hi;
+        const int n = blocks_of(a, b, lo, hi);
+        share = n;
+        at = (int64_t)((int)blockIdx.x - b * rows_of) * n;
+        end = at + n;
+    } else {
+        // blocks of a row in all sequences, then (again) up to the one where this share begins
+        int64_t total = 0;
+        for (int b0 = 0; b0 < a.c.batch; b0 += 64 * kWaves) {
+            int lo, hi, n = b0 + tid < a.c.batch ? blocks_of(a, b0 + tid, lo, hi) : 0;
+            for (int w = 1; w < 64; w <<= 1) n += __shfl_xor(n, w, 64);
+            __syncthreads();
+            if (lane == 0) sums[wave] = n;
+            __syncthreads();
+            total += (int64_t)sums[0] + sums[1] + sums[2] + sums[3];
+        }
+        total *= rows_of;
+        share = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, a.min_share);
+        at = share * blockIdx.x;
+        end = std::min(at + share, total);
+        if (!a.by_row && tid == 0) a.joined[blockIdx.x] = make_int2(-1, -1);
+        if (at >= end) return;
+        for (int b0 = 0; b0 < a.c.batch; b0 += 64 * kWaves) {
+            int lo, hi;
+            const int mine = b0 + tid < a.c.batch ? blocks_of(a, b0 + tid, lo, hi) : 0;
+            int n = mine;
+            for (int w = 1; w < 64; w <<= 1) {
+                const int u = __shfl_up(n, w, 64);
+                if (lane >= w) n += u;
+            }
+            __syncthreads();
+            if (lane == 63) sums[wave] = n;
+            if (tid == 0) start[0] = -1;
+            __syncthreads();
+            int64_t first = base;
+            for (int w = 0; w < wave; ++w) first += (int64_t)sums[w] * rows_of;
+            const int64_t upto = first + (int64_t)n * rows_of;
+            if (mine && at >= upto - (int64_t)mine * rows_of && at < upto) {
+                start[0] = b0 + tid;
+                start[1] = n - mine;  // blocks before it in its wave
+            }
+            __syncthreads();
+            if (start[0] >= 0) {
+                b = __builtin_amdgcn_readfirstlane(start[0]);
+                for (int w = 0; w < (b - b0) / 64; ++w) base += (int64_t)sums[w] * rows_of;
+                base += (int64_t)start[1] * rows_of;
+                break;
+            }
+            base += ((int64_t)sums[0] + sums[1] + sums[2] + sums[3]) * rows_of;
+        }
     }
-    for (int d = tid; d < D; d += 256) {
-        const int64_t at = row * a.q_stride + (int64_t)head * D + d;
-        qs[d] = a.q_f16 ? (float)static_cast<const _Float16 *>(a.q)[at] : static_cast<const float *>(a.q)[at];
-    }
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[(D + 255) / 256] = {};
-    for (int p0 = lo; p0 < hi; p0 += 256) {
-        const int p = p0 + tid, page = p < hi ? doe::mx4_page(a.c, b, p) : -1, x = p & ((1 << shift) - 1);
-        float s = -INFINITY;
-        if (page >= 0) {
-            const uint8_t *slab = a.c.pool + ((int64_t)page * a.c.kv_heads + kvh) * S::bytes(shift);
-            s = 0.0f;
-            for (int g = 0; g < D / 32; ++g) {
-                const float f = scale_of(slab[S::k_scale(shift, x) + g]);
-                for (int d = 32 * g; d < 32 * g + 32; d += 2) {
-                    const h2 k = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(slab[S::k_code(x) + d / 2], f, 0);
-                    s = fmaf(qs[d], (float)k[0], s);
-                    s = fmaf(qs[d + 1], (float)k[1], s);
+    while (at < end) {
+        int lo, hi;
+        const int n = blocks_of(a, b, lo, hi);
+        const int r = (int)((at - base) / n);  // row of the sequence
+        if (r >= rows_of) {
+            base += (int64_t)rows_of * n;
+            ++b;
+            continue;
+        }
+        const int64_t row0 = base + (int64_t)r * n;
+        const int first = (int)(at - row0), last = (int)(std::min(row0 + n, end) - row0);  // blocks of this row
+        const int kvh = r / a.groups, head0 = kvh * a.group + (r - kvh * a.groups) * a.heads;
+        const int heads = std::min(a.heads, (kvh + 1) * a.group - head0);
+        const int blk0 = lo / 32 + first + wave, count = (last - first - wave + kWaves - 1) / kWaves;
+        State<D> st;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) st.o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        st.m = -INFINITY;
+        st.l = 0.0f;
+        if (count > 0) {
+            h8 qf[D / 32];
+            float rowf;
+            load_query<D>(a, qf, rowf, b, head0, heads, c16, g4);
+            // the pages of up to 64 of this wave's blocks, a lane each
+            const int32_t *table = a.c.table + (int64_t)b * a.c.table_stride;
+            auto pages = [&](int i0) {
+                const int blk = blk0 + kWaves * (i0 + lane);
+                int page = -1;
+                if (i0 + lane < count && blk * 32 < hi) {
+                    page = table[blk >> (shift - 5)];
+                    if (page < 0 || page >= a.c.num_pages) page = -1;
+                }
+                return page;
+            };
+            int mine = pages(0);
+            auto page_of = [&](int i) { return __builtin_amdgcn_readlane(mine, i & 63); };
+            auto fetch = [&](Block<D> &blk, int i, int page) {
+                const uint8_t *slab = a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
+                load_block<D>(blk, slab, shift, ((blk0 + kWaves * i) * 32) & ((1 << shift) - 1), c16, g4);
+            };
+            Block<D> buf[2];
+            int page = page_of(0), next = -1;
+            fetch(buf[0], 0, page);
+            for (int i = 0; i < count; i += 2) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (i + u >= count) break;
+                    const int in = std::min(i + u + 1, count - 1);
+                    if ((in & 63) == 0 && in) mine = pages(in);
+                    next = page_of(in);
+                    fetch(buf[1 - u], in, next);
+                    if (page >= 0) attend<D>(a, st, qf, buf[u], rowf, (blk0 + kWaves * (i + u)) * 32, lo, hi, c16, g4);
+                    page = next;
                 }
             }
-            s *= a.scale;
-            if (a.softcap > 0.0f) s = tanhf(s / a.softcap) * a.softcap;
         }
-        page_[tid] = page;
-        float top = s;
-        for (int w = 1; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = top;
+        // the row's four waves together
+        float l = st.l + __shfl_xor(st.l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        __syncthreads();  // the last row's sums have been read
+        if (lane < kHeads) sm.ml[wave][lane] = make_float2(st.m, l);
         __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float mref = mn == -INFINITY ? 0.0f : mn, corr = expf(m - mref);
-        p_[tid] = expf(s - mref);
-        m = mn;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm.ml[w][c16 & 7].x);
+        const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - M);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+                const float v = st.o[t][i] * corr, sum = v + other_half(v);
+                if (c16 < kHeads) sm.o[wave][c16][(4 * g4 + i) * (D / 16) + t] = sum;
+            }
         __syncthreads();
-        l *= corr;
-        for (int i = 0; i < (D + 255) / 256; ++i) o[i] *= corr;
-        for (int j = 0; j < 256; ++j) {
-            if (page_[j] < 0) continue;
-            const float pj = p_[j];
-            l += pj;
-            const int xj = (p0 + j) & ((1 << shift) - 1);
-            const uint8_t *slab = a.c.pool + ((int64_t)page_[j] * a.c.kv_heads + kvh) * S::bytes(shift);
-            for (int i = 0; i < (D + 255) / 256; ++i) {
-                const int d = tid + 256 * i;
-                if (d >= D) continue;
-                const float f = scale_of(slab[S::v_scale(shift, xj, d / 32)]);
-                const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(slab[S::v_code(shift, xj, d / (D / 16)) + d % (D / 16) / 2], f, 0);
-                o[i] = fmaf(pj, (float)v[d & 1], o[i]);
+        const bool split = first > 0 || last < n;
+        const int slot = first > 0 ? 0 : 1;  // begun before this workgroup, or here
+        for (int e = tid; e < heads * (D / 4); e += 64 * kWaves) {
+            const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
+            float M2 = -INFINITY, lt = 0.0f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) M2 = fmaxf(M2, sm.ml[w][h].x);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 ml = sm.ml[w][h];
+                const float4 o = *reinterpret_cast<const float4 *>(&sm.o[w][h][d]);
+                lt += ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - M2);
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+            }
+            if (split) {
+                const int64_t p = ((int64_t)blockIdx.x * 2 + slot) * kHeads + h;
+                *reinterpret_cast<float4 *>(a.part + p * D + d) = v;
+                if (d == 0) reinterpret_cast<float2 *>(a.part + (int64_t)gridDim.x * 2 * kHeads * D)[p] = make_float2(M2, lt);
+            } else {
+                const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+                const int64_t to = ((int64_t)b * a.num_heads + head0 + h) * D + d;
+                if (a.out_f16) {
+                    _Float16 *o = static_cast<_Float16 *>(a.out) + to;
+                    o[0] = (_Float16)(v.x * inv), o[1] = (_Float16)(v.y * inv), o[2] = (_Float16)(v.z * inv), o[3] = (_Float16)(v.w * inv);
+                } else {
+                    *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) =
+                        make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                }
             }
         }
-        __syncthreads();
-    }
-    for (int i = 0; i < (D + 255) / 256; ++i) {
-        const int d = tid + 256 * i;
-        if (d >= D) continue;
-        const int64_t at = row * a.out_stride + (int64_t)head * D + d;
-        const float v = l != 0.0f ? o[i] / l : 0.0f;
-        if (a.out_f16) static_cast<_Float16 *>(a.out)[at] = (_Float16)v;
-        else static_cast<float *>(a.out)[at] = v;
+        // the workgroup in which a row ends says where its parts are
+        if (!a.per_row && tid == 0 && last == n && (a.by_row || first > 0)) {
+            const int row = b * rows_of + r, from = first > 0 ? (int)(row0 / share) : -1;
+            a.joined[a.by_row ? row : (int)blockIdx.x] = make_int2(from, a.by_row ? (int)blockIdx.x : row);
+        }
+        at = row0 + last;
     }
 }
 
-int attention(Args &a, const doe_mx4_cache *cache, int64_t num_heads, int64_t sliding_window, void *workspace,
-              int64_t workspace_bytes, int64_t need, hipStream_t st) {
-    const int64_t d = cache->head_dim;
-    DOE_REQUIRE(isfinite(a.scale) && isfinite(a.softcap) && a.softcap >= 0.0f, DOE_E_INVALID, "scale %g, softcap %g",
-                (double)a.scale, (double)a.softcap);
-    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
-                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
-    DOE_REQUIRE(num_heads > 0 && num_heads <= 65535 && num_heads % a.c.kv_heads == 0, DOE_E_INVALID,
-                "num_heads %lld is not a positive multiple of num_kv_heads %d", (long long)num_heads, a.c.kv_heads);
-    DOE_REQUIRE(sliding_window >= 0 && sliding_window < ((int64_t)1 << 30), DOE_E_INVALID, "sliding_window %lld",
-                (long long)sliding_window);
-    DOE_REQUIRE(a.rows >= 0 && a.rows * num_heads < ((int64_t)1 << 31), DOE_E_INVALID, "%lld rows of %lld heads",
-                (long long)a.rows, (long long)num_heads);
-    DOE_REQUIRE(a.row_starts || a.rows == a.c.batch, DOE_E_INVALID,
-                "without row_starts a call takes one row a sequence (%lld rows, batch %d)", (long long)a.rows, a.c.batch);
-    DOE_REQUIRE(a.q_stride >= num_heads * d && a.out_stride >= num_heads * d && a.q_stride * (a.q_f16 ? 2 : 4) % 16 == 0 &&
-                    a.out_stride * (a.out_f16 ? 2 : 4) % 16 == 0,
-                DOE_E_INVALID, "row strides below a row, or not multiples of 16 bytes");
-    DOE_REQUIRE(a.rows == 0 || (a.q && a.out), DOE_E_INVALID, "null pointer");
-    DOE_REQUIRE(((uintptr_t)a.q & 15) == 0 && ((uintptr_t)a.out & 15) == 0, DOE_E_INVALID, "q and out must be 16-byte aligned");
-    const int rc = doe::require_init();
-    if (rc) return rc;
-    if (a.rows == 0 || a.c.batch == 0) return DOE_OK;
-    a.num_heads = (int)num_heads;
-    a.window = (int)sliding_window;
-    const dim3 grid((unsigned)(a.rows * num_heads));
-    switch (d) {
-        case 64: hipLaunchKernelGGL(attn_mx4_rows_kernel<64>, grid, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL(attn_mx4_rows_kernel<128>, grid, dim3(256), 0, st, a); break;
-        case 160: hipLaunchKernelGGL(attn_mx4_rows_kernel<160>, grid, dim3(256), 0, st, a); break;
-        case 256: hipLaunchKernelGGL(attn_mx4_rows_kernel<256>, grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(attn_mx4_rows_kernel<512>, grid, dim3(256), 0, st, a); break;
+// A split row's head: its parts, of the workgroups first .. last, in the order
+// of a fixed tree.  D / 4 lanes hold the dims, kJoin / (D / 4) groups take every
+// so manieth part and meet in LDS.
+constexpr int kJoin = 512;
+template <int D>
+__global__ __launch_bounds__(kJoin) void attn_mx4_join_kernel(TokenArgs a, int wgs) {
+    constexpr int L = D / 4, GROUPS = kJoin / L;
+    __shared__ float4 so[GROUPS][L];
+    __shared__ float2 sml[GROUPS];
+    const int2 j = a.joined[blockIdx.x];
+    if (j.x < 0) return;
+    const int first = j.x, last = a.by_row ? j.y : (int)blockIdx.x, row = a.by_row ? (int)blockIdx.x : j.y;
+    const int rows_of = a.c.kv_heads * a.groups, b = row / rows_of, r = row - b * rows_of, kvh = r / a.groups;
+    const int head0 = kvh * a.group + (r - kvh * a.groups) * a.heads, h = blockIdx.y;
+    if (h >= std::min(a.heads, (kvh + 1) * a.group - head0)) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)wgs * 2 * kHeads * D);
+    const int grp = threadIdx.x / L, d = (threadIdx.x - grp * L) * 4;
+    float M = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp < GROUPS) {
+#pragma unroll 4
+        for (int s = first + grp; s <= last; s += GROUPS) {
+            const int64_t p = ((int64_t)s * 2 + (s == first)) * kHeads + h;
+            const float2 e = ml[p];
+            const float4 o = *reinterpret_cast<const float4 *>(a.part + p * D + d);
+            const float mn = fmaxf(M, e.x), f0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+            const float f1 = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - mn);
+            M = mn;
+            l = l * f0 + e.y * f1;
+            v.x = v.x * f0 + o.x * f1, v.y = v.y * f0 + o.y * f1, v.z = v.z * f0 + o.z * f1, v.w = v.w * f0 + o.w * f1;
+        }
+        so[grp][d / 4] = v;
+        if (d == 0) sml[grp] = make_float2(M, l);
     }
-    DOE_LAUNCH_CHECK("attn_mx4_rows_kernel");
-    return DOE_OK;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int g = 0; g < GROUPS; ++g) M = fmaxf(M, sml[g].x);
+    l = 0.0f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = 0; g < GROUPS; ++g) {
+        const float2 e = sml[g];
+        const float4 o = so[g][d / 4];
+        const float f = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - M);
+        l += e.y * f;
+        v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int64_t to = ((int64_t)b * a.num_heads + head0 + h) * D + d;
+    if (a.out_f16) {
+        _Float16 *o = static_cast<_Float16 *>(a.out) + to;
+        o[0] = (_Float16)(v.x * inv), o[1] = (_Float16)(v.y * inv), o[2] = (_Float16)(v.z * inv), o[3] = (_Float16)(v.w * inv);
+    } else {
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    }
 }
 
-int workspace_size(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t *bytes) {
-    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
-    int64_t page = 0;
-    const int rc = doe_mx4_page_bytes(32, num_kv_heads, head_dim, &page);
-    if (rc) return rc;
-    DOE_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && num_heads > 0 && num_heads <= 65535 &&
-                    num_heads % num_kv_heads == 0 && rows * num_heads < ((int64_t)1 << 31),
-                DOE_E_INVALID, "batch %lld, %lld rows, %lld heads over %lld", (long long)batch, (long long)rows,
-                (long long)num_heads, (long long)num_kv_heads);
-    *bytes = 16;
+template <int D>
+int64_t workspace() {
+    return (int64_t)workgroups<D>() * (2 * kHeads * (D + 2) * 4 + 8);
+}
+
+int64_t workspace_of(int64_t head_dim) {
+    switch (head_dim) {
+        case 64: return workspace<64>();
+        case 128: return workspace<128>();
+        case 160: return workspace<160>();
+        case 256: return workspace<256>();
+        default: return workspace<512>();
+    }
+}
+
+template <int D>
+int launch(TokenArgs &a, void *ws, hipStream_t st) {
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_token_kernel<D>,
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(TokenLds<D>));
+    DOE_HIP_CHECK(attr_rc);
+    const int64_t rows = (int64_t)a.c.batch * a.c.kv_heads * a.groups;
+    int64_t most = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;  // blocks of a row, as far as the host knows
+    if (a.window > 0) most = std::min<int64_t>(most, a.window / 32 + 2);
+    a.min_share = kWaves;
+    a.per_row = most <= 2 * kWaves;
+    int64_t wgs = rows;
+    if (!a.per_row) {
+        wgs = std::min<int64_t>(workgroups<D>(), rows * ((most + a.min_share - 1) / a.min_share));
+        a.by_row = rows <= wgs;
+        a.part = static_cast<float *>(ws);
+        a.joined = reinterpret_cast<int2 *>(a.part + wgs * 2 * kHeads * (D + 2));
+    }
+    hipLaunchKernelGGL(attn_mx4_token_kernel<D>, dim3((unsigned)wgs), dim3(64 * kWaves), sizeof(TokenLds<D>), st, a);
+    DOE_LAUNCH_CHECK("attn_mx4_token_kernel");
+    if (a.per_row) return DOE_OK;
+    hipLaunchKernelGGL(attn_mx4_join_kernel<D>, dim3((unsigned)(a.by_row ? rows : wgs), (unsigned)a.heads), dim3(kJoin), 0, st, a,
+                       (int)wgs);
+    DOE_LAUNCH_CHECK("attn_mx4_join_kernel");
     return DOE_OK;
 }
 
@@ -165,49 +571,47 @@ extern "C" {
 
 int doe_attn_mx4_decode_workspace(int64_t batch, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                                   int64_t *bytes) {
-    return workspace_size(batch, batch, num_heads, num_kv_heads, head_dim, bytes);
+    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
+    int64_t page = 0;
+    const int rc = doe_mx4_page_bytes(32, num_kv_heads, head_dim, &page);
+    if (rc) return rc;
+    DOE_REQUIRE(batch >= 0 && batch <= 65535 && num_heads > 0 && num_heads <= 65535 && num_heads % num_kv_heads == 0,
+                DOE_E_INVALID, "batch %lld, %lld heads over %lld", (long long)batch, (long long)num_heads, (long long)num_kv_heads);
+    *bytes = workspace_of(head_dim);
+    return DOE_OK;
 }
 
 int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, void *out, int out_f16, int64_t num_heads,
                         float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
                         doe_stream_t stream) {
-    Args a{};
-    const int rc = doe::mx4_view(cache, &a.c);
+    TokenArgs a{};
+    int rc = doe::mx4_view(cache, &a.c);
     if (rc) return rc;
+    if ((rc = doe::mx4_attention_checks(a.c, num_heads, scale, softcap, sliding_window, q, out))) return rc;
+    const int64_t need = workspace_of(cache->head_dim);
+    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
+                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
+    if ((rc = doe::require_init())) return rc;
+    if (a.c.batch == 0) return DOE_OK;
     a.q = q;
     a.out = out;
-    a.rows = a.c.batch;
-    a.q_stride = a.out_stride = num_heads * cache->head_dim;
-    a.q_f16 = q_f16;
-    a.out_f16 = out_f16;
+    a.q_f16 = q_f16 != 0;
+    a.out_f16 = out_f16 != 0;
+    a.num_heads = (int)num_heads;
+    a.group = (int)(num_heads / a.c.kv_heads);
+    a.groups = (a.group + kHeads - 1) / kHeads;
+    a.heads = (a.group + a.groups - 1) / a.groups;
+    a.groups = (a.group + a.heads - 1) / a.heads;
+    a.window = (int)sliding_window;
     a.scale = scale;
     a.softcap = softcap;
-    return attention(a, cache, num_heads, sliding_window, workspace, workspace_bytes, 16, (hipStream_t)stream);
-}
-
-int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
-                                  int64_t head_dim, int64_t *bytes) {
-    return workspace_size(batch, rows, num_heads, num_kv_heads, head_dim, bytes);
-}
-
-int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,
-                        int out_f16, int64_t out_row_stride, const int32_t *row_starts, int64_t rows, int64_t num_heads,
-                        float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
-                        doe_stream_t stream) {
-    Args a{};
-    const int rc = doe::mx4_view(cache, &a.c);
-    if (rc) return rc;
-    a.q = q;
-    a.out = out;
-    a.row_starts = row_starts;
-    a.rows = rows;
-    a.q_stride = q_row_stride;
-    a.out_stride = out_row_stride;
-    a.q_f16 = q_f16;
-    a.out_f16 = out_f16;
-    a.scale = scale;
-    a.softcap = softcap;
-    return attention(a, cache, num_heads, sliding_window, workspace, workspace_bytes, 16, (hipStream_t)stream);
+    switch (cache->head_dim) {
+        case 64: return launch<64>(a, workspace, (hipStream_t)stream);
+        case 128: return launch<128>(a, workspace, (hipStream_t)stream);
+        case 160: return launch<160>(a, workspace, (hipStream_t)stream);
+        case 256: return launch<256>(a, workspace, (hipStream_t)stream);
+        default: return launch<512>(a, workspace, (hipStream_t)stream);
+    }
 }
 
 }  // extern "C"

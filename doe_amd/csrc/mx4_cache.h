@@ -80,5 +80,8 @@ __device__ __forceinline__ int mx4_page(const Mx4View &c, int b, int pos) {
 
 // Checks a cache and turns it into the kernels' form; returns a DOE status.
 int mx4_view(const doe_mx4_cache *cache, Mx4View *view);
+// What both attentions check of a call.
+int mx4_attention_checks(const Mx4View &c, int64_t num_heads, float scale, float softcap, int64_t sliding_window,
+                         const void *q, const void *out);
 
 }  // namespace doe

@@ -9,6 +9,8 @@
 // infinity or a NaN keeps scale byte 255 (codes 0) and reads as NaN throughout.
 #include "mx4_cache.h"
 
+#include <math.h>
+
 namespace {
 
 using doe::Mx4Slab;
@@ -214,6 +216,19 @@ int mx4_view(const doe_mx4_cache *cache, Mx4View *view) {
     view->kv_heads = (int)c.num_kv_heads;
     view->batch = (int)c.batch;
     view->table_stride = (int)c.table_stride;
+    return DOE_OK;
+}
+
+int mx4_attention_checks(const Mx4View &c, int64_t num_heads, float scale, float softcap, int64_t sliding_window,
+                         const void *q, const void *out) {
+    DOE_REQUIRE(num_heads > 0 && num_heads <= 65535 && num_heads % c.kv_heads == 0, DOE_E_INVALID,
+                "num_heads %lld is not a positive multiple of num_kv_heads %d", (long long)num_heads, c.kv_heads);
+    DOE_REQUIRE(isfinite(scale) && isfinite(softcap) && softcap >= 0.0f, DOE_E_INVALID, "scale %g, softcap %g", (double)scale,
+                (double)softcap);
+    DOE_REQUIRE(sliding_window >= 0 && sliding_window < ((int64_t)1 << 30), DOE_E_INVALID, "sliding_window %lld",
+                (long long)sliding_window);
+    DOE_REQUIRE(c.batch == 0 || (q && out), DOE_E_INVALID, "null pointer");
+    DOE_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0, DOE_E_INVALID, "q and out must be 16-byte aligned");
     return DOE_OK;
 }
 
