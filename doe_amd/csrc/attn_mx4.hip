@@ -50,9 +50,12 @@ struct TokenArgs {
     int2 *joined;   // rows to join: first and last workgroup
 };
 
-// Workgroups that fill the device: as many waves as the registers allow.
+// Workgroups of four waves that a CU holds at once, by the registers that a wave
+// takes, and those that fill the device's 256 CUs in one round.
 template <int D>
-constexpr int workgroups() { return D <= 128 ? 1024 : (D <= 256 ? 512 : 256); }
+constexpr int per_cu() { return D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 256 ? 2 : 1)); }
+template <int D>
+constexpr int workgroups() { return 256 * per_cu<D>(); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -61,20 +64,38 @@ __device__ __forceinline__ float dpp(float v) {
 // The same query row's value in the other half (hi / lo) of its sixteen.
 __device__ __forceinline__ float other_half(float v) { return dpp<0x128>(v); }
 
-// Blocks of sequence b's rows: positions [lo, hi), at least one block.
-__device__ __forceinline__ int blocks_of(const TokenArgs &a, int b, int &lo, int &hi) {
-    hi = doe::mx4_len(a.c, b);
-    lo = a.window > 0 && hi > a.window ? hi - a.window : 0;
-    const int n = (hi + 31) / 32 - lo / 32;
+// Inclusive sum over the wave's lanes, in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xf>(v);  // one lane further within sixteen, two, four, eight
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);        // the last lane of a sixteen to the next (rows 1 and 3)
+    return dpp_add<0x143, 0xc>(v);     // lane 31 to rows 2 and 3
+}
+
+// Blocks of the rows of a sequence of hi positions, the first seen one at lo; at
+// least one (of an empty sequence it gives the zeros).
+__device__ __forceinline__ int first_seen(const TokenArgs &a, int hi) { return a.window > 0 && hi > a.window ? hi - a.window : 0; }
+__device__ __forceinline__ int blocks_of(const TokenArgs &a, int hi) {
+    const int n = ((hi + 31) >> 5) - (first_seen(a, hi) >> 5);
     return n < 1 ? 1 : n;
 }
 
-// A lane's bytes of a block.
+// A lane's bytes of a block: its dims of K at two positions, with their scale
+// bytes, and its dims of V at eight with theirs (head_dim 160: of both groups
+// that its dims may lie in).
 template <int D>
-struct Block {
-    uint32_t k[2][D / 32], v[D / 16];
-    uint32_t ks[2];                     // scale bytes of its dims, for the two 16-position tiles
-    uint32_t vs[D == 160 ? 4 : 2];      // of its eight positions (160: of both groups its dims may lie in)
+struct KBlock {
+    uint32_t k[2][D / 32], ks[2];
+};
+template <int D>
+struct VBlock {
+    uint32_t v[D / 16], vs[D == 160 ? 4 : 2];
 };
 
 // n dwords at p (aligned to 4 bytes, 8 or 16 where n is a multiple of 2 or 4 and so the layout).
@@ -100,7 +121,7 @@ __device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *p) {
 
 // Lane (c16, g4) of the block at position x of a page.
 template <int D>
-__device__ __forceinline__ void load_block(Block<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
+__device__ __forceinline__ void load_k(KBlock<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
     using S = Mx4Slab<D>;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -112,6 +133,10 @@ __device__ __forceinline__ void load_block(Block<D> &b, const uint8_t *slab, int
         else if constexpr (D == 256) b.ks[t] = *reinterpret_cast<const uint16_t *>(ks + 2 * g4);
         else b.ks[t] = *reinterpret_cast<const uint32_t *>(ks + 4 * g4);
     }
+}
+template <int D>
+__device__ __forceinline__ void load_v(VBlock<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
+    using S = Mx4Slab<D>;
     load_words<D / 16>(b.v, slab + S::v_code(shift, x, 0) + (g4 * 16 + c16) * (D / 4));
     const int group = c16 * (D / 16) / 32;
     const uint8_t *vs = slab + S::v_scale(shift, x, 0) + g4 * (D / 32) * 8;
@@ -143,10 +168,10 @@ struct State {
     float m, l;
 };
 
+// S^T of a block: query row c16, positions 16 t + 4 g4 + i at s[t][i], hi and lo
+// parts of the query in their own rows.
 template <int D>
-__device__ __forceinline__ void attend(const TokenArgs &a, State<D> &st, const h8 *qf, const Block<D> &b, float rowf,
-                                       int p0, int lo, int hi, int c16, int g4) {
-    f32x4 s[2];
+__device__ __forceinline__ void scores(f32x4 *s, const h8 *qf, const KBlock<D> &b, int g4) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -161,7 +186,13 @@ __device__ __forceinline__ void attend(const TokenArgs &a, State<D> &st, const h
             s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i], s[t], 0, 0, 0);
         }
     }
-    // lane: query row c16, positions p0 + 16 t + 4 g4 + i at 4 t + i
+}
+
+// P^T of a block at positions p0 .. (those in [lo, hi) are seen), the state's
+// maximum raised and its sum carried on.
+template <int D>
+__device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f32x4 *s, float rowf, int p0, int lo, int hi,
+                                      int c16, int g4) {
     float x[8];
     const float kLog2e = 1.4426950408889634f;
 #pragma unroll
@@ -204,14 +235,20 @@ __device__ __forceinline__ void attend(const TokenArgs &a, State<D> &st, const h
         const _Float16 ph = (_Float16)p;
         pf[j] = c16 < 8 ? ph : (_Float16)(p - (float)ph);
     }
-    // V: position j of the lane's eight at bytes j D / 32 ..; scale 0 where masked (0 times a NaN is one)
+    return pf;
+}
+
+// O^T += V^T P^T.  Position j of the lane's eight is at bytes j D / 32 ..; scale
+// 0 where it is not seen (0 times a NaN is one).
+template <int D>
+__device__ __forceinline__ void values(State<D> &st, const h8 pf, const VBlock<D> &b, int p0, int lo, int hi, int c16, int g4) {
     float vs[8], vs2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         vs[j] = byte_scale(b.vs[j >> 2], j & 3);
         if constexpr (D == 160) vs2[j] = byte_scale(b.vs[2 + (j >> 2)], j & 3);
     }
-    if (!whole) {
+    if (p0 < lo || p0 + 32 > hi) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int p = p0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
@@ -237,183 +274,189 @@ __device__ __forceinline__ void attend(const TokenArgs &a, State<D> &st, const h
     }
 }
 
-// Query operands of a row in a wave: lane (c16, g4) the dims g4 D / 4 + 8 i ..
-// of head c16 % 8, scaled by a power of two (max near 2^14), hi or lo part;
-// rowf takes the scale out of a score again.
 template <int D>
-__device__ __forceinline__ void load_query(const TokenArgs &a, h8 *qf, float &rowf, int b, int head0, int heads, int c16, int g4) {
-    const int head = c16 & 7;
-    const bool real = head < heads;
-    const int64_t at = ((int64_t)b * a.num_heads + head0 + (real ? head : 0)) * D + g4 * (D / 4);
-    float f[D / 4];
+struct TokenLds {
+    static constexpr int kRow = D + 4;
+    h8 q[D / 32][64];  // a row's query operands
+    float rowf[kHeads];
+    float o[kWaves][kHeads][kRow];
+    float2 ml[kWaves][kHeads];
+};
+
+// A row's queries, two heads a wave and D / 32 dims a lane, into operand order:
+// lane (c16, g4) of step i takes dims g4 D / 4 + 8 i .. of head c16 % 8, scaled
+// by a power of two (max near 2^14), the f16 hi part (c16 < 8) or the lo part;
+// rowf takes the scale out of a score again.  Heads that the row lacks are 0.
+template <int D>
+struct RawQuery {
+    static constexpr int N = D / 32;
+    float f[N];
+};
+template <int D>
+__device__ __forceinline__ void read_query(RawQuery<D> &r, const TokenArgs &a, int64_t row, int heads, int wave, int lane) {
+    constexpr int N = RawQuery<D>::N;
+    const int head = 2 * wave + (lane >> 5);
+    const int64_t at = row + (head < heads ? head : 0) * D + (lane & 31) * N;
     if (a.q_f16) {
+        const _Float16 *p = static_cast<const _Float16 *>(a.q) + at;
 #pragma unroll
-        for (int i = 0; i < D / 4; i += 8) {
-            const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + at + i);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
-        }
+        for (int i = 0; i < N; ++i) r.f[i] = (float)p[i];
     } else {
+        const float *p = static_cast<const float *>(a.q) + at;
 #pragma unroll
-        for (int i = 0; i < D / 4; i += 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + i);
-            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
-        }
+        for (int i = 0; i < N; ++i) r.f[i] = p[i];
     }
+}
+template <int D>
+__device__ __forceinline__ void stage_query(const TokenArgs &a, const RawQuery<D> &r, TokenLds<D> &sm, int heads, int wave, int lane) {
+    constexpr int N = RawQuery<D>::N;
+    const int head = 2 * wave + (lane >> 5);
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) amax = fmaxf(amax, fabsf(f[i]));
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(r.f[i]));
+    amax = fmaxf(amax, dpp<0xB1>(amax));
+    amax = fmaxf(amax, dpp<0x4E>(amax));
+    amax = fmaxf(amax, dpp<0x141>(amax));
+    amax = fmaxf(amax, dpp<0x140>(amax));
     amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
     int sg = 0;
     if (amax > 0.0f && amax <= 3.0e38f) {
         sg = 14 - __builtin_amdgcn_frexp_expf(amax);
         sg = sg < -100 ? -100 : (sg > 100 ? 100 : sg);
     }
-    const float sc = real ? __builtin_amdgcn_ldexpf(1.0f, sg) : 0.0f;
+    const float sc = head < heads ? __builtin_amdgcn_ldexpf(1.0f, sg) : 0.0f;
+    _Float16 *q = reinterpret_cast<_Float16 *>(sm.q);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float v = f[8 * i + e] * sc;
-            const _Float16 h = (_Float16)v;
-            qf[i][e] = c16 < 8 ? h : (_Float16)(v - (float)h);
-        }
-    rowf = a.scale * __builtin_amdgcn_ldexpf(1.0f, -sg);
-    rowf = a.softcap > 0.0f ? rowf / a.softcap : rowf * 1.4426950408889634f;
+    for (int i = 0; i < N; ++i) {
+        const int d = (lane & 31) * N + i, in = d % (D / 4);
+        const float v = head < heads ? r.f[i] * sc : 0.0f;
+        const _Float16 h = (_Float16)v;
+        _Float16 *to = q + ((in / 8) * 64 + d / (D / 4) * 16 + head) * 8 + in % 8;
+        to[0] = h;
+        to[64] = (_Float16)(v - (float)h);
+    }
+    if ((lane & 31) == 0) {
+        const float f = a.scale * __builtin_amdgcn_ldexpf(1.0f, -sg);
+        sm.rowf[head] = a.softcap > 0.0f ? f / a.softcap : f * 1.4426950408889634f;
+    }
 }
 
 template <int D>
-struct TokenLds {
-    static constexpr int kRow = D + 4;
-    float o[kWaves][kHeads][kRow];
-    float2 ml[kWaves][kHeads];
-};
-
-template <int D>
-__global__ __launch_bounds__(64 * kWaves) void attn_mx4_token_kernel(TokenArgs a) {
+__global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kernel(TokenArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     TokenLds<D> &sm = *reinterpret_cast<TokenLds<D> *>(lds_raw);
-    __shared__ int sums[kWaves], start[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4, shift = a.c.page_shift;
     const int rows_of = a.c.kv_heads * a.groups;  // rows of a sequence
-    // this workgroup's blocks [at, end) of all, the first of them in sequence b
-    int64_t at, end, share, base = 0;  // base: the first block of sequence b
-    int b = 0;
+    // this workgroup's blocks [at, end) of all, the first of them in sequence b;
+    // the host sees to it that a count of blocks fits 31 bits unless per_row
+    int at, end, share, base = 0, b = 0;  // base: the first block of sequence b
+    int b0 = 0, lens = 0;                 // lane i: the length of sequence b0 + i
+    auto read_lens = [&](int from) {
+        b0 = from;
+        lens = b0 + lane < a.c.batch ? doe::mx4_len(a.c, b0 + lane) : 0;
+    };
+    auto blocks = [&] { return b0 + lane < a.c.batch ? blocks_of(a, lens) : 0; };
     if (a.per_row) {
         b = (int)blockIdx.x / rows_of;
-        int lo, hi;
-        const int n = blocks_of(a, b, lo, hi);
-        share = n;
-        at = (int64_t)((int)blockIdx.x - b * rows_of) * n;
-        end = at + n;
+        read_lens(b);
+        share = blocks_of(a, __builtin_amdgcn_readfirstlane(lens));
+        at = ((int)blockIdx.x - b * rows_of) * share;
+        end = at + share;
     } else {
-        // blocks of a row in all sequences, then (again) up to the one where this share begins
-        int64_t total = 0;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 64 * kWaves) {
-            int lo, hi, n = b0 + tid < a.c.batch ? blocks_of(a, b0 + tid, lo, hi) : 0;
-            for (int w = 1; w < 64; w <<= 1) n += __shfl_xor(n, w, 64);
-            __syncthreads();
-            if (lane == 0) sums[wave] = n;
-            __syncthreads();
-            total += (int64_t)sums[0] + sums[1] + sums[2] + sums[3];
+        // each wave for itself: the sum over all sequences, then the one where the share begins
+        int sum = 0;
+        for (int from = (a.c.batch - 1) & ~63; from >= 0; from -= 64) {
+            read_lens(from);
+            sum += blocks();
         }
-        total *= rows_of;
-        share = std::max<int64_t>((total + gridDim.x - 1) / gridDim.x, a.min_share);
-        at = share * blockIdx.x;
-        end = std::min(at + share, total);
+        const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * rows_of;
+        share = std::max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), a.min_share);
+        const int64_t at64 = (int64_t)share * blockIdx.x;
         if (!a.by_row && tid == 0) a.joined[blockIdx.x] = make_int2(-1, -1);
-        if (at >= end) return;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 64 * kWaves) {
-            int lo, hi;
-            const int mine = b0 + tid < a.c.batch ? blocks_of(a, b0 + tid, lo, hi) : 0;
-            int n = mine;
-            for (int w = 1; w < 64; w <<= 1) {
-                const int u = __shfl_up(n, w, 64);
-                if (lane >= w) n += u;
-            }
-            __syncthreads();
-            if (lane == 63) sums[wave] = n;
-            if (tid == 0) start[0] = -1;
-            __syncthreads();
-            int64_t first = base;
-            for (int w = 0; w < wave; ++w) first += (int64_t)sums[w] * rows_of;
-            const int64_t upto = first + (int64_t)n * rows_of;
-            if (mine && at >= upto - (int64_t)mine * rows_of && at < upto) {
-                start[0] = b0 + tid;
-                start[1] = n - mine;  // blocks before it in its wave
-            }
-            __syncthreads();
-            if (start[0] >= 0) {
-                b = __builtin_amdgcn_readfirstlane(start[0]);
-                for (int w = 0; w < (b - b0) / 64; ++w) base += (int64_t)sums[w] * rows_of;
-                base += (int64_t)start[1] * rows_of;
+        if (at64 >= total) return;
+        at = (int)at64;
+        end = (int)std::min<int64_t>(at64 + share, total);
+        for (;;) {
+            const int mine = blocks(), upto = wave_scan(mine);
+            const uint64_t behind = __ballot(base + upto * rows_of > at);
+            if (behind) {
+                const int i = __builtin_ctzll(behind);
+                b = b0 + i;
+                base += __builtin_amdgcn_readlane(upto - mine, i) * rows_of;
                 break;
             }
-            base += ((int64_t)sums[0] + sums[1] + sums[2] + sums[3]) * rows_of;
+            base += __builtin_amdgcn_readlane(upto, 63) * rows_of;
+            read_lens(b0 + 64);
         }
     }
     while (at < end) {
-        int lo, hi;
-        const int n = blocks_of(a, b, lo, hi);
-        const int r = (int)((at - base) / n);  // row of the sequence
+        if (b >= b0 + 64) read_lens(b);
+        const int hi = __builtin_amdgcn_readlane(lens, b - b0), lo = first_seen(a, hi), n = blocks_of(a, hi);
+        const int r = (int)((uint32_t)(at - base) / (uint32_t)n);  // row of the sequence
         if (r >= rows_of) {
-            base += (int64_t)rows_of * n;
+            base += rows_of * n;
             ++b;
             continue;
         }
-        const int64_t row0 = base + (int64_t)r * n;
-        const int first = (int)(at - row0), last = (int)(std::min(row0 + n, end) - row0);  // blocks of this row
+        const int row0 = base + r * n, first = at - row0, last = std::min(row0 + n, end) - row0;  // blocks of this row
         const int kvh = r / a.groups, head0 = kvh * a.group + (r - kvh * a.groups) * a.heads;
         const int heads = std::min(a.heads, (kvh + 1) * a.group - head0);
         const int blk0 = lo / 32 + first + wave, count = (last - first - wave + kWaves - 1) / kWaves;
+        // the pages of up to 64 of this wave's blocks, a lane each; -1: none to see
+        const int32_t *table = a.c.table + (int64_t)b * a.c.table_stride;
+        auto pages = [&](int i0) __attribute__((always_inline)) {
+            const int blk = blk0 + kWaves * (i0 + lane);
+            int page = -1;
+            if (i0 + lane < count && blk * 32 < hi) page = table[blk >> (shift - 5)];
+            return page < a.c.num_pages ? page : -1;
+        };
+        int list = pages(0);
+        RawQuery<D> raw;
+        read_query<D>(raw, a, ((int64_t)b * a.num_heads + head0) * D, heads, wave, lane);
+        auto slab_of = [&](int page) __attribute__((always_inline)) {
+            return a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
+        };
+        auto place = [&](int i) __attribute__((always_inline)) { return ((blk0 + kWaves * i) * 32) & ((1 << shift) - 1); };
+        KBlock<D> kb;
+        VBlock<D> vb;
+        int page = __builtin_amdgcn_readfirstlane(list);
+        load_k<D>(kb, slab_of(page), shift, place(0), c16, g4);
+        load_v<D>(vb, slab_of(page), shift, place(0), c16, g4);
+        stage_query<D>(a, raw, sm, heads, wave, lane);  // (while the first block is under way)
+        __syncthreads();
+        h8 qf[D / 32];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) qf[i] = sm.q[i][lane];
+        const float rowf = sm.rowf[c16 & 7];
         State<D> st;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) st.o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         st.m = -INFINITY;
         st.l = 0.0f;
-        if (count > 0) {
-            h8 qf[D / 32];
-            float rowf;
-            load_query<D>(a, qf, rowf, b, head0, heads, c16, g4);
-            // the pages of up to 64 of this wave's blocks, a lane each
-            const int32_t *table = a.c.table + (int64_t)b * a.c.table_stride;
-            auto pages = [&](int i0) {
-                const int blk = blk0 + kWaves * (i0 + lane);
-                int page = -1;
-                if (i0 + lane < count && blk * 32 < hi) {
-                    page = table[blk >> (shift - 5)];
-                    if (page < 0 || page >= a.c.num_pages) page = -1;
-                }
-                return page;
-            };
-            int mine = pages(0);
-            auto page_of = [&](int i) { return __builtin_amdgcn_readlane(mine, i & 63); };
-            auto fetch = [&](Block<D> &blk, int i, int page) {
-                const uint8_t *slab = a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
-                load_block<D>(blk, slab, shift, ((blk0 + kWaves * i) * 32) & ((1 << shift) - 1), c16, g4);
-            };
-            Block<D> buf[2];
-            int page = page_of(0), next = -1;
-            fetch(buf[0], 0, page);
-            for (int i = 0; i < count; i += 2) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (i + u >= count) break;
-                    const int in = std::min(i + u + 1, count - 1);
-                    if ((in & 63) == 0 && in) mine = pages(in);
-                    next = page_of(in);
-                    fetch(buf[1 - u], in, next);
-                    if (page >= 0) attend<D>(a, st, qf, buf[u], rowf, (blk0 + kWaves * (i + u)) * 32, lo, hi, c16, g4);
-                    page = next;
-                }
-            }
+        for (int i = 0; i < count; ++i) {
+            // the next block's K follows this one's into its registers, and V likewise
+            // (the last block again at the end: not used)
+            const int in = std::min(i + 1, count - 1);
+            if ((in & 63) == 0 && in) list = pages(in);
+            const int next = __builtin_amdgcn_readlane(list, in & 63);
+            const uint8_t *slab = slab_of(next);
+            const int p0 = (blk0 + kWaves * i) * 32, top = page < 0 ? 0 : hi;
+            f32x4 s[2];
+            scores<D>(s, qf, kb, g4);
+            __builtin_amdgcn_sched_barrier(0);
+            load_k<D>(kb, slab, shift, place(in), c16, g4);
+            __builtin_amdgcn_sched_barrier(0);
+            const h8 pf = weights<D>(a, st, s, rowf, p0, lo, top, c16, g4);
+            values<D>(st, pf, vb, p0, lo, top, c16, g4);
+            __builtin_amdgcn_sched_barrier(0);
+            load_v<D>(vb, slab, shift, place(in), c16, g4);
+            __builtin_amdgcn_sched_barrier(0);
+            page = next;
         }
         // the row's four waves together
         float l = st.l + __shfl_xor(st.l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        __syncthreads();  // the last row's sums have been read
         if (lane < kHeads) sm.ml[wave][lane] = make_float2(st.m, l);
         __syncthreads();
         float M = -INFINITY;
@@ -421,12 +464,20 @@ __global__ __launch_bounds__(64 * kWaves) void attn_mx4_token_kernel(TokenArgs a
         for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm.ml[w][c16 & 7].x);
         const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - M);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-                const float v = st.o[t][i] * corr, sum = v + other_half(v);
-                if (c16 < kHeads) sm.o[wave][c16][(4 * g4 + i) * (D / 16) + t] = sum;
+            for (int i = 0; i < 4; ++i) {
+                const float v = st.o[t][i] * corr;
+                st.o[t][i] = v + other_half(v);
             }
+        if (c16 < kHeads) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float *to = &sm.o[wave][c16][(4 * g4 + i) * (D / 16)];
+#pragma unroll
+                for (int t = 0; t + 1 < D / 16; t += 2) *reinterpret_cast<float2 *>(to + t) = make_float2(st.o[t][i], st.o[t + 1][i]);
+            }
+        }
         __syncthreads();
         const bool split = first > 0 || last < n;
         const int slot = first > 0 ? 0 : 1;  // begun before this workgroup, or here
@@ -461,7 +512,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_mx4_token_kernel(TokenArgs a
         }
         // the workgroup in which a row ends says where its parts are
         if (!a.per_row && tid == 0 && last == n && (a.by_row || first > 0)) {
-            const int row = b * rows_of + r, from = first > 0 ? (int)(row0 / share) : -1;
+            const int row = b * rows_of + r, from = first > 0 ? (int)((uint32_t)row0 / (uint32_t)share) : -1;
             a.joined[a.by_row ? row : (int)blockIdx.x] = make_int2(from, a.by_row ? (int)blockIdx.x : row);
         }
         at = row0 + last;
@@ -548,7 +599,7 @@ int launch(TokenArgs &a, void *ws, hipStream_t st) {
     int64_t most = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;  // blocks of a row, as far as the host knows
     if (a.window > 0) most = std::min<int64_t>(most, a.window / 32 + 2);
     a.min_share = kWaves;
-    a.per_row = most <= 2 * kWaves;
+    a.per_row = most <= 2 * kWaves || rows * most >= ((int64_t)1 << 31);
     int64_t wgs = rows;
     if (!a.per_row) {
         wgs = std::min<int64_t>(workgroups<D>(), rows * ((most + a.min_share - 1) / a.min_share));
