@@ -2,11 +2,11 @@
 // bits (doe_attn_mx4_decode): o = softmax(cap(q . k scale)) v for one query a
 // sequence, whose length the kernel reads.
 //
-// A row is a sequence and up to eight query heads of one KV head.  Rows are
-// cut in blocks of 32 positions; all rows' blocks, one after another, are
-// divided evenly among the workgroups, whatever the lengths.  A row that falls
-// into several workgroups leaves its parts (o, m, l) in the caller's workspace
-// and a second kernel joins them.
+// A row is a sequence and up to eight query heads of one KV head, and is cut in
+// blocks of 32 positions.  Rows with more blocks than an even share of the
+// device's are split into equal pieces; a workgroup takes one piece (or row), its
+// waves every fourth block.  Pieces leave their parts (o, m, l) in the caller's
+// workspace and a second kernel joins them.
 //   * S^T = K Q^T on v_mfma_f32_16x16x32_f16: 16 positions x 16 query rows, of
 //     which 0..7 are the heads' f16 hi parts and 8..15 their lo parts (one
 //     exchange of lane halves adds them: f32 quality for no more matrix work).
@@ -22,6 +22,7 @@
 // No wave waits for another until a row's end.
 #include "mx4_cache.h"
 
+#include <limits.h>
 #include <math.h>
 #include <algorithm>
 
@@ -37,23 +38,23 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4, kHeads = 8;
-constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P above the running max, and how far that may lag
+constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P of the running max, and how far that may lag
 
 struct TokenArgs {
     Mx4View c;
     const void *q;
     void *out;
     int q_f16, out_f16, num_heads, group, heads, groups;  // query heads of a KV head, of a row, rows of a KV head
-    int window, per_row, by_row, min_share;
+    int window, per_row, by_row;
     float scale, softcap;
-    float *part;    // [workgroup][2][kHeads][D], then [workgroup][2][kHeads][2]
-    int2 *joined;   // rows to join: first and last workgroup
+    float *part;    // split items' [gridDim.x][kHeads][D], then [gridDim.x][kHeads][2]
+    int2 *joined;   // by_row: a row's first part (-1: not split) and their number; else at a row's first part the row and that number (others: -1)
 };
 
 // Workgroups of four waves that a CU holds at once, by the registers that a wave
 // takes, and those that fill the device's 256 CUs in one round.
 template <int D>
-constexpr int per_cu() { return D <= 64 ? 4 : (D <= 128 ? 3 : (D <= 256 ? 2 : 1)); }
+constexpr int per_cu() { return D <= 128 ? 4 : (D <= 160 ? 3 : (D <= 256 ? 2 : 1)); }
 template <int D>
 constexpr int workgroups() { return 256 * per_cu<D>(); }
 
@@ -119,33 +120,47 @@ __device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *p) {
     }
 }
 
-// Lane (c16, g4) of the block at position x of a page.
+// A lane's (c16, g4) place within a block's sections: fixed, so that a load is a
+// wave's address and this offset.
 template <int D>
-__device__ __forceinline__ void load_k(KBlock<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
+struct Place {
+    uint32_t k, ks, v, vs;
+    __device__ __forceinline__ Place(int c16, int g4)
+        : k(c16 * (D / 2) + g4 * (D / 8)),
+          ks(c16 * (D / 32) + (D == 64 ? g4 >> 1 : (D <= 160 ? g4 : g4 * (D / 128)))),
+          v((g4 * 16 + c16) * (D / 4)),
+          vs((g4 * (D / 32) + c16 * (D / 16) / 32) * 8) {}
+};
+
+// The block at position x of a page.
+template <int D>
+__device__ __forceinline__ void load_k(KBlock<D> &b, const uint8_t *slab, int shift, int x, const Place<D> &at) {
     using S = Mx4Slab<D>;
+    const uint8_t *k = slab + S::k_code(x), *ks = slab + S::k_scale(shift, x);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        load_words<D / 32>(b.k[t], slab + S::k_code(x + 16 * t + c16) + g4 * (D / 8));
-        const uint8_t *ks = slab + S::k_scale(shift, x + 16 * t + c16);
-        if constexpr (D == 64) b.ks[t] = ks[g4 >> 1];
-        else if constexpr (D == 128) b.ks[t] = ks[g4];
-        else if constexpr (D == 160) b.ks[t] = ks[g4] | (uint32_t)ks[g4 + 1] << 8;
-        else if constexpr (D == 256) b.ks[t] = *reinterpret_cast<const uint16_t *>(ks + 2 * g4);
-        else b.ks[t] = *reinterpret_cast<const uint32_t *>(ks + 4 * g4);
+        load_words<D / 32>(b.k[t], k + at.k + 16 * t * (D / 2));
+        const uint8_t *s = ks + at.ks + 16 * t * (D / 32);
+        if constexpr (D <= 128) b.ks[t] = s[0];
+        else if constexpr (D == 160) b.ks[t] = s[0] | (uint32_t)s[1] << 8;
+        else if constexpr (D == 256) b.ks[t] = *reinterpret_cast<const uint16_t *>(s);
+        else b.ks[t] = *reinterpret_cast<const uint32_t *>(s);
     }
 }
 template <int D>
-__device__ __forceinline__ void load_v(VBlock<D> &b, const uint8_t *slab, int shift, int x, int c16, int g4) {
+__device__ __forceinline__ void load_v(VBlock<D> &b, const uint8_t *slab, int shift, int x, const Place<D> &at) {
     using S = Mx4Slab<D>;
-    load_words<D / 16>(b.v, slab + S::v_code(shift, x, 0) + (g4 * 16 + c16) * (D / 4));
-    const int group = c16 * (D / 16) / 32;
-    const uint8_t *vs = slab + S::v_scale(shift, x, 0) + g4 * (D / 32) * 8;
-    load_words<2>(b.vs, vs + group * 8);
-    if constexpr (D == 160) load_words<2>(b.vs + 2, vs + min(group + 1, 4) * 8);
+    load_words<D / 16>(b.v, slab + S::v_code(shift, x, 0) + at.v);
+    const uint8_t *vs = slab + S::v_scale(shift, x, 0) + at.vs;
+    load_words<2>(b.vs, vs);
+    // (the second group of columns 13 .. 15 is the same one: their dims lie in it whole)
+    if constexpr (D == 160) load_words<2>(b.vs + 2, vs + (at.vs / 8 % 5 < 4 ? 8 : 0));
 }
 
+// A scale byte as the conversions take it: they look at the exponent field alone,
+// so the other bits may hold the byte's neighbours.
 __device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
-    return __uint_as_float((word >> (8 * byte) & 255u) << 23);
+    return __uint_as_float(byte == 3 ? word >> 1 : word << (23 - 8 * byte));
 }
 template <int BYTE>
 __device__ __forceinline__ h2 pair(uint32_t word, float s) {
@@ -161,7 +176,7 @@ __device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
 }
 
 // A row's running state in a wave: O^T tile T, dims (4 g4 + i) D / 16 + T of
-// query row c16.
+// query row c16; P is 2^(score - m), l its sum.
 template <int D>
 struct State {
     f32x4 o[D / 16];
@@ -171,69 +186,74 @@ struct State {
 // S^T of a block: query row c16, positions 16 t + 4 g4 + i at s[t][i], hi and lo
 // parts of the query in their own rows.
 template <int D>
-__device__ __forceinline__ void scores(f32x4 *s, const h8 *qf, const KBlock<D> &b, int g4) {
+__device__ __forceinline__ void scores(f32x4 *s, const h8 (*q)[64], const KBlock<D> &b, int lane, int g4) {
+    s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 32; ++i) {
+        const h8 qf = q[i][lane];
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
+        for (int t = 0; t < 2; ++t) {
             float f;
             if constexpr (D == 160) f = byte_scale(g4 + i >= 4 ? b.ks[t] >> 8 : b.ks[t], 0);
             else f = byte_scale(b.ks[t], D >= 128 ? i / 4 : 0);
             const uint32_t w = b.k[t][i];
             const h2 k0 = pair<0>(w, f), k1 = pair<1>(w, f), k2 = pair<2>(w, f), k3 = pair<3>(w, f);
             const h8 kf = {k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]};
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i], s[t], 0, 0, 0);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, s[t], 0, 0, 0);
         }
     }
 }
 
 // P^T of a block at positions p0 .. (those in [lo, hi) are seen), the state's
-// maximum raised and its sum carried on.
+// reference raised and its sum carried on.  `lo_part`: 1 in the lanes of P's lo
+// part, 0 in those of its hi part.
 template <int D>
-__device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f32x4 *s, float rowf, int p0, int lo, int hi,
-                                      int c16, int g4) {
-    float x[8];
-    const float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f32x4 *s, float rowf, float lo_part, int p0,
+                                      int lo, int hi, int g4) {
+    float v[8], y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float v = s[j >> 2][j & 3];
-        x[j] = (v + other_half(v)) * rowf;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3]);
     if (a.softcap > 0.0f) {
-        const float f = a.softcap * kLog2e;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = tanhf(x[j]) * f;
+        for (int j = 0; j < 8; ++j) v[j] = tanhf(v[j] * rowf);
+        rowf = a.softcap * 1.4426950408889634f;
     }
     const bool whole = p0 >= lo && p0 + 32 <= hi;
-    if (!whole) {
+    // log2 of P: the score less the reference (first -inf: any seen score gives +inf)
+    auto logs = [&](float ref) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int p = p0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
-            x[j] = p >= lo && p < hi ? x[j] : -INFINITY;
+        for (int j = 0; j < 8; ++j) y[j] = fmaf(v[j], rowf, -ref);
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int p = p0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
+                y[j] = p >= lo && p < hi ? y[j] : -INFINITY;
+            }
         }
-    }
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(top > st.m + kLazy)) {  // (m = -inf: any score)
+        return fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+    };
+    if (__any(logs(st.m) > kBias + kLazy)) {
+        float top = logs(0.0f);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = top > st.m + kLazy ? top : st.m;
-        const float corr = mn == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - mn);
-        st.m = mn;
+        const float ref = top - kBias > st.m + kLazy ? top - kBias : st.m;
+        const float corr = ref == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - ref);
+        st.m = ref;
         st.l *= corr;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) st.o[t][i] *= corr;
+        logs(ref);
     }
-    const float mref = st.m == -INFINITY ? 0.0f : st.m - kBias;
     h8 pf;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float p = __builtin_amdgcn_exp2f(x[j] - mref);
-        st.l += p;
-        const _Float16 ph = (_Float16)p;
-        pf[j] = c16 < 8 ? ph : (_Float16)(p - (float)ph);
+    for (int j = 0; j < 8; j += 2) {
+        const float p0_ = __builtin_amdgcn_exp2f(y[j]), p1_ = __builtin_amdgcn_exp2f(y[j + 1]);
+        st.l += p0_ + p1_;
+        const h2 hi_part = {(_Float16)p0_, (_Float16)p1_};
+        pf[j] = (_Float16)fmaf(-lo_part, (float)hi_part[0], p0_);
+        pf[j + 1] = (_Float16)fmaf(-lo_part, (float)hi_part[1], p1_);
     }
     return pf;
 }
@@ -348,58 +368,70 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4, shift = a.c.page_shift;
     const int rows_of = a.c.kv_heads * a.groups;  // rows of a sequence
-    // this workgroup's blocks [at, end) of all, the first of them in sequence b;
-    // the host sees to it that a count of blocks fits 31 bits unless per_row
-    int at, end, share, base = 0, b = 0;  // base: the first block of sequence b
-    int b0 = 0, lens = 0;                 // lane i: the length of sequence b0 + i
-    auto read_lens = [&](int from) {
+    // the sequences b0 .. b0 + 63, a lane each: their lengths, the items of their
+    // rows, and those of rows that are split
+    int b0 = 0, lens = 0, share = INT_MAX;
+    auto read_lens = [&](int from) __attribute__((always_inline)) {
         b0 = from;
         lens = b0 + lane < a.c.batch ? doe::mx4_len(a.c, b0 + lane) : 0;
     };
-    auto blocks = [&] { return b0 + lane < a.c.batch ? blocks_of(a, lens) : 0; };
+    auto pieces_of = [&](int n) __attribute__((always_inline)) { return (int)(((uint32_t)n + share - 1) / (uint32_t)share); };
+    int item = blockIdx.x, items0 = 0, slots0 = 0;  // items and split ones before sequence b0
     if (a.per_row) {
-        b = (int)blockIdx.x / rows_of;
-        read_lens(b);
-        share = blocks_of(a, __builtin_amdgcn_readfirstlane(lens));
-        at = ((int)blockIdx.x - b * rows_of) * share;
-        end = at + share;
+        read_lens(item / rows_of);
     } else {
-        // each wave for itself: the sum over all sequences, then the one where the share begins
+        // the share of an item, so that no more than gridDim.x are split ones: with few
+        // rows there are at most blocks / share + rows items, else those of split rows
+        // are at most twice blocks / share
         int sum = 0;
         for (int from = (a.c.batch - 1) & ~63; from >= 0; from -= 64) {
             read_lens(from);
-            sum += blocks();
+            sum += b0 + lane < a.c.batch ? blocks_of(a, lens) : 0;
         }
-        const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63) * rows_of;
-        share = std::max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), a.min_share);
-        const int64_t at64 = (int64_t)share * blockIdx.x;
-        if (!a.by_row && tid == 0) a.joined[blockIdx.x] = make_int2(-1, -1);
-        if (at64 >= total) return;
-        at = (int)at64;
-        end = (int)std::min<int64_t>(at64 + share, total);
-        for (;;) {
-            const int mine = blocks(), upto = wave_scan(mine);
-            const uint64_t behind = __ballot(base + upto * rows_of > at);
-            if (behind) {
-                const int i = __builtin_ctzll(behind);
-                b = b0 + i;
-                base += __builtin_amdgcn_readlane(upto - mine, i) * rows_of;
-                break;
+        const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_scan(sum), 63) * rows_of, rows = a.c.batch * rows_of;
+        const uint32_t room = rows <= gridDim.x / 2 ? gridDim.x - rows : gridDim.x / 2;
+        share = std::max((int)((total + room - 1) / room), kWaves);
+        share = (share + kWaves - 1) & -kWaves;
+        if (!a.by_row) {  // records of no row
+            int split = 0;
+            for (int from = 0; from < a.c.batch; from += 64) {
+                if (from) read_lens(from);
+                const int n = b0 + lane < a.c.batch ? pieces_of(blocks_of(a, lens)) : 0;
+                split += n > 1 ? n : 0;
             }
-            base += __builtin_amdgcn_readlane(upto, 63) * rows_of;
-            read_lens(b0 + 64);
+            if (a.c.batch > 64) read_lens(0);
+            split = __builtin_amdgcn_readlane(wave_scan(split), 63) * rows_of;
+            if (tid == 0 && (int)blockIdx.x >= split) a.joined[blockIdx.x] = make_int2(-1, 0);
         }
     }
-    while (at < end) {
-        if (b >= b0 + 64) read_lens(b);
-        const int hi = __builtin_amdgcn_readlane(lens, b - b0), lo = first_seen(a, hi), n = blocks_of(a, hi);
-        const int r = (int)((uint32_t)(at - base) / (uint32_t)n);  // row of the sequence
-        if (r >= rows_of) {
-            base += rows_of * n;
-            ++b;
-            continue;
+    for (;; item += gridDim.x) {
+        int b, first_item, first_slot;
+        if (a.per_row) {
+            if (item != (int)blockIdx.x) return;
+            b = b0;
+            first_item = b * rows_of;
+            first_slot = 0;
+        } else {
+            for (;;) {
+                if (b0 >= a.c.batch) return;
+                const int n = b0 + lane < a.c.batch ? pieces_of(blocks_of(a, lens)) : 0;
+                const int upto = wave_scan(n), split = wave_scan(n > 1 ? n : 0);
+                const uint64_t behind = __ballot(items0 + upto * rows_of > item);
+                if (behind) {
+                    const int i = __builtin_ctzll(behind), own = __builtin_amdgcn_readlane(n, i);
+                    b = b0 + i;
+                    first_item = items0 + (__builtin_amdgcn_readlane(upto, i) - own) * rows_of;
+                    first_slot = slots0 + (__builtin_amdgcn_readlane(split, i) - (own > 1 ? own : 0)) * rows_of;
+                    break;
+                }
+                items0 += __builtin_amdgcn_readlane(upto, 63) * rows_of;
+                slots0 += __builtin_amdgcn_readlane(split, 63) * rows_of;
+                read_lens(b0 + 64);
+            }
         }
-        const int row0 = base + r * n, first = at - row0, last = std::min(row0 + n, end) - row0;  // blocks of this row
+        const int hi = __builtin_amdgcn_readlane(lens, b - b0), lo = first_seen(a, hi), n = blocks_of(a, hi);
+        const int pieces = a.per_row ? 1 : pieces_of(n), r = (item - first_item) / pieces, piece = item - first_item - r * pieces;
+        const int per = ((uint32_t)n + pieces - 1) / (uint32_t)pieces, first = piece * per, last = std::min(n, first + per);
         const int kvh = r / a.groups, head0 = kvh * a.group + (r - kvh * a.groups) * a.heads;
         const int heads = std::min(a.heads, (kvh + 1) * a.group - head0);
         const int blk0 = lo / 32 + first + wave, count = (last - first - wave + kWaves - 1) / kWaves;
@@ -418,17 +450,15 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             return a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
         };
         auto place = [&](int i) __attribute__((always_inline)) { return ((blk0 + kWaves * i) * 32) & ((1 << shift) - 1); };
+        const Place<D> at_lane(c16, g4);
         KBlock<D> kb;
         VBlock<D> vb;
         int page = __builtin_amdgcn_readfirstlane(list);
-        load_k<D>(kb, slab_of(page), shift, place(0), c16, g4);
-        load_v<D>(vb, slab_of(page), shift, place(0), c16, g4);
+        load_k<D>(kb, slab_of(page), shift, place(0), at_lane);
+        load_v<D>(vb, slab_of(page), shift, place(0), at_lane);
         stage_query<D>(a, raw, sm, heads, wave, lane);  // (while the first block is under way)
         __syncthreads();
-        h8 qf[D / 32];
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) qf[i] = sm.q[i][lane];
-        const float rowf = sm.rowf[c16 & 7];
+        const float rowf = sm.rowf[c16 & 7], lo_part = c16 < 8 ? 0.0f : 1.0f;
         State<D> st;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) st.o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -443,14 +473,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             const uint8_t *slab = slab_of(next);
             const int p0 = (blk0 + kWaves * i) * 32, top = page < 0 ? 0 : hi;
             f32x4 s[2];
-            scores<D>(s, qf, kb, g4);
+            scores<D>(s, sm.q, kb, lane, g4);
             __builtin_amdgcn_sched_barrier(0);
-            load_k<D>(kb, slab, shift, place(in), c16, g4);
+            load_k<D>(kb, slab, shift, place(in), at_lane);
             __builtin_amdgcn_sched_barrier(0);
-            const h8 pf = weights<D>(a, st, s, rowf, p0, lo, top, c16, g4);
+            const h8 pf = weights<D>(a, st, s, rowf, lo_part, p0, lo, top, g4);
             values<D>(st, pf, vb, p0, lo, top, c16, g4);
             __builtin_amdgcn_sched_barrier(0);
-            load_v<D>(vb, slab, shift, place(in), c16, g4);
+            load_v<D>(vb, slab, shift, place(in), at_lane);
             __builtin_amdgcn_sched_barrier(0);
             page = next;
         }
@@ -479,8 +509,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             }
         }
         __syncthreads();
-        const bool split = first > 0 || last < n;
-        const int slot = first > 0 ? 0 : 1;  // begun before this workgroup, or here
+        const int slot = first_slot + r * pieces + piece;
         for (int e = tid; e < heads * (D / 4); e += 64 * kWaves) {
             const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
             float M2 = -INFINITY, lt = 0.0f;
@@ -494,10 +523,10 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
                 lt += ml.x == -INFINITY ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - M2);
                 v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
             }
-            if (split) {
-                const int64_t p = ((int64_t)blockIdx.x * 2 + slot) * kHeads + h;
+            if (pieces > 1) {
+                const int64_t p = (int64_t)slot * kHeads + h;
                 *reinterpret_cast<float4 *>(a.part + p * D + d) = v;
-                if (d == 0) reinterpret_cast<float2 *>(a.part + (int64_t)gridDim.x * 2 * kHeads * D)[p] = make_float2(M2, lt);
+                if (d == 0) reinterpret_cast<float2 *>(a.part + (int64_t)gridDim.x * kHeads * D)[p] = make_float2(M2, lt);
             } else {
                 const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
                 const int64_t to = ((int64_t)b * a.num_heads + head0 + h) * D + d;
@@ -510,17 +539,15 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
                 }
             }
         }
-        // the workgroup in which a row ends says where its parts are
-        if (!a.per_row && tid == 0 && last == n && (a.by_row || first > 0)) {
-            const int row = b * rows_of + r, from = first > 0 ? (int)((uint32_t)row0 / (uint32_t)share) : -1;
-            a.joined[a.by_row ? row : (int)blockIdx.x] = make_int2(from, a.by_row ? (int)blockIdx.x : row);
+        if (!a.per_row && tid == 0) {
+            const int row = b * rows_of + r;
+            if (!a.by_row && pieces > 1) a.joined[slot] = piece ? make_int2(-1, 0) : make_int2(row, pieces);
+            if (a.by_row && piece == 0) a.joined[row] = make_int2(pieces > 1 ? slot : -1, pieces);
         }
-        at = row0 + last;
     }
 }
 
-// A split row's head: its parts, of the workgroups first .. last, in the order
-// of a fixed tree.  D / 4 lanes hold the dims, kJoin / (D / 4) groups take every
+// A split row's head: its parts, in the order of a fixed tree.  D / 4 lanes hold the dims, kJoin / (D / 4) groups take every
 // so manieth part and meet in LDS.
 constexpr int kJoin = 512;
 template <int D>
@@ -530,18 +557,18 @@ __global__ __launch_bounds__(kJoin) void attn_mx4_join_kernel(TokenArgs a, int w
     __shared__ float2 sml[GROUPS];
     const int2 j = a.joined[blockIdx.x];
     if (j.x < 0) return;
-    const int first = j.x, last = a.by_row ? j.y : (int)blockIdx.x, row = a.by_row ? (int)blockIdx.x : j.y;
+    const int row = a.by_row ? (int)blockIdx.x : j.x, slot = a.by_row ? j.x : (int)blockIdx.x, pieces = j.y;
     const int rows_of = a.c.kv_heads * a.groups, b = row / rows_of, r = row - b * rows_of, kvh = r / a.groups;
     const int head0 = kvh * a.group + (r - kvh * a.groups) * a.heads, h = blockIdx.y;
     if (h >= std::min(a.heads, (kvh + 1) * a.group - head0)) return;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)wgs * 2 * kHeads * D);
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + (int64_t)wgs * kHeads * D);
     const int grp = threadIdx.x / L, d = (threadIdx.x - grp * L) * 4;
     float M = -INFINITY, l = 0.0f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (grp < GROUPS) {
 #pragma unroll 4
-        for (int s = first + grp; s <= last; s += GROUPS) {
-            const int64_t p = ((int64_t)s * 2 + (s == first)) * kHeads + h;
+        for (int s = grp; s < pieces; s += GROUPS) {
+            const int64_t p = (int64_t)(slot + s) * kHeads + h;
             const float2 e = ml[p];
             const float4 o = *reinterpret_cast<const float4 *>(a.part + p * D + d);
             const float mn = fmaxf(M, e.x), f0 = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
@@ -577,7 +604,7 @@ __global__ __launch_bounds__(kJoin) void attn_mx4_join_kernel(TokenArgs a, int w
 
 template <int D>
 int64_t workspace() {
-    return (int64_t)workgroups<D>() * (2 * kHeads * (D + 2) * 4 + 8);
+    return (int64_t)workgroups<D>() * (kHeads * (D + 2) * 4 + 8);
 }
 
 int64_t workspace_of(int64_t head_dim) {
@@ -598,14 +625,13 @@ int launch(TokenArgs &a, void *ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.c.batch * a.c.kv_heads * a.groups;
     int64_t most = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;  // blocks of a row, as far as the host knows
     if (a.window > 0) most = std::min<int64_t>(most, a.window / 32 + 2);
-    a.min_share = kWaves;
     a.per_row = most <= 2 * kWaves || rows * most >= ((int64_t)1 << 31);
     int64_t wgs = rows;
     if (!a.per_row) {
-        wgs = std::min<int64_t>(workgroups<D>(), rows * ((most + a.min_share - 1) / a.min_share));
+        wgs = std::min<int64_t>(workgroups<D>(), 2 * rows * ((most + kWaves - 1) / kWaves));
         a.by_row = rows <= wgs;
         a.part = static_cast<float *>(ws);
-        a.joined = reinterpret_cast<int2 *>(a.part + wgs * 2 * kHeads * (D + 2));
+        a.joined = reinterpret_cast<int2 *>(a.part + wgs * kHeads * (D + 2));
     }
     hipLaunchKernelGGL(attn_mx4_token_kernel<D>, dim3((unsigned)wgs), dim3(64 * kWaves), sizeof(TokenLds<D>), st, a);
     DOE_LAUNCH_CHECK("attn_mx4_token_kernel");
