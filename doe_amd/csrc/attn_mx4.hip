@@ -51,6 +51,8 @@ struct TokenArgs {
     int2 *joined;   // by_row: a row's first part (-1: not split) and their number; else at a row's first part the row and that number (others: -1)
 };
 
+constexpr int64_t kCacheBytes = (int64_t)256 << 20;
+
 // Workgroups of four waves that a CU holds at once, by the registers that a wave
 // takes, and those that fill the device's 256 CUs in one round.
 template <int D>
@@ -99,24 +101,30 @@ struct VBlock {
     uint32_t v[D / 16], vs[D == 160 ? 4 : 2];
 };
 
-// n dwords at p (aligned to 4 bytes, 8 or 16 where n is a multiple of 2 or 4 and so the layout).
-template <int N>
+// n dwords at p (aligned to 4 bytes, 8 or 16 where n is a multiple of 2 or 4 and so
+// the layout).  NT: past the caches.
+template <bool NT, typename T>
+__device__ __forceinline__ T load(const uint8_t *p) {
+    if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+    else return *reinterpret_cast<const T *>(p);
+}
+template <bool NT, int N>
 __device__ __forceinline__ void load_words(uint32_t *dst, const uint8_t *p) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(p + 4 * i);
+            const u32x4 v = load<NT, u32x4>(p + 4 * i);
             dst[i] = v[0], dst[i + 1] = v[1], dst[i + 2] = v[2], dst[i + 3] = v[3];
         }
     } else if constexpr (N % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const u32x2 v = *reinterpret_cast<const u32x2 *>(p + 4 * i);
+            const u32x2 v = load<NT, u32x2>(p + 4 * i);
             dst[i] = v[0], dst[i + 1] = v[1];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) dst[i] = *reinterpret_cast<const uint32_t *>(p + 4 * i);
+        for (int i = 0; i < N; ++i) dst[i] = load<NT, uint32_t>(p + 4 * i);
     }
 }
 
@@ -133,13 +141,13 @@ struct Place {
 };
 
 // The block at position x of a page.
-template <int D>
+template <int D, bool NT>
 __device__ __forceinline__ void load_k(KBlock<D> &b, const uint8_t *slab, int shift, int x, const Place<D> &at) {
     using S = Mx4Slab<D>;
     const uint8_t *k = slab + S::k_code(x), *ks = slab + S::k_scale(shift, x);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        load_words<D / 32>(b.k[t], k + at.k + 16 * t * (D / 2));
+        load_words<NT, D / 32>(b.k[t], k + at.k + 16 * t * (D / 2));
         const uint8_t *s = ks + at.ks + 16 * t * (D / 32);
         if constexpr (D <= 128) b.ks[t] = s[0];
         else if constexpr (D == 160) b.ks[t] = s[0] | (uint32_t)s[1] << 8;
@@ -147,14 +155,14 @@ __device__ __forceinline__ void load_k(KBlock<D> &b, const uint8_t *slab, int sh
         else b.ks[t] = *reinterpret_cast<const uint32_t *>(s);
     }
 }
-template <int D>
+template <int D, bool NT>
 __device__ __forceinline__ void load_v(VBlock<D> &b, const uint8_t *slab, int shift, int x, const Place<D> &at) {
     using S = Mx4Slab<D>;
-    load_words<D / 16>(b.v, slab + S::v_code(shift, x, 0) + at.v);
+    load_words<NT, D / 16>(b.v, slab + S::v_code(shift, x, 0) + at.v);
     const uint8_t *vs = slab + S::v_scale(shift, x, 0) + at.vs;
-    load_words<2>(b.vs, vs);
+    load_words<NT, 2>(b.vs, vs);
     // (the second group of columns 13 .. 15 is the same one: their dims lie in it whole)
-    if constexpr (D == 160) load_words<2>(b.vs + 2, vs + (at.vs / 8 % 5 < 4 ? 8 : 0));
+    if constexpr (D == 160) load_words<NT, 2>(b.vs + 2, vs + (at.vs / 8 % 5 < 4 ? 8 : 0));
 }
 
 // A scale byte as the conversions take it: they look at the exponent field alone,
@@ -361,76 +369,107 @@ __device__ __forceinline__ void stage_query(const TokenArgs &a, const RawQuery<D
     }
 }
 
-template <int D>
+template <int D, bool NT>
 __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kernel(TokenArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_raw[];
     TokenLds<D> &sm = *reinterpret_cast<TokenLds<D> *>(lds_raw);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4, shift = a.c.page_shift;
     const int rows_of = a.c.kv_heads * a.groups;  // rows of a sequence
-    // the sequences b0 .. b0 + 63, a lane each: their lengths, the items of their
-    // rows, and those of rows that are split
-    int b0 = 0, lens = 0, share = INT_MAX;
+    // the sequences b0 .. b0 + 63, a lane each: their lengths and the pieces of their rows
+    int b0 = 0, lens = 0, pieces_ = 0;
+    uint32_t share = 0;
     auto read_lens = [&](int from) __attribute__((always_inline)) {
         b0 = from;
         lens = b0 + lane < a.c.batch ? doe::mx4_len(a.c, b0 + lane) : 0;
     };
-    auto pieces_of = [&](int n) __attribute__((always_inline)) { return (int)(((uint32_t)n + share - 1) / (uint32_t)share); };
+    auto cut = [&] { pieces_ = b0 + lane < a.c.batch ? (int)(((uint32_t)blocks_of(a, lens) + share - 1) / share) : 0; };
+    auto sum_of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(v), 63) * rows_of; };
     int item = blockIdx.x, items0 = 0, slots0 = 0;  // items and split ones before sequence b0
+    bool dense = true;                              // as many slots as items
+    const bool one = a.c.batch == 1 && a.by_row;
     if (a.per_row) {
         read_lens(item / rows_of);
+    } else if (one) {
+        // one sequence: as many pieces a row as workgroups, of a round of the waves at least
+        read_lens(0);
+        const uint32_t n = blocks_of(a, __builtin_amdgcn_readfirstlane(lens));
+        pieces_ = std::min(gridDim.x / rows_of, (n + kWaves - 1) / kWaves);
+        share = (n + pieces_ - 1) / (uint32_t)pieces_;
+        pieces_ = (n + share - 1) / share;
     } else {
-        // the share of an item, so that no more than gridDim.x are split ones: with few
-        // rows there are at most blocks / share + rows items, else those of split rows
-        // are at most twice blocks / share
-        int sum = 0;
+        // the share of an item: the least that leaves no more items than workgroups, of
+        // an even share, a half more at most, and what does in any case (with few rows
+        // there are at most blocks / share + rows items, else those of split rows are at
+        // most twice blocks / share)
+        int sum = 0, items = INT_MAX;
         for (int from = (a.c.batch - 1) & ~63; from >= 0; from -= 64) {
             read_lens(from);
             sum += b0 + lane < a.c.batch ? blocks_of(a, lens) : 0;
         }
-        const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_scan(sum), 63) * rows_of, rows = a.c.batch * rows_of;
-        const uint32_t room = rows <= gridDim.x / 2 ? gridDim.x - rows : gridDim.x / 2;
-        share = std::max((int)((total + room - 1) / room), kWaves);
-        share = (share + kWaves - 1) & -kWaves;
-        if (!a.by_row) {  // records of no row
-            int split = 0;
-            for (int from = 0; from < a.c.batch; from += 64) {
-                if (from) read_lens(from);
-                const int n = b0 + lane < a.c.batch ? pieces_of(blocks_of(a, lens)) : 0;
-                split += n > 1 ? n : 0;
-            }
-            if (a.c.batch > 64) read_lens(0);
-            split = __builtin_amdgcn_readlane(wave_scan(split), 63) * rows_of;
-            if (tid == 0 && (int)blockIdx.x >= split) a.joined[blockIdx.x] = make_int2(-1, 0);
+        const uint32_t total = (uint32_t)sum_of(sum), rows = a.c.batch * rows_of;
+        const uint32_t even = (total + gridDim.x - 1) / gridDim.x, room = rows <= gridDim.x / 2 ? gridDim.x - rows : gridDim.x / 2;
+        auto rounded = [](uint32_t n) { return n <= 4 * kWaves ? (n + kWaves - 1) & -kWaves : n; };  // whole rounds of the waves
+        for (int more = 0; more < 5 && a.c.batch <= 64 && items > (int)gridDim.x; ++more) {
+            share = rounded(even + even * more / 8);
+            cut();
+            items = sum_of(pieces_);
         }
+        if (items > (int)gridDim.x) {
+            share = rounded((total + room - 1) / room);
+            int split = 0;
+            items = 0;
+            for (int from = (a.c.batch - 1) & ~63; from >= 0; from -= 64) {
+                read_lens(from);
+                cut();
+                items += pieces_;
+                split += pieces_ > 1 ? pieces_ : 0;
+            }
+            items = sum_of(items);
+            split = sum_of(split);
+            dense = items <= (int)gridDim.x;
+            if (!dense) items = split;
+        }
+        if (!a.by_row && tid == 0 && (int)blockIdx.x >= items) a.joined[blockIdx.x] = make_int2(-1, 0);  // of no row
     }
-    for (;; item += gridDim.x) {
-        int b, first_item, first_slot;
+    for (bool again = false;; again = true) {
+        if (again) {  // (rarely: read once more rather than held over a row)
+            item += gridDim.x;
+            read_lens(b0);
+            if (!a.per_row) cut();
+            if (one) return;
+        }
+        int b, pieces = 1, first_item, first_slot = 0;
         if (a.per_row) {
             if (item != (int)blockIdx.x) return;
             b = b0;
             first_item = b * rows_of;
-            first_slot = 0;
+        } else if (one) {
+            b = first_item = 0;
+            pieces = __builtin_amdgcn_readfirstlane(pieces_);
+            if (item >= pieces * rows_of) return;
         } else {
             for (;;) {
                 if (b0 >= a.c.batch) return;
-                const int n = b0 + lane < a.c.batch ? pieces_of(blocks_of(a, lens)) : 0;
-                const int upto = wave_scan(n), split = wave_scan(n > 1 ? n : 0);
+                const int upto = wave_scan(pieces_);
                 const uint64_t behind = __ballot(items0 + upto * rows_of > item);
+                const int split = dense ? 0 : wave_scan(pieces_ > 1 ? pieces_ : 0);
                 if (behind) {
-                    const int i = __builtin_ctzll(behind), own = __builtin_amdgcn_readlane(n, i);
+                    const int i = __builtin_ctzll(behind);
+                    pieces = __builtin_amdgcn_readlane(pieces_, i);
                     b = b0 + i;
-                    first_item = items0 + (__builtin_amdgcn_readlane(upto, i) - own) * rows_of;
-                    first_slot = slots0 + (__builtin_amdgcn_readlane(split, i) - (own > 1 ? own : 0)) * rows_of;
+                    first_item = items0 + (__builtin_amdgcn_readlane(upto, i) - pieces) * rows_of;
+                    first_slot = dense ? first_item : slots0 + (__builtin_amdgcn_readlane(split, i) - (pieces > 1 ? pieces : 0)) * rows_of;
                     break;
                 }
                 items0 += __builtin_amdgcn_readlane(upto, 63) * rows_of;
                 slots0 += __builtin_amdgcn_readlane(split, 63) * rows_of;
                 read_lens(b0 + 64);
+                cut();
             }
         }
         const int hi = __builtin_amdgcn_readlane(lens, b - b0), lo = first_seen(a, hi), n = blocks_of(a, hi);
-        const int pieces = a.per_row ? 1 : pieces_of(n), r = (item - first_item) / pieces, piece = item - first_item - r * pieces;
+        const int r = (uint32_t)(item - first_item) / (uint32_t)pieces, piece = item - first_item - r * pieces;
         const int per = ((uint32_t)n + pieces - 1) / (uint32_t)pieces, first = piece * per, last = std::min(n, first + per);
         const int kvh = r / a.groups, head0 = kvh * a.group + (r - kvh * a.groups) * a.heads;
         const int heads = std::min(a.heads, (kvh + 1) * a.group - head0);
@@ -450,12 +489,14 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             return a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
         };
         auto place = [&](int i) __attribute__((always_inline)) { return ((blk0 + kWaves * i) * 32) & ((1 << shift) - 1); };
-        const Place<D> at_lane(c16, g4);
+        int in_wave = lane;
+        __asm__ volatile("" : "+v"(in_wave));
+        const Place<D> at_lane(in_wave & 15, in_wave >> 4);
         KBlock<D> kb;
         VBlock<D> vb;
         int page = __builtin_amdgcn_readfirstlane(list);
-        load_k<D>(kb, slab_of(page), shift, place(0), at_lane);
-        load_v<D>(vb, slab_of(page), shift, place(0), at_lane);
+        load_k<D, NT>(kb, slab_of(page), shift, place(0), at_lane);
+        load_v<D, NT>(vb, slab_of(page), shift, place(0), at_lane);
         stage_query<D>(a, raw, sm, heads, wave, lane);  // (while the first block is under way)
         __syncthreads();
         const float rowf = sm.rowf[c16 & 7], lo_part = c16 < 8 ? 0.0f : 1.0f;
@@ -475,16 +516,20 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             f32x4 s[2];
             scores<D>(s, sm.q, kb, lane, g4);
             __builtin_amdgcn_sched_barrier(0);
-            load_k<D>(kb, slab, shift, place(in), at_lane);
+            load_k<D, NT>(kb, slab, shift, place(in), at_lane);
             __builtin_amdgcn_sched_barrier(0);
             const h8 pf = weights<D>(a, st, s, rowf, lo_part, p0, lo, top, g4);
             values<D>(st, pf, vb, p0, lo, top, c16, g4);
             __builtin_amdgcn_sched_barrier(0);
-            load_v<D>(vb, slab, shift, place(in), at_lane);
+            load_v<D, NT>(vb, slab, shift, place(in), at_lane);
             __builtin_amdgcn_sched_barrier(0);
             page = next;
         }
-        // the row's four waves together
+        // the row's four waves together (the lane's places formed anew: held over the
+        // blocks they would take the registers that O needs)
+        int tid = threadIdx.x;
+        __asm__ volatile("" : "+v"(tid));
+        const int lane = tid & 63, c16 = lane & 15, g4 = lane >> 4;
         float l = st.l + __shfl_xor(st.l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (lane < kHeads) sm.ml[wave][lane] = make_float2(st.m, l);
@@ -541,7 +586,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
         }
         if (!a.per_row && tid == 0) {
             const int row = b * rows_of + r;
-            if (!a.by_row && pieces > 1) a.joined[slot] = piece ? make_int2(-1, 0) : make_int2(row, pieces);
+            if (!a.by_row && (dense || pieces > 1)) a.joined[slot] = piece || pieces == 1 ? make_int2(-1, 0) : make_int2(row, pieces);
             if (a.by_row && piece == 0) a.joined[row] = make_int2(pieces > 1 ? slot : -1, pieces);
         }
     }
@@ -617,24 +662,33 @@ int64_t workspace_of(int64_t head_dim) {
     }
 }
 
-template <int D>
-int launch(TokenArgs &a, void *ws, hipStream_t st) {
-    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_token_kernel<D>,
+template <int D, bool NT>
+int launch_token(const TokenArgs &a, unsigned wgs, hipStream_t st) {
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_token_kernel<D, NT>,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(TokenLds<D>));
     DOE_HIP_CHECK(attr_rc);
+    hipLaunchKernelGGL((attn_mx4_token_kernel<D, NT>), dim3(wgs), dim3(64 * kWaves), sizeof(TokenLds<D>), st, a);
+    DOE_LAUNCH_CHECK("attn_mx4_token_kernel");
+    return DOE_OK;
+}
+
+template <int D>
+int launch(TokenArgs &a, void *ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.c.batch * a.c.kv_heads * a.groups;
     int64_t most = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;  // blocks of a row, as far as the host knows
     if (a.window > 0) most = std::min<int64_t>(most, a.window / 32 + 2);
     a.per_row = most <= 2 * kWaves || rows * most >= ((int64_t)1 << 31);
     int64_t wgs = rows;
     if (!a.per_row) {
-        wgs = std::min<int64_t>(workgroups<D>(), 2 * rows * ((most + kWaves - 1) / kWaves));
+        wgs = std::min<int64_t>(workgroups<D>(), rows * ((most + kWaves - 1) / kWaves));
         a.by_row = rows <= wgs;
         a.part = static_cast<float *>(ws);
         a.joined = reinterpret_cast<int2 *>(a.part + wgs * kHeads * (D + 2));
     }
-    hipLaunchKernelGGL(attn_mx4_token_kernel<D>, dim3((unsigned)wgs), dim3(64 * kWaves), sizeof(TokenLds<D>), st, a);
-    DOE_LAUNCH_CHECK("attn_mx4_token_kernel");
+    // A pool that the 256 MB last-level cache cannot hold is read past it.
+    const bool stream = ((int64_t)a.c.num_pages * a.c.kv_heads * (D + D / 16) << a.c.page_shift) > kCacheBytes;
+    const int rc = stream ? launch_token<D, true>(a, (unsigned)wgs, st) : launch_token<D, false>(a, (unsigned)wgs, st);
+    if (rc) return rc;
     if (a.per_row) return DOE_OK;
     hipLaunchKernelGGL(attn_mx4_join_kernel<D>, dim3((unsigned)(a.by_row ? rows : wgs), (unsigned)a.heads), dim3(kJoin), 0, st, a,
                        (int)wgs);
