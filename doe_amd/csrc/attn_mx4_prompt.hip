@@ -1,14 +1,32 @@
 // attn_mx4_prompt.hip -- causal GQA attention of prompt rows over the paged KV
 // cache held in 4 bits (doe_attn_mx4_prompt).
 //
-// o = sum_p softmax_p(cap(q . k_p scale)) v_p over the positions p that a row
-// sees: p <= pos, p < kv_len, with a window p > pos - window.
-//
-// One workgroup a row and head: 256 positions at a time, a thread one score;
-// then the running maximum and sum, and a thread one or two dims of P V.
+// o = softmax(cap(q . k_p scale)) v over the positions p that a row sees: p <=
+// pos, with a window p > pos - window; row i of a sequence's n is at position
+// kv_len - n + i.  The query heads of a KV head share its K and V: a tile is 32 or
+// 128 (row, head) pairs of one KV head, a wave 32 of them, a lane column one.
+//   * S^T = K Q^T on v_mfma_scale_f32_32x32x64_f8f6f4: K's codes and scale bytes are
+//     the matrix cores' own 4-bit format, a lane's operand one block of 32 dims as
+//     it stands in the page, with no conversion at all.  Q is cut into digits of
+//     radix 32 below the largest value of its block, each an integer of [-16, 16]
+//     and so a 6-bit float (E2M3 holds all multiples of 1/8 up to 2) under a scale
+//     of its own; all digits' products add up in one f32 accumulator.  Five digits
+//     carry 25 bits of a block's largest value, four 20; the 4- and 6-bit formats
+//     run at four times the f16 rate, so five cost 1.25 f16 products, where f16 hi
+//     + lo over converted K would cost two.
+//   * S^T's sums are P^T's operand order of O^T = V^T P^T, on
+//     v_mfma_f32_32x32x16_f16: P as f16 hi + lo, or one f16 where q and out are
+//     f16 (2^-12 of P's each, below the output's own rounding).
+//   * V goes to f16 with its scales (v_cvt_scalef32_pk_f16_fp4) once for the waves
+//     that share it, into LDS in operand order: the page layout holds the eight
+//     positions of a lane half together, so a lane writes and reads 16-byte pieces.
+//   * The running max is raised only when a score exceeds it by 2^8; P lies 2^7
+//     above it, so that f16's small values lose nothing.
 #include "mx4_cache.h"
 
 #include <math.h>
+#include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -16,139 +34,656 @@ using doe::Mx4Slab;
 using doe::Mx4View;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
-struct Args {
+constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P of the running max, and how far that may lag
+constexpr int kWaves = 4;
+
+struct PromptArgs {
     Mx4View c;
     const void *q;
     void *out;
     const int32_t *row_starts;
-    int64_t rows, q_stride, out_stride;
-    int q_f16, out_f16, num_heads, window;
+    int64_t q_stride, out_stride;
+    int q_f16, out_f16, rows, num_heads, group, window, splits, tiles;
     float scale, softcap;
+    float *part;  // [split][row][head][D], then [split][row][head][2]
 };
 
-__device__ __forceinline__ float scale_of(int s) {
-    return __uint_as_float(s == doe::kMx4NanScale ? 0x7fc00000u : (uint32_t)s << 23);
+// TEAM waves share a block's V (4: a tile of 128 pairs, 1: of 32, the waves taking
+// every fourth block); head_dim 512: each wave holds a quarter of the dims of one
+// tile of 32, and the waves add up their parts of a score.
+template <int D, int TEAM>
+struct Shape {
+    static constexpr int kSlices = D == 512 ? 4 : 1, kDims = D / kSlices;  // of a wave
+    static constexpr int kRows = D == 512 ? 32 : 32 * TEAM;                // pairs of a tile
+    static constexpr int kBlocks = TEAM;                                   // blocks of a step
+    static constexpr int kSteps = (kDims + 63) / 64, kTiles = kDims / 32;
+    static constexpr int kV = 32 * kDims * 2;                              // bytes of a block's V
+    static constexpr int kBuffers = D == 512 ? 4 : (TEAM == 4 ? 8 : 4);    // two steps of four, or a block a wave
+    static constexpr int kMerge = TEAM == 4 || D == 512 ? 0 : kWaves * 32 * D * 4;  // the waves' O at the end
+    static constexpr int kScores = D == 512 ? kWaves * 32 * 32 * 4 : 0;
+    static constexpr int kData = kBuffers * kV > kMerge ? kBuffers * kV : kMerge;
+    static constexpr int kLds = kData + kScores + 1024;
+};
+
+template <int BYTE>
+__device__ __forceinline__ h2 pair(uint32_t word, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, s, BYTE);
+}
+__device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
+    switch (byte & 3) {
+        case 0: return pair<0>(word, s);
+        case 1: return pair<1>(word, s);
+        case 2: return pair<2>(word, s);
+        default: return pair<3>(word, s);
+    }
+}
+
+// A lane's K of a block: position lane % 32, the 32 dims of half lane / 32 of
+// each step, and their scale bytes (step s in byte 2 (s % 2) of word s / 2).
+template <int D, int TEAM>
+struct KBlock {
+    u32x4 k[Shape<D, TEAM>::kSteps];
+    uint32_t s[(Shape<D, TEAM>::kSteps + 1) / 2];
+};
+template <int D, int TEAM>
+__device__ __forceinline__ void load_k(KBlock<D, TEAM> &b, const uint8_t *slab, int shift, int x, int lane, int slice) {
+    using S = Mx4Slab<D>;
+    using P = Shape<D, TEAM>;
+    const int m = lane & 31, lh = lane >> 5;
+    const uint8_t *k = slab + S::k_code(x) + slice * (P::kDims / 2) + (m * (D / 2) + lh * 16);
+    const uint8_t *s = slab + S::k_scale(shift, x) + slice * (P::kDims / 32) + m * (D / 32);
+#pragma unroll
+    for (int i = 0; i < P::kSteps; ++i) {
+        // (head_dim 160: the last step's second half is nothing; the query has zeros there)
+        const int at = P::kDims % 64 && i == P::kSteps - 1 ? i * 32 - lh * 16 : i * 32;
+        b.k[i] = *reinterpret_cast<const u32x4 *>(k + at);
+    }
+    if constexpr (D == 64) {
+        b.s[0] = *reinterpret_cast<const uint16_t *>(s) >> (8 * lh);
+    } else if constexpr (D == 160) {
+        b.s[0] = s[lh] | (uint32_t)s[2 + lh] << 16;
+        b.s[1] = s[4];
+    } else {
+#pragma unroll
+        for (int i = 0; i < P::kSteps / 2; ++i) b.s[i] = *reinterpret_cast<const uint32_t *>(s + 4 * i) >> (8 * lh);
+    }
+}
+
+// A lane's V of a block: quarter lane / 16 of the positions (eight), column
+// lane % 16, with the scales of the one or two groups that its dims lie in.
+template <int D, int TEAM>
+struct VBlock {
+    static constexpr int kBytes = Shape<D, TEAM>::kDims / 32;  // of a position
+    uint32_t v[2 * kBytes], s[D == 160 ? 4 : 2];
+};
+template <int D, int TEAM>
+__device__ __forceinline__ void load_v(VBlock<D, TEAM> &b, const uint8_t *slab, int shift, int x, int lane, int slice) {
+    using S = Mx4Slab<D>;
+    constexpr int N = VBlock<D, TEAM>::kBytes;
+    const int c = lane & 15, g = lane >> 4;
+    const uint8_t *v = slab + S::v_code(shift, x, 0) + lane * (D / 4) + slice * N;
+    if constexpr (D == 512) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b.v[j] = *reinterpret_cast<const uint32_t *>(v + j * (D / 32));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2 * N; i += 2) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(v + 4 * i);
+            b.v[i] = w[0], b.v[i + 1] = w[1];
+        }
+    }
+    const int group = c * (D / 16) / 32;
+    const uint8_t *s = slab + S::v_scale(shift, x, 0) + (g * (D / 32) + group) * 8;
+    const u32x2 w = *reinterpret_cast<const u32x2 *>(s);
+    b.s[0] = w[0], b.s[1] = w[1];
+    if constexpr (D == 160) {
+        const u32x2 u = *reinterpret_cast<const u32x2 *>(s + (group < 4 ? 8 : 0));
+        b.s[2] = u[0], b.s[3] = u[1];
+    }
+}
+
+// A scale byte as the conversions take it (they look at the exponent field alone).
+__device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
+    return __uint_as_float(byte == 3 ? word >> 1 : word << (23 - 8 * byte));
+}
+// Whether one of the word's bytes is 255.
+__device__ __forceinline__ bool any_nan_scale(uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; }
+
+// V as f16 to LDS: piece (g, t, c) holds the eight positions of quarter g of dim c
+// D / 16 + t.  Positions outside [lo, hi) and NaN blocks are zeros; returns
+// whether there was one of the latter (for this lane).
+template <int D, int TEAM>
+__device__ __forceinline__ bool stage_v(uint8_t *dst, const VBlock<D, TEAM> &b, int p0, int lo, int hi, int lane) {
+    using P = Shape<D, TEAM>;
+    constexpr int N = VBlock<D, TEAM>::kBytes;
+    const int c = lane & 15, g = lane >> 4;
+    float s[8], s2[8];
+    bool nan = false;
+#pragma unroll
+    for (int w = 0; w < (D == 160 ? 4 : 2); ++w) nan |= any_nan_scale(b.s[w]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        s[j] = byte_scale(b.s[j >> 2], j & 3);
+        if constexpr (D == 160) s2[j] = byte_scale(b.s[2 + (j >> 2)], j & 3);
+    }
+    if (p0 < lo || p0 + 32 > hi || __any(nan)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int p = p0 + 16 * (j >> 2) + 4 * g + (j & 3);
+            const bool in = p >= lo && p < hi;
+            s[j] = in && (b.s[j >> 2] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? s[j] : 0.0f;
+            if constexpr (D == 160) s2[j] = in && (b.s[2 + (j >> 2)] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? s2[j] : 0.0f;
+        }
+    }
+    h8 *to = reinterpret_cast<h8 *>(dst) + g * P::kDims + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        h2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = j * N + i;
+            float f = s[j];
+            if constexpr (D == 160) f = 5 * c % 16 + i >= 16 ? s2[j] : f;
+            v[j] = pair_at(b.v[at >> 2], f, at);
+        }
+        to[(2 * i) * 16] = h8{v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
+        to[(2 * i + 1) * 16] = h8{v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
+    }
+    return nan;
+}
+
+// A lane's queries: pair lane % 32, the 32 dims of half lane / 32 of each step, as
+// ND digits; scale bytes of digits 0..3 in one word, of a fifth in another.
+template <int D, int TEAM, int ND>
+struct Query {
+    u32x6 d[Shape<D, TEAM>::kSteps][ND];
+    uint32_t s[Shape<D, TEAM>::kSteps], s4[ND > 4 ? Shape<D, TEAM>::kSteps : 1];
+};
+template <int D, int TEAM, int ND>
+__device__ __forceinline__ void load_query(Query<D, TEAM, ND> &q, const PromptArgs &a, int64_t at, int lane, int slice) {
+    using P = Shape<D, TEAM>;
+    const int lh = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < P::kSteps; ++s) {
+        const bool none = P::kDims % 64 && s == P::kSteps - 1 && lh;
+        const int64_t from = at + slice * P::kDims + (none ? 0 : 64 * s + 32 * lh);
+        float f[32];
+        if (a.q_f16) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + from + i);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + from + i);
+                f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+            }
+        }
+        uint32_t top = 0;  // (as bits: a NaN is above all)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+        if (none) top = 0;
+        const bool real = top < 0x7f800000u;
+        int e = top == 0 || !real ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top));
+        e = e < -106 ? -106 : e;
+        f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            even[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i], 4 - e);
+            odd[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i + 1], 4 - e);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            f32x16 x, y;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = __builtin_rintf(even[i]);
+                y[i] = __builtin_rintf(odd[i]);
+                even[i] = (even[i] - x[i]) * 32.0f;
+                odd[i] = (odd[i] - y[i]) * 32.0f;
+            }
+            u32x6 packed = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x, y, 8.0f);
+            // (the sources outlive it: with a destination that begins inside one of them,
+            // which the compiler allows itself, the instruction overwrites what it has yet to read)
+            __asm__ volatile("" : "+v"(packed) : "v"(x), "v"(y));
+            q.d[s][d] = packed;
+        }
+        // digit d counts 2^(e - 1 - 5 d) times its 6-bit float; 255: not a number
+        const uint32_t b = e + 126;
+        q.s[s] = real ? b | (b - 5) << 8 | (b - 10) << 16 | (ND > 3 ? (b - 15) << 24 : 0u) : 0xffffffffu;
+        if constexpr (ND > 4) q.s4[s] = real ? b - 20 : 255u;
+    }
+}
+
+template <int D, int TEAM, int ND, int S, int DIGIT>
+__device__ __forceinline__ f32x16 score_digit(const Query<D, TEAM, ND> &q, const i32x8 &k, uint32_t ks, f32x16 acc) {
+    i32x8 b = {};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) b[i] = (int)q.d[S][DIGIT][i];
+    if constexpr (DIGIT < 4)
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, b, acc, 4, 2, 2 * (S % 2), (int)ks, DIGIT, (int)q.s[S]);
+    else
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, b, acc, 4, 2, 2 * (S % 2), (int)ks, 0, (int)q.s4[S]);
+}
+template <int D, int TEAM, int ND, int S>
+__device__ __forceinline__ void score_step(const Query<D, TEAM, ND> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
+    if constexpr (S < Shape<D, TEAM>::kSteps) {
+        i32x8 a = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = (int)k.k[S][i];
+        acc = score_digit<D, TEAM, ND, S, 0>(q, a, k.s[S / 2], acc);
+        acc = score_digit<D, TEAM, ND, S, 1>(q, a, k.s[S / 2], acc);
+        acc = score_digit<D, TEAM, ND, S, 2>(q, a, k.s[S / 2], acc);
+        if constexpr (ND > 3) acc = score_digit<D, TEAM, ND, S, 3>(q, a, k.s[S / 2], acc);
+        if constexpr (ND > 4) acc = score_digit<D, TEAM, ND, S, 4>(q, a, k.s[S / 2], acc);
+        score_step<D, TEAM, ND, S + 1>(q, k, acc);
+    }
+}
+
+// Inclusive sum over the wave's lanes, in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    return dpp_add<0x143, 0xc>(v);
+}
+
+// FULL: P as f16 hi + lo.
+template <int D, int TEAM, int ND, bool FULL>
+__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt_kernel(PromptArgs a) {
+    using P = Shape<D, TEAM>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr bool kShare = TEAM == 4;                 // the waves share V
+    constexpr bool kSliced = P::kSlices > 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int n32 = lane & 31, lh = lane >> 5, shift = a.c.page_shift, G = a.group;
+    const int slice = kSliced ? wave : 0;
+    const int kvh = blockIdx.x % a.c.kv_heads;
+    // the last tiles first: they see the most positions
+    int tile = a.tiles - 1 - blockIdx.x / a.c.kv_heads, b = 0, start = 0, count = 1, all = 1;
+    if (a.row_starts) {
+        for (int b0 = 0;; b0 += 64) {
+            if (b0 >= a.c.batch) return;
+            const int i = b0 + lane;
+            const int lo_ = i < a.c.batch ? a.row_starts[i] : 0, hi_ = i < a.c.batch ? a.row_starts[i + 1] : 0;
+            const int rows = lo_ < 0 ? 0 : std::max(0, std::min(hi_, a.rows) - lo_);
+            const int upto = wave_scan((int)(((int64_t)rows * G + P::kRows - 1) / P::kRows));
+            const uint64_t behind = __ballot(upto > tile);
+            if (behind) {
+                const int at = __builtin_ctzll(behind);
+                b = b0 + at;
+                start = __builtin_amdgcn_readlane(lo_, at);
+                count = __builtin_amdgcn_readlane(rows, at);
+                all = __builtin_amdgcn_readlane(hi_, at) - start;
+                tile -= at ? __builtin_amdgcn_readlane(upto, at - 1) : 0;
+                break;
+            }
+            tile -= __builtin_amdgcn_readlane(upto, 63);
+        }
+    } else {
+        const int each = (G + P::kRows - 1) / P::kRows;
+        b = tile / each;
+        tile -= b * each;
+        start = b;
+    }
+    const int L = doe::mx4_len(a.c, b), pairs = count * G, pair0 = tile * P::kRows;
+    // positions [seen_from, seen_to) of a pair; pairs behind the last repeat it
+    auto to_of = [&](int pr) { return std::max(0, L - all + pr / G + 1); };
+    auto from_of = [&](int pr) { return a.window > 0 ? std::max(0, to_of(pr) - a.window) : 0; };
+    const int wave0 = pair0 + (kShare ? 32 * wave : 0);          // this wave's first pair
+    const int tile1 = std::min(pair0 + P::kRows, pairs) - 1, wave1 = std::min(wave0 + 32, pairs) - 1;
+    const bool idle = wave1 < wave0;
+    const int klo = from_of(pair0), khi = to_of(tile1);          // the tile's
+    const int wlo = from_of(wave0), whi = idle ? 0 : to_of(wave1);  // the wave's
+    const int flo = idle ? 0 : from_of(wave1), fhi = to_of(std::min(wave0, pairs - 1));  // seen by all of its pairs
+    const int mine = std::min(wave0 + n32, pairs - 1);
+    const int lo = from_of(mine), hi = to_of(mine);
+    const int row = start + mine / G, head = kvh * G + mine % G;
+
+    // this split's blocks [b0, b1)
+    int b0 = klo / 32, b1 = khi > klo ? (khi + 31) / 32 : b0;
+    if (a.splits > 1) {
+        int per = (b1 - b0 + a.splits - 1) / a.splits;
+        per = (per + P::kBlocks - 1) / P::kBlocks * P::kBlocks;
+        b0 += (int)blockIdx.y * per;
+        b1 = std::min(b1, b0 + per);
+    }
+    // pages of 128 blocks from base on, two lists of a lane each; -1: nothing to see
+    const int32_t *table = a.c.table + (int64_t)b * a.c.table_stride;
+    auto pages = [&](int blk) __attribute__((always_inline)) {
+        blk += lane;
+        int page = -1;
+        if (blk < b1) page = table[blk >> (shift - 5)];
+        return page < a.c.num_pages ? page : -1;
+    };
+    int base = b0, list0 = pages(b0), list1 = pages(b0 + 64);
+    auto page_of = [&](int blk) __attribute__((always_inline)) {
+        const int i = blk - base;
+        return i < 64 ? __builtin_amdgcn_readlane(list0, i) : (i < 128 ? __builtin_amdgcn_readlane(list1, i - 64) : -1);
+    };
+    auto slab_of = [&](int page) __attribute__((always_inline)) {
+        return a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
+    };
+    auto place = [&](int blk) __attribute__((always_inline)) { return (blk * 32) & ((1 << shift) - 1); };
+
+    uint8_t *vbuf = lds;
+    float *sx = reinterpret_cast<float *>(lds + P::kData);                 // scores of the slices
+    int *flags = reinterpret_cast<int *>(lds + P::kData + P::kScores);     // [buffer]: a NaN among the block's V
+    constexpr int kStride = kShare || kSliced ? P::kBlocks : kWaves;       // blocks from a step to the next
+    const int blk0 = kShare || kSliced ? b0 : b0 + wave;
+    const int mine0 = kShare ? wave : 0;                                   // the block of a step that this wave stages
+
+    Query<D, TEAM, ND> q;
+    f32x16 o[P::kTiles];
+#pragma unroll
+    for (int t = 0; t < P::kTiles; ++t) o[t] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    const float rowf = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
+    const float yf = a.softcap > 0.0f ? a.softcap * 1.4426950408889634f : rowf;
+
+    KBlock<D, TEAM> kb;
+    VBlock<D, TEAM> vb;
+    auto stage = [&](int blk, int buffer) __attribute__((always_inline)) {
+        const int page = page_of(blk);
+        const bool nan = stage_v<D, TEAM>(vbuf + buffer * P::kV, vb, blk * 32, klo, page < 0 ? 0 : khi, lane);
+        const bool some = __any(nan);
+        if (lane == 0) flags[buffer] = some;
+    };
+    load_v<D, TEAM>(vb, slab_of(page_of(blk0 + mine0)), shift, place(blk0 + mine0), lane, slice);
+    load_k<D, TEAM>(kb, slab_of(page_of(blk0)), shift, place(blk0), lane, slice);
+    load_query<D, TEAM, ND>(q, a, (int64_t)row * a.q_stride + (int64_t)head * D, lane, slice);
+    int buffer = kShare ? 0 : wave;  // of the step's first block
+    stage(blk0 + mine0, buffer + mine0);
+    if (kShare) __syncthreads();
+
+    for (int step = blk0; step < b1; step += kStride) {
+        if (step - base >= 64) {
+            base += 64;
+            list0 = list1;
+            list1 = pages(base + 64);
+        }
+        const int next = step + kStride;
+        if (next < b1) load_v<D, TEAM>(vb, slab_of(page_of(next + mine0)), shift, place(next + mine0), lane, slice);
+#pragma unroll 1
+        for (int u = 0; u < P::kBlocks; ++u) {
+            const int blk = step + u, p0 = blk * 32, page = page_of(blk);
+            // the next block's K follows this one's into its registers
+            const int after = u + 1 < P::kBlocks ? blk + 1 : next;
+            const bool skip = blk >= b1 || page < 0 || p0 >= whi || p0 + 32 <= wlo;
+            f32x16 s = {};
+            if (!skip || kSliced) score_step<D, TEAM, ND, 0>(q, kb, s);
+            __builtin_amdgcn_sched_barrier(0);
+            load_k<D, TEAM>(kb, slab_of(page_of(after)), shift, place(after), lane, slice);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (kSliced) {
+                // [slice][r / 4][lane] float4
+                float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
+                __syncthreads();  // the last block's scores have been read
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[64 * r] = make_float4(s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]);
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) {
+                        const float4 e = reinterpret_cast<const float4 *>(sx)[w * 256 + 64 * r + lane];
+                        v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
+                    }
+                    s[4 * r] = v.x, s[4 * r + 1] = v.y, s[4 * r + 2] = v.z, s[4 * r + 3] = v.w;
+                }
+            }
+            if (skip) continue;
+            // lane: pair n32, positions p0 + 8 (r / 4) + 4 lh + r % 4
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = tanhf(s[r] * rowf);
+            }
+            float y[16];
+            const bool whole = p0 >= flo && p0 + 32 <= fhi;
+            auto logs = [&](float ref) __attribute__((always_inline)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) y[r] = fmaf(s[r], yf, -ref);
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int p = p0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                        y[r] = p >= lo && p < hi ? y[r] : -INFINITY;
+                    }
+                }
+                float top = y[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, y[r]);
+                return top;
+            };
+            if (__any(logs(m) > kBias + kLazy)) {  // (m = -inf: any score)
+                float top = logs(0.0f);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float ref = top - kBias > m + kLazy ? top - kBias : m;
+                const float corr = ref == m ? 1.0f : __builtin_amdgcn_exp2f(m - ref);
+                m = ref;
+                l *= corr;
+#pragma unroll
+                for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[t][r] *= corr;
+                logs(ref);
+            }
+            // P^T operands: step h of two takes the positions of quarter lh + 2 h
+            h8 ph[2], pl[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const int r = 4 * (h + 2 * (j >> 2)) + (j & 3);
+                    const float e0 = __builtin_amdgcn_exp2f(y[r]), e1 = __builtin_amdgcn_exp2f(y[r + 1]);
+                    l += e0 + e1;
+                    ph[h][j] = (_Float16)e0, ph[h][j + 1] = (_Float16)e1;
+                    if constexpr (FULL) {
+                        pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
+                        pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
+                    }
+                }
+            const h8 *v = reinterpret_cast<const h8 *>(vbuf + (buffer + u) * P::kV) + lh * P::kDims + n32;
+#pragma unroll
+            for (int t = 0; t < P::kTiles; ++t) {
+                const h8 v0 = v[32 * t], v1 = v[2 * P::kDims + 32 * t];
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[t], 0, 0, 0);
+                if constexpr (FULL) {
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[t], 0, 0, 0);
+                }
+            }
+            if (flags[buffer + u]) {
+                // NaN blocks were left out of V: they reach the pairs that see them
+                const uint8_t *slab = slab_of(page);
+                for (int x = 0; x < 32; ++x)
+                    for (int g = 0; g < D / 32; ++g) {
+                        if (slab[Mx4Slab<D>::v_scale(shift, place(blk) + x, g)] != doe::kMx4NanScale) continue;
+                        const float bad = p0 + x >= lo && p0 + x < hi ? NAN : 0.0f;
+#pragma unroll
+                        for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int w = 8 * (r >> 2) + 4 * lh + (r & 3);
+                                const int dim = (w & 15) * (D / 16) + slice * (P::kDims / 16) + 2 * t + (w >> 4);
+                                o[t][r] += dim / 32 == g ? bad : 0.0f;
+                            }
+                    }
+            }
+        }
+        if (next < b1) {
+            if (kShare) buffer ^= 4;
+            stage(next + mine0, buffer + mine0);
+        }
+        if (kShare) __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    const int64_t parts = (int64_t)a.splits * a.rows * a.num_heads;
+    // dims d .. d + N - 1 of the pair (row, head), or its part of a split
+    auto put = [&](int row, int head, int d, const float *v, auto n, float M, float sum, bool first) __attribute__((always_inline)) {
+        constexpr int N = decltype(n)::value;
+        if (a.splits > 1) {
+            const int64_t at = ((int64_t)blockIdx.y * a.rows + row) * a.num_heads + head;
+            float *to = a.part + at * D + d;
+#pragma unroll
+            for (int i = 0; i < N; ++i) to[i] = v[i];
+            if (first) reinterpret_cast<float2 *>(a.part + parts * D)[at] = make_float2(M, sum);
+            return;
+        }
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        const int64_t at = (int64_t)row * a.out_stride + (int64_t)head * D + d;
+        if (a.out_f16) {
+            _Float16 *to = static_cast<_Float16 *>(a.out) + at;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) *reinterpret_cast<h2 *>(to + i) = h2{(_Float16)(v[i] * inv), (_Float16)(v[i + 1] * inv)};
+        } else {
+            float *to = static_cast<float *>(a.out) + at;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) *reinterpret_cast<float2 *>(to + i) = make_float2(v[i] * inv, v[i + 1] * inv);
+        }
+    };
+    if constexpr (kShare || kSliced) {
+        if (idle || wave0 + n32 >= pairs) return;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int c = 8 * (r >> 2) + 4 * lh + (r & 3);
+            float v[2 * P::kTiles];
+#pragma unroll
+            for (int t = 0; t < P::kTiles; ++t) v[2 * t] = o[t][r], v[2 * t + 1] = o[t][r + 8];
+            put(row, head, c * (D / 16) + slice * (P::kDims / 16), v, std::integral_constant<int, 2 * P::kTiles>(), m, l,
+                r == 0 && lh == 0 && slice == 0);
+        }
+    } else {
+        // the waves' parts of the tile together: each wave's O as [4 t + position / 4][pair] float4
+        __syncthreads();
+        float4 *om = reinterpret_cast<float4 *>(lds) + wave * (32 * D / 4);
+        float2 *ml = reinterpret_cast<float2 *>(lds + P::kData);  // [wave][pair]
+        if (lh == 0) ml[wave * 32 + n32] = make_float2(m, l);
+#pragma unroll
+        for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                om[(t * 8 + 2 * r + lh) * 32 + n32] = make_float4(o[t][4 * r], o[t][4 * r + 1], o[t][4 * r + 2], o[t][4 * r + 3]);
+        __syncthreads();
+        // a thread two columns (D / 16 dims) of a pair: position c + 16 h of tile t is dim c D / 16 + 2 t + h
+        for (int id = threadIdx.x; id < 512; id += 64 * kWaves) {
+            const int pr = (id >> 2) & 31, c = (id >> 7) * 4 + (id & 3);
+            if (pair0 + pr >= pairs) continue;
+            float M = -INFINITY, lt = 0.0f, v[D / 16], f[kWaves];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w * 32 + pr].x);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 e = ml[w * 32 + pr];
+                f[w] = e.x == -INFINITY ? (e.y != e.y ? e.y : 0.0f) : __builtin_amdgcn_exp2f(e.x - M);  // (a NaN stays one)
+                lt += e.y * f[w];
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                v[i] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w)
+                    v[i] += f[w] * reinterpret_cast<const float *>(lds)[((w * (D / 4) + (i >> 1) * 8 + (i & 1) * 4 + (c >> 2)) * 32 + pr) * 4 + (c & 3)];
+            }
+            const int pr_ = pair0 + pr;
+            put(start + pr_ / G, kvh * G + pr_ % G, c * (D / 16), v, std::integral_constant<int, D / 16>(), M, lt, c == 0);
+        }
+    }
+}
+
+// The splits of a (row, head) joined; pairs of rows of no sequence have none and are left alone.
+template <int D>
+__global__ __launch_bounds__(256) void attn_mx4_prompt_join_kernel(PromptArgs a) {
+    const int64_t pairs = (int64_t)a.rows * a.num_heads;
+    const int64_t at = (int64_t)blockIdx.x * (1024 / D) + threadIdx.x / (D / 4);
+    const int d = (int)(threadIdx.x % (D / 4)) * 4;
+    if (threadIdx.x / (D / 4) >= 1024 / D || at >= pairs) return;
+    const int64_t row = at / a.num_heads;
+    if (a.row_starts && (row < a.row_starts[0] || row >= a.row_starts[a.c.batch])) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part + a.splits * pairs * D);
+    float M = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int z = 0; z < a.splits; ++z) M = fmaxf(M, ml[z * pairs + at].x);
+    for (int z = 0; z < a.splits; ++z) {
+        const float2 e = ml[z * pairs + at];
+        const float f = e.x == -INFINITY ? (e.y != e.y ? e.y : 0.0f) : __builtin_amdgcn_exp2f(e.x - M);
+        const float4 o = *reinterpret_cast<const float4 *>(a.part + (z * pairs + at) * D + d);
+        l += e.y * f;
+        v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int64_t to = row * a.out_stride + (at - row * a.num_heads) * D + d;
+    if (a.out_f16) {
+        _Float16 *o = static_cast<_Float16 *>(a.out) + to;
+        o[0] = (_Float16)(v.x * inv), o[1] = (_Float16)(v.y * inv), o[2] = (_Float16)(v.z * inv), o[3] = (_Float16)(v.w * inv);
+    } else {
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    }
+}
+
+constexpr int kCus = 256, kMaxSplits = 16;
+
+// Tiles of `rows` pairs that a call may have, by what the host knows.
+int64_t tiles_of(bool starts, int64_t batch, int64_t rows, int64_t group, int tile_rows) {
+    return starts ? rows * group / tile_rows + std::min(batch, rows) : batch * ((group + tile_rows - 1) / tile_rows);
+}
+// Whether tiles of 128 pairs, whose waves share V, are many enough to fill the device.
+bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    return head_dim < 512 && tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= 2 * kCus;
+}
+int64_t splits_of(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    const int tile = shared(head_dim, starts, batch, rows, num_heads, kv_heads) ? 128 : 32;
+    const int64_t wgs = std::max<int64_t>(1, tiles_of(starts, batch, rows, num_heads / kv_heads, tile) * kv_heads);
+    return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kCus / wgs));
+}
+int64_t workspace_of(int64_t head_dim, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    int64_t splits = splits_of(head_dim, true, batch, rows, num_heads, kv_heads);
+    if (rows == batch) splits = std::max(splits, splits_of(head_dim, false, batch, rows, num_heads, kv_heads));
+    return splits == 1 ? 16 : splits * rows * num_heads * (head_dim + 2) * 4;
+}
+
+template <int D, int TEAM, int ND, bool FULL>
+int launch(const PromptArgs &a, hipStream_t st) {
+    constexpr int lds = Shape<D, TEAM>::kLds;
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_prompt_kernel<D, TEAM, ND, FULL>,
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    DOE_HIP_CHECK(attr_rc);
+    const dim3 grid((unsigned)(a.tiles * a.c.kv_heads), (unsigned)a.splits);
+    hipLaunchKernelGGL((attn_mx4_prompt_kernel<D, TEAM, ND, FULL>), grid, dim3(64 * kWaves), lds, st, a);
+    DOE_LAUNCH_CHECK("attn_mx4_prompt_kernel");
+    if (a.splits == 1) return DOE_OK;
+    const int64_t pairs = (int64_t)a.rows * a.num_heads, each = 1024 / D;
+    hipLaunchKernelGGL(attn_mx4_prompt_join_kernel<D>, dim3((unsigned)((pairs + each - 1) / each)), dim3(256), 0, st, a);
+    DOE_LAUNCH_CHECK("attn_mx4_prompt_join_kernel");
+    return DOE_OK;
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void attn_mx4_rows_kernel(Args a) {
-    using S = Mx4Slab<D>;
-    __shared__ float qs[D], p_[256], red[4];
-    __shared__ int page_[256];
-    const int tid = threadIdx.x, head = blockIdx.x % a.num_heads;
-    const int64_t row = blockIdx.x / a.num_heads;
-    int b, pos;
-    const bool seen = doe::mx4_row(a.c, a.row_starts, row, b, pos);
-    if (a.row_starts && (row < a.row_starts[0] || row >= a.row_starts[a.c.batch])) return;
-    const int kvh = head / (a.num_heads / a.c.kv_heads), shift = a.c.page_shift;
-    int hi = 0, lo = 0;
-    if (seen) {
-        hi = min(pos + 1, doe::mx4_len(a.c, b));
-        if (a.window > 0) lo = max(0, pos - a.window + 1);
+int launch_d(PromptArgs &a, bool share, hipStream_t st) {
+    const bool full = !(a.q_f16 && a.out_f16);
+    if constexpr (D < 512) {
+        if (share) return full ? launch<D, 4, 5, true>(a, st) : launch<D, 4, 4, false>(a, st);
     }
-    for (int d = tid; d < D; d += 256) {
-        const int64_t at = row * a.q_stride + (int64_t)head * D + d;
-        qs[d] = a.q_f16 ? (float)static_cast<const _Float16 *>(a.q)[at] : static_cast<const float *>(a.q)[at];
-    }
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[(D + 255) / 256] = {};
-    for (int p0 = lo; p0 < hi; p0 += 256) {
-        const int p = p0 + tid, page = p < hi ? doe::mx4_page(a.c, b, p) : -1, x = p & ((1 << shift) - 1);
-        float s = -INFINITY;
-        if (page >= 0) {
-            const uint8_t *slab = a.c.pool + ((int64_t)page * a.c.kv_heads + kvh) * S::bytes(shift);
-            s = 0.0f;
-            for (int g = 0; g < D / 32; ++g) {
-                const float f = scale_of(slab[S::k_scale(shift, x) + g]);
-                for (int d = 32 * g; d < 32 * g + 32; d += 2) {
-                    const h2 k = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(slab[S::k_code(x) + d / 2], f, 0);
-                    s = fmaf(qs[d], (float)k[0], s);
-                    s = fmaf(qs[d + 1], (float)k[1], s);
-                }
-            }
-            s *= a.scale;
-            if (a.softcap > 0.0f) s = tanhf(s / a.softcap) * a.softcap;
-        }
-        page_[tid] = page;
-        float top = s;
-        for (int w = 1; w < 64; w <<= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = top;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float mref = mn == -INFINITY ? 0.0f : mn, corr = expf(m - mref);
-        p_[tid] = expf(s - mref);
-        m = mn;
-        __syncthreads();
-        l *= corr;
-        for (int i = 0; i < (D + 255) / 256; ++i) o[i] *= corr;
-        for (int j = 0; j < 256; ++j) {
-            if (page_[j] < 0) continue;
-            const float pj = p_[j];
-            l += pj;
-            const int xj = (p0 + j) & ((1 << shift) - 1);
-            const uint8_t *slab = a.c.pool + ((int64_t)page_[j] * a.c.kv_heads + kvh) * S::bytes(shift);
-            for (int i = 0; i < (D + 255) / 256; ++i) {
-                const int d = tid + 256 * i;
-                if (d >= D) continue;
-                const float f = scale_of(slab[S::v_scale(shift, xj, d / 32)]);
-                const h2 v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(slab[S::v_code(shift, xj, d / (D / 16)) + d % (D / 16) / 2], f, 0);
-                o[i] = fmaf(pj, (float)v[d & 1], o[i]);
-            }
-        }
-        __syncthreads();
-    }
-    for (int i = 0; i < (D + 255) / 256; ++i) {
-        const int d = tid + 256 * i;
-        if (d >= D) continue;
-        const int64_t at = row * a.out_stride + (int64_t)head * D + d;
-        const float v = l != 0.0f ? o[i] / l : 0.0f;
-        if (a.out_f16) static_cast<_Float16 *>(a.out)[at] = (_Float16)v;
-        else static_cast<float *>(a.out)[at] = v;
-    }
-}
-
-int attention(Args &a, const doe_mx4_cache *cache, int64_t num_heads, int64_t sliding_window, void *workspace,
-              int64_t workspace_bytes, int64_t need, hipStream_t st) {
-    const int64_t d = cache->head_dim;
-    int rc = doe::mx4_attention_checks(a.c, num_heads, a.scale, a.softcap, sliding_window, a.q, a.out);
-    if (rc) return rc;
-    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
-                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
-    DOE_REQUIRE(a.rows >= 0 && a.rows * num_heads < ((int64_t)1 << 31), DOE_E_INVALID, "%lld rows of %lld heads",
-                (long long)a.rows, (long long)num_heads);
-    DOE_REQUIRE(a.row_starts || a.rows == a.c.batch, DOE_E_INVALID,
-                "without row_starts a call takes one row a sequence (%lld rows, batch %d)", (long long)a.rows, a.c.batch);
-    DOE_REQUIRE(a.q_stride >= num_heads * d && a.out_stride >= num_heads * d && a.q_stride * (a.q_f16 ? 2 : 4) % 16 == 0 &&
-                    a.out_stride * (a.out_f16 ? 2 : 4) % 16 == 0,
-                DOE_E_INVALID, "row strides below a row, or not multiples of 16 bytes");
-    if ((rc = doe::require_init())) return rc;
-    if (a.rows == 0 || a.c.batch == 0) return DOE_OK;
-    a.num_heads = (int)num_heads;
-    a.window = (int)sliding_window;
-    const dim3 grid((unsigned)(a.rows * num_heads));
-    switch (d) {
-        case 64: hipLaunchKernelGGL(attn_mx4_rows_kernel<64>, grid, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL(attn_mx4_rows_kernel<128>, grid, dim3(256), 0, st, a); break;
-        case 160: hipLaunchKernelGGL(attn_mx4_rows_kernel<160>, grid, dim3(256), 0, st, a); break;
-        case 256: hipLaunchKernelGGL(attn_mx4_rows_kernel<256>, grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(attn_mx4_rows_kernel<512>, grid, dim3(256), 0, st, a); break;
-    }
-    DOE_LAUNCH_CHECK("attn_mx4_rows_kernel");
-    return DOE_OK;
-}
-
-int workspace_size(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t *bytes) {
-    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
-    int64_t page = 0;
-    const int rc = doe_mx4_page_bytes(32, num_kv_heads, head_dim, &page);
-    if (rc) return rc;
-    DOE_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && num_heads > 0 && num_heads <= 65535 &&
-                    num_heads % num_kv_heads == 0 && rows * num_heads < ((int64_t)1 << 31),
-                DOE_E_INVALID, "batch %lld, %lld rows, %lld heads over %lld", (long long)batch, (long long)rows,
-                (long long)num_heads, (long long)num_kv_heads);
-    *bytes = 16;
-    return DOE_OK;
+    return full ? launch<D, 1, 5, true>(a, st) : launch<D, 1, 4, false>(a, st);
 }
 
 }  // namespace
@@ -157,27 +692,69 @@ extern "C" {
 
 int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
                                   int64_t head_dim, int64_t *bytes) {
-    return workspace_size(batch, rows, num_heads, num_kv_heads, head_dim, bytes);
+    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
+    int64_t page = 0;
+    const int rc = doe_mx4_page_bytes(32, num_kv_heads, head_dim, &page);
+    if (rc) return rc;
+    DOE_REQUIRE(batch >= 0 && batch <= 65535 && rows >= 0 && num_heads > 0 && num_heads <= 65535 &&
+                    num_heads % num_kv_heads == 0 && rows < ((int64_t)1 << 31) && rows * num_heads < ((int64_t)1 << 31),
+                DOE_E_INVALID, "batch %lld, %lld rows, %lld heads over %lld", (long long)batch, (long long)rows,
+                (long long)num_heads, (long long)num_kv_heads);
+    *bytes = workspace_of(head_dim, batch, rows, num_heads, num_kv_heads);
+    return DOE_OK;
 }
 
 int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,
                         int out_f16, int64_t out_row_stride, const int32_t *row_starts, int64_t rows, int64_t num_heads,
                         float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
                         doe_stream_t stream) {
-    Args a{};
-    const int rc = doe::mx4_view(cache, &a.c);
+    PromptArgs a{};
+    int rc = doe::mx4_view(cache, &a.c);
     if (rc) return rc;
+    if ((rc = doe::mx4_attention_checks(a.c, num_heads, scale, softcap, sliding_window, q, out))) return rc;
+    const int64_t d = cache->head_dim;
+    DOE_REQUIRE(rows >= 0 && rows < ((int64_t)1 << 31) && rows * num_heads < ((int64_t)1 << 31), DOE_E_INVALID,
+                "%lld rows of %lld heads", (long long)rows, (long long)num_heads);
+    DOE_REQUIRE(row_starts || rows == a.c.batch, DOE_E_INVALID,
+                "without row_starts a call takes one row a sequence (%lld rows, batch %d)", (long long)rows, a.c.batch);
+    DOE_REQUIRE(q_row_stride >= num_heads * d && out_row_stride >= num_heads * d && q_row_stride * (q_f16 ? 2 : 4) % 16 == 0 &&
+                    out_row_stride * (out_f16 ? 2 : 4) % 16 == 0,
+                DOE_E_INVALID, "row strides below a row, or not multiples of 16 bytes");
+    const int64_t need = workspace_of(d, a.c.batch, rows, num_heads, a.c.kv_heads);
+    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
+                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
+    const bool starts = row_starts != nullptr, share = shared(d, starts, a.c.batch, rows, num_heads, a.c.kv_heads);
+    const int64_t tiles = tiles_of(starts, a.c.batch, rows, num_heads / a.c.kv_heads, share ? 128 : 32);
+    DOE_REQUIRE(tiles * a.c.kv_heads < ((int64_t)1 << 31), DOE_E_UNSUPPORTED, "too many rows");
+    if ((rc = doe::require_init())) return rc;
+    if (rows == 0 || a.c.batch == 0) return DOE_OK;
     a.q = q;
     a.out = out;
     a.row_starts = row_starts;
-    a.rows = rows;
+    a.rows = (int)rows;
     a.q_stride = q_row_stride;
     a.out_stride = out_row_stride;
-    a.q_f16 = q_f16;
-    a.out_f16 = out_f16;
+    a.q_f16 = q_f16 != 0;
+    a.out_f16 = out_f16 != 0;
+    a.num_heads = (int)num_heads;
+    a.group = (int)(num_heads / a.c.kv_heads);
+    a.window = (int)sliding_window;
     a.scale = scale;
     a.softcap = softcap;
-    return attention(a, cache, num_heads, sliding_window, workspace, workspace_bytes, 16, (hipStream_t)stream);
+    a.tiles = (int)tiles;
+    // no more splits than there are steps of eight blocks to share out
+    int64_t blocks = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;
+    if (a.window > 0) blocks = std::min<int64_t>(blocks, (a.window + rows) / 32 + 2);
+    a.splits = (int)std::max<int64_t>(1, std::min(splits_of(d, starts, a.c.batch, rows, num_heads, a.c.kv_heads), blocks / 8));
+    a.part = static_cast<float *>(workspace);
+    const hipStream_t st = (hipStream_t)stream;
+    switch (d) {
+        case 64: return launch_d<64>(a, share, st);
+        case 128: return launch_d<128>(a, share, st);
+        case 160: return launch_d<160>(a, share, st);
+        case 256: return launch_d<256>(a, share, st);
+        default: return launch_d<512>(a, share, st);
+    }
 }
 
 }  // extern "C"
