@@ -65,7 +65,7 @@ struct Shape {
     static constexpr int kBlocks = TEAM;                                   // blocks of a step
     static constexpr int kSteps = (kDims + 63) / 64, kTiles = kDims / 32;
     static constexpr int kV = 32 * kDims * 2;                              // bytes of a block's V
-    static constexpr int kBuffers = D == 512 ? 4 : (TEAM == 4 ? 8 : 4);    // two steps of four, or a block a wave
+    static constexpr int kBuffers = 8;                                     // two steps of four, or two blocks a wave
     static constexpr int kMerge = TEAM == 4 || D == 512 ? 0 : kWaves * 32 * D * 4;  // the waves' O at the end
     static constexpr int kScores = D == 512 ? kWaves * 32 * 32 * 4 : 0;
     static constexpr int kData = kBuffers * kV > kMerge ? kBuffers * kV : kMerge;
@@ -157,46 +157,50 @@ __device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
 __device__ __forceinline__ bool any_nan_scale(uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; }
 
 // V as f16 to LDS: piece (g, t, c) holds the eight positions of quarter g of dim c
-// D / 16 + t.  Positions outside [lo, hi) and NaN blocks are zeros; returns
-// whether there was one of the latter (for this lane).
+// D / 16 + t.  Positions outside [lo, hi) and NaN blocks are zeros.
 template <int D, int TEAM>
-__device__ __forceinline__ bool stage_v(uint8_t *dst, const VBlock<D, TEAM> &b, int p0, int lo, int hi, int lane) {
-    using P = Shape<D, TEAM>;
-    constexpr int N = VBlock<D, TEAM>::kBytes;
-    const int c = lane & 15, g = lane >> 4;
-    float s[8], s2[8];
-    bool nan = false;
+struct VScale {
+    float s[8], s2[D == 160 ? 8 : 1];
+    bool nan;  // one of the latter (in this lane)
+};
+template <int D, int TEAM>
+__device__ __forceinline__ void v_scales(VScale<D, TEAM> &f, const VBlock<D, TEAM> &b, int p0, int lo, int hi, int lane) {
+    const int g = lane >> 4;
+    f.nan = false;
 #pragma unroll
-    for (int w = 0; w < (D == 160 ? 4 : 2); ++w) nan |= any_nan_scale(b.s[w]);
+    for (int w = 0; w < (D == 160 ? 4 : 2); ++w) f.nan |= any_nan_scale(b.s[w]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        s[j] = byte_scale(b.s[j >> 2], j & 3);
-        if constexpr (D == 160) s2[j] = byte_scale(b.s[2 + (j >> 2)], j & 3);
+        f.s[j] = byte_scale(b.s[j >> 2], j & 3);
+        if constexpr (D == 160) f.s2[j] = byte_scale(b.s[2 + (j >> 2)], j & 3);
     }
-    if (p0 < lo || p0 + 32 > hi || __any(nan)) {
+    if (p0 < lo || p0 + 32 > hi || __any(f.nan)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int p = p0 + 16 * (j >> 2) + 4 * g + (j & 3);
             const bool in = p >= lo && p < hi;
-            s[j] = in && (b.s[j >> 2] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? s[j] : 0.0f;
-            if constexpr (D == 160) s2[j] = in && (b.s[2 + (j >> 2)] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? s2[j] : 0.0f;
+            f.s[j] = in && (b.s[j >> 2] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? f.s[j] : 0.0f;
+            if constexpr (D == 160)
+                f.s2[j] = in && (b.s[2 + (j >> 2)] >> 8 * (j & 3) & 255) != doe::kMx4NanScale ? f.s2[j] : 0.0f;
         }
     }
-    h8 *to = reinterpret_cast<h8 *>(dst) + g * P::kDims + c;
+}
+// Dims 2 i and 2 i + 1 of a lane's.
+template <int D, int TEAM>
+__device__ __forceinline__ void stage_v(uint8_t *dst, const VBlock<D, TEAM> &b, const VScale<D, TEAM> &f, int i, int lane) {
+    constexpr int N = VBlock<D, TEAM>::kBytes;
+    const int c = lane & 15, g = lane >> 4;
+    h8 *to = reinterpret_cast<h8 *>(dst) + g * Shape<D, TEAM>::kDims + c;
+    h2 v[8];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        h2 v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int at = j * N + i;
-            float f = s[j];
-            if constexpr (D == 160) f = 5 * c % 16 + i >= 16 ? s2[j] : f;
-            v[j] = pair_at(b.v[at >> 2], f, at);
-        }
-        to[(2 * i) * 16] = h8{v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
-        to[(2 * i + 1) * 16] = h8{v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
+    for (int j = 0; j < 8; ++j) {
+        const int at = j * N + i;
+        float s = f.s[j];
+        if constexpr (D == 160) s = 5 * c % 16 + i >= 16 ? f.s2[j] : s;
+        v[j] = pair_at(b.v[at >> 2], s, at);
     }
-    return nan;
+    to[(2 * i) * 16] = h8{v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
+    to[(2 * i + 1) * 16] = h8{v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
 }
 
 // A lane's queries: pair lane % 32, the 32 dims of half lane / 32 of each step, as
@@ -265,28 +269,33 @@ __device__ __forceinline__ void load_query(Query<D, TEAM, ND> &q, const PromptAr
     }
 }
 
-template <int D, int TEAM, int ND, int S, int DIGIT>
-__device__ __forceinline__ f32x16 score_digit(const Query<D, TEAM, ND> &q, const i32x8 &k, uint32_t ks, f32x16 acc) {
-    i32x8 b = {};
-#pragma unroll
-    for (int i = 0; i < 6; ++i) b[i] = (int)q.d[S][DIGIT][i];
-    if constexpr (DIGIT < 4)
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, b, acc, 4, 2, 2 * (S % 2), (int)ks, DIGIT, (int)q.s[S]);
-    else
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, b, acc, 4, 2, 2 * (S % 2), (int)ks, 0, (int)q.s4[S]);
-}
-template <int D, int TEAM, int ND, int S>
-__device__ __forceinline__ void score_step(const Query<D, TEAM, ND> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
-    if constexpr (S < Shape<D, TEAM>::kSteps) {
-        i32x8 a = {};
+// The products [FROM, TO) of a block's scores, step and digit in order.
+template <int D, int TEAM, int ND, int FROM, int TO>
+__device__ __forceinline__ void scores(const Query<D, TEAM, ND> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
+    if constexpr (FROM < TO) {
+        constexpr int S = FROM / ND, DIGIT = FROM % ND;
+        i32x8 a = {}, b = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = (int)k.k[S][i];
-        acc = score_digit<D, TEAM, ND, S, 0>(q, a, k.s[S / 2], acc);
-        acc = score_digit<D, TEAM, ND, S, 1>(q, a, k.s[S / 2], acc);
-        acc = score_digit<D, TEAM, ND, S, 2>(q, a, k.s[S / 2], acc);
-        if constexpr (ND > 3) acc = score_digit<D, TEAM, ND, S, 3>(q, a, k.s[S / 2], acc);
-        if constexpr (ND > 4) acc = score_digit<D, TEAM, ND, S, 4>(q, a, k.s[S / 2], acc);
-        score_step<D, TEAM, ND, S + 1>(q, k, acc);
+#pragma unroll
+        for (int i = 0; i < 6; ++i) b[i] = (int)q.d[S][DIGIT][i];
+        const int ks = (int)k.s[S / 2];
+        if constexpr (DIGIT < 4)
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 2, 2 * (S % 2), ks, DIGIT, (int)q.s[S]);
+        else
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 2, 2 * (S % 2), ks, 0, (int)q.s4[S]);
+        scores<D, TEAM, ND, FROM + 1, TO>(q, k, acc);
+    }
+}
+
+// The instruction scheduler's order for what stands before it in a block of code:
+// one matrix instruction, then so many vector ones, N times.
+template <int N, int VALU>
+__device__ __forceinline__ void interleave() {
+    if constexpr (N > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        interleave<N - 1, VALU>();
     }
 }
 
@@ -364,33 +373,34 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         b0 += (int)blockIdx.y * per;
         b1 = std::min(b1, b0 + per);
     }
-    // pages of 128 blocks from base on, two lists of a lane each; -1: nothing to see
+    // this wave's blocks: first, first + stride, .. (all of the tile's, or every fourth);
+    // slabs of 64 of them at a time, a lane each: -1 where there is nothing to see
+    constexpr int kStride = kShare || kSliced ? 1 : kWaves;
+    const int first = kShare || kSliced ? b0 : b0 + wave, blocks = std::max(0, (b1 - first + kStride - 1) / kStride);
     const int32_t *table = a.c.table + (int64_t)b * a.c.table_stride;
-    auto pages = [&](int blk) __attribute__((always_inline)) {
-        blk += lane;
+    auto slabs = [&](int i0) __attribute__((always_inline)) {
+        const int blk = first + (i0 + lane) * kStride;
         int page = -1;
         if (blk < b1) page = table[blk >> (shift - 5)];
-        return page < a.c.num_pages ? page : -1;
+        return page >= 0 && page < a.c.num_pages ? page * a.c.kv_heads + kvh : -1;
     };
-    int base = b0, list0 = pages(b0), list1 = pages(b0 + 64);
-    auto page_of = [&](int blk) __attribute__((always_inline)) {
-        const int i = blk - base;
-        return i < 64 ? __builtin_amdgcn_readlane(list0, i) : (i < 128 ? __builtin_amdgcn_readlane(list1, i - 64) : -1);
+    int list0 = slabs(0), list1 = slabs(64), base = 0;  // blocks base .. base + 127
+    auto slab_index = [&](int i) __attribute__((always_inline)) {
+        const int k = i - base;
+        return __builtin_amdgcn_readlane(k < 64 ? list0 : list1, k & 63);
     };
-    auto slab_of = [&](int page) __attribute__((always_inline)) {
-        return a.c.pool + ((int64_t)std::max(page, 0) * a.c.kv_heads + kvh) * Mx4Slab<D>::bytes(shift);
+    auto slab_at = [&](int index) __attribute__((always_inline)) {
+        return a.c.pool + (uint64_t)(uint32_t)std::max(index, 0) * (uint32_t)Mx4Slab<D>::bytes(shift);
     };
-    auto place = [&](int blk) __attribute__((always_inline)) { return (blk * 32) & ((1 << shift) - 1); };
+    auto place = [&](int i) __attribute__((always_inline)) { return ((first + i * kStride) * 32) & ((1 << shift) - 1); };
 
-    uint8_t *vbuf = lds;
     float *sx = reinterpret_cast<float *>(lds + P::kData);                 // scores of the slices
     int *flags = reinterpret_cast<int *>(lds + P::kData + P::kScores);     // [buffer]: a NaN among the block's V
-    constexpr int kStride = kShare || kSliced ? P::kBlocks : kWaves;       // blocks from a step to the next
-    const int blk0 = kShare || kSliced ? b0 : b0 + wave;
-    const int mine0 = kShare ? wave : 0;                                   // the block of a step that this wave stages
+    const int ahead = kShare ? wave : 0;       // the block of a step that this wave stages
+    const int buffers = kShare ? 0 : 2 * wave;  // this wave's first buffer
 
     Query<D, TEAM, ND> q;
-    f32x16 o[P::kTiles];
+    f32x16 o[P::kTiles], s;
 #pragma unroll
     for (int t = 0; t < P::kTiles; ++t) o[t] = f32x16{};
     float m = -INFINITY, l = 0.0f;
@@ -399,141 +409,176 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
 
     KBlock<D, TEAM> kb;
     VBlock<D, TEAM> vb;
-    auto stage = [&](int blk, int buffer) __attribute__((always_inline)) {
-        const int page = page_of(blk);
-        const bool nan = stage_v<D, TEAM>(vbuf + buffer * P::kV, vb, blk * 32, klo, page < 0 ? 0 : khi, lane);
-        const bool some = __any(nan);
+    VScale<D, TEAM> vs;
+    int ahead_slab = slab_index(ahead);  // of the block in vb
+    auto fetch_v = [&](int i) __attribute__((always_inline)) {
+        ahead_slab = slab_index(i);
+        load_v<D, TEAM>(vb, slab_at(ahead_slab), shift, place(i), lane, slice);
+    };
+    auto scale_v = [&](int i, int buffer) __attribute__((always_inline)) {
+        v_scales<D, TEAM>(vs, vb, (first + i * kStride) * 32, klo, ahead_slab < 0 ? 0 : khi, lane);
+        const bool some = __any(vs.nan);
         if (lane == 0) flags[buffer] = some;
     };
-    load_v<D, TEAM>(vb, slab_of(page_of(blk0 + mine0)), shift, place(blk0 + mine0), lane, slice);
-    load_k<D, TEAM>(kb, slab_of(page_of(blk0)), shift, place(blk0), lane, slice);
+    fetch_v(ahead);
+    int slab0 = slab_index(0), slab1 = slab_index(1);  // of the block at hand and the next
+    load_k<D, TEAM>(kb, slab_at(slab0), shift, place(0), lane, slice);
     load_query<D, TEAM, ND>(q, a, (int64_t)row * a.q_stride + (int64_t)head * D, lane, slice);
-    int buffer = kShare ? 0 : wave;  // of the step's first block
-    stage(blk0 + mine0, buffer + mine0);
+    scale_v(ahead, buffers + ahead);
+#pragma unroll
+    for (int t = 0; t < P::kTiles; ++t) stage_v<D, TEAM>(lds + (buffers + ahead) * P::kV, vb, vs, t, lane);
+    fetch_v(ahead + P::kBlocks);
+    constexpr int kProducts = P::kSteps * ND, kEarly = kProducts / 4;  // of a block's scores; those beside the logs
+    s = f32x16{};
+    scores<D, TEAM, ND, 0, kProducts>(q, kb, s);
+    load_k<D, TEAM>(kb, slab_at(slab1), shift, place(1), lane, slice);
     if (kShare) __syncthreads();
 
-    for (int step = blk0; step < b1; step += kStride) {
-        if (step - base >= 64) {
+    // Block i: its weights beside the next one's scores, its P V beside the next V's
+    // way into LDS (of a step's next V a quarter at each of its four blocks).
+    auto block = [&](int i, auto u_) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_)::value;
+        const int p0 = (first + i * kStride) * 32;
+        const int buffer = kShare ? (i & 4) + u : buffers + (i & 1);
+        const int into = kShare ? ((i & 4) ^ 4) + wave : buffers + (~i & 1);
+        f32x16 next = f32x16{};
+        if constexpr (kSliced) {
+            // [slice][r / 4][lane] float4
+            float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
+            __syncthreads();  // the last block's scores have been read
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[64 * r] = make_float4(s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]);
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float4 e = reinterpret_cast<const float4 *>(sx)[w * 256 + 64 * r + lane];
+                    v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
+                }
+                s[4 * r] = v.x, s[4 * r + 1] = v.y, s[4 * r + 2] = v.z, s[4 * r + 3] = v.w;
+            }
+        }
+        // lane: pair n32, positions p0 + 8 (r / 4) + 4 lh + r % 4
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = tanhf(s[r] * rowf);
+        }
+        float y[16];
+        const int top_ = slab0 < 0 ? 0 : hi;
+        const bool whole = slab0 >= 0 && p0 >= flo && p0 + 32 <= fhi;
+        auto logs = [&](float ref) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[r] = fmaf(s[r], yf, -ref);
+        };
+        auto mask = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int p = p0 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                y[r] = p >= lo && p < top_ ? y[r] : -INFINITY;
+            }
+        };
+        auto most = [&]() __attribute__((always_inline)) {
+            float top = y[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, y[r]);
+            return top;
+        };
+        logs(m);
+        if (!whole) mask();
+        const float over = most();
+        scores<D, TEAM, ND, 0, kEarly>(q, kb, next);
+        interleave<kEarly, 6>();
+        if (__any(over > kBias + kLazy)) {  // (m = -inf: any score)
+            logs(0.0f);
+            if (!whole) mask();
+            float top = most();
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float ref = top - kBias > m + kLazy ? top - kBias : m;
+            const float corr = ref == m ? 1.0f : __builtin_amdgcn_exp2f(m - ref);
+            m = ref;
+            l *= corr;
+#pragma unroll
+            for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[t][r] *= corr;
+            logs(ref);
+            if (!whole) mask();
+        }
+        // P^T operands: step h of two takes the positions of quarter lh + 2 h
+        h8 ph[2], pl[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const int r = 4 * (h + 2 * (j >> 2)) + (j & 3);
+                const float e0 = __builtin_amdgcn_exp2f(y[r]), e1 = __builtin_amdgcn_exp2f(y[r + 1]);
+                l += e0 + e1;
+                ph[h][j] = (_Float16)e0, ph[h][j + 1] = (_Float16)e1;
+                if constexpr (FULL) {
+                    pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
+                    pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
+                }
+            }
+        scores<D, TEAM, ND, kEarly, kProducts>(q, kb, next);
+        interleave<kProducts - kEarly, FULL ? 6 : 4>();
+        __builtin_amdgcn_sched_barrier(0);
+        // the block after next follows the next one's K into its registers
+        const int slab2 = slab_index(i + 2);
+        load_k<D, TEAM>(kb, slab_at(slab2), shift, place(i + 2), lane, slice);
+        if constexpr (u == 0) scale_v(i + P::kBlocks + ahead, into);
+        __builtin_amdgcn_sched_barrier(0);
+        const h8 *v = reinterpret_cast<const h8 *>(lds + buffer * P::kV) + lh * P::kDims + n32;
+        uint8_t *to = lds + into * P::kV;
+        constexpr int each = (P::kTiles + P::kBlocks - 1) / P::kBlocks;  // pieces staged at a block of a step
+#pragma unroll
+        for (int t = 0; t < P::kTiles; ++t) {
+            const h8 v0 = v[32 * t], v1 = v[2 * P::kDims + 32 * t];
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[t], 0, 0, 0);
+            if constexpr (FULL) {
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[t], 0, 0, 0);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[t], 0, 0, 0);
+            }
+            if (t < each && u * each + t < P::kTiles) stage_v<D, TEAM>(to, vb, vs, u * each + t, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (u == P::kBlocks - 1) fetch_v(i + 1 + P::kBlocks + ahead);
+        if (flags[buffer]) {
+            // NaN blocks were left out of V: they reach the pairs that see them
+            const uint8_t *slab = slab_at(slab0);
+            for (int x = 0; x < 32; ++x)
+                for (int g = 0; g < D / 32; ++g) {
+                    if (slab[Mx4Slab<D>::v_scale(shift, place(i) + x, g)] != doe::kMx4NanScale) continue;
+                    const float bad = p0 + x >= lo && p0 + x < top_ ? NAN : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < P::kTiles; ++t)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int w = 8 * (r >> 2) + 4 * lh + (r & 3);
+                            const int dim = (w & 15) * (D / 16) + slice * (P::kDims / 16) + 2 * t + (w >> 4);
+                            o[t][r] += dim / 32 == g ? bad : 0.0f;
+                        }
+                }
+        }
+        s = next;
+        slab0 = slab1;
+        slab1 = slab2;
+    };
+    for (int i = 0; i < blocks; i += P::kBlocks) {
+        if (i - base >= 64) {  // (after the last use of a block below base + 64: those ahead are at most eleven on)
             base += 64;
             list0 = list1;
-            list1 = pages(base + 64);
+            list1 = slabs(base + 64);
         }
-        const int next = step + kStride;
-        if (next < b1) load_v<D, TEAM>(vb, slab_of(page_of(next + mine0)), shift, place(next + mine0), lane, slice);
-#pragma unroll 1
-        for (int u = 0; u < P::kBlocks; ++u) {
-            const int blk = step + u, p0 = blk * 32, page = page_of(blk);
-            // the next block's K follows this one's into its registers
-            const int after = u + 1 < P::kBlocks ? blk + 1 : next;
-            const bool skip = blk >= b1 || page < 0 || p0 >= whi || p0 + 32 <= wlo;
-            f32x16 s = {};
-            if (!skip || kSliced) score_step<D, TEAM, ND, 0>(q, kb, s);
-            __builtin_amdgcn_sched_barrier(0);
-            load_k<D, TEAM>(kb, slab_of(page_of(after)), shift, place(after), lane, slice);
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (kSliced) {
-                // [slice][r / 4][lane] float4
-                float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
-                __syncthreads();  // the last block's scores have been read
-#pragma unroll
-                for (int r = 0; r < 4; ++r) to[64 * r] = make_float4(s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]);
-                __syncthreads();
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) {
-                        const float4 e = reinterpret_cast<const float4 *>(sx)[w * 256 + 64 * r + lane];
-                        v.x += e.x, v.y += e.y, v.z += e.z, v.w += e.w;
-                    }
-                    s[4 * r] = v.x, s[4 * r + 1] = v.y, s[4 * r + 2] = v.z, s[4 * r + 3] = v.w;
-                }
-            }
-            if (skip) continue;
-            // lane: pair n32, positions p0 + 8 (r / 4) + 4 lh + r % 4
-            if (a.softcap > 0.0f) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = tanhf(s[r] * rowf);
-            }
-            float y[16];
-            const bool whole = p0 >= flo && p0 + 32 <= fhi;
-            auto logs = [&](float ref) __attribute__((always_inline)) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) y[r] = fmaf(s[r], yf, -ref);
-                if (!whole) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int p = p0 + 8 * (r >> 2) + 4 * lh + (r & 3);
-                        y[r] = p >= lo && p < hi ? y[r] : -INFINITY;
-                    }
-                }
-                float top = y[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, y[r]);
-                return top;
-            };
-            if (__any(logs(m) > kBias + kLazy)) {  // (m = -inf: any score)
-                float top = logs(0.0f);
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float ref = top - kBias > m + kLazy ? top - kBias : m;
-                const float corr = ref == m ? 1.0f : __builtin_amdgcn_exp2f(m - ref);
-                m = ref;
-                l *= corr;
-#pragma unroll
-                for (int t = 0; t < P::kTiles; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[t][r] *= corr;
-                logs(ref);
-            }
-            // P^T operands: step h of two takes the positions of quarter lh + 2 h
-            h8 ph[2], pl[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const int r = 4 * (h + 2 * (j >> 2)) + (j & 3);
-                    const float e0 = __builtin_amdgcn_exp2f(y[r]), e1 = __builtin_amdgcn_exp2f(y[r + 1]);
-                    l += e0 + e1;
-                    ph[h][j] = (_Float16)e0, ph[h][j + 1] = (_Float16)e1;
-                    if constexpr (FULL) {
-                        pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
-                        pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
-                    }
-                }
-            const h8 *v = reinterpret_cast<const h8 *>(vbuf + (buffer + u) * P::kV) + lh * P::kDims + n32;
-#pragma unroll
-            for (int t = 0; t < P::kTiles; ++t) {
-                const h8 v0 = v[32 * t], v1 = v[2 * P::kDims + 32 * t];
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[t], 0, 0, 0);
-                if constexpr (FULL) {
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[t], 0, 0, 0);
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[t], 0, 0, 0);
-                }
-            }
-            if (flags[buffer + u]) {
-                // NaN blocks were left out of V: they reach the pairs that see them
-                const uint8_t *slab = slab_of(page);
-                for (int x = 0; x < 32; ++x)
-                    for (int g = 0; g < D / 32; ++g) {
-                        if (slab[Mx4Slab<D>::v_scale(shift, place(blk) + x, g)] != doe::kMx4NanScale) continue;
-                        const float bad = p0 + x >= lo && p0 + x < hi ? NAN : 0.0f;
-#pragma unroll
-                        for (int t = 0; t < P::kTiles; ++t)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                const int w = 8 * (r >> 2) + 4 * lh + (r & 3);
-                                const int dim = (w & 15) * (D / 16) + slice * (P::kDims / 16) + 2 * t + (w >> 4);
-                                o[t][r] += dim / 32 == g ? bad : 0.0f;
-                            }
-                    }
-            }
+        block(i, std::integral_constant<int, 0>());
+        if constexpr (kShare) {
+            block(i + 1, std::integral_constant<int, 1>());
+            block(i + 2, std::integral_constant<int, 2>());
+            block(i + 3, std::integral_constant<int, 3>());
+            __syncthreads();
         }
-        if (next < b1) {
-            if (kShare) buffer ^= 4;
-            stage(next + mine0, buffer + mine0);
-        }
-        if (kShare) __syncthreads();
     }
 
     l += __shfl_xor(l, 32, 64);
@@ -646,8 +691,11 @@ constexpr int kCus = 256, kMaxSplits = 16;
 int64_t tiles_of(bool starts, int64_t batch, int64_t rows, int64_t group, int tile_rows) {
     return starts ? rows * group / tile_rows + std::min(batch, rows) : batch * ((group + tile_rows - 1) / tile_rows);
 }
+int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
+
 // Whether tiles of 128 pairs, whose waves share V, are many enough to fill the device.
 bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    if (g_tile) return head_dim < 512 && g_tile == 128;
     return head_dim < 512 && tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= 2 * kCus;
 }
 int64_t splits_of(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
@@ -687,6 +735,16 @@ int launch_d(PromptArgs &a, bool share, hipStream_t st) {
 }
 
 }  // namespace
+
+namespace doe {
+
+int mx4_set_tile(int value) {
+    DOE_REQUIRE(value == 0 || value == 32 || value == 128, DOE_E_INVALID, "attn_mx4.tile is 0, 32 or 128");
+    g_tile = value;
+    return DOE_OK;
+}
+
+}  // namespace doe
 
 extern "C" {
 

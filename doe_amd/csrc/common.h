@@ -38,6 +38,7 @@ int attn_scratch_setup(int device);
 int attn_set_splits(int value);
 int mq_set_splits(int value);
 int mq_set_queries(int value);
+int mx4_set_tile(int value);
 int attn_set_waves(int value);
 int attn_set_combine(int value);
 int gemm_set_f16_operands(int value);

@@ -1758,6 +1758,8 @@ int doe_tune_set(const char *key, int value) {
         return doe::mq_set_splits(value);
     } else if (!strcmp(key, "attn_mq.queries")) {
         return doe::mq_set_queries(value);
+    } else if (!strcmp(key, "attn_mx4.tile")) {
+        return doe::mx4_set_tile(value);
     } else if (!strcmp(key, "attn_decode.splits")) {
         return doe::attn_set_splits(value);
     } else if (!strcmp(key, "attn_decode.waves")) {

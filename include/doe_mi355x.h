@@ -809,7 +809,9 @@ int doe_decode_advance(int32_t *state, int32_t *token, int32_t *ids, int64_t max
  * "int4_gemv.xcd" (1: workgroup ids in plain order, not a row block's K
  * ranges grouped on one XCD), "q8_0_gemv.rows" (1, 2 or 4 rows per wave group), "q8_0_gemv.depth" (1 or
  * 2 blocks loaded ahead), "attn_mq.splits" (1..16 key splits of the
- * multi-query attention), "attn_mq.queries" (16: its 16-query form, with P in
+ * multi-query attention), "attn_mx4.tile" (32 or 128 (row, head) pairs a tile
+ * of the 4-bit cache's prompt attention; a workspace has to be asked for under
+ * the same setting), "attn_mq.queries" (16: its 16-query form, with P in
  * one f16, at any head_dim), "attn_decode.splits",
  * "attn_decode.waves" (4: narrow workgroups; 8 or 16: the wide short-context
  * workgroup where the head shape allows it), "attn_decode.combine" (1: the

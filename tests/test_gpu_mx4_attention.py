@@ -167,7 +167,7 @@ def test_lengths_beyond_the_table(dev, form):
     assert np.isfinite(got).all() and not got[0].any()
 
 
-def test_a_nan_block_reaches_its_own_sequence_and_head_only(dev):
+def test_a_nan_block_reaches_its_own_sequence_and_head_only(dev, tile):
     rng = np.random.default_rng(12)
     case = Case(rng, [100, 100], head_dim=128, num_kv_heads=2, page_size=32)
     page = case.table[0, 1]
@@ -185,7 +185,59 @@ def test_a_nan_block_reaches_its_own_sequence_and_head_only(dev):
     q = rng.standard_normal((100, 4, 128)).astype(np.float32)
     got = prompt(case, q, rows, sliding_window=10)
     assert np.isfinite(got[:, :2]).all() and np.isfinite(got[50:]).all()
+    # of a prompt's rows it reaches those that see it, from its own position on
+    case = Case(rng, [100], head_dim=128, num_kv_heads=2, page_size=32)
+    case.vs[case.table[0, 1], 1, 3, 2] = mx4.NAN_SCALE
+    case.ks[case.table[0, 2], 0, 6, 1] = mx4.NAN_SCALE  # position 70, head 0
+    case.upload()
+    q = rng.standard_normal((90, 4, 128)).astype(np.float32)
+    got = prompt(case, q, [90])
+    bad = np.zeros(got.shape, bool)
+    bad[25:, 2:, 64:96] = True
+    bad[60:, :2] = True
+    assert np.array_equal(np.isnan(got), bad)
+    got = prompt(case, q, [90], sliding_window=5)
+    bad[30:] = False
+    bad[60:65, :2] = True
+    assert np.array_equal(np.isnan(got), bad)
 
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 16, 2), (128, 8, 2), (160, 8, 4), (256, 8, 4), (512, 4, 2)])
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("f16", [False, True])
+def test_long_prompts(dev, tile, d, hq, hkv, window, f16):
+    """Rows enough for several tiles and positions for several lists of pages;
+    checked at some of the rows."""
+    rng = np.random.default_rng(d + window)
+    rows, lens = [300, 70], [300 + 4700, 70]
+    case = Case(rng, lens, head_dim=d, num_kv_heads=hkv, page_size=32)
+    case.upload()
+    q = rng.standard_normal((sum(rows), hq, d)).astype(np.float16 if f16 else np.float32)
+    got = prompt(case, q, rows, f16=f16, sliding_window=window)
+    for at in (0, 31, 150, 299, 300, 340, 369):
+        b, i = (0, at) if at < 300 else (1, at - 300)
+        one = Case.__new__(Case)
+        one.__dict__.update(case.__dict__, lens=[lens[b] - rows[b] + i + 1], table=case.table[b:b + 1], batch=1)
+        want, bound, mass = attention(one, q[at:at + 1], [1], d ** -0.5, 0.0, window)
+        check(got[at:at + 1], want, bound, got.dtype, mass if f16 else None)
+
+
+@pytest.mark.parametrize("d", [64, 128, 160, 256])
+def test_tokens_of_a_pool_beyond_the_last_level_cache(dev, d):
+    """The form that reads past the caches gives the same bits."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [700, 31, 2000], head_dim=d, num_kv_heads=2, page_size=64)
+    case.upload()
+    q = rng.standard_normal((3, 8, d)).astype(np.float32)
+    small = token(case, q)
+    size = mx4.page_bytes(64, 2, d)
+    case.num_pages = (300 << 20) // size
+    pool = DeviceBuffer(case.num_pages * size)
+    pool.view(0, case.pool.nbytes).upload(case.pages())
+    case.cache = ops.Mx4Cache(pool, case.table_dev, case.lens_dev, num_pages=case.num_pages, page_size=64, num_kv_heads=2,
+                              head_dim=d, batch=3, table_stride=case.stride)
+    assert np.array_equal(token(case, q), small)
+    pool.free()
 
 PROMPTS = [
     # rows and lengths by sequence, head_dim, heads, page size
@@ -201,9 +253,17 @@ PROMPTS = [
 ]
 
 
+@pytest.fixture(params=[32, 128])
+def tile(request, dev):
+    """Both tile sizes of the prompt's kernel (head_dim 512 has one)."""
+    ops.tune("attn_mx4.tile", request.param)
+    yield request.param
+    ops.tune("attn_mx4.tile", 0)
+
+
 @pytest.mark.parametrize("rows,lens,d,hq,hkv,ps", PROMPTS)
 @pytest.mark.parametrize("f16", [False, True])
-def test_prompts(dev, rows, lens, d, hq, hkv, ps, f16):
+def test_prompts(dev, tile, rows, lens, d, hq, hkv, ps, f16):
     """Prompts from one row on, behind contexts of all lengths, more rows than
     positions among them; rows of nobody before and behind."""
     rng = np.random.default_rng(sum(rows) + d)
@@ -218,7 +278,7 @@ def test_prompts(dev, rows, lens, d, hq, hkv, ps, f16):
 
 @pytest.mark.parametrize("d,hq,hkv", [(64, 4, 2), (128, 6, 2), (160, 4, 4), (256, 4, 2), (512, 2, 1)])
 @pytest.mark.parametrize("window,softcap", [(1, 0.0), (40, 0.0), (64, 20.0), (0, 5.0), (5000, 0.0)])
-def test_prompts_window_and_softcap(dev, d, hq, hkv, window, softcap):
+def test_prompts_window_and_softcap(dev, tile, d, hq, hkv, window, softcap):
     rng = np.random.default_rng(d + window)
     rows, lens = [70, 1, 33], [150, 90, 33]
     case = Case(rng, lens, head_dim=d, num_kv_heads=hkv, page_size=64)
