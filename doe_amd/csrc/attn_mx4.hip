@@ -223,7 +223,7 @@ __device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f3
     for (int j = 0; j < 8; ++j) v[j] = s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3]);
     if (a.softcap > 0.0f) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tanhf(v[j] * rowf);
+        for (int j = 0; j < 8; ++j) v[j] = doe::mx4_tanh(v[j] * rowf);
         rowf = a.softcap * 1.4426950408889634f;
     }
     const bool whole = p0 >= lo && p0 + 32 <= hi;

@@ -97,22 +97,23 @@ __device__ __forceinline__ void load_k(KBlock<D, TEAM> &b, const uint8_t *slab, 
     using S = Mx4Slab<D>;
     using P = Shape<D, TEAM>;
     const int m = lane & 31, lh = lane >> 5;
-    const uint8_t *k = slab + S::k_code(x) + slice * (P::kDims / 2) + (m * (D / 2) + lh * 16);
-    const uint8_t *s = slab + S::k_scale(shift, x) + slice * (P::kDims / 32) + m * (D / 32);
+    const uint8_t *k = slab + (uint32_t)(S::k_code(x) + slice * (P::kDims / 2));
+    const uint32_t at_k = m * (D / 2) + lh * 16, at_s = m * (D / 32);
+    const uint8_t *s = slab + (uint32_t)(S::k_scale(shift, x) + slice * (P::kDims / 32));
 #pragma unroll
     for (int i = 0; i < P::kSteps; ++i) {
         // (head_dim 160: the last step's second half is nothing; the query has zeros there)
         const int at = P::kDims % 64 && i == P::kSteps - 1 ? i * 32 - lh * 16 : i * 32;
-        b.k[i] = *reinterpret_cast<const u32x4 *>(k + at);
+        b.k[i] = *reinterpret_cast<const u32x4 *>(k + (uint32_t)(at_k + at));
     }
     if constexpr (D == 64) {
-        b.s[0] = *reinterpret_cast<const uint16_t *>(s) >> (8 * lh);
+        b.s[0] = *reinterpret_cast<const uint16_t *>(s + at_s) >> (8 * lh);
     } else if constexpr (D == 160) {
-        b.s[0] = s[lh] | (uint32_t)s[2 + lh] << 16;
-        b.s[1] = s[4];
+        b.s[0] = s[at_s + lh] | (uint32_t)s[at_s + 2 + lh] << 16;
+        b.s[1] = s[at_s + 4];
     } else {
 #pragma unroll
-        for (int i = 0; i < P::kSteps / 2; ++i) b.s[i] = *reinterpret_cast<const uint32_t *>(s + 4 * i) >> (8 * lh);
+        for (int i = 0; i < P::kSteps / 2; ++i) b.s[i] = *reinterpret_cast<const uint32_t *>(s + (uint32_t)(at_s + 4 * i)) >> (8 * lh);
     }
 }
 
@@ -288,6 +289,12 @@ __device__ __forceinline__ void scores(const Query<D, TEAM, ND> &q, const KBlock
     }
 }
 
+// A value is wanted here: otherwise the compiler computes it where it is used.
+template <typename T>
+__device__ __forceinline__ void here(T &v) {
+    __asm__ volatile("" : "+v"(v));
+}
+
 // The instruction scheduler's order for what stands before it in a block of code:
 // one matrix instruction, then so many vector ones, N times.
 template <int N, int VALU>
@@ -415,10 +422,11 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         ahead_slab = slab_index(i);
         load_v<D, TEAM>(vb, slab_at(ahead_slab), shift, place(i), lane, slice);
     };
+    int nans = 0, nans_ahead = 0;  // NaN blocks among the V of the step at hand, of the one being staged
     auto scale_v = [&](int i, int buffer) __attribute__((always_inline)) {
         v_scales<D, TEAM>(vs, vb, (first + i * kStride) * 32, klo, ahead_slab < 0 ? 0 : khi, lane);
-        const bool some = __any(vs.nan);
-        if (lane == 0) flags[buffer] = some;
+        nans_ahead = __any(vs.nan);
+        if (kShare && lane == 0) flags[buffer] = nans_ahead;
     };
     fetch_v(ahead);
     int slab0 = slab_index(0), slab1 = slab_index(1);  // of the block at hand and the next
@@ -442,6 +450,14 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         const int buffer = kShare ? (i & 4) + u : buffers + (i & 1);
         const int into = kShare ? ((i & 4) ^ 4) + wave : buffers + (~i & 1);
         f32x16 next = f32x16{};
+        if constexpr (u == 0) {
+            if constexpr (kShare) {
+                const int4 f = *reinterpret_cast<const int4 *>(flags + (i & 4));
+                nans = f.x | f.y | f.z | f.w;
+            } else {
+                nans = nans_ahead;
+            }
+        }
         if constexpr (kSliced) {
             // [slice][r / 4][lane] float4
             float4 *to = reinterpret_cast<float4 *>(sx) + wave * 256 + lane;
@@ -463,7 +479,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         // lane: pair n32, positions p0 + 8 (r / 4) + 4 lh + r % 4
         if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = tanhf(s[r] * rowf);
+            for (int r = 0; r < 16; ++r) s[r] = doe::mx4_tanh(s[r] * rowf);
         }
         float y[16];
         const int top_ = slab0 < 0 ? 0 : hi;
@@ -490,6 +506,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         const float over = most();
         scores<D, TEAM, ND, 0, kEarly>(q, kb, next);
         interleave<kEarly, 6>();
+        here(next);
         if (__any(over > kBias + kLazy)) {  // (m = -inf: any score)
             logs(0.0f);
             if (!whole) mask();
@@ -523,6 +540,8 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
             }
         scores<D, TEAM, ND, kEarly, kProducts>(q, kb, next);
         interleave<kProducts - kEarly, FULL ? 6 : 4>();
+        here(next);
+        here(l);
         __builtin_amdgcn_sched_barrier(0);
         // the block after next follows the next one's K into its registers
         const int slab2 = slab_index(i + 2);
@@ -545,7 +564,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (u == P::kBlocks - 1) fetch_v(i + 1 + P::kBlocks + ahead);
-        if (flags[buffer]) {
+        if (__builtin_amdgcn_readfirstlane(nans)) {
             // NaN blocks were left out of V: they reach the pairs that see them
             const uint8_t *slab = slab_at(slab0);
             for (int x = 0; x < 32; ++x)
