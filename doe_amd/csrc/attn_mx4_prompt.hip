@@ -211,63 +211,62 @@ struct Query {
     u32x6 d[Shape<D, TEAM>::kSteps][ND];
     uint32_t s[Shape<D, TEAM>::kSteps], s4[ND > 4 ? Shape<D, TEAM>::kSteps : 1];
 };
+// Step s of them.
 template <int D, int TEAM, int ND>
-__device__ __forceinline__ void load_query(Query<D, TEAM, ND> &q, const PromptArgs &a, int64_t at, int lane, int slice) {
+__device__ __forceinline__ void load_query(u32x6 *digits, uint32_t &scales, uint32_t &scale4, const PromptArgs &a, int64_t at, int s,
+                                           int lane, int slice) {
     using P = Shape<D, TEAM>;
     const int lh = lane >> 5;
+    const bool none = P::kDims % 64 && s == P::kSteps - 1 && lh;
+    const int64_t from = at + slice * P::kDims + (none ? 0 : 64 * s + 32 * lh);
+    float f[32];
+    if (a.q_f16) {
 #pragma unroll
-    for (int s = 0; s < P::kSteps; ++s) {
-        const bool none = P::kDims % 64 && s == P::kSteps - 1 && lh;
-        const int64_t from = at + slice * P::kDims + (none ? 0 : 64 * s + 32 * lh);
-        float f[32];
-        if (a.q_f16) {
+        for (int i = 0; i < 32; i += 8) {
+            const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + from + i);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-                const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + from + i);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + from + i);
-                f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
-            }
+            for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
         }
-        uint32_t top = 0;  // (as bits: a NaN is above all)
+    } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-        if (none) top = 0;
-        const bool real = top < 0x7f800000u;
-        int e = top == 0 || !real ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top));
-        e = e < -106 ? -106 : e;
-        f32x16 even, odd;
+        for (int i = 0; i < 32; i += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + from + i);
+            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+        }
+    }
+    uint32_t top = 0;  // (as bits: a NaN is above all)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    if (none) top = 0;
+    const bool real = top < 0x7f800000u;
+    int e = top == 0 || !real ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top));
+    e = e < -106 ? -106 : e;
+    f32x16 even, odd;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        even[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i], 4 - e);
+        odd[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i + 1], 4 - e);
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        f32x16 x, y;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            even[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i], 4 - e);
-            odd[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i + 1], 4 - e);
+            x[i] = __builtin_rintf(even[i]);
+            y[i] = __builtin_rintf(odd[i]);
+            even[i] = (even[i] - x[i]) * 32.0f;
+            odd[i] = (odd[i] - y[i]) * 32.0f;
         }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            f32x16 x, y;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = __builtin_rintf(even[i]);
-                y[i] = __builtin_rintf(odd[i]);
-                even[i] = (even[i] - x[i]) * 32.0f;
-                odd[i] = (odd[i] - y[i]) * 32.0f;
-            }
-            u32x6 packed = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x, y, 8.0f);
-            // (the sources outlive it: with a destination that begins inside one of them,
-            // which the compiler allows itself, the instruction overwrites what it has yet to read)
-            __asm__ volatile("" : "+v"(packed) : "v"(x), "v"(y));
-            q.d[s][d] = packed;
-        }
-        // digit d counts 2^(e - 1 - 5 d) times its 6-bit float; 255: not a number
-        const uint32_t b = e + 126;
-        q.s[s] = real ? b | (b - 5) << 8 | (b - 10) << 16 | (ND > 3 ? (b - 15) << 24 : 0u) : 0xffffffffu;
-        if constexpr (ND > 4) q.s4[s] = real ? b - 20 : 255u;
+        u32x6 packed = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x, y, 8.0f);
+        // (the sources outlive it: with a destination that begins inside one of them,
+        // which the compiler allows itself, the instruction overwrites what it has yet to read)
+        __asm__ volatile("" : "+v"(packed) : "v"(x), "v"(y));
+        digits[d] = packed;
     }
+    // digit d counts 2^(e - 1 - 5 d) times its 6-bit float; 255: not a number
+    const uint32_t b = e + 126;
+    scales = real ? b | (b - 5) << 8 | (b - 10) << 16 | (ND > 3 ? (b - 15) << 24 : 0u) : 0xffffffffu;
+    scale4 = real ? b - 20 : 255u;
 }
 
 // The products [FROM, TO) of a block's scores, step and digit in order.
@@ -431,7 +430,43 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
     fetch_v(ahead);
     int slab0 = slab_index(0), slab1 = slab_index(1);  // of the block at hand and the next
     load_k<D, TEAM>(kb, slab_at(slab0), shift, place(0), lane, slice);
-    load_query<D, TEAM, ND>(q, a, (int64_t)row * a.q_stride + (int64_t)head * D, lane, slice);
+    {
+        const int64_t at = (int64_t)row * a.q_stride + (int64_t)head * D;
+        uint32_t s4 = 0;
+        if constexpr (kShare || kSliced) {
+#pragma unroll
+            for (int s = 0; s < P::kSteps; ++s) {
+                load_query<D, TEAM, ND>(q.d[s], q.s[s], s4, a, at, s, lane, slice);
+                if constexpr (ND > 4) q.s4[s] = s4;
+            }
+        } else {
+            // the waves have the same pairs: a step or none each, passed on in V's place
+            u32x2 *x = reinterpret_cast<u32x2 *>(lds);
+            if (wave < P::kSteps) {
+                u32x6 d[ND];
+                uint32_t sc = 0;
+                load_query<D, TEAM, ND>(d, sc, s4, a, at, wave, lane, slice);
+                u32x2 *to = x + wave * (3 * ND + 1) * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < 3 * ND; ++i) to[64 * i] = u32x2{d[i / 3][i % 3 * 2], d[i / 3][i % 3 * 2 + 1]};
+                to[64 * 3 * ND] = u32x2{sc, s4};
+            }
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < P::kSteps; ++s) {
+                const u32x2 *from = x + s * (3 * ND + 1) * 64 + lane;
+#pragma unroll
+                for (int i = 0; i < 3 * ND; ++i) {
+                    const u32x2 w = from[64 * i];
+                    q.d[s][i / 3][i % 3 * 2] = w[0], q.d[s][i / 3][i % 3 * 2 + 1] = w[1];
+                }
+                const u32x2 w = from[64 * 3 * ND];
+                q.s[s] = w[0];
+                if constexpr (ND > 4) q.s4[s] = w[1];
+            }
+            __syncthreads();
+        }
+    }
     scale_v(ahead, buffers + ahead);
 #pragma unroll
     for (int t = 0; t < P::kTiles; ++t) stage_v<D, TEAM>(lds + (buffers + ahead) * P::kV, vb, vs, t, lane);
