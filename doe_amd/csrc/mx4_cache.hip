@@ -66,8 +66,9 @@ struct Place {
 };
 
 // A workgroup takes kRowsPerWg rows; a thread four dims of K and V of a row's head.
-template <int D, bool F16>
+template <bool F16>
 __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
+    constexpr int D = 160;
     __shared__ Place place[kRowsPerWg];
     const int64_t row0 = (int64_t)blockIdx.x * kRowsPerWg;
     if (threadIdx.x < kRowsPerWg) {
@@ -103,13 +104,9 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         const uint32_t kc = quantise(k, ks), vc = quantise(v, vs);
         uint8_t *slab = a.c.pool + (p.page + head) * S::bytes(shift);
         *reinterpret_cast<uint16_t *>(slab + S::k_code(p.x) + d / 2) = (uint16_t)kc;
-        if constexpr (D == 160) {  // columns of five bytes
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                slab[S::v_code(shift, p.x, (d + 2 * e) / 10) + (d + 2 * e) % 10 / 2] = (uint8_t)(vc >> (8 * e));
-        } else {
-            *reinterpret_cast<uint16_t *>(slab + S::v_code(shift, p.x, d / (D / 16)) + d % (D / 16) / 2) = (uint16_t)vc;
-        }
+        for (int e = 0; e < 2; ++e)
+            slab[S::v_code(shift, p.x, (d + 2 * e) / 10) + (d + 2 * e) % 10 / 2] = (uint8_t)(vc >> (8 * e));
         if ((d & 31) == 0) {
             slab[S::k_scale(shift, p.x) + d / 32] = (uint8_t)ks;
             slab[S::v_scale(shift, p.x, d / 32)] = (uint8_t)vs;
@@ -123,8 +120,8 @@ __device__ __forceinline__ float4 values(uint32_t codes, int scale) {
     return make_float4((float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]);
 }
 
-template <int D>
 __global__ __launch_bounds__(256) void mx4_read_kernel(RowArgs a) {
+    constexpr int D = 160;
     __shared__ Place place[kRowsPerWg];
     __shared__ bool mine[kRowsPerWg];
     const int64_t row0 = (int64_t)blockIdx.x * kRowsPerWg;
@@ -152,17 +149,183 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(RowArgs a) {
         if (p.page >= 0) {
             const uint8_t *slab = a.c.pool + (p.page + head) * S::bytes(shift);
             const uint32_t kc = *reinterpret_cast<const uint16_t *>(slab + S::k_code(p.x) + d / 2);
-            uint32_t vc;
-            if constexpr (D == 160) {
-                vc = slab[S::v_code(shift, p.x, d / 10) + d % 10 / 2] |
-                     (uint32_t)slab[S::v_code(shift, p.x, (d + 2) / 10) + (d + 2) % 10 / 2] << 8;
-            } else {
-                vc = *reinterpret_cast<const uint16_t *>(slab + S::v_code(shift, p.x, d / (D / 16)) + d % (D / 16) / 2);
-            }
+            const uint32_t vc = slab[S::v_code(shift, p.x, d / 10) + d % 10 / 2] |
+                                (uint32_t)slab[S::v_code(shift, p.x, (d + 2) / 10) + (d + 2) % 10 / 2] << 8;
             k = values(kc, slab[S::k_scale(shift, p.x) + d / 32]);
             v = values(vc, slab[S::v_scale(shift, p.x, d / 32)]);
         }
         const int64_t at = (row0 + r) * a.row_stride + (int64_t)head * D + d;
+        *reinterpret_cast<float4 *>(a.k_out + at) = k;
+        *reinterpret_cast<float4 *>(a.v_out + at) = v;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The other head dims: a unit is four consecutive positions, from a multiple of
+// four on, of one head, and D / 4 lanes take four dims of each.  V's codes of a
+// column's four positions lie in a row (D / 8 bytes), so the lanes hand them round
+// through LDS, each to its own wave's lanes only, and move eight bytes each.  The rows of a sequence get rows / 4 + 2 places for units (as
+// many as they can touch from any position on), so that a place's sequence is
+// found in row_starts.
+struct Four {
+    int pos0, from, last;  // positions pos0 .. pos0 + 3; those in [from, last] have rows, those below 0 hold nothing
+    int64_t row0;          // row of position pos0
+    int page;              // -1: none
+};
+template <int D>
+__device__ __forceinline__ bool find_four(const RowArgs &a, Four &f, int &head) {
+    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 4), place = unit / a.c.kv_heads;
+    head = (int)(unit - place * a.c.kv_heads);
+    int b = 0;
+    int64_t at = place, n = 1, four = 0;
+    if (a.row_starts) {
+        int hi = a.c.batch;  // the last b whose places begin at or before this one
+        while (hi - b > 1) {
+            const int mid = (b + hi) >> 1;
+            if ((a.row_starts[mid] >> 2) + 2 * (int64_t)mid <= place) b = mid;
+            else hi = mid;
+        }
+        at = a.row_starts[b];
+        n = a.row_starts[b + 1] - at;
+        four = place - (at >> 2) - 2 * (int64_t)b;
+    } else {
+        if (place >= a.c.batch) return false;
+        b = (int)place;
+    }
+    if (at < 0 || n <= 0 || four < 0) return false;
+    const int len = doe::mx4_len(a.c, b);
+    f.from = (int)(len - n);
+    f.last = len - 1;
+    four += f.from >> 2;
+    if (four > (f.last >> 2)) return false;
+    f.pos0 = (int)four * 4;
+    f.row0 = at + (f.pos0 - f.from);
+    f.page = f.pos0 < 0 ? -1 : doe::mx4_page(a.c, b, f.pos0);
+    return true;
+}
+
+// Codes of V of a unit between the lanes' order (a lane's four dims of position
+// i: 16 bits of the 64) and the page's.  LDS operations of a wave are in order.
+template <int D>
+struct Exchange {
+    static constexpr int C = D / 16, PER = C / 4;  // lanes of a column
+    uint8_t *mine, *column;
+    int at;
+    __device__ __forceinline__ explicit Exchange(uint8_t *lds)
+        : mine(lds + threadIdx.x * 8), column(lds + (threadIdx.x / PER) * PER * 8), at(threadIdx.x % PER * 2) {}
+    __device__ __forceinline__ uint64_t to_page(const uint32_t *codes) const {
+        if constexpr (PER == 1) return codes[0] | codes[1] << 16 | (uint64_t)(codes[2] | codes[3] << 16) << 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint16_t *>(column + i * (C / 2) + at) = (uint16_t)codes[i];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        return *reinterpret_cast<const uint64_t *>(mine);
+    }
+    __device__ __forceinline__ void from_page(uint64_t w, uint32_t *codes) const {
+        if constexpr (PER == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) codes[i] = (uint32_t)(w >> (16 * i)) & 0xffff;
+        } else {
+            *reinterpret_cast<uint64_t *>(mine) = w;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) codes[i] = *reinterpret_cast<const uint16_t *>(column + i * (C / 2) + at);
+        }
+    }
+};
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
+    using S = Mx4Slab<D>;
+    constexpr int C = D / 16;
+    __shared__ __align__(16) uint8_t lds[256 * 8];
+    const Exchange<D> x(lds);
+    Four f;
+    int head;
+    if (!find_four<D>(a, f, head) || f.page < 0) return;  // (all lanes of a unit)
+    const int shift = a.c.page_shift, x0 = f.pos0 & ((1 << shift) - 1), d = threadIdx.x % (D / 4) * 4;
+    uint8_t *slab = a.c.pool + ((int64_t)f.page * a.c.kv_heads + head) * S::bytes(shift);
+    bool in[4], all = true;
+    float4 k[4] = {}, v[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = f.row0 + i;
+        in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && row < a.rows;
+        all = all && in[i];
+        if (!in[i]) continue;
+        const int64_t at = row * a.row_stride + (int64_t)head * D + d;
+        if constexpr (F16) {
+            const h4 kh = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.k) + at);
+            const h4 vh = *reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.v) + at);
+            k[i] = make_float4((float)kh[0], (float)kh[1], (float)kh[2], (float)kh[3]);
+            v[i] = make_float4((float)vh[0], (float)vh[1], (float)vh[2], (float)vh[3]);
+        } else {
+            k[i] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.k) + at);
+            v[i] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.v) + at);
+        }
+    }
+    uint32_t vc[4] = {};
+    int vs[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!in[i]) continue;
+        int ks;
+        const uint32_t kc = quantise(k[i], ks);
+        vc[i] = quantise(v[i], vs[i]);
+        *reinterpret_cast<uint16_t *>(slab + S::k_code(x0 + i) + d / 2) = (uint16_t)kc;
+        if ((d & 31) == 0) slab[S::k_scale(shift, x0 + i) + d / 32] = (uint8_t)ks;
+    }
+    uint8_t *vsat = slab + S::v_scale(shift, x0, d / 32);
+    if (all) {
+        const uint64_t w = x.to_page(vc);
+        *reinterpret_cast<uint64_t *>(slab + S::v_code(shift, x0, d / C) + d % C * 2) = w;
+        if ((d & 31) == 0) *reinterpret_cast<uint32_t *>(vsat) = vs[0] | vs[1] << 8 | vs[2] << 16 | (uint32_t)vs[3] << 24;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!in[i]) continue;
+            *reinterpret_cast<uint16_t *>(slab + S::v_code(shift, x0 + i, d / C) + d % C / 2) = (uint16_t)vc[i];
+            if ((d & 31) == 0) vsat[i] = (uint8_t)vs[i];
+        }
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void mx4_read_fours_kernel(RowArgs a) {
+    using S = Mx4Slab<D>;
+    constexpr int C = D / 16;
+    __shared__ __align__(16) uint8_t lds[256 * 8];
+    const Exchange<D> x(lds);
+    Four f;
+    int head;
+    if (!find_four<D>(a, f, head)) return;  // (all lanes of a unit)
+    const int shift = a.c.page_shift, x0 = f.pos0 & ((1 << shift) - 1), d = threadIdx.x % (D / 4) * 4;
+    uint32_t kc[4] = {}, vc[4] = {}, vs = 0;
+    int ks[4] = {};
+    if (f.page >= 0) {
+        const uint8_t *slab = a.c.pool + ((int64_t)f.page * a.c.kv_heads + head) * S::bytes(shift);
+        const uint64_t w = *reinterpret_cast<const uint64_t *>(slab + S::v_code(shift, x0, d / C) + d % C * 2);
+        vs = *reinterpret_cast<const uint32_t *>(slab + S::v_scale(shift, x0, d / 32));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            kc[i] = *reinterpret_cast<const uint16_t *>(slab + S::k_code(x0 + i) + d / 2);
+            ks[i] = slab[S::k_scale(shift, x0 + i) + d / 32];
+        }
+        x.from_page(w, vc);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = f.row0 + i;
+        if (f.pos0 + i < f.from || f.pos0 + i > f.last || row >= a.rows) continue;
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;  // (positions below 0, pages outside the pool)
+        if (f.page >= 0) {
+            k = values(kc[i], ks[i]);
+            v = values(vc[i], vs >> (8 * i) & 0xff);
+        }
+        const int64_t at = row * a.row_stride + (int64_t)head * D + d;
         *reinterpret_cast<float4 *>(a.k_out + at) = k;
         *reinterpret_cast<float4 *>(a.v_out + at) = v;
     }
@@ -181,10 +344,29 @@ int row_checks(const Mx4View &c, int64_t head_dim, int64_t rows, int64_t row_str
     return DOE_OK;
 }
 
+// Workgroups for the rows' units.
 template <int D>
-void launch_write(bool f16, dim3 grid, hipStream_t st, const RowArgs &a) {
-    if (f16) hipLaunchKernelGGL((mx4_write_kernel<D, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((mx4_write_kernel<D, false>), grid, dim3(256), 0, st, a);
+dim3 fours_grid(const RowArgs &a) {
+    const int64_t places = a.row_starts ? a.rows / 4 + 2 * (int64_t)a.c.batch : a.c.batch;
+    return dim3((unsigned)((places * a.c.kv_heads * (D / 4) + 255) / 256));
+}
+dim3 rows_grid(const RowArgs &a) { return dim3((unsigned)((a.rows + kRowsPerWg - 1) / kRowsPerWg)); }
+
+template <int D>
+void launch_write(bool f16, hipStream_t st, const RowArgs &a) {
+    if constexpr (D == 160) {
+        if (f16) hipLaunchKernelGGL((mx4_write_kernel<true>), rows_grid(a), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((mx4_write_kernel<false>), rows_grid(a), dim3(256), 0, st, a);
+    } else {
+        if (f16) hipLaunchKernelGGL((mx4_write_fours_kernel<D, true>), fours_grid<D>(a), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((mx4_write_fours_kernel<D, false>), fours_grid<D>(a), dim3(256), 0, st, a);
+    }
+}
+
+template <int D>
+void launch_read(hipStream_t st, const RowArgs &a) {
+    if constexpr (D == 160) hipLaunchKernelGGL(mx4_read_kernel, rows_grid(a), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mx4_read_fours_kernel<D>), fours_grid<D>(a), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -266,14 +448,13 @@ int doe_mx4_kv_write(const doe_mx4_cache *cache, const void *k, const void *v, i
     a.row_starts = row_starts;
     a.rows = rows;
     a.row_stride = row_stride;
-    const dim3 grid((unsigned)((rows + kRowsPerWg - 1) / kRowsPerWg));
     const hipStream_t st = (hipStream_t)stream;
     switch (cache->head_dim) {
-        case 64: launch_write<64>(in_f16, grid, st, a); break;
-        case 128: launch_write<128>(in_f16, grid, st, a); break;
-        case 160: launch_write<160>(in_f16, grid, st, a); break;
-        case 256: launch_write<256>(in_f16, grid, st, a); break;
-        default: launch_write<512>(in_f16, grid, st, a); break;
+        case 64: launch_write<64>(in_f16, st, a); break;
+        case 128: launch_write<128>(in_f16, st, a); break;
+        case 160: launch_write<160>(in_f16, st, a); break;
+        case 256: launch_write<256>(in_f16, st, a); break;
+        default: launch_write<512>(in_f16, st, a); break;
     }
     DOE_LAUNCH_CHECK("mx4_write_kernel");
     return DOE_OK;
@@ -292,14 +473,13 @@ int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_
     a.row_starts = row_starts;
     a.rows = rows;
     a.row_stride = row_stride;
-    const dim3 grid((unsigned)((rows + kRowsPerWg - 1) / kRowsPerWg));
     const hipStream_t st = (hipStream_t)stream;
     switch (cache->head_dim) {
-        case 64: hipLaunchKernelGGL(mx4_read_kernel<64>, grid, dim3(256), 0, st, a); break;
-        case 128: hipLaunchKernelGGL(mx4_read_kernel<128>, grid, dim3(256), 0, st, a); break;
-        case 160: hipLaunchKernelGGL(mx4_read_kernel<160>, grid, dim3(256), 0, st, a); break;
-        case 256: hipLaunchKernelGGL(mx4_read_kernel<256>, grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(mx4_read_kernel<512>, grid, dim3(256), 0, st, a); break;
+        case 64: launch_read<64>(st, a); break;
+        case 128: launch_read<128>(st, a); break;
+        case 160: launch_read<160>(st, a); break;
+        case 256: launch_read<256>(st, a); break;
+        default: launch_read<512>(st, a); break;
     }
     DOE_LAUNCH_CHECK("mx4_read_kernel");
     return DOE_OK;
