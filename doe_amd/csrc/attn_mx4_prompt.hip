@@ -745,22 +745,32 @@ constexpr int kCus = 256, kMaxSplits = 16;
 int64_t tiles_of(bool starts, int64_t batch, int64_t rows, int64_t group, int tile_rows) {
     return starts ? rows * group / tile_rows + std::min(batch, rows) : batch * ((group + tile_rows - 1) / tile_rows);
 }
-int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
+int g_tile = 0;  // 0 automatic, 32 or 128 pairs (where there are such tiles)
 
-// Whether tiles of 128 pairs, whose waves share V, are many enough to fill the device.
-bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
-    if (g_tile) return head_dim < 512 && g_tile == 128;
-    return head_dim < 512 && tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= 2 * kCus;
+// Whether a call takes tiles of 128 pairs, whose waves share V's way into LDS, or of
+// 32, whose waves take every fourth block.  The large ones need many tiles to fill
+// the device (two a CU).  At head_dim 256 with f32 in or out their kernel spills
+// (1500 rows after 2000 of 8 sequences: 468 us against 366 in tiles of 32) and there is none;
+// with f16 in and out it is ahead (304 against 321), and so it is at 160 (f32 913
+// against 1106, f16 766 against 983).
+bool shared(int64_t head_dim, bool full, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    if (head_dim == 512 || (head_dim == 256 && full)) return false;
+    if (g_tile) return g_tile == 128;
+    return tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= 2 * kCus;
 }
-int64_t splits_of(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
-    const int tile = shared(head_dim, starts, batch, rows, num_heads, kv_heads) ? 128 : 32;
-    const int64_t wgs = std::max<int64_t>(1, tiles_of(starts, batch, rows, num_heads / kv_heads, tile) * kv_heads);
+int64_t splits_of(bool share, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    const int64_t wgs =
+        std::max<int64_t>(1, tiles_of(starts, batch, rows, num_heads / kv_heads, share ? 128 : 32) * kv_heads);
     return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kCus / wgs));
 }
+// (larger tiles make the splits more, never fewer: enough for any types)
 int64_t workspace_of(int64_t head_dim, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
-    int64_t splits = splits_of(head_dim, true, batch, rows, num_heads, kv_heads);
-    if (rows == batch) splits = std::max(splits, splits_of(head_dim, false, batch, rows, num_heads, kv_heads));
-    return splits == 1 ? 16 : splits * rows * num_heads * (head_dim + 2) * 4;
+    auto splits = [&](bool starts) {
+        return splits_of(shared(head_dim, false, starts, batch, rows, num_heads, kv_heads), starts, batch, rows, num_heads,
+                         kv_heads);
+    };
+    const int64_t most = rows == batch ? std::max(splits(true), splits(false)) : splits(true);
+    return most == 1 ? 16 : most * rows * num_heads * (head_dim + 2) * 4;
 }
 
 template <int D, int TEAM, int ND, bool FULL>
@@ -782,8 +792,11 @@ int launch(const PromptArgs &a, hipStream_t st) {
 template <int D>
 int launch_d(PromptArgs &a, bool share, hipStream_t st) {
     const bool full = !(a.q_f16 && a.out_f16);
+    if constexpr (D < 256) {
+        if (share && full) return launch<D, 4, 5, true>(a, st);
+    }
     if constexpr (D < 512) {
-        if (share) return full ? launch<D, 4, 5, true>(a, st) : launch<D, 4, 4, false>(a, st);
+        if (share) return launch<D, 4, 4, false>(a, st);
     }
     return full ? launch<D, 1, 5, true>(a, st) : launch<D, 1, 4, false>(a, st);
 }
@@ -835,7 +848,8 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
     const int64_t need = workspace_of(d, a.c.batch, rows, num_heads, a.c.kv_heads);
     DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
                 "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
-    const bool starts = row_starts != nullptr, share = shared(d, starts, a.c.batch, rows, num_heads, a.c.kv_heads);
+    const bool starts = row_starts != nullptr,
+               share = shared(d, !(q_f16 && out_f16), starts, a.c.batch, rows, num_heads, a.c.kv_heads);
     const int64_t tiles = tiles_of(starts, a.c.batch, rows, num_heads / a.c.kv_heads, share ? 128 : 32);
     DOE_REQUIRE(tiles * a.c.kv_heads < ((int64_t)1 << 31), DOE_E_UNSUPPORTED, "too many rows");
     if ((rc = doe::require_init())) return rc;
@@ -857,7 +871,7 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
     // no more splits than there are steps of eight blocks to share out
     int64_t blocks = ((int64_t)a.c.table_stride << a.c.page_shift) / 32;
     if (a.window > 0) blocks = std::min<int64_t>(blocks, (a.window + rows) / 32 + 2);
-    a.splits = (int)std::max<int64_t>(1, std::min(splits_of(d, starts, a.c.batch, rows, num_heads, a.c.kv_heads), blocks / 8));
+    a.splits = (int)std::max<int64_t>(1, std::min(splits_of(share, starts, a.c.batch, rows, num_heads, a.c.kv_heads), blocks / 8));
     a.part = static_cast<float *>(workspace);
     const hipStream_t st = (hipStream_t)stream;
     switch (d) {
