@@ -722,8 +722,6 @@ int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, vo
     const int64_t need = workspace_of(cache->head_dim);
     DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
                 "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
-    if ((rc = doe::require_init())) return rc;
-    if (a.c.batch == 0) return DOE_OK;
     a.q = q;
     a.out = out;
     a.q_f16 = q_f16 != 0;
@@ -736,6 +734,10 @@ int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, vo
     a.window = (int)sliding_window;
     a.scale = scale;
     a.softcap = softcap;
+    DOE_REQUIRE((int64_t)a.c.batch * a.c.kv_heads * a.groups < ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "batch %d of %d KV heads",
+                a.c.batch, a.c.kv_heads);  // (a workgroup each: a launch has fewer than 2^32 threads)
+    if ((rc = doe::require_init())) return rc;
+    if (a.c.batch == 0) return DOE_OK;
     switch (cache->head_dim) {
         case 64: return launch<64>(a, workspace, (hipStream_t)stream);
         case 128: return launch<128>(a, workspace, (hipStream_t)stream);

@@ -851,7 +851,8 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
     const bool starts = row_starts != nullptr,
                share = shared(d, !(q_f16 && out_f16), starts, a.c.batch, rows, num_heads, a.c.kv_heads);
     const int64_t tiles = tiles_of(starts, a.c.batch, rows, num_heads / a.c.kv_heads, share ? 128 : 32);
-    DOE_REQUIRE(tiles * a.c.kv_heads < ((int64_t)1 << 31), DOE_E_UNSUPPORTED, "too many rows");
+    DOE_REQUIRE(tiles * a.c.kv_heads < ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %lld heads in one call",
+                (long long)rows, (long long)num_heads);  // (a launch has fewer than 2^32 threads)
     if ((rc = doe::require_init())) return rc;
     if (rows == 0 || a.c.batch == 0) return DOE_OK;
     a.q = q;

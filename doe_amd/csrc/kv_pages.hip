@@ -243,9 +243,8 @@ __global__ __launch_bounds__(256) void pages_free_kernel(PageArgs a) {
         if (threadIdx.x == 0) *a.status = bad ? -1 : 0;
     }
     __syncthreads();
-    const int len = len_;
-    if (len <= 0) return;
-    const int held = min((int64_t)pages_of(a, len), (int64_t)a.table_stride);
+    if (len_ <= 0) return;
+    const int held = pages_of(a, (int)min((int64_t)len_, (int64_t)a.table_stride * a.page_size));
     for (int col = threadIdx.x; col < a.table_stride; col += 256) {
         int32_t *e = &a.table[(int64_t)s * a.table_stride + col];
         if (col < held && *e >= 0 && *e < a.num_pages) atomicSub(&a.refs[*e], 1);
@@ -256,15 +255,14 @@ __global__ __launch_bounds__(256) void pages_free_kernel(PageArgs a) {
 __global__ __launch_bounds__(kPlan) void pages_compact_plan_kernel(PageArgs a) {
     __shared__ int wave_sums[kPlan / 64];
     int mine = 0, total;
-    for (int p = threadIdx.x; p < a.num_pages; p += kPlan) mine += a.refs[p] > 0;
+    for (int p = threadIdx.x; p < a.num_pages; p += kPlan) mine += a.refs[p] != 0;
     scan(mine, wave_sums, total);
     const int live = total;
-    const int low = take_free(a, live, wave_sums);  // free pages in order: those below `live` take the pages above it
-    (void)low;
+    take_free(a, live, wave_sums);  // in order: those below `live` take the pages above it, as many
     int moved = 0;
     for (int p0 = 0; p0 < a.num_pages; p0 += kPlan) {
         const int p = p0 + (int)threadIdx.x;
-        const bool high = p < a.num_pages && p >= live && a.refs[p] > 0;
+        const bool high = p < a.num_pages && p >= live && a.refs[p] != 0;
         const int at = moved + scan(high, wave_sums, total) - 1;
         if (p < a.num_pages) a.by_page[p] = high ? a.taken[at] : p;
         if (high) {
@@ -325,7 +323,7 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(PageArgs a) { copy_page
 int workspace_ints(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *ints) {
     DOE_REQUIRE(num_pages > 0 && num_pages < ((int64_t)1 << 30), DOE_E_INVALID, "num_pages %lld", (long long)num_pages);
     DOE_REQUIRE(max_seqs >= 0 && max_seqs <= ((int64_t)1 << 24), DOE_E_INVALID, "max_seqs %lld", (long long)max_seqs);
-    DOE_REQUIRE(n >= 0 && n <= ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
+    DOE_REQUIRE(n >= 0 && n < ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
     *ints = 16 + 3 * num_pages + max_seqs + 3 * n;
     return DOE_OK;
 }
@@ -352,6 +350,7 @@ int pool_checks(const PageArgs &a) {
     DOE_REQUIRE(a.pools, DOE_E_INVALID, "null pools");
     DOE_REQUIRE(a.page_bytes > 0 && a.page_bytes % 16 == 0 && a.layer_stride % 16 == 0 && ((uintptr_t)a.pools & 15) == 0,
                 DOE_E_INVALID, "pools, page_bytes and layer_stride must be multiples of 16");
+    DOE_REQUIRE(a.page_bytes < ((int64_t)1 << 32), DOE_E_INVALID, "page_bytes %lld", (long long)a.page_bytes);
     DOE_REQUIRE(a.layer_stride >= a.num_pages * a.page_bytes, DOE_E_INVALID, "layer_stride %lld below %d pages of %lld bytes",
                 (long long)a.layer_stride, a.num_pages, (long long)a.page_bytes);
     return DOE_OK;
@@ -360,7 +359,7 @@ int pool_checks(const PageArgs &a) {
 int page_args(PageArgs &a, const doe_kv_pages *p, const int32_t *first, const int32_t *second, int64_t n, bool lists,
               int32_t *status) {
     DOE_REQUIRE(p && p->page_table && p->kv_lens && p->page_refs && status, DOE_E_INVALID, "null pointer");
-    DOE_REQUIRE(n >= 0 && n <= ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
+    DOE_REQUIRE(n >= 0 && n < ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
     DOE_REQUIRE(n == 0 || !lists || first, DOE_E_INVALID, "null list");
     DOE_REQUIRE(p->max_seqs > 0 && p->max_seqs <= ((int64_t)1 << 24), DOE_E_INVALID, "max_seqs %lld", (long long)p->max_seqs);
     DOE_REQUIRE(p->num_pages > 0 && p->num_pages < ((int64_t)1 << 30), DOE_E_INVALID, "num_pages %lld", (long long)p->num_pages);
@@ -389,7 +388,7 @@ int page_args(PageArgs &a, const doe_kv_pages *p, const int32_t *first, const in
 
 // Workgroups of a wide kernel: one for each 16 KB piece and 256 entries, at most eight a CU.
 unsigned wide_grid(const PageArgs &a, int64_t copies, int64_t entries) {
-    const int64_t pieces = a.layers > 0 ? copies * a.layers * ((a.page_bytes + 16383) / 16384) : 0;
+    const int64_t pieces = a.layers > 0 ? std::min<int64_t>(copies * a.layers, 2048) * ((a.page_bytes + 16383) / 16384) : 0;
     const int64_t want = std::max(pieces, (entries + 255) / 256);
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(want, 2048));
 }
@@ -470,7 +469,7 @@ int doe_kv_pages_copy(void *pools, int64_t layers, int64_t layer_stride, int64_t
                       const int32_t *sources, const int32_t *destinations, int64_t n, int32_t *status, void *workspace,
                       int64_t workspace_bytes, doe_stream_t stream) {
     DOE_REQUIRE(status, DOE_E_INVALID, "null pointer");
-    DOE_REQUIRE(n >= 0 && n <= ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
+    DOE_REQUIRE(n >= 0 && n < ((int64_t)1 << 24), DOE_E_INVALID, "n %lld", (long long)n);
     DOE_REQUIRE(n == 0 || (sources && destinations), DOE_E_INVALID, "null list");
     DOE_REQUIRE(num_pages > 0 && num_pages < ((int64_t)1 << 30), DOE_E_INVALID, "num_pages %lld", (long long)num_pages);
     PageArgs a{};

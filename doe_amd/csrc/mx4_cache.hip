@@ -347,6 +347,10 @@ int row_checks(const Mx4View &c, int64_t head_dim, int64_t rows, int64_t row_str
     DOE_REQUIRE(row_stride >= c.kv_heads * head_dim && row_stride * size % 16 == 0, DOE_E_INVALID,
                 "row stride %lld below a row of %lld, or not a multiple of 16 bytes", (long long)row_stride,
                 (long long)(c.kv_heads * head_dim));
+    // (a launch has fewer than 2^32 threads; without row_starts a unit a sequence)
+    DOE_REQUIRE((row_starts ? rows / 4 + 2 * (int64_t)c.batch : rows) * c.kv_heads * (head_dim == 160 ? 64 : head_dim / 4) <
+                    ((int64_t)1 << 32) - 256,
+                DOE_E_UNSUPPORTED, "%lld rows and %d sequences of %d heads", (long long)rows, c.batch, c.kv_heads);
     DOE_REQUIRE(rows == 0 || (k && v), DOE_E_INVALID, "null pointer");
     DOE_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0, DOE_E_INVALID, "k and v must be 16-byte aligned");
     return DOE_OK;
@@ -392,7 +396,8 @@ int mx4_view(const doe_mx4_cache *cache, Mx4View *view) {
                 (long long)c.page_size);
     DOE_REQUIRE(c.num_kv_heads > 0 && c.num_kv_heads <= 1024, DOE_E_INVALID, "num_kv_heads %lld outside 1..1024",
                 (long long)c.num_kv_heads);
-    DOE_REQUIRE(c.num_pages > 0 && c.num_pages < ((int64_t)1 << 31), DOE_E_INVALID, "num_pages %lld", (long long)c.num_pages);
+    DOE_REQUIRE(c.num_pages > 0 && c.num_pages < ((int64_t)1 << 31) && c.num_pages * c.num_kv_heads < ((int64_t)1 << 31),
+                DOE_E_INVALID, "num_pages %lld of %lld heads", (long long)c.num_pages, (long long)c.num_kv_heads);
     DOE_REQUIRE(c.batch >= 0 && c.batch <= 65535, DOE_E_INVALID, "batch %lld outside 0..65535", (long long)c.batch);
     DOE_REQUIRE(c.table_stride > 0 && c.table_stride * c.page_size < ((int64_t)1 << 30), DOE_E_INVALID,
                 "table_stride %lld: a sequence holds fewer than 2^30 positions", (long long)c.table_stride);
@@ -415,6 +420,8 @@ int mx4_attention_checks(const Mx4View &c, int64_t num_heads, float scale, float
                 "num_heads %lld is not a positive multiple of num_kv_heads %d", (long long)num_heads, c.kv_heads);
     DOE_REQUIRE(isfinite(scale) && isfinite(softcap) && softcap >= 0.0f, DOE_E_INVALID, "scale %g, softcap %g", (double)scale,
                 (double)softcap);
+    DOE_REQUIRE(softcap == 0.0f || isfinite(scale / softcap), DOE_E_INVALID, "softcap %g too small for scale %g",
+                (double)softcap, (double)scale);
     DOE_REQUIRE(sliding_window >= 0 && sliding_window < ((int64_t)1 << 30), DOE_E_INVALID, "sliding_window %lld",
                 (long long)sliding_window);
     DOE_REQUIRE(c.batch == 0 || (q && out), DOE_E_INVALID, "null pointer");

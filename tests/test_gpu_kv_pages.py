@@ -210,6 +210,24 @@ def test_bookkeeping_without_pools(dev):
     h.same()
 
 
+def test_free_and_compact_of_a_damaged_state(dev):
+    """A length beyond the table row counts as what the row holds; a page with a
+    count below 0 is in use for all that moves."""
+    rng = np.random.default_rng(8)
+    h = Host(rng, 3, 4, 20, 16, [64, 30, 0])
+    h.dev[1].upload(i32([2**31 - 1, 30, 0]).view(np.uint8))
+    ops.kv_pages_free(h.pages, up(i32([0])), 1, status=h.status)
+    h.free([0])
+    h.same()
+    h.refs[h.table[1, :2]] = -3
+    h.dev[2].upload(h.refs.view(np.uint8))
+    h.refs = np.abs(h.refs)
+    ops.kv_pages_compact(h.pages, status=h.status, workspace=h.ws)
+    h.compact()
+    h.refs = -h.refs
+    h.same()
+
+
 def test_copy(dev):
     rng = np.random.default_rng(6)
     h = Host(rng, 1, 1, 50, 16, layers=3, page_bytes=16400, extra=48)

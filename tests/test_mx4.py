@@ -152,10 +152,12 @@ def test_cache_calls_refuse_bad_arguments():
         refused("aligned", call, c, FakeBuf(1 << 30, 8), BIG, 3)
         refused("null", call, c, BIG, FakeBuf(1 << 30, 0), 3)
         refused("rows", call, c, BIG, BIG, -1, row_starts=BIG)
+        refused("2147483647 rows", call, c, BIG, BIG, (1 << 31) - 1, row_starts=BIG)
     refused("row stride", ops.mx4_kv_write, c, BIG, BIG, 3, row_stride=260, in_f16=True)
     refused("pool", ops.mx4_kv_write, cache(FakeBuf(1 << 40, 24)), BIG, BIG, 3)
     for bad, match in ((dict(num_pages=0), "num_pages"), (dict(batch=70000), "batch"), (dict(table_stride=0), "table_stride"),
-                       (dict(table_stride=1 << 24), "positions"), (dict(num_kv_heads=2000), "num_kv_heads")):
+                       (dict(table_stride=1 << 24), "positions"), (dict(num_kv_heads=2000), "num_kv_heads"),
+                       (dict(num_pages=1 << 30), "num_pages")):
         c2 = cache(**bad)
         refused(match, ops.mx4_kv_write, c2, BIG, BIG, c2.batch)
 
@@ -170,6 +172,7 @@ def test_attention_calls_refuse_bad_arguments():
     for bad, match in ((dict(num_heads=7), "multiple"), (dict(num_heads=0), "multiple"), (dict(sliding_window=-1), "window"),
                        (dict(sliding_window=1 << 40), "window"), (dict(softcap=-1.0), "softcap"),
                        (dict(softcap=float("nan")), "softcap"), (dict(scale=float("inf")), "scale"),
+                       (dict(scale=1e30, softcap=1e-10), "softcap"),
                        (dict(workspace=FakeBuf(8)), "workspace"), (dict(workspace=FakeBuf(1 << 40, 4)), "workspace")):
         refused(match, ops.attention_mx4, c, BIG, BIG, **{**token, **bad})
         refused(match, ops.attention_mx4_prompt, c, BIG, BIG, 500, row_starts=BIG, **{**token, **bad})
@@ -180,10 +183,31 @@ def test_attention_calls_refuse_bad_arguments():
     refused("strides", ops.attention_mx4_prompt, c, BIG, BIG, 5, row_starts=BIG, q_row_stride=1023, **token)
     refused("strides", ops.attention_mx4_prompt, c, BIG, BIG, 5, row_starts=BIG, out_row_stride=1026, **token)
     refused("rows", ops.attention_mx4_prompt, c, BIG, BIG, 1 << 40, row_starts=BIG, **token)
+    many = cache(batch=65535, num_kv_heads=512)
+    refused("KV heads", ops.attention_mx4, many, BIG, BIG, **{**token, "num_heads": 512})
+    refused("in one call", ops.attention_mx4_prompt, many, BIG, BIG, 65535, **{**token, "num_heads": 512})
     for f in (lambda: ops.attention_mx4_workspace(3, 7, 2, 128), lambda: ops.attention_mx4_workspace(3, 8, 2, 96),
               lambda: ops.attention_mx4_workspace(-1, 8, 2, 128), lambda: ops.attention_mx4_workspace(3, 8, 2, 128, -1)):
         with pytest.raises(DoeError):
             f()
+
+
+def test_tile_setting():
+    try:
+        for v in (32, 128, 0):
+            ops.tune("attn_mx4.tile", v)
+        for v in (-1, 1, 64, 256):
+            refused("attn_mx4.tile", ops.tune, "attn_mx4.tile", v)
+    finally:
+        ops.tune("attn_mx4.tile", 0)
+
+
+def test_prompt_workspace_grows_with_the_splits_only():
+    # (row, head) pairs times splits; many rows need none
+    assert ops.attention_mx4_workspace(1, 8, 2, 128, 1 << 20) == 16
+    one = ops.attention_mx4_workspace(1, 8, 2, 128, 17)
+    assert one > 16 and one % (17 * 8 * 130 * 4) == 0
+    assert ops.attention_mx4_workspace(1, 8, 2, 128, 0) >= 0
 
 
 def pages(**change):
@@ -206,11 +230,12 @@ def test_page_calls_refuse_bad_arguments():
         refused("workspace", call, p, BIG, BIG, 4, status=BIG, workspace=FakeBuf(100))
         refused("workspace", call, p, BIG, BIG, 4, status=BIG, workspace=FakeBuf(1 << 30, 8))
         refused("n -1", call, p, BIG, BIG, -1, **how)
+        refused("n 16777216", call, p, BIG, BIG, 1 << 24, **how)
         refused("null", call, p, BIG, BIG, 4, status=FakeBuf(4, 0), workspace=BIG)
         refused("null list", call, p, FakeBuf(16, 0), BIG, 4, **how)
         refused("null list", call, p, BIG, FakeBuf(16, 0), 4, **how)
     refused("null list", ops.kv_pages_free, p, FakeBuf(16, 0), 4, status=BIG)
-    for bad, match in ((dict(page_bytes=4100), "multiples of 16"), (dict(layer_stride=4096), "layer_stride"),
+    for bad, match in ((dict(page_bytes=4100), "multiples of 16"), (dict(page_bytes=1 << 32), "page_bytes"), (dict(layer_stride=4096), "layer_stride"),
                        (dict(pools=FakeBuf(1 << 40, 8)), "multiples of 16")):
         refused(match, ops.kv_pages_compact, pages(**bad), **how)
         refused(match, ops.kv_pages_fork, pages(**bad), BIG, BIG, 4, **how)
