@@ -125,6 +125,28 @@ def test_write_prompts(dev, d, h, ps, pad):
         assert np.array_equal(o, e, equal_nan=True)
 
 
+@pytest.mark.parametrize("d,h,ps", [(64, 1, 32), (128, 3, 64), (160, 1, 32), (512, 2, 128)])
+def test_write_many_short_prompts(dev, d, h, ps):
+    """More sequences than a wave has lanes, of no rows to a few, at any place in a four."""
+    rng = np.random.default_rng(d)
+    rows = rng.integers(0, 10, 150).tolist()
+    lens = [int(n + rng.integers(-2, 40)) if n else 7 for n in rows]
+    p = Pool(rng, lens, d, h, ps)
+    total = sum(rows)
+    starts = up(np.cumsum([0] + rows).astype(np.int32))
+    k, v = special(rng, (total, h, d)), special(rng, (total, h, d))
+    ops.mx4_kv_write(p.cache, up(k), up(v), total, row_starts=starts)
+    want, back = p.expect(k, v, rows)
+    assert np.array_equal(p.dev.download(), want)
+    out = [up(np.full(k.shape, -5, np.float32)) for _ in "kv"]
+    ops.mx4_kv_read(p.cache, *out, total, row_starts=starts)
+    out = [o.download() for o in out]
+    assert sorted(back) == list(range(total))
+    for i, b in back.items():
+        for o, x in zip(out, b):
+            assert np.array_equal(o[i], np.broadcast_to(x, o[i].shape), equal_nan=True)
+
+
 def test_every_border_and_scale(dev):
     """Values next to every rounding border, under every scale."""
     near = []
