@@ -69,7 +69,7 @@ struct Shape {
     static constexpr int kMerge = TEAM == 4 || D == 512 ? 0 : kWaves * 32 * D * 4;  // the waves' O at the end
     static constexpr int kScores = D == 512 ? kWaves * 32 * 32 * 4 : 0;
     static constexpr int kData = kBuffers * kV > kMerge ? kBuffers * kV : kMerge;
-    static constexpr int kLds = kData + kScores + 1024;
+    static constexpr int kLds = kData + kScores + (D == 512 ? 0 : 1024);  // (512: half a CU's, to the byte)
 };
 
 template <int BYTE>
@@ -321,7 +321,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // FULL: P as f16 hi + lo.
 template <int D, int TEAM, int ND, bool FULL>
-__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D <= 128 || D == 512 ? 2 : 1) void attn_mx4_prompt_kernel(PromptArgs a) {
     using P = Shape<D, TEAM>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool kShare = TEAM == 4;                 // the waves share V
@@ -477,6 +477,12 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
     load_k<D, TEAM>(kb, slab_at(slab1), shift, place(1), lane, slice);
     if (kShare) __syncthreads();
 
+    // O stays in the accumulation registers between the matrix instructions where it
+    // takes many (the compiler would move it out at every block for the rare rescaling)
+    auto keep = [&](f32x16 &v) __attribute__((always_inline)) {
+        if constexpr (P::kTiles > 4) __asm__ volatile("" : "+a"(v));
+    };
+
     // Block i: its weights beside the next one's scores, its P V beside the next V's
     // way into LDS (of a step's next V a quarter at each of its four blocks).
     auto block = [&](int i, auto u_) __attribute__((always_inline)) {
@@ -551,10 +557,15 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
             const float corr = ref == m ? 1.0f : __builtin_amdgcn_exp2f(m - ref);
             m = ref;
             l *= corr;
+            if (i > 0) {  // (O is 0 before)
 #pragma unroll
-            for (int t = 0; t < P::kTiles; ++t)
+                for (int t = 0; t < P::kTiles; ++t) {
+                    keep(o[t]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[t][r] *= corr;
+                    for (int r = 0; r < 16; ++r) o[t][r] *= corr;
+                    keep(o[t]);
+                }
+            }
             logs(ref);
             if (!whole) mask();
         }
@@ -607,13 +618,16 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void attn_mx4_prompt
                     if (slab[Mx4Slab<D>::v_scale(shift, place(i) + x, g)] != doe::kMx4NanScale) continue;
                     const float bad = p0 + x >= lo && p0 + x < top_ ? NAN : 0.0f;
 #pragma unroll
-                    for (int t = 0; t < P::kTiles; ++t)
+                    for (int t = 0; t < P::kTiles; ++t) {
+                        keep(o[t]);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int w = 8 * (r >> 2) + 4 * lh + (r & 3);
                             const int dim = (w & 15) * (D / 16) + slice * (P::kDims / 16) + 2 * t + (w >> 4);
                             o[t][r] += dim / 32 == g ? bad : 0.0f;
                         }
+                        keep(o[t]);
+                    }
                 }
         }
         s = next;
@@ -745,29 +759,28 @@ constexpr int kCus = 256, kMaxSplits = 16;
 int64_t tiles_of(bool starts, int64_t batch, int64_t rows, int64_t group, int tile_rows) {
     return starts ? rows * group / tile_rows + std::min(batch, rows) : batch * ((group + tile_rows - 1) / tile_rows);
 }
-int g_tile = 0;  // 0 automatic, 32 or 128 pairs (where there are such tiles)
+int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
 
 // Whether a call takes tiles of 128 pairs, whose waves share V's way into LDS, or of
-// 32, whose waves take every fourth block.  The large ones need many tiles to fill
-// the device (two a CU).  At head_dim 256 with f32 in or out their kernel spills
-// (1500 rows after 2000 of 8 sequences: 468 us against 366 in tiles of 32) and there is none;
-// with f16 in and out it is ahead (304 against 321), and so it is at 160 (f32 913
-// against 1106, f16 766 against 983).
-bool shared(int64_t head_dim, bool full, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
-    if (head_dim == 512 || (head_dim == 256 && full)) return false;
+// 32, whose waves take every fourth block.  The large ones need as many tiles as the
+// device holds workgroups (a CU two up to head_dim 128, else one).  1500 rows after
+// 2000 of 8 sequences, 32 against 128, f32 and f16: head_dim 64 181 / 165 and 129 /
+// 117 us, 128 258 / 234 and 202 / 159, 160 1010 / 799 and 907 / 619, 256 316 / 300
+// and 285 / 231; one prompt of 1000 rows (fewer tiles): 16 / 28, 21 / 36 and 28 / 44
+// at 64, 128 and 256, but 67 / 60 and 59 / 47 at 160, where 16 KV heads make 256 tiles.
+bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
+    if (head_dim == 512) return false;
     if (g_tile) return g_tile == 128;
-    return tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= 2 * kCus;
+    return tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= (head_dim <= 128 ? 2 : 1) * kCus;
 }
 int64_t splits_of(bool share, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     const int64_t wgs =
         std::max<int64_t>(1, tiles_of(starts, batch, rows, num_heads / kv_heads, share ? 128 : 32) * kv_heads);
     return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, kCus / wgs));
 }
-// (larger tiles make the splits more, never fewer: enough for any types)
 int64_t workspace_of(int64_t head_dim, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     auto splits = [&](bool starts) {
-        return splits_of(shared(head_dim, false, starts, batch, rows, num_heads, kv_heads), starts, batch, rows, num_heads,
-                         kv_heads);
+        return splits_of(shared(head_dim, starts, batch, rows, num_heads, kv_heads), starts, batch, rows, num_heads, kv_heads);
     };
     const int64_t most = rows == batch ? std::max(splits(true), splits(false)) : splits(true);
     return most == 1 ? 16 : most * rows * num_heads * (head_dim + 2) * 4;
@@ -792,11 +805,8 @@ int launch(const PromptArgs &a, hipStream_t st) {
 template <int D>
 int launch_d(PromptArgs &a, bool share, hipStream_t st) {
     const bool full = !(a.q_f16 && a.out_f16);
-    if constexpr (D < 256) {
-        if (share && full) return launch<D, 4, 5, true>(a, st);
-    }
     if constexpr (D < 512) {
-        if (share) return launch<D, 4, 4, false>(a, st);
+        if (share) return full ? launch<D, 4, 5, true>(a, st) : launch<D, 4, 4, false>(a, st);
     }
     return full ? launch<D, 1, 5, true>(a, st) : launch<D, 1, 4, false>(a, st);
 }
@@ -848,8 +858,7 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
     const int64_t need = workspace_of(d, a.c.batch, rows, num_heads, a.c.kv_heads);
     DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need, DOE_E_INVALID,
                 "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)need, (long long)workspace_bytes);
-    const bool starts = row_starts != nullptr,
-               share = shared(d, !(q_f16 && out_f16), starts, a.c.batch, rows, num_heads, a.c.kv_heads);
+    const bool starts = row_starts != nullptr, share = shared(d, starts, a.c.batch, rows, num_heads, a.c.kv_heads);
     const int64_t tiles = tiles_of(starts, a.c.batch, rows, num_heads / a.c.kv_heads, share ? 128 : 32);
     DOE_REQUIRE(tiles * a.c.kv_heads < ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %lld heads in one call",
                 (long long)rows, (long long)num_heads);  // (a launch has fewer than 2^32 threads)
