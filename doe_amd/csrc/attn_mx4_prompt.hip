@@ -43,6 +43,10 @@ typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
 constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P of the running max, and how far that may lag
 constexpr int kWaves = 4;
+// Workgroups that a CU holds, by their registers (at 512 by LDS as well).  64: three
+// cost seven spilled registers at most and win (12 ragged prompts of up to 777 rows, a window,
+// capped scores: 49.6 to 41.3 us); 512: 648 us for 1050 with one.
+constexpr int per_cu(int head_dim) { return head_dim == 64 ? 3 : (head_dim == 128 || head_dim == 512 ? 2 : 1); }
 
 struct PromptArgs {
     Mx4View c;
@@ -321,7 +325,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // FULL: P as f16 hi + lo.
 template <int D, int TEAM, int ND, bool FULL>
-__global__ __launch_bounds__(64 * kWaves, D <= 128 || D == 512 ? 2 : 1) void attn_mx4_prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel(PromptArgs a) {
     using P = Shape<D, TEAM>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool kShare = TEAM == 4;                 // the waves share V
@@ -763,15 +767,14 @@ int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
 
 // Whether a call takes tiles of 128 pairs, whose waves share V's way into LDS, or of
 // 32, whose waves take every fourth block.  The large ones need as many tiles as the
-// device holds workgroups (a CU two up to head_dim 128, else one).  1500 rows after
-// 2000 of 8 sequences, 32 against 128, f32 and f16: head_dim 64 181 / 165 and 129 /
-// 117 us, 128 258 / 234 and 202 / 159, 160 1010 / 799 and 907 / 619, 256 316 / 300
+// device holds workgroups.  1500 rows after 2000 of 8 sequences, 32 against 128, f32
+// and f16: head_dim 64 163 / 157 and 131 / 117 us, 128 258 / 234 and 202 / 159, 160 1010 / 799 and 907 / 619, 256 316 / 300
 // and 285 / 231; one prompt of 1000 rows (fewer tiles): 16 / 28, 21 / 36 and 28 / 44
 // at 64, 128 and 256, but 67 / 60 and 59 / 47 at 160, where 16 KV heads make 256 tiles.
 bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     if (head_dim == 512) return false;
     if (g_tile) return g_tile == 128;
-    return tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= (head_dim <= 128 ? 2 : 1) * kCus;
+    return tiles_of(starts, batch, rows, num_heads / kv_heads, 128) * kv_heads >= per_cu((int)head_dim) * kCus;
 }
 int64_t splits_of(bool share, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     const int64_t wgs =
