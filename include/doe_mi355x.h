@@ -552,11 +552,15 @@ int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, vo
 /* The prompt form: rows of q and out as in doe_mx4_kv_write (row_starts,
  * rows; q_row_stride and out_row_stride elements apart), row i of the n of a
  * sequence at position kv_lens[b] - n + i, causal.  Rows of no sequence are
- * left as they were; a row at a position below 0 gives zeros.  f32 queries are
- * carried as f16 hi + lo and probabilities as f16 hi + lo (2-4e-7 from
- * float64); with q_f16 and out_f16 the probabilities are f16 (below the
- * output's own rounding).  A short prompt over a long cache splits its keys
- * over the device and joins them through the workspace. */
+ * left as they were; a row at a position below 0 gives zeros.  Scores are
+ * products of the cache's codes as they stand and digits of the queries: 25
+ * bits of the largest value of every 32 dims, 20 with q_f16 and out_f16 (a dim
+ * 2^n below that keeps n fewer); probabilities are f16 hi + lo, with q_f16 and
+ * out_f16 one f16.  2-4e-7 from float64 with normal queries, 1.5e-5 with single
+ * dims 2^11 above the others where the keys are zero; with f16 both ways 3e-4
+ * (the output's rounding 2e-4 of it), 5e-4.  A short
+ * prompt over a long cache splits its keys over the device and joins them
+ * through the workspace. */
 int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
                                   int64_t head_dim, int64_t *bytes);
 int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,
@@ -810,8 +814,8 @@ int doe_decode_advance(int32_t *state, int32_t *token, int32_t *ids, int64_t max
  * ranges grouped on one XCD), "q8_0_gemv.rows" (1, 2 or 4 rows per wave group), "q8_0_gemv.depth" (1 or
  * 2 blocks loaded ahead), "attn_mq.splits" (1..16 key splits of the
  * multi-query attention), "attn_mx4.tile" (32 or 128 (row, head) pairs a tile
- * of the 4-bit cache's prompt attention; a workspace has to be asked for under
- * the same setting), "attn_mq.queries" (16: its 16-query form, with P in
+ * of the 4-bit cache's prompt attention, up to head_dim 256; a workspace has to
+ * be asked for under the same setting), "attn_mq.queries" (16: its 16-query form, with P in
  * one f16, at any head_dim), "attn_decode.splits",
  * "attn_decode.waves" (4: narrow workgroups; 8 or 16: the wide short-context
  * workgroup where the head shape allows it), "attn_decode.combine" (1: the

@@ -4,10 +4,14 @@ The pages are made on the host (doe_amd.mx4), the reference works on the values
 they stand for.  ``bound`` is how far a result may be, element by element:
 probabilities carry a relative error of at most 2 ds (numerator and sum), ds
 the error of a score, and every output rounding half a step.  ds: the query's
-f16 hi + lo parts leave 2^-22 of it, the D products of a score are summed in
+f16 hi + lo parts leave 2^-22 of it (prompts: `attention`'s `digits`), the D products of a score are summed in
 f32 in at most D / 16 + 8 steps of 2^-24 each and scaled once, softcap's tanh
 is good to 2^-21 of the cap; the exponential, its argument (up to 150, in
-steps of 2^-24 of itself) and the sums over positions add 2^-16 and 2^-18."""
+steps of 2^-24 of itself) and the sums over positions add 2^-16 and 2^-18.  A
+probability is held in f16 parts, where f16 has no steps below 2^-24: at most
+2^-25 is lost of each, the largest being 2^7 or more (it lies 2^7 above the
+running reference when that is raised, and the reference is only raised), so
+2^-32 of |v| summed over the positions whatever they weigh."""
 from __future__ import annotations
 
 import numpy as np
@@ -67,10 +71,11 @@ class Case:
         return k, v, has
 
 
-def attention(case, q, rows, scale, softcap=0.0, window=0):
+def attention(case, q, rows, scale, softcap=0.0, window=0, digits=None):
     """(out, bound, mass) [total rows][heads][D] in 64 bits: q the rows of
     sequence 0, 1, ..., rows[b] of them each, at its last positions; mass is
-    sum p |v|."""
+    sum p |v|.  `digits` (prompts whose dims differ widely): what the queries'
+    digits leave of the largest of each 32 dims, 2^-24 or 2^-19 of it."""
     q = np.asarray(q, np.float64)
     hq, g = q.shape[1], q.shape[1] // case.h
     out, bound, mass = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
@@ -92,13 +97,16 @@ def attention(case, q, rows, scale, softcap=0.0, window=0):
                 s = kk @ q[at + i, head] * scale
                 big = np.max(np.abs(kk) @ np.abs(q[at + i, head])) * abs(scale)
                 ds = big * (2.0 ** -22 + (case.d / 16 + 9) * 2.0 ** -24)
+                if digits:
+                    top = np.abs(q[at + i, head]).reshape(-1, 32).max(1)
+                    ds += digits * abs(scale) * np.max(np.abs(kk).reshape(len(kk), -1, 32).sum(2) @ top)
                 if softcap:
                     s = np.tanh(s / softcap) * softcap
                     ds += softcap * 2.0 ** -21
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 out[at + i, head], mass[at + i, head] = p @ vv, p @ np.abs(vv)
-                bound[at + i, head] = (2 * ds + 2.0 ** -16 + 2.0 ** -18) * mass[at + i, head]
+                bound[at + i, head] = (2 * ds + 2.0 ** -16 + 2.0 ** -18) * mass[at + i, head] + 2.0 ** -32 * np.abs(vv).sum(0)
         at += n
     return out, bound, mass
 

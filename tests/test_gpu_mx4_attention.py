@@ -290,6 +290,30 @@ def test_prompts_window_and_softcap(dev, tile, d, hq, hkv, window, softcap):
     check(got, want, bound, got.dtype)
 
 
+@pytest.mark.parametrize("d", [64, 160, 512])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("zero", [False, True])
+def test_queries_with_wide_dims(dev, tile, d, f16, zero):
+    """Dims of a query up to 2^11 times the others, scores in the thousands; or the
+    keys are zero there: the digits hold the others to a part of the largest, and
+    no worse."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [70, 40], head_dim=d, num_kv_heads=1, page_size=32)
+    wide = np.arange(0, d, 32) + 2 * rng.integers(0, 16, d // 32)
+    if zero:
+        case.kc[..., wide] = 0
+    case.upload()
+    q = rng.standard_normal((50, 3, d)).astype(np.float16 if f16 else np.float32)
+    q[..., wide] *= np.exp2(rng.integers(0, 12, q[..., wide].shape)).astype(q.dtype)
+    print(f"[wide] d={d} f16={f16}", flush=True)
+    got = prompt(case, q, [30, 20], f16=f16)
+    want, bound, mass = attention(case, q, [30, 20], d ** -0.5, digits=2.0 ** (-19 if f16 else -24))
+    check(got, want, bound, got.dtype, mass if f16 else None)
+    if not f16:  # tokens carry each dim with 22 bits of its own
+        got = token(case, q[:2])
+        check(got, *attention(case, q[:2], [1, 1], d ** -0.5)[:2], got.dtype)
+
+
 def test_a_prompt_row_equals_its_token(dev):
     """Rows of a prompt are what single tokens at the same lengths are."""
     rng = np.random.default_rng(13)
