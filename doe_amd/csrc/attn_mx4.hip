@@ -18,8 +18,14 @@
 //   * O^T = V^T P^T: the page layout gives a lane its eight positions x D / 16 dims
 //     in one piece; pairs of positions are brought together by v_perm.
 //   * The running max is raised only when a score exceeds it by 2^8, P lies
-//     2^7 above it, so that f16's small values lose nothing.
-// No wave waits for another until a row's end.
+//     2^7 above it, so that f16's small values lose no more than 2^-32 of the largest.
+// No wave waits for another until a row's end.  Bound by the cache's bytes where
+// there are many: 8 sequences of 32768, 64 / 8 heads of 128 dims (285 MB): 55.6 us with
+// the join, the rate of a large copy (5.1 TB/s).  Bound by two dependent launches and
+// a chain of cold reads (length, page table, K, then parts) where there are few: one
+// of 4096, 8 / 4 heads of 256: 10.5 us, 7.7 + 2.8 of them in the kernels.  A wave has
+// a block's K and V under way while it works on the one before, which asks for enough
+// waves more than for more blocks a wave: per_cu() is as many as the registers allow.
 #include "mx4_cache.h"
 
 #include <limits.h>
@@ -54,9 +60,10 @@ struct TokenArgs {
 constexpr int64_t kCacheBytes = (int64_t)256 << 20;
 
 // Workgroups of four waves that a CU holds at once, by the registers that a wave
-// takes, and those that fill the device's 256 CUs in one round.
+// takes, and those that fill the device's 256 CUs in one round (head_dim 128: four
+// leave a wave fewer registers, 56.6 us for 55.6 over 8 sequences of 32768).
 template <int D>
-constexpr int per_cu() { return D <= 128 ? 4 : (D <= 160 ? 3 : (D <= 256 ? 2 : 1)); }
+constexpr int per_cu() { return D <= 160 ? 3 : (D <= 256 ? 2 : 1); }
 template <int D>
 constexpr int workgroups() { return 256 * per_cu<D>(); }
 
@@ -592,8 +599,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
     }
 }
 
-// A split row's head: its parts, in the order of a fixed tree.  D / 4 lanes hold the dims, kJoin / (D / 4) groups take every
-// so manieth part and meet in LDS.
+// A split row's head: its parts, in the order of a fixed tree.  D / 4 lanes hold the
+// dims, kJoin / (D / 4) groups take every so manieth part and meet in LDS.  2.7 - 4.7
+// us: a dependent launch and two reads after one another, whatever the parts.
 constexpr int kJoin = 512;
 template <int D>
 __global__ __launch_bounds__(kJoin) void attn_mx4_join_kernel(TokenArgs a, int wgs) {
@@ -685,7 +693,9 @@ int launch(TokenArgs &a, void *ws, hipStream_t st) {
         a.part = static_cast<float *>(ws);
         a.joined = reinterpret_cast<int2 *>(a.part + wgs * kHeads * (D + 2));
     }
-    // A pool that the 256 MB last-level cache cannot hold is read past it.
+    // A pool that the 256 MB last-level cache cannot hold is read past it (8 sequences
+    // of 32768 in 302 MB: 55.6 us, through it 60.7; 48 ragged ones in 90 MB through it
+    // 23.6, past it 25.9).
     const bool stream = ((int64_t)a.c.num_pages * a.c.kv_heads * (D + D / 16) << a.c.page_shift) > kCacheBytes;
     const int rc = stream ? launch_token<D, true>(a, (unsigned)wgs, st) : launch_token<D, false>(a, (unsigned)wgs, st);
     if (rc) return rc;

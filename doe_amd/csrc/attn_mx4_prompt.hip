@@ -28,7 +28,7 @@
 // A block's steps overlap with its neighbours': its weights stand beside the next
 // one's scores, its P V beside the next V's way into LDS, so that the matrix and
 // vector units of a SIMD work at once with one or two waves on it.  2048 rows after
-// 30720 positions, 32 / 8 heads of 128 dims, f16: 315 us, 981 TFLOP/s of the 4 D
+// 8192 positions, 32 / 8 heads of 128 dims, f16: 315 us, 981 TFLOP/s of the 4 D
 // operations a pair and position, where a large f16 matrix product reaches 1139; the
 // matrix units are busy 43 % of the cycles, vector issue and the latency of a chain
 // of them by two waves the rest (without the exponentials it would be 3 % less,
