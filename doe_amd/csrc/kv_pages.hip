@@ -6,10 +6,10 @@
 // page_refs [num_pages], the number of sequences that hold a page (0: free).
 // What is copied is bound by its bytes: 96 last pages of 26 layers (290 MB read and
 // written, part of it from the last-level cache) 39 us, half of a pool (746 MB) 147 us,
-// the rate of a large copy.  A plan is one workgroup's chain of dependent reads: 6 - 7
-// us for 256 sequences of a pool of 40000 pages (entries and sums kept in registers
-// and LDS rather than read again made no difference).  Splitting it over workgroups
-// would take launches of 3 - 4 us each between its steps.
+// the rate of a large copy.  A plan is one workgroup's chain of dependent reads and of
+// its own code's lines, fetched as it runs: 5.1 us for 256 sequences of a pool of 40000
+// pages (7.3 with sums through memory, unrolled scans and the compiler's divisions).
+// Splitting it over workgroups would take launches of 3 - 4 us each between its steps.
 // A plan kernel of one workgroup checks the call as a whole, takes the lowest
 // free pages in the order of the call's entries and writes *status; the copies
 // and the long tables are a second, wide kernel that reads the plan.  A call
@@ -28,74 +28,92 @@ struct PageArgs {
     int32_t *table, *lens, *refs, *status;
     const int32_t *first, *second;  // the call's two lists (sequences, amounts; parents, children; sources, destinations)
     int n, max_seqs, table_stride, num_pages, page_size;
+    double page_inv;  // 1 / page_size
     // workspace: plan[0] pages to copy; by_seq [max_seqs] and by_page [num_pages]
     // hold the entry that names a sequence or page; need [n] running sums of pages;
     // taken [num_pages] free pages in order; pair [2 n or num_pages] copies
     int32_t *plan, *by_seq, *by_page, *need, *taken, *pair;
 };
 
+// Inclusive sums over the lanes of a wave, in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int scan16(int v) {  // of each sixteen
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    return dpp_add<0x118, 0xf>(v);
+}
 // Inclusive sum over the workgroup; `total` the last thread's.
-__device__ int scan(int v, int *wave_sums, int &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
+__device__ __forceinline__ int scan(int v, int *wave_sums, int &total) {
+    static_assert(kPlan == 1024, "sixteen waves");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    v = dpp_add<0x142, 0xa>(scan16(v));
+    v = dpp_add<0x143, 0xc>(v);
     __syncthreads();  // the last call's sums have been read
     if (lane == 63) wave_sums[wave] = v;
     __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kPlan / 64; ++w) {
-        const int s = wave_sums[w];
-        if (w < wave) before += s;
-        total += s;
-    }
-    return before + v;
+    const int upto = scan16(wave_sums[lane & 15]);
+    total = __builtin_amdgcn_readlane(upto, 15);
+    return v + (wave ? __builtin_amdgcn_readlane(upto, wave - 1) : 0);
 }
 
-// The lowest free pages into a.taken, at least `want` of them where there are as
-// many; returns how many were found (the same for every thread).
-__device__ int take_free(const PageArgs &a, int want, int *wave_sums) {
+// Which of a thread's four pages p .. are free, a bit each.
+__device__ __forceinline__ uint32_t free_bits(const PageArgs &a, int p) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bits |= p + j < a.num_pages && a.refs[p + j] == 0 ? 1u << j : 0u;
+    return bits;
+}
+
+// The lowest free pages into a.taken (and the first kPlan into `near`, in LDS), at
+// least `want` of them where there are as many; returns how many were found (the
+// same for every thread).  `bits`: those of the first pages, read before.
+__device__ int take_free(const PageArgs &a, int want, uint32_t bits, int *wave_sums, int *near) {
     int found = 0;
     for (int p0 = 0; p0 < a.num_pages && found < want; p0 += 4 * kPlan) {
         const int p = p0 + 4 * (int)threadIdx.x;
-        bool free_[4];
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            free_[j] = p + j < a.num_pages && a.refs[p + j] == 0;
-            mine += free_[j];
-        }
+        if (p0) bits = free_bits(a, p);
+        const int mine = __popc(bits);
         int total;
         int at = found + scan(mine, wave_sums, total) - mine;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (free_[j]) a.taken[at++] = p + j;
+            if (bits >> j & 1) {
+                if (at < kPlan) near[at] = p + j;
+                else if (at < want) a.taken[at] = p + j;
+                ++at;
+            }
         found += total;
     }
     __syncthreads();
     return found;
 }
+__device__ __forceinline__ int taken(const PageArgs &a, const int *near, int t) { return t < kPlan ? near[t] : a.taken[t]; }
 
-// Every entry's count of pages (count(i)) summed into a.need; the total.
+// Every entry's count of pages (count(i)) summed into a.need (the first kPlan into
+// `near`, in LDS, instead); the total.
 template <typename F>
-__device__ int sum_needs(const PageArgs &a, int *wave_sums, const F &count) {
+__device__ int sum_needs(const PageArgs &a, int *wave_sums, int *near, const F &count) {
     int sum = 0;
     for (int i0 = 0; i0 < a.n; i0 += kPlan) {
         const int i = i0 + (int)threadIdx.x;
         int total;
         const int upto = scan(i < a.n ? count(i) : 0, wave_sums, total);
-        if (i < a.n) a.need[i] = sum + upto;
+        if (i < kPlan) near[i] = sum + upto;
+        else if (i < a.n) a.need[i] = sum + upto;
         sum += total;
     }
     __syncthreads();
     return sum;
 }
 
-__device__ __forceinline__ int pages_of(const PageArgs &a, int len) { return (len + a.page_size - 1) / a.page_size; }
+// The full ones of len positions' pages (the reciprocal's error is far below the half
+// by which len + 1/2 clears the quotients' borders), and all of them.
+__device__ __forceinline__ int full_pages(const PageArgs &a, int len) { return (int)(((double)len + 0.5) * a.page_inv); }
+__device__ __forceinline__ int pages_of(const PageArgs &a, int len) { return full_pages(a, len + a.page_size - 1); }
 
 // Each of `list` marks its place; afterwards mark[list[i]] == i for every i where no value comes twice.
 __device__ void mark_all(const int32_t *list, int n, int limit, int32_t *mark) {
@@ -104,50 +122,87 @@ __device__ void mark_all(const int32_t *list, int n, int limit, int32_t *mark) {
     __syncthreads();
 }
 
+// The chain of dependent reads is all this kernel's time: a thread's first entry
+// and the first pages' counts are read once, all at the start; places, sums and pages of
+// the first kPlan entries go through LDS, and so do the marks of sequences as far as
+// they fit there.
 __global__ __launch_bounds__(kPlan) void pages_extend_kernel(PageArgs a) {
-    __shared__ int wave_sums[kPlan / 64];
-    mark_all(a.first, a.n, a.max_seqs, a.by_seq);
+    constexpr int kMarks = 1 << 16;
+    __shared__ int wave_sums[kPlan / 64], sums[kPlan], pages[kPlan];
+    __shared__ int2 place[kPlan];
+    __shared__ uint32_t marks[kMarks / 32];
+    const int tid = threadIdx.x;
+    struct Entry {
+        int s, add, len;
+    };
+    auto read = [&](int i) {
+        Entry e{-1, 0, 0};
+        if (i < a.n) {
+            e.s = a.first[i];
+            e.add = a.second[i];
+            if (e.s >= 0 && e.s < a.max_seqs) e.len = a.lens[e.s];
+        }
+        return e;
+    };
+    const uint32_t bits = free_bits(a, 4 * tid);
+    const Entry mine = read(tid);
+    auto entry = [&](int i) { return i == tid ? mine : read(i); };
+    const bool few = a.max_seqs <= kMarks;
+    if (few) {
+        for (int w = tid; w < (a.max_seqs + 31) / 32; w += kPlan) marks[w] = 0;
+        __syncthreads();
+    } else {
+        mark_all(a.first, a.n, a.max_seqs, a.by_seq);
+    }
+    auto twice = [&](int s, int i) { return few ? (atomicOr(&marks[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) != 0 : a.by_seq[s] != i; };
     bool bad = false;
-    for (int i = threadIdx.x; i < a.n; i += kPlan) {
-        const int s = a.first[i], add = a.second[i];
-        if (s < 0 || s >= a.max_seqs || a.by_seq[s] != i || add < 0) {
+    for (int i = tid; i < a.n; i += kPlan) {
+        const Entry e = entry(i);
+        if (e.s < 0 || e.s >= a.max_seqs || twice(e.s, i) || e.add < 0) {
             bad = true;
             continue;
         }
-        const int64_t len = a.lens[s];
-        bad = bad || len < 0 || len + add > (int64_t)a.table_stride * a.page_size;
+        bad = bad || e.len < 0 || (int64_t)e.len + e.add > (int64_t)a.table_stride * a.page_size;
     }
     if (__syncthreads_or(bad)) {
-        if (threadIdx.x == 0) *a.status = -1;
+        if (tid == 0) *a.status = -1;
         return;
     }
-    const int want = sum_needs(a, wave_sums, [&](int i) {
-        const int len = a.lens[a.first[i]];
-        return pages_of(a, len + a.second[i]) - pages_of(a, len);
+    const int want = sum_needs(a, wave_sums, sums, [&](int i) {
+        const Entry e = entry(i);
+        const int held = pages_of(a, e.len);
+        if (i < kPlan) place[i] = make_int2(e.s, held);
+        return pages_of(a, e.len + e.add) - held;
     });
-    const int found = take_free(a, want, wave_sums);
+    const int found = take_free(a, want, bits, wave_sums, pages);
     if (found < want) {
-        if (threadIdx.x == 0) *a.status = want - found;
+        if (tid == 0) *a.status = want - found;
         return;
     }
-    for (int t = threadIdx.x; t < want; t += kPlan) {
+    auto sum = [&](int i) { return i < kPlan ? sums[i] : a.need[i]; };
+    for (int t = tid; t < want; t += kPlan) {
         int lo = 0, hi = a.n - 1;  // the first entry whose running sum is above t
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (a.need[mid] > t) hi = mid;
+            if (sum(mid) > t) hi = mid;
             else lo = mid + 1;
         }
-        const int s = a.first[lo], before = lo ? a.need[lo - 1] : 0, page = a.taken[t];
-        a.table[(int64_t)s * a.table_stride + pages_of(a, a.lens[s]) + t - before] = page;
+        const int2 at = lo < kPlan ? place[lo] : make_int2(a.first[lo], pages_of(a, a.lens[a.first[lo]]));
+        const int page = taken(a, pages, t);
+        a.table[(int64_t)at.x * a.table_stride + at.y + t - (lo ? sum(lo - 1) : 0)] = page;
         a.refs[page] = 1;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.n; i += kPlan) a.lens[a.first[i]] += a.second[i];
-    if (threadIdx.x == 0) *a.status = 0;
+    if (a.n > kPlan) __syncthreads();
+    for (int i = tid; i < a.n; i += kPlan) {
+        const Entry e = entry(i);
+        a.lens[e.s] = e.len + e.add;
+    }
+    if (tid == 0) *a.status = 0;
 }
 
 __global__ __launch_bounds__(kPlan) void pages_fork_plan_kernel(PageArgs a) {
-    __shared__ int wave_sums[kPlan / 64];
+    __shared__ int wave_sums[kPlan / 64], sums[kPlan], pages[kPlan];
+    const uint32_t bits = free_bits(a, 4 * (int)threadIdx.x);
     mark_all(a.second, a.n, a.max_seqs, a.by_seq);
     bool bad = false;
     for (int i = threadIdx.x; i < a.n; i += kPlan) {
@@ -168,8 +223,11 @@ __global__ __launch_bounds__(kPlan) void pages_fork_plan_kernel(PageArgs a) {
         }
         return;
     }
-    const int want = sum_needs(a, wave_sums, [&](int i) { return a.lens[a.first[i]] % a.page_size != 0; });
-    const int found = take_free(a, want, wave_sums);
+    const int want = sum_needs(a, wave_sums, sums, [&](int i) {
+        const int len = a.lens[a.first[i]];
+        return pages_of(a, len) - full_pages(a, len);
+    });
+    const int found = take_free(a, want, bits, wave_sums, pages);
     if (found < want) {
         if (threadIdx.x == 0) {
             *a.status = want - found;
@@ -179,9 +237,11 @@ __global__ __launch_bounds__(kPlan) void pages_fork_plan_kernel(PageArgs a) {
     }
     for (int i = threadIdx.x; i < a.n; i += kPlan) {
         const int len = a.lens[a.first[i]];
-        if (len % a.page_size == 0) continue;
-        const int t = a.need[i] - 1, page = a.taken[t];
-        a.pair[2 * t] = a.table[(int64_t)a.first[i] * a.table_stride + len / a.page_size];
+        const int full = full_pages(a, len);
+        if (len == full * a.page_size) continue;
+        const int t = (i < kPlan ? sums[i] : a.need[i]) - 1, page = taken(a, pages, t);
+        if (i < kPlan) a.need[i] = t + 1;  // (the copying kernel reads it)
+        a.pair[2 * t] = a.table[(int64_t)a.first[i] * a.table_stride + full];
         a.pair[2 * t + 1] = page;
         a.refs[page] = 1;
     }
@@ -220,12 +280,12 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PageArgs a) {
     const int64_t entries = (int64_t)a.n * a.table_stride;
     for (int64_t t = tid; t < entries; t += step) {
         const int i = (int)(t / a.table_stride), col = (int)(t - (int64_t)i * a.table_stride);
-        const int p = a.first[i], c = a.second[i], len = a.lens[p], full = len / a.page_size;
+        const int p = a.first[i], c = a.second[i], len = a.lens[p], full = full_pages(a, len);
         int page = -1;
         if (col < full) {
             page = a.table[(int64_t)p * a.table_stride + col];
             if (page >= 0 && page < a.num_pages) atomicAdd(&a.refs[page], 1);
-        } else if (col == full && len % a.page_size) {
+        } else if (col == full && len != full * a.page_size) {
             page = a.pair[2 * (a.need[i] - 1) + 1];
         }
         a.table[(int64_t)c * a.table_stride + col] = page;
@@ -259,21 +319,22 @@ __global__ __launch_bounds__(256) void pages_free_kernel(PageArgs a) {
 }
 
 __global__ __launch_bounds__(kPlan) void pages_compact_plan_kernel(PageArgs a) {
-    __shared__ int wave_sums[kPlan / 64];
+    __shared__ int wave_sums[kPlan / 64], pages[kPlan];
     int mine = 0, total;
     for (int p = threadIdx.x; p < a.num_pages; p += kPlan) mine += a.refs[p] != 0;
     scan(mine, wave_sums, total);
     const int live = total;
-    take_free(a, live, wave_sums);  // in order: those below `live` take the pages above it, as many
+    take_free(a, live, free_bits(a, 4 * (int)threadIdx.x), wave_sums, pages);  // in order: those below `live` take the pages above it, as many
     int moved = 0;
     for (int p0 = 0; p0 < a.num_pages; p0 += kPlan) {
         const int p = p0 + (int)threadIdx.x;
         const bool high = p < a.num_pages && p >= live && a.refs[p] != 0;
         const int at = moved + scan(high, wave_sums, total) - 1;
-        if (p < a.num_pages) a.by_page[p] = high ? a.taken[at] : p;
+        const int to = high ? taken(a, pages, at) : p;
+        if (p < a.num_pages) a.by_page[p] = to;
         if (high) {
             a.pair[2 * at] = p;
-            a.pair[2 * at + 1] = a.taken[at];
+            a.pair[2 * at + 1] = to;
         }
         moved += total;
     }
@@ -389,6 +450,7 @@ int page_args(PageArgs &a, const doe_kv_pages *p, const int32_t *first, const in
     a.table_stride = (int)p->table_stride;
     a.num_pages = (int)p->num_pages;
     a.page_size = (int)p->page_size;
+    a.page_inv = 1.0 / a.page_size;
     return DOE_OK;
 }
 

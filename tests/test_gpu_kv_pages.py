@@ -210,6 +210,37 @@ def test_bookkeeping_without_pools(dev):
     h.same()
 
 
+def test_extend_among_very_many_sequences(dev):
+    """More sequences than are marked in LDS; more entries, and more pages, than are kept there."""
+    rng = np.random.default_rng(70000)
+    h = Host(rng, 70000, 2, 9000, 16, [16 * (i % 2) + i % 3 for i in range(4000)])
+    for n in (1, 1500, 3000):
+        seqs, add = rng.choice(70000, n, replace=False), rng.integers(0, 15, n)
+        add = np.minimum(add, 32 - h.lens[seqs])
+        print(f"[extend] 70000 sequences, {n} entries", flush=True)
+        ops.kv_pages_extend(h.pages, up(i32(seqs)), up(i32(add)), n, status=h.status, workspace=h.ws)
+        h.same(h.extend(seqs, add))
+    for seqs in ([69999, 5, 69999], [70000], [-1]):
+        ops.kv_pages_extend(h.pages, up(i32(seqs)), up(i32([1] * len(seqs))), len(seqs), status=h.status, workspace=h.ws)
+        h.same(-1)
+
+
+def test_fork_and_compact_of_many_pages(dev):
+    """More copies than are kept in LDS."""
+    rng = np.random.default_rng(2)
+    h = Host(rng, 4000, 2, 9000, 16, [1 + i % 31 for i in range(1900)] + [0] * 2100)
+    parents, children = rng.integers(0, 1900, 1800), 1900 + rng.permutation(2100)[:1800]
+    ops.kv_pages_fork(h.pages, up(i32(parents)), up(i32(children)), 1800, status=h.status, workspace=h.ws)
+    h.same(h.fork(parents, children))
+    gone = rng.choice(3700, 1200, replace=False)
+    ops.kv_pages_free(h.pages, up(i32(gone)), 1200, status=h.status)
+    h.free(gone)
+    h.same()
+    ops.kv_pages_compact(h.pages, status=h.status, workspace=h.ws)
+    h.compact()
+    h.same()
+
+
 def test_free_and_compact_of_a_damaged_state(dev):
     """A length beyond the table row counts as what the row holds; a page with a
     count below 0 is in use for all that moves."""
