@@ -11,15 +11,15 @@
 //     radix 32 below the largest value of its block, each an integer of [-16, 16]
 //     and so a 6-bit float (E2M3 holds all multiples of 1/8 up to 2) under a scale
 //     of its own; all digits' products add up in one f32 accumulator.  Five digits
-//     carry 25 bits of a block's largest value, four (q and out f16) 20: an error
+//     carry 25 bits of a block's largest value: an error
 //     of the scale of the block's products, as their f32 sum has it too.  A dim far
 //     below the largest has it alone where the keys are zero at the large one
 //     (2^11 apart: 1.5e-5 of the output).  The 4- and 6-bit formats run at four
 //     times the f16 rate, so five cost 1.25 f16 products, where f16 hi + lo over
 //     converted K would cost two.
 //   * S^T's sums are P^T's operand order of O^T = V^T P^T, on
-//     v_mfma_f32_32x32x16_f16: P as f16 hi + lo, or one f16 where q and out are
-//     f16 (2^-12 of P's each, below the output's own rounding).
+//     v_mfma_f32_32x32x16_f16: P as f16 hi + lo whatever the output's type (one f16
+//     of P would cost an f16 output as much again as its own rounding, 2e-4).
 //   * V goes to f16 with its scales (v_cvt_scalef32_pk_f16_fp4) once for the waves
 //     that share it, into LDS in operand order: the page layout holds the eight
 //     positions of a lane half together, so a lane writes and reads 16-byte pieces.
@@ -56,6 +56,7 @@ typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
 constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P of the running max, and how far that may lag
 constexpr int kWaves = 4;
+constexpr int kDigits = 5;  // of a query
 // Workgroups that a CU holds, by their registers (at 512 by LDS as well).  64: three
 // cost seven spilled registers at most and win (12 ragged prompts of up to 777 rows, a window,
 // capped scores: 49.6 to 41.3 us); 512: 648 us for 1050 with one.
@@ -336,13 +337,13 @@ __device__ __forceinline__ int wave_scan(int v) {
     return dpp_add<0x143, 0xc>(v);
 }
 
-// FULL: P as f16 hi + lo.
-template <int D, int TEAM, int ND, bool FULL>
+template <int D, int TEAM>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel(PromptArgs a) {
     using P = Shape<D, TEAM>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool kShare = TEAM == 4;                 // the waves share V
     constexpr bool kSliced = P::kSlices > 1;
+    constexpr int ND = kDigits;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n32 = lane & 31, lh = lane >> 5, shift = a.c.page_shift, G = a.group;
     const int slice = kSliced ? wave : 0;
@@ -596,13 +597,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
                 const float e0 = __builtin_amdgcn_exp2f(y[r]), e1 = __builtin_amdgcn_exp2f(y[r + 1]);
                 l += e0 + e1;
                 ph[h][j] = (_Float16)e0, ph[h][j + 1] = (_Float16)e1;
-                if constexpr (FULL) {
-                    pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
-                    pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
-                }
+                pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
+                pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
             }
         scores<D, TEAM, ND, kEarly, kProducts>(q, kb, next);
-        interleave<kProducts - kEarly, FULL ? 6 : 4>();
+        interleave<kProducts - kEarly, 6>();
         here(next);
         here(l);
         __builtin_amdgcn_sched_barrier(0);
@@ -619,10 +618,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
             const h8 v0 = v[32 * t], v1 = v[2 * P::kDims + 32 * t];
             o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], o[t], 0, 0, 0);
             o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], o[t], 0, 0, 0);
-            if constexpr (FULL) {
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[t], 0, 0, 0);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[t], 0, 0, 0);
-            }
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], o[t], 0, 0, 0);
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], o[t], 0, 0, 0);
             if (t < each && u * each + t < P::kTiles) stage_v<D, TEAM>(to, vb, vs, u * each + t, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -802,14 +799,14 @@ int64_t workspace_of(int64_t head_dim, int64_t batch, int64_t rows, int64_t num_
     return most == 1 ? 16 : most * rows * num_heads * (head_dim + 2) * 4;
 }
 
-template <int D, int TEAM, int ND, bool FULL>
+template <int D, int TEAM>
 int launch(const PromptArgs &a, hipStream_t st) {
     constexpr int lds = Shape<D, TEAM>::kLds;
-    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_prompt_kernel<D, TEAM, ND, FULL>,
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_prompt_kernel<D, TEAM>,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     DOE_HIP_CHECK(attr_rc);
     const dim3 grid((unsigned)(a.tiles * a.c.kv_heads), (unsigned)a.splits);
-    hipLaunchKernelGGL((attn_mx4_prompt_kernel<D, TEAM, ND, FULL>), grid, dim3(64 * kWaves), lds, st, a);
+    hipLaunchKernelGGL((attn_mx4_prompt_kernel<D, TEAM>), grid, dim3(64 * kWaves), lds, st, a);
     DOE_LAUNCH_CHECK("attn_mx4_prompt_kernel");
     if (a.splits == 1) return DOE_OK;
     const int64_t pairs = (int64_t)a.rows * a.num_heads, each = 1024 / D;
@@ -820,11 +817,10 @@ int launch(const PromptArgs &a, hipStream_t st) {
 
 template <int D>
 int launch_d(PromptArgs &a, bool share, hipStream_t st) {
-    const bool full = !(a.q_f16 && a.out_f16);
     if constexpr (D < 512) {
-        if (share) return full ? launch<D, 4, 5, true>(a, st) : launch<D, 4, 4, false>(a, st);
+        if (share) return launch<D, 4>(a, st);
     }
-    return full ? launch<D, 1, 5, true>(a, st) : launch<D, 1, 4, false>(a, st);
+    return launch<D, 1>(a, st);
 }
 
 }  // namespace

@@ -554,13 +554,11 @@ int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, vo
  * sequence at position kv_lens[b] - n + i, causal.  Rows of no sequence are
  * left as they were; a row at a position below 0 gives zeros.  Scores are
  * products of the cache's codes as they stand and digits of the queries: 25
- * bits of the largest value of every 32 dims, 20 with q_f16 and out_f16 (a dim
- * 2^n below that keeps n fewer); probabilities are f16 hi + lo, with q_f16 and
- * out_f16 one f16.  2-4e-7 from float64 with normal queries, 1.5e-5 with single
- * dims 2^11 above the others where the keys are zero; with f16 both ways 3e-4
- * (the output's rounding 2e-4 of it), 5e-4.  A short
- * prompt over a long cache splits its keys over the device and joins them
- * through the workspace. */
+ * bits of the largest value of every 32 dims (a dim 2^n below that keeps n
+ * fewer); probabilities are f16 hi + lo.  2-4e-7 from float64 with normal queries,
+ * 1.5e-5 with single dims 2^11 above the others where the keys are zero; an f16
+ * output adds its rounding, 2e-4.  A short prompt over a long cache splits its
+ * keys over the device and joins them through the workspace. */
 int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
                                   int64_t head_dim, int64_t *bytes);
 int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,
