@@ -5,21 +5,16 @@
 // pos, with a window p > pos - window; row i of a sequence's n is at position
 // kv_len - n + i.  The query heads of a KV head share its K and V: a tile is 32 or
 // 128 (row, head) pairs of one KV head, a wave 32 of them, a lane column one.
-//   * S^T = K Q^T on v_mfma_scale_f32_32x32x64_f8f6f4: K's codes and scale bytes are
-//     the matrix cores' own 4-bit format, a lane's operand one block of 32 dims as
-//     it stands in the page, with no conversion at all.  Q is cut into digits of
-//     radix 32 below the largest value of its block, each an integer of [-16, 16]
-//     and so a 6-bit float (E2M3 holds all multiples of 1/8 up to 2) under a scale
-//     of its own; all digits' products add up in one f32 accumulator.  Five digits
-//     carry 25 bits of a block's largest value: an error
-//     of the scale of the block's products, as their f32 sum has it too.  A dim far
-//     below the largest has it alone where the keys are zero at the large one
-//     (2^11 apart: 1.5e-5 of the output).  The 4- and 6-bit formats run at four
-//     times the f16 rate, so five cost 1.25 f16 products, where f16 hi + lo over
-//     converted K would cost two.
-//   * S^T's sums are P^T's operand order of O^T = V^T P^T, on
-//     v_mfma_f32_32x32x16_f16: P as f16 hi + lo whatever the output's type (one f16
-//     of P would cost an f16 output as much again as its own rounding, 2e-4).
+//   * S^T = K Q^T on v_mfma_f32_32x32x16_f16: K's codes go to f16 with their scales in
+//     four conversions an operand, exactly.  f16 queries are operands as they stand,
+//     f32 ones in hi and lo parts of one power of two for the row: 22 bits of each
+//     dim, whatever the others are (down to 2^-38 of the largest).  The matrix cores'
+//     own 4-bit operands against digits of Q in 6 bits (25 bits of the largest of 32
+//     dims) took 2-15 % less, but lost dims far below the largest where the keys are
+//     zero at the large ones: 1e-3 of the output at 2^15.
+//   * S^T's sums are P^T's operand order of O^T = V^T P^T, on the same instruction:
+//     P as f16 hi + lo whatever the output's type (one f16 of P would cost an f16
+//     output as much again as its own rounding, 2e-4).
 //   * V goes to f16 with its scales (v_cvt_scalef32_pk_f16_fp4) once for the waves
 //     that share it, into LDS in operand order: the page layout holds the eight
 //     positions of a lane half together, so a lane writes and reads 16-byte pieces.
@@ -28,13 +23,11 @@
 // A block's steps overlap with its neighbours': its weights stand beside the next
 // one's scores, its P V beside the next V's way into LDS, so that the matrix and
 // vector units of a SIMD work at once with one or two waves on it.  2048 rows after
-// 8192 positions, 32 / 8 heads of 128 dims, f16: 315 us, 981 TFLOP/s of the 4 D
-// operations a pair and position, where a large f16 matrix product reaches 1139; the
-// matrix units are busy 43 % of the cycles, vector issue and the latency of a chain
-// of them by two waves the rest (without the exponentials it would be 3 % less,
-// without the staging 9 %, without the scores 18 %).  1000 rows at 8 / 4 heads of
-// 256 dims, f32: 27 us, of which 8 are a prologue (row, page table and query read one
-// after the other, digits) that 252 tiles on 256 CUs go through at once.
+// 8192 positions, 32 / 8 heads of 128 dims, f16: 460 us, 672 TFLOP/s of the 4 D
+// operations a pair and position, where a large f16 matrix product reaches 1139: P's
+// two parts are three products for two.  1000 rows at 8 / 4 heads of 256 dims, f32: 28
+// us, of which 8 are a prologue (row, page table and query read one after the other)
+// that 252 tiles on 256 CUs go through at once.
 #include "mx4_cache.h"
 
 #include <math.h>
@@ -43,23 +36,22 @@
 
 namespace {
 
+using doe::Mx4Factor;
 using doe::Mx4Slab;
 using doe::Mx4View;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
 constexpr float kBias = 7.0f, kLazy = 8.0f;  // log2: P of the running max, and how far that may lag
 constexpr int kWaves = 4;
-constexpr int kDigits = 5;  // of a query
 // Workgroups that a CU holds, by their registers (at 512 by LDS as well).  64: three
-// cost seven spilled registers at most and win (12 ragged prompts of up to 777 rows, a window,
-// capped scores: 49.6 to 41.3 us); 512: 648 us for 1050 with one.
+// cost eight spilled registers at most and win (12 ragged prompts of up to 777 rows, a window,
+// capped scores: 49.6 to 41.3 us); 512: 1500 rows after 2000 of 8 sequences at 8 / 1 heads
+// 648 us for 1050 with one.
 constexpr int per_cu(int head_dim) { return head_dim == 64 ? 3 : (head_dim == 128 || head_dim == 512 ? 2 : 1); }
 
 struct PromptArgs {
@@ -81,7 +73,7 @@ struct Shape {
     static constexpr int kSlices = D == 512 ? 4 : 1, kDims = D / kSlices;  // of a wave
     static constexpr int kRows = D == 512 ? 32 : 32 * TEAM;                // pairs of a tile
     static constexpr int kBlocks = TEAM;                                   // blocks of a step
-    static constexpr int kSteps = (kDims + 63) / 64, kTiles = kDims / 32;
+    static constexpr int kSteps = (kDims + 63) / 64, kTiles = kDims / 32, kOps = kDims / 16;
     static constexpr int kV = 32 * kDims * 2;                              // bytes of a block's V
     static constexpr int kBuffers = 8;                                     // two steps of four, or two blocks a wave
     static constexpr int kMerge = TEAM == 4 || D == 512 ? 0 : kWaves * 32 * D * 4;  // the waves' O at the end
@@ -103,12 +95,20 @@ __device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
     }
 }
 
-// A lane's K of a block: position lane % 32, the 32 dims of half lane / 32 of
-// each step, and their scale bytes (step s in byte 2 (s % 2) of word s / 2).
+// A lane's dims of a row, of K and of the queries alike: operand o has eight, of the
+// 32 of group 2 (o / 4) + half (half: lane / 32); of a last group without a second
+// (head_dim 160) each half has 16.
+template <int D, int TEAM>
+__device__ __forceinline__ constexpr int dims_of(int o, int half) {
+    constexpr int PAIRED = Shape<D, TEAM>::kDims / 64 * 4;
+    return o < PAIRED ? 64 * (o / 4) + 32 * half + 8 * (o % 4) : 16 * PAIRED + 16 * half + 8 * (o - PAIRED);
+}
+
+// A lane's K of a block: position lane % 32, the codes of an operand a word, and the
+// scale bytes (operands 4 s .. 4 s + 3 in byte 2 (s % 2) of word s / 2).
 template <int D, int TEAM>
 struct KBlock {
-    u32x4 k[Shape<D, TEAM>::kSteps];
-    uint32_t s[(Shape<D, TEAM>::kSteps + 1) / 2];
+    uint32_t k[Shape<D, TEAM>::kOps], s[(Shape<D, TEAM>::kSteps + 1) / 2];
 };
 template <int D, int TEAM>
 __device__ __forceinline__ void load_k(KBlock<D, TEAM> &b, const uint8_t *slab, int shift, int x, int lane, int slice) {
@@ -119,10 +119,13 @@ __device__ __forceinline__ void load_k(KBlock<D, TEAM> &b, const uint8_t *slab, 
     const uint32_t at_k = m * (D / 2) + lh * 16, at_s = m * (D / 32);
     const uint8_t *s = slab + (uint32_t)(S::k_scale(shift, x) + slice * (P::kDims / 32));
 #pragma unroll
-    for (int i = 0; i < P::kSteps; ++i) {
-        // (head_dim 160: the last step's second half is nothing; the query has zeros there)
-        const int at = P::kDims % 64 && i == P::kSteps - 1 ? i * 32 - lh * 16 : i * 32;
-        b.k[i] = *reinterpret_cast<const u32x4 *>(k + (uint32_t)(at_k + at));
+    for (int o = 0; o + 4 <= P::kOps; o += 4) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(k + (uint32_t)(at_k + 8 * o));
+        b.k[o] = w[0], b.k[o + 1] = w[1], b.k[o + 2] = w[2], b.k[o + 3] = w[3];
+    }
+    if constexpr (P::kOps % 4 != 0) {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(k + (uint32_t)(at_k - lh * 8 + 8 * (P::kOps - 2)));
+        b.k[P::kOps - 2] = w[0], b.k[P::kOps - 1] = w[1];
     }
     if constexpr (D == 64) {
         b.s[0] = *reinterpret_cast<const uint16_t *>(s + at_s) >> (8 * lh);
@@ -222,87 +225,54 @@ __device__ __forceinline__ void stage_v(uint8_t *dst, const VBlock<D, TEAM> &b, 
     to[(2 * i + 1) * 16] = h8{v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
 }
 
-// A lane's queries: pair lane % 32, the 32 dims of half lane / 32 of each step, as
-// ND digits; scale bytes of digits 0..3 in one word, of a fifth in another.
-template <int D, int TEAM, int ND>
+// A lane's queries as operands, pair lane % 32: f16 as they are (HALF), f32 as f16 hi
+// and lo parts of q 2^e.
+template <int D, int TEAM, bool HALF>
 struct Query {
-    u32x6 d[Shape<D, TEAM>::kSteps][ND];
-    uint32_t s[Shape<D, TEAM>::kSteps], s4[ND > 4 ? Shape<D, TEAM>::kSteps : 1];
+    static constexpr int kOps = Shape<D, TEAM>::kOps, kLo = HALF ? 1 : kOps;
+    h8 hi[kOps], lo[kLo];
 };
-// Step s of them.
-template <int D, int TEAM, int ND>
-__device__ __forceinline__ void load_query(u32x6 *digits, uint32_t &scales, uint32_t &scale4, const PromptArgs &a, int64_t at, int s,
-                                           int lane, int slice) {
-    using P = Shape<D, TEAM>;
-    const int lh = lane >> 5;
-    const bool none = P::kDims % 64 && s == P::kSteps - 1 && lh;
-    const int64_t from = at + slice * P::kDims + (none ? 0 : 64 * s + 32 * lh);
-    float f[32];
-    if (a.q_f16) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            const h8 v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + from + i);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[i + e] = (float)v[e];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + from + i);
-            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
-        }
-    }
+// N operands of f32 queries from `first` on.
+template <int D, int TEAM, int N>
+struct RawQuery {
+    float f[8 * N];
+};
+template <int D, int TEAM, int N>
+__device__ __forceinline__ uint32_t read_query(RawQuery<D, TEAM, N> &r, const float *q, int first, int half) {
     uint32_t top = 0;  // (as bits: a NaN is above all)
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    if (none) top = 0;
-    const bool real = top < 0x7f800000u;
-    int e = top == 0 || !real ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top));
-    e = e < -106 ? -106 : e;
-    f32x16 even, odd;
+    for (int o = 0; o < N; ++o) {
+        const int from = dims_of<D, TEAM>(first + o, half);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        even[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i], 4 - e);
-        odd[i] = none || !real ? 0.0f : __builtin_amdgcn_ldexpf(f[2 * i + 1], 4 - e);
-    }
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-        f32x16 x, y;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_rintf(even[i]);
-            y[i] = __builtin_rintf(odd[i]);
-            even[i] = (even[i] - x[i]) * 32.0f;
-            odd[i] = (odd[i] - y[i]) * 32.0f;
+        for (int i = 0; i < 8; i += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(q + from + i);
+            r.f[8 * o + i] = v.x, r.f[8 * o + i + 1] = v.y, r.f[8 * o + i + 2] = v.z, r.f[8 * o + i + 3] = v.w;
         }
-        u32x6 packed = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x, y, 8.0f);
-        // (the sources outlive it: with a destination that begins inside one of them,
-        // which the compiler allows itself, the instruction overwrites what it has yet to read)
-        __asm__ volatile("" : "+v"(packed) : "v"(x), "v"(y));
-        digits[d] = packed;
     }
-    // digit d counts 2^(e - 1 - 5 d) times its 6-bit float; 255: not a number
-    const uint32_t b = e + 126;
-    scales = real ? b | (b - 5) << 8 | (b - 10) << 16 | (ND > 3 ? (b - 15) << 24 : 0u) : 0xffffffffu;
-    scale4 = real ? b - 20 : 255u;
+#pragma unroll
+    for (int i = 0; i < 8 * N; ++i) top = max(top, __float_as_uint(r.f[i]) & 0x7fffffffu);
+    return max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+}
+__device__ __forceinline__ void split_query(h8 &hi, h8 &lo, const float *f, int e) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = __builtin_amdgcn_ldexpf(f[i], e);
+        hi[i] = (_Float16)v;
+        lo[i] = (_Float16)(v - (float)hi[i]);
+    }
 }
 
-// The products [FROM, TO) of a block's scores, step and digit in order.
-template <int D, int TEAM, int ND, int FROM, int TO>
-__device__ __forceinline__ void scores(const Query<D, TEAM, ND> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
+// The products [FROM, TO) of a block's scores, operand by operand.
+template <int D, int TEAM, bool HALF, int FROM, int TO>
+__device__ __forceinline__ void scores(const Query<D, TEAM, HALF> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
     if constexpr (FROM < TO) {
-        constexpr int S = FROM / ND, DIGIT = FROM % ND;
-        i32x8 a = {}, b = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = (int)k.k[S][i];
-#pragma unroll
-        for (int i = 0; i < 6; ++i) b[i] = (int)q.d[S][DIGIT][i];
-        const int ks = (int)k.s[S / 2];
-        if constexpr (DIGIT < 4)
-            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 2, 2 * (S % 2), ks, DIGIT, (int)q.s[S]);
-        else
-            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 2, 2 * (S % 2), ks, 0, (int)q.s4[S]);
-        scores<D, TEAM, ND, FROM + 1, TO>(q, k, acc);
+        const float f = byte_scale(k.s[FROM / 8], FROM / 4 % 2 * 2);
+        const uint32_t w = k.k[FROM];
+        const h2 k0 = pair<0>(w, f), k1 = pair<1>(w, f), k2 = pair<2>(w, f), k3 = pair<3>(w, f);
+        const h8 kf = {k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]};
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q.hi[FROM], acc, 0, 0, 0);
+        if constexpr (!HALF) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q.lo[FROM], acc, 0, 0, 0);
+        scores<D, TEAM, HALF, FROM + 1, TO>(q, k, acc);
     }
 }
 
@@ -337,13 +307,14 @@ __device__ __forceinline__ int wave_scan(int v) {
     return dpp_add<0x143, 0xc>(v);
 }
 
-template <int D, int TEAM>
+// HALF: f16 queries.
+template <int D, int TEAM, bool HALF>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel(PromptArgs a) {
     using P = Shape<D, TEAM>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     constexpr bool kShare = TEAM == 4;                 // the waves share V
     constexpr bool kSliced = P::kSlices > 1;
-    constexpr int ND = kDigits;
+    constexpr int kParts = HALF ? 1 : 2;               // matrix instructions of an operand
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int n32 = lane & 31, lh = lane >> 5, shift = a.c.page_shift, G = a.group;
     const int slice = kSliced ? wave : 0;
@@ -423,13 +394,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
     const int ahead = kShare ? wave : 0;       // the block of a step that this wave stages
     const int buffers = kShare ? 0 : 2 * wave;  // this wave's first buffer
 
-    Query<D, TEAM, ND> q;
+    Query<D, TEAM, HALF> q;
     f32x16 o[P::kTiles], s;
 #pragma unroll
     for (int t = 0; t < P::kTiles; ++t) o[t] = f32x16{};
     float m = -INFINITY, l = 0.0f;
-    const float rowf = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
-    const float yf = a.softcap > 0.0f ? a.softcap * 1.4426950408889634f : rowf;
+    Mx4Factor rowf;  // of a score
 
     KBlock<D, TEAM> kb;
     VBlock<D, TEAM> vb;
@@ -449,49 +419,79 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
     int slab0 = slab_index(0), slab1 = slab_index(1);  // of the block at hand and the next
     load_k<D, TEAM>(kb, slab_at(slab0), shift, place(0), lane, slice);
     {
-        const int64_t at = (int64_t)row * a.q_stride + (int64_t)head * D;
-        uint32_t s4 = 0;
-        if constexpr (kShare || kSliced) {
+        const int64_t at = (int64_t)row * a.q_stride + (int64_t)head * D + slice * P::kDims;
+        const float f = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
+        if constexpr (HALF) {
+            typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+            u16x8 top = {};
 #pragma unroll
-            for (int s = 0; s < P::kSteps; ++s) {
-                load_query<D, TEAM, ND>(q.d[s], q.s[s], s4, a, at, s, lane, slice);
-                if constexpr (ND > 4) q.s4[s] = s4;
+            for (int o = 0; o < P::kOps; ++o) {
+                q.hi[o] = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(a.q) + at + dims_of<D, TEAM>(o, lh));
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, q.hi[o]) & (unsigned short)0x7fff);
             }
+            int bad = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bad |= top[i] >= 0x7c00;
+            bad |= __shfl_xor(bad, 32, 64);
+            if constexpr (kSliced) {  // (a slice that is no number: the pair's scores are none)
+                if (bad) q.hi[0][0] = (_Float16)NAN;
+                bad = 0;
+            }
+            rowf = doe::mx4_factor(f, bad ? 0x7f800000u : 0u, 0);
+        } else if constexpr (kShare) {
+            RawQuery<D, TEAM, P::kOps> raw;
+            const uint32_t top = read_query(raw, static_cast<const float *>(a.q) + at, 0, lh);
+            const int e = doe::mx4_query_exp(top);
+#pragma unroll
+            for (int o = 0; o < P::kOps; ++o) split_query(q.hi[o], q.lo[o], raw.f + 8 * o, e);
+            rowf = doe::mx4_factor(f, top, e);
         } else {
-            // the waves have the same pairs: a step or none each, passed on in V's place
-            u32x2 *x = reinterpret_cast<u32x2 *>(lds);
-            if (wave < P::kSteps) {
-                u32x6 d[ND];
-                uint32_t sc = 0;
-                load_query<D, TEAM, ND>(d, sc, s4, a, at, wave, lane, slice);
-                u32x2 *to = x + wave * (3 * ND + 1) * 64 + lane;
-#pragma unroll
-                for (int i = 0; i < 3 * ND; ++i) to[64 * i] = u32x2{d[i / 3][i % 3 * 2], d[i / 3][i % 3 * 2 + 1]};
-                to[64 * 3 * ND] = u32x2{sc, s4};
-            }
+            // the waves have the same pairs: a step or none each (or, sliced, a part of the
+            // dims), one scale for them all, passed on in V's place
+            uint32_t *tops = reinterpret_cast<uint32_t *>(lds);
+            h8 *x = reinterpret_cast<h8 *>(lds);
+            constexpr int N = kSliced ? P::kOps : 4;
+            RawQuery<D, TEAM, N> raw;
+            uint32_t top = 0;
+            const bool have = kSliced || wave < P::kSteps;
+            // (the last step of head_dim 160 has two operands: its others are read again)
+            const int op0 = kSliced ? 0 : std::min(4 * wave, P::kOps - N);
+            if (have) top = read_query(raw, static_cast<const float *>(a.q) + at, op0, lh);
+            if (lh == 0) tops[wave * 32 + n32] = top;
             __syncthreads();
 #pragma unroll
-            for (int s = 0; s < P::kSteps; ++s) {
-                const u32x2 *from = x + s * (3 * ND + 1) * 64 + lane;
+            for (int w = 0; w < kWaves; ++w) top = max(top, tops[w * 32 + n32]);
+            __syncthreads();
+            const int e = doe::mx4_query_exp(top);
+            rowf = doe::mx4_factor(f, top, e);
+            if constexpr (kSliced) {
 #pragma unroll
-                for (int i = 0; i < 3 * ND; ++i) {
-                    const u32x2 w = from[64 * i];
-                    q.d[s][i / 3][i % 3 * 2] = w[0], q.d[s][i / 3][i % 3 * 2 + 1] = w[1];
+                for (int o = 0; o < P::kOps; ++o) split_query(q.hi[o], q.lo[o], raw.f + 8 * o, e);
+            } else {
+                if (have) {
+#pragma unroll
+                    for (int o = 0; o < N; ++o) {
+                        h8 hi, lo;
+                        split_query(hi, lo, raw.f + 8 * o, e);
+                        x[(op0 + o) * 128 + lane] = hi, x[(op0 + o) * 128 + 64 + lane] = lo;
+                    }
                 }
-                const u32x2 w = from[64 * 3 * ND];
-                q.s[s] = w[0];
-                if constexpr (ND > 4) q.s4[s] = w[1];
+                __syncthreads();
+#pragma unroll
+                for (int o = 0; o < P::kOps; ++o) q.hi[o] = x[o * 128 + lane], q.lo[o] = x[o * 128 + 64 + lane];
+                __syncthreads();
             }
-            __syncthreads();
         }
     }
+    const float yf = a.softcap > 0.0f ? a.softcap * 1.4426950408889634f : rowf.post;
+    const bool large = __any(rowf.pre != 1.0f);
     scale_v(ahead, buffers + ahead);
 #pragma unroll
     for (int t = 0; t < P::kTiles; ++t) stage_v<D, TEAM>(lds + (buffers + ahead) * P::kV, vb, vs, t, lane);
     fetch_v(ahead + P::kBlocks);
-    constexpr int kProducts = P::kSteps * ND, kEarly = kProducts / 4;  // of a block's scores; those beside the logs
+    constexpr int kEarly = P::kOps / 4;  // operands of a block's scores that go beside the logs
     s = f32x16{};
-    scores<D, TEAM, ND, 0, kProducts>(q, kb, s);
+    scores<D, TEAM, HALF, 0, P::kOps>(q, kb, s);
     load_k<D, TEAM>(kb, slab_at(slab1), shift, place(1), lane, slice);
     if (kShare) __syncthreads();
 
@@ -536,9 +536,13 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
             }
         }
         // lane: pair n32, positions p0 + 8 (r / 4) + 4 lh + r % 4
+        if (large) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= rowf.pre;
+        }
         if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = doe::mx4_tanh(s[r] * rowf);
+            for (int r = 0; r < 16; ++r) s[r] = doe::mx4_tanh(s[r] * rowf.post);
         }
         float y[16];
         const int top_ = slab0 < 0 ? 0 : hi;
@@ -563,8 +567,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
         logs(m);
         if (!whole) mask();
         const float over = most();
-        scores<D, TEAM, ND, 0, kEarly>(q, kb, next);
-        interleave<kEarly, 6>();
+        scores<D, TEAM, HALF, 0, kEarly>(q, kb, next);
+        interleave<kEarly * kParts, 6>();
         here(next);
         if (__any(over > kBias + kLazy)) {  // (m = -inf: any score)
             logs(0.0f);
@@ -600,8 +604,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
                 pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
                 pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
             }
-        scores<D, TEAM, ND, kEarly, kProducts>(q, kb, next);
-        interleave<kProducts - kEarly, 6>();
+        scores<D, TEAM, HALF, kEarly, P::kOps>(q, kb, next);
+        interleave<(P::kOps - kEarly) * kParts, 6>();
         here(next);
         here(l);
         __builtin_amdgcn_sched_barrier(0);
@@ -778,9 +782,10 @@ int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
 // Whether a call takes tiles of 128 pairs, whose waves share V's way into LDS, or of
 // 32, whose waves take every fourth block.  The large ones need as many tiles as the
 // device holds workgroups.  1500 rows after 2000 of 8 sequences, 32 against 128, f32
-// and f16: head_dim 64 163 / 157 and 131 / 117 us, 128 258 / 234 and 202 / 159, 160 1010 / 799 and 907 / 619, 256 316 / 300
-// and 285 / 231; one prompt of 1000 rows (fewer tiles): 16 / 28, 21 / 36 and 28 / 44
-// at 64, 128 and 256, but 67 / 60 and 59 / 47 at 160, where 16 KV heads make 256 tiles.
+// and f16: 16 / 4 heads of 64 174 / 173 and 151 / 157 us, 16 / 4 of 128 279 / 270 and 244 /
+// 226, 32 / 16 of 160 1046 / 815 and 928 / 676, 8 / 4 of 256 335 / 328 and 294 / 273; one
+// prompt of 1000 rows (fewer tiles), f32: 16 / 29, 21 / 37 and 29 / 43 at 64, 128 and 256,
+// but 67 / 61 at 160, where 16 KV heads make 256 tiles.
 bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     if (head_dim == 512) return false;
     if (g_tile) return g_tile == 128;
@@ -799,14 +804,14 @@ int64_t workspace_of(int64_t head_dim, int64_t batch, int64_t rows, int64_t num_
     return most == 1 ? 16 : most * rows * num_heads * (head_dim + 2) * 4;
 }
 
-template <int D, int TEAM>
+template <int D, int TEAM, bool HALF>
 int launch(const PromptArgs &a, hipStream_t st) {
     constexpr int lds = Shape<D, TEAM>::kLds;
-    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_prompt_kernel<D, TEAM>,
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)attn_mx4_prompt_kernel<D, TEAM, HALF>,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     DOE_HIP_CHECK(attr_rc);
     const dim3 grid((unsigned)(a.tiles * a.c.kv_heads), (unsigned)a.splits);
-    hipLaunchKernelGGL((attn_mx4_prompt_kernel<D, TEAM>), grid, dim3(64 * kWaves), lds, st, a);
+    hipLaunchKernelGGL((attn_mx4_prompt_kernel<D, TEAM, HALF>), grid, dim3(64 * kWaves), lds, st, a);
     DOE_LAUNCH_CHECK("attn_mx4_prompt_kernel");
     if (a.splits == 1) return DOE_OK;
     const int64_t pairs = (int64_t)a.rows * a.num_heads, each = 1024 / D;
@@ -818,9 +823,9 @@ int launch(const PromptArgs &a, hipStream_t st) {
 template <int D>
 int launch_d(PromptArgs &a, bool share, hipStream_t st) {
     if constexpr (D < 512) {
-        if (share) return launch<D, 4>(a, st);
+        if (share) return a.q_f16 ? launch<D, 4, true>(a, st) : launch<D, 4, false>(a, st);
     }
-    return launch<D, 1>(a, st);
+    return a.q_f16 ? launch<D, 1, true>(a, st) : launch<D, 1, false>(a, st);
 }
 
 }  // namespace

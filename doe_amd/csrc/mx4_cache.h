@@ -89,6 +89,27 @@ __device__ __forceinline__ float mx4_tanh(float x) {
     return u < 0.3f ? x * p : copysignf(q, x);
 }
 
+// A query's f32 values go to the matrix cores as f16 hi and lo parts of q 2^e, e such
+// that the largest (its bits without the sign: `top`) lies in [2^13, 2^14): of a value
+// at most 2^-22 is lost, or 2^-38 of the largest where that is more.
+__device__ __forceinline__ int mx4_query_exp(uint32_t top) {
+    if (top == 0 || top >= 0x7f800000u) return 0;
+    const int e = 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));  // (-114 at the least)
+    return e > 100 ? 100 : e;
+}
+// Takes that 2^e out of a score again, with the call's own factor f: s = s * pre * post.
+// pre is 1 unless f 2^-e overflows (then f > 1, so that s pre overflows with s only).
+// A query that is no number has scores that are none.
+struct Mx4Factor {
+    float pre, post;
+};
+__device__ __forceinline__ Mx4Factor mx4_factor(float f, uint32_t top, int e) {
+    if (top >= 0x7f800000u) return {1.0f, __uint_as_float(0x7fc00000u)};
+    const float post = __builtin_amdgcn_ldexpf(f, -e);
+    if (fabsf(post) < __uint_as_float(0x7f800000u)) return {1.0f, post};
+    return {__builtin_amdgcn_ldexpf(1.0f, -e), f};
+}
+
 // Checks a cache and turns it into the kernels' form; returns a DOE status.
 int mx4_view(const doe_mx4_cache *cache, Mx4View *view);
 // What both attentions check of a call.

@@ -539,8 +539,9 @@ int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_
  * > 0 keeps the last sliding_window positions; softcap > 0 applies tanh(s /
  * cap) * cap; a sequence without keys gives zeros.  num_heads any multiple of
  * num_kv_heads.  f32-accurate (2-4e-7 from float64 with f32 queries and
- * output).  The work is divided over the device by the lengths that the
- * kernel reads, so ragged batches fill it evenly.
+ * output): f32 queries keep 22 bits of each dim, down to 2^-38 of a head's
+ * largest.  The work is divided over the device by the lengths that the kernel
+ * reads, so ragged batches fill it evenly.
  * The workspace (16-byte aligned, doe_attn_mx4_decode_workspace bytes) is the
  * caller's: calls that may overlap, and captured graphs that may be replayed
  * side by side, each take their own.  Nothing is kept in it between calls. */
@@ -552,13 +553,11 @@ int doe_attn_mx4_decode(const doe_mx4_cache *cache, const void *q, int q_f16, vo
 /* The prompt form: rows of q and out as in doe_mx4_kv_write (row_starts,
  * rows; q_row_stride and out_row_stride elements apart), row i of the n of a
  * sequence at position kv_lens[b] - n + i, causal.  Rows of no sequence are
- * left as they were; a row at a position below 0 gives zeros.  Scores are
- * products of the cache's codes as they stand and digits of the queries: 25
- * bits of the largest value of every 32 dims (a dim 2^n below that keeps n
- * fewer); probabilities are f16 hi + lo.  2-4e-7 from float64 with normal queries,
- * 1.5e-5 with single dims 2^11 above the others where the keys are zero; an f16
- * output adds its rounding, 2e-4.  A short prompt over a long cache splits its
- * keys over the device and joins them through the workspace. */
+ * left as they were; a row at a position below 0 gives zeros.  f16 queries are
+ * taken as they are, f32 ones as in the token form; probabilities are f16 hi +
+ * lo.  2-3e-7 from float64, and an f16 output's rounding, 2e-4.  A short prompt
+ * over a long cache splits its keys over the device and joins them through the
+ * workspace. */
 int doe_attn_mx4_prompt_workspace(int64_t batch, int64_t rows, int64_t num_heads, int64_t num_kv_heads,
                                   int64_t head_dim, int64_t *bytes);
 int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, int64_t q_row_stride, void *out,

@@ -3,8 +3,9 @@ little but an output's rounding may be lost (tests/mx4_cases.py derives the boun
 import numpy as np
 import pytest
 
+from doe_amd import DeviceBuffer, mx4, ops
 from mx4_cases import Case, attention, check
-from test_gpu_mx4_attention import prompt, tile  # noqa: F401  (a fixture)
+from test_gpu_mx4_attention import prompt, tile, up  # noqa: F401  (a fixture among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +24,46 @@ def test_f16_prompts_lose_their_rounding_only(dev, tile, d, hq, hkv):  # noqa: F
     got = prompt(case, q, rows, f16=True)
     want, bound, _ = attention(case, q, rows, d ** -0.5, digits=2.0 ** -24)
     check(got, want, bound, got.dtype)
+
+
+@pytest.mark.parametrize("d", [64, 128, 160, 256, 512])
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_dims_far_below_the_largest(dev, tile, d, f16):  # noqa: F811
+    """Dims of 2^15 (f16: the largest of the type) among normal ones, keys zero there: the
+    others make the scores and keep their bits.  f16 queries lose nothing, of f32 ones
+    2^-38 of the largest may be lost beside the 2^-22 that the bound counts of each."""
+    rng = np.random.default_rng(d)
+    rows, lens, hq = [30, 20], [70, 40], 3
+    case = Case(rng, lens, head_dim=d, num_kv_heads=1, page_size=32)
+    wide = np.arange(0, d, 32) + 2 * rng.integers(0, 16, d // 32)
+    case.kc[..., wide] = 0
+    case.upload()
+    q = rng.standard_normal((sum(rows), hq, d)).astype(np.float16 if f16 else np.float32)
+    q[..., wide] = rng.choice([-65504.0, 65504.0] if f16 else [-32768.0, 32768.0], q[..., wide].shape)
+    print(f"[far] d={d} f16={f16}", flush=True)
+    starts, out = up(np.cumsum([0] + rows).astype(np.int32)), up(np.zeros(q.shape, np.float32))
+    ws = DeviceBuffer(ops.attention_mx4_workspace(2, hq, 1, d, len(q)))
+    ops.attention_mx4_prompt(case.cache, up(q), out, len(q), row_starts=starts, num_heads=hq, scale=d ** -0.5, q_f16=f16,
+                             workspace=ws)
+    # (the scores' sum by the dims that the keys have: the others add nothing to it)
+    want, bound, mass = attention(case, q * (~np.isin(np.arange(d), wide)), rows, d ** -0.5)
+    if not f16:
+        keys = np.abs(np.where(case.ks[..., None] == mx4.NAN_SCALE, 0, mx4.dequantise(case.kc, np.minimum(case.ks, 140))
+                               .reshape(*case.ks.shape, 32))).sum((-1, -2)).max()
+        bound = bound + 2 * 2.0 ** -38 * 32768 * d ** -0.5 * keys * mass
+    check(out.download(), want, bound, np.float32)
+
+
+@pytest.mark.parametrize("d", [64, 160, 512])
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompt_queries_that_are_no_numbers(dev, tile, d, f16):  # noqa: F811
+    """A NaN or an infinity in any dim of a query makes its own output NaN, and no other."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [70], head_dim=d, num_kv_heads=1, page_size=32)
+    case.upload()
+    q = rng.standard_normal((40, 3, d)).astype(np.float16 if f16 else np.float32)
+    bad = np.zeros((40, 3), bool)
+    for row, head, dim, value in ((0, 0, 0, np.nan), (7, 2, d - 1, np.inf), (20, 1, d // 2 + 3, -np.inf), (39, 0, 37, -np.nan)):
+        q[row, head, dim], bad[row, head] = value, True
+    got = prompt(case, q, [40], f16=f16)
+    assert np.array_equal(np.isnan(got), np.repeat(bad[..., None], d, -1))
