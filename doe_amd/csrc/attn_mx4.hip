@@ -34,6 +34,7 @@
 
 namespace {
 
+using doe::Mx4Factor;
 using doe::Mx4Slab;
 using doe::Mx4View;
 
@@ -70,6 +71,10 @@ constexpr int workgroups() { return 256 * per_cu<D>(); }
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return std::max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
 }
 // The same query row's value in the other half (hi / lo) of its sixteen.
 __device__ __forceinline__ float other_half(float v) { return dpp<0x128>(v); }
@@ -223,11 +228,15 @@ __device__ __forceinline__ void scores(f32x4 *s, const h8 (*q)[64], const KBlock
 // reference raised and its sum carried on.  `lo_part`: 1 in the lanes of P's lo
 // part, 0 in those of its hi part.
 template <int D>
-__device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f32x4 *s, float rowf, float lo_part, int p0,
-                                      int lo, int hi, int g4) {
-    float v[8], y[8];
+__device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f32x4 *s, const Mx4Factor &factor, bool large,
+                                      float lo_part, int p0, int lo, int hi, int g4) {
+    float v[8], y[8], rowf = factor.post;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3]);
+    if (large) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= factor.pre;
+    }
     if (a.softcap > 0.0f) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = doe::mx4_tanh(v[j] * rowf);
@@ -313,15 +322,15 @@ template <int D>
 struct TokenLds {
     static constexpr int kRow = D + 4;
     h8 q[D / 32][64];  // a row's query operands
-    float rowf[kHeads];
+    Mx4Factor rowf[kHeads];
     float o[kWaves][kHeads][kRow];
     float2 ml[kWaves][kHeads];
 };
 
 // A row's queries, two heads a wave and D / 32 dims a lane, into operand order:
 // lane (c16, g4) of step i takes dims g4 D / 4 + 8 i .. of head c16 % 8, scaled
-// by a power of two (max near 2^14), the f16 hi part (c16 < 8) or the lo part;
-// rowf takes the scale out of a score again.  Heads that the row lacks are 0.
+// by a power of two, the f16 hi part (c16 < 8) or the lo part; rowf takes the
+// scale out of a score again.  Heads that the row lacks are 0.
 template <int D>
 struct RawQuery {
     static constexpr int N = D / 32;
@@ -346,33 +355,25 @@ template <int D>
 __device__ __forceinline__ void stage_query(const TokenArgs &a, const RawQuery<D> &r, TokenLds<D> &sm, int heads, int wave, int lane) {
     constexpr int N = RawQuery<D>::N;
     const int head = 2 * wave + (lane >> 5);
-    float amax = 0.0f;
+    uint32_t top = 0;  // (as bits: a NaN is above all)
 #pragma unroll
-    for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(r.f[i]));
-    amax = fmaxf(amax, dpp<0xB1>(amax));
-    amax = fmaxf(amax, dpp<0x4E>(amax));
-    amax = fmaxf(amax, dpp<0x141>(amax));
-    amax = fmaxf(amax, dpp<0x140>(amax));
-    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    int sg = 0;
-    if (amax > 0.0f && amax <= 3.0e38f) {
-        sg = 14 - __builtin_amdgcn_frexp_expf(amax);
-        sg = sg < -100 ? -100 : (sg > 100 ? 100 : sg);
-    }
-    const float sc = head < heads ? __builtin_amdgcn_ldexpf(1.0f, sg) : 0.0f;
+    for (int i = 0; i < N; ++i) top = std::max(top, __float_as_uint(r.f[i]) & 0x7fffffffu);
+    top = dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(top))));
+    top = std::max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    const int e = doe::mx4_query_exp(top);
     _Float16 *q = reinterpret_cast<_Float16 *>(sm.q);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int d = (lane & 31) * N + i, in = d % (D / 4);
-        const float v = head < heads ? r.f[i] * sc : 0.0f;
+        const float v = head < heads ? __builtin_amdgcn_ldexpf(r.f[i], e) : 0.0f;
         const _Float16 h = (_Float16)v;
         _Float16 *to = q + ((in / 8) * 64 + d / (D / 4) * 16 + head) * 8 + in % 8;
         to[0] = h;
         to[64] = (_Float16)(v - (float)h);
     }
     if ((lane & 31) == 0) {
-        const float f = a.scale * __builtin_amdgcn_ldexpf(1.0f, -sg);
-        sm.rowf[head] = a.softcap > 0.0f ? f / a.softcap : f * 1.4426950408889634f;
+        const float f = a.softcap > 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
+        sm.rowf[head] = doe::mx4_factor(f, top, e);
     }
 }
 
@@ -506,7 +507,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
         load_v<D, NT>(vb, slab_of(page), shift, place(0), at_lane);
         stage_query<D>(a, raw, sm, heads, wave, lane);  // (while the first block is under way)
         __syncthreads();
-        const float rowf = sm.rowf[c16 & 7], lo_part = c16 < 8 ? 0.0f : 1.0f;
+        const Mx4Factor rowf = sm.rowf[c16 & 7];
+        const float lo_part = c16 < 8 ? 0.0f : 1.0f;
+        const bool large = __any(rowf.pre != 1.0f);
         State<D> st;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) st.o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -525,7 +528,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
             __builtin_amdgcn_sched_barrier(0);
             load_k<D, NT>(kb, slab, shift, place(in), at_lane);
             __builtin_amdgcn_sched_barrier(0);
-            const h8 pf = weights<D>(a, st, s, rowf, lo_part, p0, lo, top, g4);
+            const h8 pf = weights<D>(a, st, s, rowf, large, lo_part, p0, lo, top, g4);
             values<D>(st, pf, vb, p0, lo, top, c16, g4);
             __builtin_amdgcn_sched_barrier(0);
             load_v<D, NT>(vb, slab, shift, place(in), at_lane);

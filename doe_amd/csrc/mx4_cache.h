@@ -94,8 +94,7 @@ __device__ __forceinline__ float mx4_tanh(float x) {
 // at most 2^-22 is lost, or 2^-38 of the largest where that is more.
 __device__ __forceinline__ int mx4_query_exp(uint32_t top) {
     if (top == 0 || top >= 0x7f800000u) return 0;
-    const int e = 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));  // (-114 at the least)
-    return e > 100 ? 100 : e;
+    return 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));  // -114 .. 162
 }
 // Takes that 2^e out of a score again, with the call's own factor f: s = s * pre * post.
 // pre is 1 unless f 2^-e overflows (then f > 1, so that s pre overflows with s only).

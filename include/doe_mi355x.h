@@ -540,8 +540,9 @@ int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_
  * cap) * cap; a sequence without keys gives zeros.  num_heads any multiple of
  * num_kv_heads.  f32-accurate (2-4e-7 from float64 with f32 queries and
  * output): f32 queries keep 22 bits of each dim, down to 2^-38 of a head's
- * largest.  The work is divided over the device by the lengths that the kernel
- * reads, so ragged batches fill it evenly.
+ * largest; scores beyond f32's range are no numbers unless capped.  The work is
+ * divided over the device by the lengths that the kernel reads, so ragged batches
+ * fill it evenly.
  * The workspace (16-byte aligned, doe_attn_mx4_decode_workspace bytes) is the
  * caller's: calls that may overlap, and captured graphs that may be replayed
  * side by side, each take their own.  Nothing is kept in it between calls. */

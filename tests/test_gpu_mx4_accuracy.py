@@ -5,7 +5,7 @@ import pytest
 
 from doe_amd import DeviceBuffer, mx4, ops
 from mx4_cases import Case, attention, check
-from test_gpu_mx4_attention import prompt, tile, up  # noqa: F401  (a fixture among them)
+from test_gpu_mx4_attention import prompt, tile, token, up  # noqa: F401  (a fixture among them)
 
 pytestmark = pytest.mark.gpu
 
@@ -66,4 +66,51 @@ def test_prompt_queries_that_are_no_numbers(dev, tile, d, f16):  # noqa: F811
     for row, head, dim, value in ((0, 0, 0, np.nan), (7, 2, d - 1, np.inf), (20, 1, d // 2 + 3, -np.inf), (39, 0, 37, -np.nan)):
         q[row, head, dim], bad[row, head] = value, True
     got = prompt(case, q, [40], f16=f16)
+    assert np.array_equal(np.isnan(got), np.repeat(bad[..., None], d, -1))
+
+
+@pytest.mark.parametrize("form", ["token", "prompt"])
+@pytest.mark.parametrize("d", [64, 160, 512])
+def test_queries_at_the_end_of_the_range(dev, form, d):
+    """Finite f32 queries up to the type's largest, whatever the scale: scores that f32
+    holds are right, also zero ones of a scale that overflows with the query's, and a
+    cap holds those that overflow."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [300, 40], head_dim=d, num_kv_heads=1, page_size=32)
+    case.kc[..., 5] = 0
+    case.upload()
+    call = token if form == "token" else (lambda c, q, **kw: prompt(c, q, [1, 1], **kw))
+    normal = rng.standard_normal((2, 2, d)).astype(np.float32)
+    largest = normal.copy()
+    largest[..., 5] = np.finfo(np.float32).max
+    for name, q, scale, softcap in (("1e36", normal * np.float32(1e36), 1e-37, 0.0), ("1e36", normal * np.float32(1e36), 1e-36, 5.0),
+                                    ("1e37", normal * np.float32(3e37), 3e-39, 0.0), ("1e-40", normal * np.float32(1e-40), 1e38, 0.0),
+                                    ("largest", largest * np.float32(1), 1e-30, 0.0)):
+        print(f"[{form}] d={d} {name} scale={scale} softcap={softcap}", flush=True)
+        got = call(case, q, scale=scale, softcap=softcap)
+        check(got, *attention(case, q.astype(np.float32) * (name != "largest"), [1, 1], float(np.float32(scale)), softcap)[:2], got.dtype)
+    # 2 ds + 2^-16 + 2^-18 of the mass, ds 2^-21 of the cap: no other part of the scores is left
+    q = normal * np.float32(1e36)
+    got = call(case, q, scale=1e5, softcap=30.0)
+    want, _, mass = attention(case, q, [1, 1], 1e5, 30.0)
+    check(got, want, (60 * 2.0 ** -21 + 2.0 ** -16 + 2.0 ** -18) * mass + 2.0 ** -32 * 300 * 6, got.dtype)
+    case.kc[case.ks[..., None].repeat(32, -1).reshape(case.kc.shape) != mx4.NAN_SCALE] = 0
+    case.pool.upload(case.pages())
+    for softcap in (0.0, 30.0):
+        got = call(case, q, scale=1e5, softcap=softcap)
+        check(got, *attention(case, q, [1, 1], 1e5, softcap)[:2], got.dtype)
+
+
+@pytest.mark.parametrize("d", [64, 160, 512])
+@pytest.mark.parametrize("f16", [False, True])
+def test_token_queries_that_are_no_numbers(dev, d, f16):
+    """A NaN or an infinity in any dim of a query makes its own output NaN, and no other."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [70, 1, 900, 0], head_dim=d, num_kv_heads=1, page_size=32)
+    case.upload()
+    q = rng.standard_normal((4, 12, d)).astype(np.float16 if f16 else np.float32)
+    bad = np.zeros((4, 12), bool)
+    for row, head, dim, value in ((0, 0, 0, np.nan), (1, 2, d - 1, np.inf), (2, 11, d // 2 + 3, -np.inf), (2, 6, 37, -np.nan)):
+        q[row, head, dim], bad[row, head] = value, True
+    got = token(case, q, f16=f16)
     assert np.array_equal(np.isnan(got), np.repeat(bad[..., None], d, -1))
