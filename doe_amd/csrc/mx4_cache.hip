@@ -422,6 +422,9 @@ int mx4_attention_checks(const Mx4View &c, int64_t num_heads, float scale, float
                 (double)softcap);
     DOE_REQUIRE(softcap == 0.0f || isfinite(scale / softcap), DOE_E_INVALID, "softcap %g too small for scale %g",
                 (double)softcap, (double)scale);
+    // (scores and caps are held in powers of two)
+    DOE_REQUIRE(isfinite(scale * 1.4426950408889634f) && isfinite(softcap * 1.4426950408889634f), DOE_E_INVALID,
+                "scale %g or softcap %g above 2.35e38", (double)scale, (double)softcap);
     DOE_REQUIRE(sliding_window >= 0 && sliding_window < ((int64_t)1 << 30), DOE_E_INVALID, "sliding_window %lld",
                 (long long)sliding_window);
     DOE_REQUIRE(c.batch == 0 || (q && out), DOE_E_INVALID, "null pointer");
