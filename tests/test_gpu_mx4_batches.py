@@ -1,0 +1,92 @@
+"""Attention over the 4-bit cache with more sequences than a wave or the device looks at
+once, and prompts of one row a sequence without row_starts, against the formula in 64
+bits (tests/mx4_cases.py derives the bounds)."""
+import numpy as np
+import pytest
+
+from doe_amd import DeviceBuffer, ops
+from mx4_cases import Case, attention, check
+from test_gpu_mx4_attention import prompt, tile, token, up  # noqa: F401  (a fixture among them)
+
+pytestmark = pytest.mark.gpu
+
+# sequences, (share of them, shortest, longest) of their lengths, head_dim, heads, KV heads
+MANY = {
+    # more rows than workgroups (768 at 64), a few of them split
+    "more rows than workgroups": (1000, ((0.97, 0, 60), (0.03, 500, 3000)), 64, 2, 1),
+    # the same with few sequences
+    "many KV heads": (60, ((0.9, 1, 40), (0.1, 700, 1500)), 64, 16, 16),
+    # rows between half and all of the workgroups, half of them split in two: more pieces
+    # than workgroups
+    "more pieces than workgroups": (150, ((0.5, 1, 31), (0.5, 1450, 1500)), 64, 8, 4),
+    "more pieces than workgroups, few sequences": (40, ((0.5, 1, 31), (0.5, 1450, 1500)), 64, 16, 16),
+    # more than one search step, every row whole or split
+    "sequences beyond a wave": (130, ((0.9, 0, 300), (0.1, 2000, 4000)), 128, 2, 1),
+    "head_dim 512": (70, ((0.8, 0, 40), (0.2, 400, 900)), 512, 8, 4),
+    "rows of two parts of a head group": (100, ((0.9, 0, 90), (0.1, 600, 2000)), 160, 24, 2),
+}
+
+
+def lengths(rng, batch, shares):
+    lens = np.concatenate([rng.integers(lo, hi + 1, int(round(batch * part))) for part, lo, hi in shares])
+    return [int(n) for n in rng.permutation(lens)[:batch]]
+
+
+@pytest.mark.parametrize("name", MANY)
+@pytest.mark.parametrize("window", [0, 400])
+def test_tokens_of_many_sequences(dev, name, window):
+    batch, shares, d, hq, hkv = MANY[name]
+    rng = np.random.default_rng(batch)
+    case = Case(rng, lengths(rng, batch, shares), head_dim=d, num_kv_heads=hkv, page_size=32)
+    case.upload()
+    q = rng.standard_normal((case.batch, hq, d)).astype(np.float32)
+    print(f"[many] {name} window={window}", flush=True)
+    got = token(case, q, sliding_window=window)
+    want, bound, _ = attention(case, q, [1] * case.batch, d ** -0.5, 0.0, window)
+    check(got, want, bound, got.dtype)
+    assert np.array_equal(token(case, q, sliding_window=window), got)
+
+
+@pytest.mark.parametrize("batch,longest,d,hq,hkv", [
+    (3, 3000, 128, 8, 2),      # few rows: keys split
+    (150, 90, 128, 8, 2),      # none split
+    (5, 500, 64, 80, 2),       # 40 heads a KV head: two tiles of 32 a row
+    (40, 60, 64, 160, 1),      # 160: five of 32, two of 128
+    (2, 2000, 160, 160, 1),    # and split
+    (3, 700, 256, 4, 4), (2, 900, 512, 40, 1)])
+@pytest.mark.parametrize("f16", [False, True])
+def test_prompts_of_one_row_without_row_starts(dev, tile, batch, longest, d, hq, hkv, f16):  # noqa: F811
+    rng = np.random.default_rng(batch + d)
+    lens = [longest, 0] + [int(n) for n in rng.integers(1, longest, batch - 2)] if batch > 2 else [longest, 33]
+    case = Case(rng, lens, head_dim=d, num_kv_heads=hkv, page_size=32)
+    case.upload()
+    t = np.float16 if f16 else np.float32
+    q = rng.standard_normal((batch, hq, d)).astype(t)
+    out = up(np.full(q.shape, 7, t))
+    ws = DeviceBuffer(ops.attention_mx4_workspace(batch, hq, hkv, d, batch))
+    print(f"[rows] batch={batch} d={d} hq={hq} hkv={hkv} f16={f16}", flush=True)
+    ops.attention_mx4_prompt(case.cache, up(q), out, batch, num_heads=hq, scale=d ** -0.5, q_f16=f16, out_f16=f16, workspace=ws)
+    want, bound, _ = attention(case, q, [1] * batch, d ** -0.5)
+    check(out.download(), want, bound, t)
+
+
+@pytest.mark.parametrize("batch,most,longest", [(200, 5, 90), (130, 40, 60), (67, 3, 4000)])
+def test_many_short_prompts(dev, tile, batch, most, longest):  # noqa: F811
+    """Sequences without rows among them, the first 64 all of that kind."""
+    rng = np.random.default_rng(batch)
+    rows = [0] * 64 + [int(n) for n in rng.integers(0, most + 1, batch - 64)]
+    rows[-1], rows[-2] = most, 0
+    lens = [n + int(rng.integers(0, longest)) for n in rows]
+    case = Case(rng, lens, head_dim=64, num_kv_heads=1, page_size=32)
+    case.upload()
+    q = rng.standard_normal((sum(rows), 5, 64)).astype(np.float32)
+    print(f"[many] batch={batch} rows={sum(rows)}", flush=True)
+    got = prompt(case, q, rows, skip=3, behind=2)
+    want, bound, _ = attention(case, q, rows, 0.125)
+    check(got, want, bound, got.dtype)
+    # and the other way round: the last sequences without rows
+    case = Case(rng, lens[::-1], head_dim=64, num_kv_heads=1, page_size=32)
+    case.upload()
+    got = prompt(case, q, rows[::-1], skip=3, behind=2)
+    want, bound, _ = attention(case, q, rows[::-1], 0.125)
+    check(got, want, bound, got.dtype)
