@@ -58,8 +58,6 @@ struct TokenArgs {
     int2 *joined;   // by_row: a row's first part (-1: not split) and their number; else at a row's first part the row and that number (others: -1)
 };
 
-constexpr int64_t kCacheBytes = (int64_t)256 << 20;
-
 // Workgroups of four waves that a CU holds at once, by the registers that a wave
 // takes, and those that fill the device's 256 CUs in one round (head_dim 128: four
 // leave a wave fewer registers, 56.6 us for 55.6 over 8 sequences of 32768).
@@ -683,6 +681,23 @@ int launch_token(const TokenArgs &a, unsigned wgs, hipStream_t st) {
     return DOE_OK;
 }
 
+// Whether a call reads its pages past the 256 MB last-level cache: when it may read
+// more than half of that, up to head_dim 128 and with one row a KV head.  Up to there a
+// lane has its piece of K in one load; wider ones take several, and further rows the
+// same pages again, each a read of memory.  Past the cache and through it, pools of
+// layers in turn (one pool again and again in brackets), 16 sequences: 4 KV heads of 128
+// with 8 heads each 70 MB 23.7 and 24.2 us (22.7, 22.0), 140 MB 34.5 and 36.2 (33.6,
+// 31.6), 290 MB 58.0 and 62.8 (58.2, 56.7); with 16 heads each 290 MB 107 and 96; of
+// 256 290 MB 80 and 62, of 512 123 and 67; 16 of 160 74 and 64.
+template <int D>
+bool past_caches(const TokenArgs &a) {
+    if (D > 128 || a.groups > 1) return false;
+    int64_t pages = a.c.table_stride;  // of a sequence
+    if (a.window > 0) pages = std::min<int64_t>(pages, (a.window >> a.c.page_shift) + 2);
+    pages = std::min<int64_t>(a.c.num_pages, pages * a.c.batch);
+    return (pages * a.c.kv_heads * (D + D / 16) << a.c.page_shift) > ((int64_t)128 << 20);
+}
+
 template <int D>
 int launch(TokenArgs &a, void *ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.c.batch * a.c.kv_heads * a.groups;
@@ -696,11 +711,7 @@ int launch(TokenArgs &a, void *ws, hipStream_t st) {
         a.part = static_cast<float *>(ws);
         a.joined = reinterpret_cast<int2 *>(a.part + wgs * kHeads * (D + 2));
     }
-    // A pool that the 256 MB last-level cache cannot hold is read past it (8 sequences
-    // of 32768 in 302 MB: 55.6 us, through it 60.7; 48 ragged ones in 90 MB through it
-    // 23.6, past it 25.9).
-    const bool stream = ((int64_t)a.c.num_pages * a.c.kv_heads * (D + D / 16) << a.c.page_shift) > kCacheBytes;
-    const int rc = stream ? launch_token<D, true>(a, (unsigned)wgs, st) : launch_token<D, false>(a, (unsigned)wgs, st);
+    const int rc = past_caches<D>(a) ? launch_token<D, D <= 128>(a, (unsigned)wgs, st) : launch_token<D, false>(a, (unsigned)wgs, st);
     if (rc) return rc;
     if (a.per_row) return DOE_OK;
     hipLaunchKernelGGL(attn_mx4_join_kernel<D>, dim3((unsigned)(a.by_row ? rows : wgs), (unsigned)a.heads), dim3(kJoin), 0, st, a,

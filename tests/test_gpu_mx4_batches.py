@@ -4,7 +4,7 @@ bits (tests/mx4_cases.py derives the bounds)."""
 import numpy as np
 import pytest
 
-from doe_amd import DeviceBuffer, ops
+from doe_amd import DeviceBuffer, mx4, ops
 from mx4_cases import Case, attention, check
 from test_gpu_mx4_attention import prompt, tile, token, up  # noqa: F401  (a fixture among them)
 
@@ -90,3 +90,23 @@ def test_many_short_prompts(dev, tile, batch, most, longest):  # noqa: F811
     got = prompt(case, q, rows[::-1], skip=3, behind=2)
     want, bound, _ = attention(case, q, rows[::-1], 0.125)
     check(got, want, bound, got.dtype)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 2), (128, 8, 2), (128, 20, 2), (160, 8, 2), (512, 4, 2)])
+def test_tokens_that_may_read_past_the_caches(dev, d, hq, hkv):
+    """A call that may read more than half the last-level cache gives the bits of one that
+    may not, with the same table."""
+    rng = np.random.default_rng(d + hq)
+    size = mx4.page_bytes(64, hkv, d)
+    pages = (150 << 20) // size
+    case = Case(rng, [700, 31, 0, 2000], head_dim=d, num_kv_heads=hkv, page_size=64, stride=pages // 4 + 1)
+    case.upload()
+    q = rng.standard_normal((4, hq, d)).astype(np.float32)
+    small = token(case, q)
+    check(small, *attention(case, q, [1] * 4, d ** -0.5)[:2], small.dtype)
+    pool = DeviceBuffer(pages * size)
+    pool.view(0, case.pool.nbytes).upload(case.pages())
+    case.cache = ops.Mx4Cache(pool, case.table_dev, case.lens_dev, num_pages=pages, page_size=64, num_kv_heads=hkv,
+                              head_dim=d, batch=4, table_stride=case.stride)
+    assert np.array_equal(token(case, q), small)
+    pool.free()
