@@ -77,20 +77,6 @@ __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
 // The same query row's value in the other half (hi / lo) of its sixteen.
 __device__ __forceinline__ float other_half(float v) { return dpp<0x128>(v); }
 
-// Inclusive sum over the wave's lanes, in registers.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xf>(v);  // one lane further within sixteen, two, four, eight
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);        // the last lane of a sixteen to the next (rows 1 and 3)
-    return dpp_add<0x143, 0xc>(v);     // lane 31 to rows 2 and 3
-}
-
 // Blocks of the rows of a sequence of hi positions, the first seen one at lo; at
 // least one (of an empty sequence it gives the zeros).
 __device__ __forceinline__ int first_seen(const TokenArgs &a, int hi) { return a.window > 0 && hi > a.window ? hi - a.window : 0; }
@@ -175,24 +161,6 @@ __device__ __forceinline__ void load_v(VBlock<D> &b, const uint8_t *slab, int sh
     if constexpr (D == 160) load_words<NT, 2>(b.vs + 2, vs + (at.vs / 8 % 5 < 4 ? 8 : 0));
 }
 
-// A scale byte as the conversions take it: they look at the exponent field alone,
-// so the other bits may hold the byte's neighbours.
-__device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
-    return __uint_as_float(byte == 3 ? word >> 1 : word << (23 - 8 * byte));
-}
-template <int BYTE>
-__device__ __forceinline__ h2 pair(uint32_t word, float s) {
-    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, s, BYTE);
-}
-__device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
-    switch (byte & 3) {
-        case 0: return pair<0>(word, s);
-        case 1: return pair<1>(word, s);
-        case 2: return pair<2>(word, s);
-        default: return pair<3>(word, s);
-    }
-}
-
 // A row's running state in a wave: O^T tile T, dims (4 g4 + i) D / 16 + T of
 // query row c16; P is 2^(score - m), l its sum.
 template <int D>
@@ -212,10 +180,10 @@ __device__ __forceinline__ void scores(f32x4 *s, const h8 (*q)[64], const KBlock
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float f;
-            if constexpr (D == 160) f = byte_scale(g4 + i >= 4 ? b.ks[t] >> 8 : b.ks[t], 0);
-            else f = byte_scale(b.ks[t], D >= 128 ? i / 4 : 0);
+            if constexpr (D == 160) f = doe::mx4_byte_scale(g4 + i >= 4 ? b.ks[t] >> 8 : b.ks[t], 0);
+            else f = doe::mx4_byte_scale(b.ks[t], D >= 128 ? i / 4 : 0);
             const uint32_t w = b.k[t][i];
-            const h2 k0 = pair<0>(w, f), k1 = pair<1>(w, f), k2 = pair<2>(w, f), k3 = pair<3>(w, f);
+            const h2 k0 = doe::mx4_pair<0>(w, f), k1 = doe::mx4_pair<1>(w, f), k2 = doe::mx4_pair<2>(w, f), k3 = doe::mx4_pair<3>(w, f);
             const h8 kf = {k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]};
             s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, s[t], 0, 0, 0);
         }
@@ -287,8 +255,8 @@ __device__ __forceinline__ void values(State<D> &st, const h8 pf, const VBlock<D
     float vs[8], vs2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        vs[j] = byte_scale(b.vs[j >> 2], j & 3);
-        if constexpr (D == 160) vs2[j] = byte_scale(b.vs[2 + (j >> 2)], j & 3);
+        vs[j] = doe::mx4_byte_scale(b.vs[j >> 2], j & 3);
+        if constexpr (D == 160) vs2[j] = doe::mx4_byte_scale(b.vs[2 + (j >> 2)], j & 3);
     }
     if (p0 < lo || p0 + 32 > hi) {
 #pragma unroll
@@ -307,7 +275,7 @@ __device__ __forceinline__ void values(State<D> &st, const h8 pf, const VBlock<D
             const int at = j * (D / 32) + i;
             float f = vs[j];
             if constexpr (D == 160) f = 5 * c16 % 16 + i >= 16 ? vs2[j] : f;
-            v[j] = pair_at(b.v[at >> 2], f, at);
+            v[j] = doe::mx4_pair_at(b.v[at >> 2], f, at);
         }
         const h8 v0 = {v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
         const h8 v1 = {v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
@@ -390,7 +358,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
         lens = b0 + lane < a.c.batch ? doe::mx4_len(a.c, b0 + lane) : 0;
     };
     auto cut = [&] { pieces_ = b0 + lane < a.c.batch ? (int)(((uint32_t)blocks_of(a, lens) + share - 1) / share) : 0; };
-    auto sum_of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(wave_scan(v), 63) * rows_of; };
+    auto sum_of = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(doe::wave_scan(v), 63) * rows_of; };
     int item = blockIdx.x, items0 = 0, slots0 = 0;  // items and split ones before sequence b0
     bool dense = true;                              // as many slots as items
     const bool one = a.c.batch == 1 && a.by_row;
@@ -457,9 +425,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void attn_mx4_token_kerne
         } else {
             for (;;) {
                 if (b0 >= a.c.batch) return;
-                const int upto = wave_scan(pieces_);
+                const int upto = doe::wave_scan(pieces_);
                 const uint64_t behind = __ballot(items0 + upto * rows_of > item);
-                const int split = dense ? 0 : wave_scan(pieces_ > 1 ? pieces_ : 0);
+                const int split = dense ? 0 : doe::wave_scan(pieces_ > 1 ? pieces_ : 0);
                 if (behind) {
                     const int i = __builtin_ctzll(behind);
                     pieces = __builtin_amdgcn_readlane(pieces_, i);

@@ -82,19 +82,6 @@ struct Shape {
     static constexpr int kLds = kData + kScores + (D == 512 ? 0 : 1024);  // (512: half a CU's, to the byte)
 };
 
-template <int BYTE>
-__device__ __forceinline__ h2 pair(uint32_t word, float s) {
-    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, s, BYTE);
-}
-__device__ __forceinline__ h2 pair_at(uint32_t word, float s, int byte) {
-    switch (byte & 3) {
-        case 0: return pair<0>(word, s);
-        case 1: return pair<1>(word, s);
-        case 2: return pair<2>(word, s);
-        default: return pair<3>(word, s);
-    }
-}
-
 // A lane's dims of a row, of K and of the queries alike: operand o has eight, of the
 // 32 of group 2 (o / 4) + half (half: lane / 32); of a last group without a second
 // (head_dim 160) each half has 16.
@@ -171,10 +158,6 @@ __device__ __forceinline__ void load_v(VBlock<D, TEAM> &b, const uint8_t *slab, 
     }
 }
 
-// A scale byte as the conversions take it (they look at the exponent field alone).
-__device__ __forceinline__ float byte_scale(uint32_t word, int byte) {
-    return __uint_as_float(byte == 3 ? word >> 1 : word << (23 - 8 * byte));
-}
 // Whether one of the word's bytes is 255.
 __device__ __forceinline__ bool any_nan_scale(uint32_t w) { return ((~w - 0x01010101u) & w & 0x80808080u) != 0; }
 
@@ -193,8 +176,8 @@ __device__ __forceinline__ void v_scales(VScale<D, TEAM> &f, const VBlock<D, TEA
     for (int w = 0; w < (D == 160 ? 4 : 2); ++w) f.nan |= any_nan_scale(b.s[w]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        f.s[j] = byte_scale(b.s[j >> 2], j & 3);
-        if constexpr (D == 160) f.s2[j] = byte_scale(b.s[2 + (j >> 2)], j & 3);
+        f.s[j] = doe::mx4_byte_scale(b.s[j >> 2], j & 3);
+        if constexpr (D == 160) f.s2[j] = doe::mx4_byte_scale(b.s[2 + (j >> 2)], j & 3);
     }
     if (p0 < lo || p0 + 32 > hi || __any(f.nan)) {
 #pragma unroll
@@ -219,7 +202,7 @@ __device__ __forceinline__ void stage_v(uint8_t *dst, const VBlock<D, TEAM> &b, 
         const int at = j * N + i;
         float s = f.s[j];
         if constexpr (D == 160) s = 5 * c % 16 + i >= 16 ? f.s2[j] : s;
-        v[j] = pair_at(b.v[at >> 2], s, at);
+        v[j] = doe::mx4_pair_at(b.v[at >> 2], s, at);
     }
     to[(2 * i) * 16] = h8{v[0][0], v[1][0], v[2][0], v[3][0], v[4][0], v[5][0], v[6][0], v[7][0]};
     to[(2 * i + 1) * 16] = h8{v[0][1], v[1][1], v[2][1], v[3][1], v[4][1], v[5][1], v[6][1], v[7][1]};
@@ -266,9 +249,9 @@ __device__ __forceinline__ void split_query(h8 &hi, h8 &lo, const float *f, int 
 template <int D, int TEAM, bool HALF, int FROM, int TO>
 __device__ __forceinline__ void scores(const Query<D, TEAM, HALF> &q, const KBlock<D, TEAM> &k, f32x16 &acc) {
     if constexpr (FROM < TO) {
-        const float f = byte_scale(k.s[FROM / 8], FROM / 4 % 2 * 2);
+        const float f = doe::mx4_byte_scale(k.s[FROM / 8], FROM / 4 % 2 * 2);
         const uint32_t w = k.k[FROM];
-        const h2 k0 = pair<0>(w, f), k1 = pair<1>(w, f), k2 = pair<2>(w, f), k3 = pair<3>(w, f);
+        const h2 k0 = doe::mx4_pair<0>(w, f), k1 = doe::mx4_pair<1>(w, f), k2 = doe::mx4_pair<2>(w, f), k3 = doe::mx4_pair<3>(w, f);
         const h8 kf = {k0[0], k0[1], k1[0], k1[1], k2[0], k2[1], k3[0], k3[1]};
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q.hi[FROM], acc, 0, 0, 0);
         if constexpr (!HALF) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q.lo[FROM], acc, 0, 0, 0);
@@ -293,20 +276,6 @@ __device__ __forceinline__ void interleave() {
     }
 }
 
-// Inclusive sum over the wave's lanes, in registers.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xf>(v);
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);
-    return dpp_add<0x143, 0xc>(v);
-}
-
 // HALF: f16 queries.
 template <int D, int TEAM, bool HALF>
 __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel(PromptArgs a) {
@@ -327,7 +296,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
             const int i = b0 + lane;
             const int lo_ = i < a.c.batch ? a.row_starts[i] : 0, hi_ = i < a.c.batch ? a.row_starts[i + 1] : 0;
             const int rows = lo_ < 0 ? 0 : std::max(0, std::min(hi_, a.rows) - lo_);
-            const int upto = wave_scan((int)(((int64_t)rows * G + P::kRows - 1) / P::kRows));
+            const int upto = doe::wave_scan((int)(((int64_t)rows * G + P::kRows - 1) / P::kRows));
             const uint64_t behind = __ballot(upto > tile);
             if (behind) {
                 const int at = __builtin_ctzll(behind);
@@ -354,7 +323,6 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
     const int tile1 = std::min(pair0 + P::kRows, pairs) - 1, wave1 = std::min(wave0 + 32, pairs) - 1;
     const bool idle = wave1 < wave0;
     const int klo = from_of(pair0), khi = to_of(tile1);          // the tile's
-    const int wlo = from_of(wave0), whi = idle ? 0 : to_of(wave1);  // the wave's
     const int flo = idle ? 0 : from_of(wave1), fhi = to_of(std::min(wave0, pairs - 1));  // seen by all of its pairs
     const int mine = std::min(wave0 + n32, pairs - 1);
     const int lo = from_of(mine), hi = to_of(mine);

@@ -13,7 +13,6 @@
 
 namespace doe {
 
-constexpr int kMx4Block = 32;           // positions of a V block, and dims of a scale
 constexpr int kMx4MinExp = -23;         // every value exact in f16: 0.5 x 2^-23 is its
 constexpr int kMx4MaxExp = 13;          // least, 6 x 2^13 within its range
 constexpr int kMx4NanScale = 255;
@@ -76,6 +75,40 @@ __device__ __forceinline__ bool mx4_row(const Mx4View &c, const int32_t *row_sta
 __device__ __forceinline__ int mx4_page(const Mx4View &c, int b, int pos) {
     const int page = c.table[(int64_t)b * c.table_stride + (pos >> c.page_shift)];
     return page >= 0 && page < c.num_pages ? page : -1;
+}
+
+// Inclusive sum over the wave's lanes, in registers.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xf>(v);  // one lane further within sixteen, two, four, eight
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);     // the last lane of a sixteen to the next (rows 1 and 3)
+    return dpp_add<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+}
+
+// A scale byte as the conversions take it: they look at the exponent field alone,
+// so the other bits may hold the byte's neighbours.
+__device__ __forceinline__ float mx4_byte_scale(uint32_t word, int byte) {
+    return __uint_as_float(byte == 3 ? word >> 1 : word << (23 - 8 * byte));
+}
+// The two values of a byte of codes in f16, exactly.
+typedef _Float16 Mx4Pair __attribute__((ext_vector_type(2)));
+template <int BYTE>
+__device__ __forceinline__ Mx4Pair mx4_pair(uint32_t word, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, s, BYTE);
+}
+__device__ __forceinline__ Mx4Pair mx4_pair_at(uint32_t word, float s, int byte) {
+    switch (byte & 3) {
+        case 0: return mx4_pair<0>(word, s);
+        case 1: return mx4_pair<1>(word, s);
+        case 2: return mx4_pair<2>(word, s);
+        default: return mx4_pair<3>(word, s);
+    }
 }
 
 // tanh x to 2e-7 of itself, without a branch: (1 - e) / (1 + e), e = exp(-2 |x|), the

@@ -28,10 +28,6 @@ struct RowArgs {
     int64_t rows, row_stride;
 };
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
 // Bits of the largest magnitude over each 8 lanes, an infinity's or NaN's above
 // all others (as numbers a maximum would drop a NaN).
 __device__ __forceinline__ uint32_t max8(uint32_t v) {
