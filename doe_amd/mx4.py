@@ -31,7 +31,9 @@ def page_bytes(page_size: int, num_kv_heads: int, head_dim: int) -> int:
 def quantise(rows: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
     """Codes ``[..., D]`` and scale bytes ``[..., D / 32]`` (uint8) of f32 rows."""
     x = np.asarray(rows, np.float32)
-    b = x.reshape(*x.shape[:-1], -1, BLOCK)
+    if x.ndim == 0 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
+        raise ValueError(f"rows of shape {x.shape}: the last axis has to be a multiple of {BLOCK}")
+    b = x.reshape(*x.shape[:-1], x.shape[-1] // BLOCK, BLOCK)
     top = np.abs(b).max(-1)  # (a NaN is its block's maximum)
     finite = np.isfinite(top)
     bits = np.where(finite, top, 1).astype(np.float32).view(np.uint32)
@@ -55,16 +57,16 @@ def dequantise(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
     return (v.reshape(*s.shape, BLOCK) * s[..., None]).reshape(codes.shape).astype(np.float32)
 
 
-def _sections(page_size: int, head_dim: int) -> list[int]:
-    ps, d = page_size, head_dim
-    return list(np.cumsum([ps * d // 2, ps * d // 2, ps * d // 32]))
+def _widths(page_size: int, head_dim: int) -> list[int]:
+    """Bytes of a slab's K codes, V codes, K scales and V scales."""
+    return [page_size * head_dim // 2] * 2 + [page_size * head_dim // BLOCK] * 2
 
 
 def pack_pages(k_codes, k_scales, v_codes, v_scales) -> np.ndarray:
     """Pages ``[n][page_bytes]`` of codes ``[n][num_kv_heads][page_size][D]``
     and scale bytes ``[n][num_kv_heads][page_size][D / 32]``."""
     n, h, ps, d = k_codes.shape
-    page_bytes(ps, h, d)
+    size = page_bytes(ps, h, d)
 
     def two(x):
         return x[..., 0::2] | (x[..., 1::2] << 4)
@@ -72,7 +74,8 @@ def pack_pages(k_codes, k_scales, v_codes, v_scales) -> np.ndarray:
     vc = v_codes.reshape(n, h, ps // 32, 2, 4, 4, 16, d // 16).transpose(0, 1, 2, 4, 6, 3, 5, 7)
     vs = v_scales.reshape(n, h, ps // 32, 2, 4, 4, d // 32).transpose(0, 1, 2, 4, 6, 3, 5)
     parts = [two(k_codes), two(vc), k_scales, vs]
-    return np.concatenate([p.reshape(n, h, -1) for p in parts], -1).reshape(n, -1).astype(np.uint8)
+    slabs = np.concatenate([p.reshape(n, h, w) for p, w in zip(parts, _widths(ps, d))], -1)
+    return slabs.reshape(n, size).astype(np.uint8)
 
 
 def unpack_pages(pages: np.ndarray, page_size: int, num_kv_heads: int, head_dim: int):
@@ -81,7 +84,8 @@ def unpack_pages(pages: np.ndarray, page_size: int, num_kv_heads: int, head_dim:
     if pages.shape[-1] != page_bytes(ps, h, d):
         raise ValueError(f"pages of {pages.shape[-1]} bytes, expected {page_bytes(ps, h, d)}")
     n = pages.shape[0]
-    kc, vc, ks, vs = np.split(pages.reshape(n, h, -1), _sections(ps, d), axis=-1)
+    widths = _widths(ps, d)
+    kc, vc, ks, vs = np.split(pages.reshape(n, h, sum(widths)), np.cumsum(widths)[:3], axis=-1)
 
     def two(b):
         return np.stack([b & 15, b >> 4], -1)
