@@ -924,16 +924,23 @@ def tune(key: str, value: int) -> None:
 OPS = {
     "attention": attention,
     "attention_mx4": attention_mx4,
+    "attention_mx4_prompt": attention_mx4_prompt,
     "attention_prefill": attention_prefill,
     "dequant": dequant_q4k,
     "embed": embed,
     "gelu_gated": gelu_gated,
+    "kv_pages_compact": kv_pages_compact,
+    "kv_pages_copy": kv_pages_copy,
+    "kv_pages_extend": kv_pages_extend,
+    "kv_pages_fork": kv_pages_fork,
+    "kv_pages_free": kv_pages_free,
     "kv_write": kv_write,
-    "mx4_kv_write": mx4_kv_write,
     "lm_head": lm_head,
     "matmul_q4k": matmul_q4k,
     "matmul_q4k_gemm": matmul_q4k_gemm,
     "matmul_int4g32": matmul_int4g32,
+    "mx4_kv_read": mx4_kv_read,
+    "mx4_kv_write": mx4_kv_write,
     "residual": residual,
     "rmsnorm": rmsnorm,
     "rope": rope,

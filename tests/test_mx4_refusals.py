@@ -28,3 +28,8 @@ def test_rows_that_are_no_whole_blocks():
     for d in (0, 31, 48):
         with pytest.raises(ValueError, match="multiple of 32"):
             mx4.quantise(np.zeros((2, d), np.float32))
+
+
+def test_the_registry_names_every_call_of_the_cache():
+    calls = {n for n in vars(ops) if n.startswith(("attention_mx4", "mx4_kv_", "kv_pages_")) and not n.endswith("_workspace")}
+    assert len(calls) == 9 and all(ops.OPS[n] is getattr(ops, n) for n in calls)
