@@ -259,6 +259,14 @@ __device__ __forceinline__ void scores(const Query<D, TEAM, HALF> &q, const KBlo
     }
 }
 
+// What lanes of a wave write to LDS before it, its other lanes read behind it: the
+// wave's LDS operations are in order, as long as the compiler leaves them so.
+__device__ __forceinline__ void in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A value is wanted here: otherwise the compiler computes it where it is used.
 template <typename T>
 __device__ __forceinline__ void here(T &v) {
@@ -462,6 +470,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
     scores<D, TEAM, HALF, 0, P::kOps>(q, kb, s);
     load_k<D, TEAM>(kb, slab_at(slab1), shift, place(1), lane, slice);
     if (kShare) __syncthreads();
+    else in_order();
 
     // O stays in the accumulation registers between the matrix instructions where it
     // takes many (the compiler would move it out at every block for the rare rescaling)
@@ -616,6 +625,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
                     }
                 }
         }
+        if constexpr (!kShare) in_order();
         s = next;
         slab0 = slab1;
         slab1 = slab2;
