@@ -570,6 +570,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
         }
         // P^T operands: step h of two takes the positions of quarter lh + 2 h
         h8 ph[2], pl[2];
+        float minus = -1.0f;  // (a value, so that e - hi is one instruction that takes hi as f16)
+        here(minus);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -577,9 +579,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
                 const int r = 4 * (h + 2 * (j >> 2)) + (j & 3);
                 const float e0 = __builtin_amdgcn_exp2f(y[r]), e1 = __builtin_amdgcn_exp2f(y[r + 1]);
                 l += e0 + e1;
-                ph[h][j] = (_Float16)e0, ph[h][j + 1] = (_Float16)e1;
-                pl[h][j] = (_Float16)(e0 - (float)ph[h][j]);
-                pl[h][j + 1] = (_Float16)(e1 - (float)ph[h][j + 1]);
+                h2 hi_part = {(_Float16)e0, (_Float16)e1};
+                here(hi_part);  // (rounded as a pair once, not each again for the lo part)
+                ph[h][j] = hi_part[0], ph[h][j + 1] = hi_part[1];
+                pl[h][j] = (_Float16)fmaf((float)hi_part[0], minus, e0);
+                pl[h][j + 1] = (_Float16)fmaf((float)hi_part[1], minus, e1);
             }
         scores<D, TEAM, HALF, kEarly, P::kOps>(q, kb, next);
         interleave<(P::kOps - kEarly) * kParts, 6>();
