@@ -20,12 +20,13 @@
 //   * The running max is raised only when a score exceeds it by 2^8, P lies
 //     2^7 above it, so that f16's small values lose no more than 2^-32 of the largest.
 // No wave waits for another until a row's end.  Bound by the cache's bytes where
-// there are many: 8 sequences of 32768, 64 / 8 heads of 128 dims (285 MB): 55.6 us with
-// the join, the rate of a large copy (5.1 TB/s).  Bound by two dependent launches and
+// there are many: 8 sequences of 32768, 64 / 8 heads of 128 dims (285 MB): 55 us with
+// the join, the rate of a large copy (5.2 TB/s).  Bound by two dependent launches and
 // a chain of cold reads (length, page table, K, then parts) where there are few: one
-// of 4096, 8 / 4 heads of 256: 10.5 us, 7.7 + 2.8 of them in the kernels.  A wave has
-// a block's K and V under way while it works on the one before, which asks for enough
-// waves more than for more blocks a wave: per_cu() is as many as the registers allow.
+// of 4096, 8 / 4 heads of 256: 10.5 us, 7.6 + 3.1-3.7 of them in the kernels, which
+// overlap a little.  A wave has a block's K and V under way while it works on the one
+// before, which asks for enough waves more than for more blocks a wave: per_cu() is as
+// many as the registers allow.
 #include "mx4_cache.h"
 
 #include <limits.h>
@@ -60,7 +61,7 @@ struct TokenArgs {
 
 // Workgroups of four waves that a CU holds at once, by the registers that a wave
 // takes, and those that fill the device's 256 CUs in one round (head_dim 128: four
-// leave a wave fewer registers, 56.6 us for 55.6 over 8 sequences of 32768).
+// leave a wave fewer registers, 56.6 us for 55.2 over 8 sequences of 32768).
 template <int D>
 constexpr int per_cu() { return D <= 160 ? 3 : (D <= 256 ? 2 : 1); }
 template <int D>

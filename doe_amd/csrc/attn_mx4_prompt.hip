@@ -10,7 +10,7 @@
 //     f32 ones in hi and lo parts of one power of two for the row: 22 bits of each
 //     dim, whatever the others are (down to 2^-38 of the largest).  The matrix cores'
 //     own 4-bit operands against digits of Q in 6 bits (25 bits of the largest of 32
-//     dims) took 2-15 % less, but lost dims far below the largest where the keys are
+//     dims) took up to 12 % less, but lost dims far below the largest where the keys are
 //     zero at the large ones: 1e-3 of the output at 2^15.
 //   * S^T's sums are P^T's operand order of O^T = V^T P^T, on the same instruction:
 //     P as f16 hi + lo whatever the output's type (one f16 of P would cost an f16
@@ -23,11 +23,16 @@
 // A block's steps overlap with its neighbours': its weights stand beside the next
 // one's scores, its P V beside the next V's way into LDS, so that the matrix and
 // vector units of a SIMD work at once with one or two waves on it.  2048 rows after
-// 8192 positions, 32 / 8 heads of 128 dims, f16: 460 us, 672 TFLOP/s of the 4 D
-// operations a pair and position, where a large f16 matrix product reaches 1139: P's
-// two parts are three products for two.  1000 rows at 8 / 4 heads of 256 dims, f32: 28
-// us, of which 8 are a prologue (row, page table and query read one after the other)
-// that 252 tiles on 256 CUs go through at once.
+// 8192 positions, 32 / 8 heads of 128 dims, f16: 463 us, 668 TFLOP/s of the 4 D
+// operations a pair and position, where a large f16 matrix product reaches 1139; P's two
+// parts make three products of two.  Its matrix units are busy 47 % of the cycles and
+// vector instructions issue in 50: the two waves of a SIMD seldom do both at once.  32 /
+// 16 heads of 160 (1500 rows after 2000 of 8 sequences, f32): 31 and 34 % with the one wave
+// a SIMD that its registers allow, 796 us, 360 TFLOP/s; 8 / 1 of 512, whose waves add up
+// their parts of every score through LDS: 28 and 39 %, 667 us, 344.  1000 rows at 8 / 4
+// heads of 256 dims, f32: 28 us, of which 8 are a prologue (row, page table and query read
+// one after the other) and most of the rest the last tiles' eight blocks a wave, where the
+// mean is 4.3.
 #include "mx4_cache.h"
 
 #include <math.h>
@@ -764,10 +769,10 @@ int g_tile = 0;  // 0 automatic, 32 or 128 (up to head_dim 256) pairs
 // Whether a call takes tiles of 128 pairs, whose waves share V's way into LDS, or of
 // 32, whose waves take every fourth block.  The large ones need as many tiles as the
 // device holds workgroups.  1500 rows after 2000 of 8 sequences, 32 against 128, f32
-// and f16: 16 / 4 heads of 64 174 / 173 and 151 / 157 us, 16 / 4 of 128 279 / 270 and 244 /
-// 226, 32 / 16 of 160 1046 / 815 and 928 / 676, 8 / 4 of 256 335 / 328 and 294 / 273; one
-// prompt of 1000 rows (fewer tiles), f32: 16 / 29, 21 / 37 and 29 / 43 at 64, 128 and 256,
-// but 67 / 61 at 160, where 16 KV heads make 256 tiles.
+// and f16: 16 / 4 heads of 64 165 / 166 and 147 / 146 us, 16 / 4 of 128 274 / 266 and 235 /
+// 220, 32 / 16 of 160 1049 / 798 and 852 / 650, 8 / 4 of 256 331 / 324 and 290 / 264; one
+// prompt of 1000 rows (fewer tiles), f32: 16 / 28, 20 / 36 and 29 / 43 at 64, 128 and 256,
+// but 67 / 60 at 160, where 16 KV heads make 256 tiles.
 bool shared(int64_t head_dim, bool starts, int64_t batch, int64_t rows, int64_t num_heads, int64_t kv_heads) {
     if (head_dim == 512) return false;
     if (g_tile) return g_tile == 128;
