@@ -4,7 +4,7 @@ bits (tests/mx4_cases.py derives the bounds)."""
 import numpy as np
 import pytest
 
-from doe_amd import DeviceBuffer, mx4, ops
+from doe_amd import DeviceBuffer, Graph, Stream, mx4, ops, synchronize
 from mx4_cases import Case, attention, check
 from test_gpu_mx4_attention import prompt, tile, token, up  # noqa: F401  (a fixture among them)
 
@@ -110,3 +110,83 @@ def test_tokens_that_may_read_past_the_caches(dev, d, hq, hkv):
                               head_dim=d, batch=4, table_stride=case.stride)
     assert np.array_equal(token(case, q), small)
     pool.free()
+
+
+def guarded(size, fill=0x5a):
+    """A workspace of `size` bytes within a buffer that is `fill` around it."""
+    buf = up(np.full(size + 8192, fill, np.uint8))
+    return buf, buf.view(4096, size)
+
+
+def intact(buf, size, fill=0x5a):
+    host = buf.download()
+    return (host[:4096] == fill).all() and (host[4096 + size:] == fill).all()
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 16, 2), (128, 5, 1), (160, 40, 4), (256, 4, 4), (512, 9, 1)])
+@pytest.mark.parametrize("f16", [False, True])
+def test_workspaces_and_rows_are_all_that_is_written(dev, d, hq, hkv, f16):
+    """Workspaces of the size asked for, queries in the wide rows of a fused projection,
+    outputs in rows of another width: what lies around them stays as it was."""
+    rng = np.random.default_rng(d + hq)
+    rows, lens = [3, 0, 40, 1], [2000, 7, 40, 300]
+    case = Case(rng, lens, head_dim=d, num_kv_heads=hkv, page_size=32)
+    case.upload()
+    t = np.float16 if f16 else np.float32
+    how = dict(num_heads=hq, scale=d ** -0.5, q_f16=f16, out_f16=f16)
+    print(f"[around] d={d} hq={hq} hkv={hkv} f16={f16}", flush=True)
+    q = rng.standard_normal((4, hq, d)).astype(t)
+    size = ops.attention_mx4_workspace(4, hq, hkv, d)
+    buf, ws = guarded(size)
+    out = up(np.full((6, hq * d), 7, t))
+    ops.attention_mx4(case.cache, up(q), out.view(hq * d * out.dtype.itemsize, 4 * hq * d * out.dtype.itemsize), workspace=ws, **how)
+    got = out.download()
+    assert intact(buf, size) and (got[0] == 7).all() and (got[5] == 7).all()
+    check(got[1:5].reshape(q.shape), *attention(case, q, [1] * 4, d ** -0.5)[:2], t)
+    n, wide, narrow = sum(rows), (hq + 2 * hkv) * d, hq * d + 32
+    q = rng.standard_normal((n, hq, d)).astype(t)
+    fused = np.full((n, wide), np.nan, t)
+    fused[:, :hq * d] = q.reshape(n, -1)
+    size = ops.attention_mx4_workspace(4, hq, hkv, d, n)
+    buf, ws = guarded(size)
+    out = up(np.full((n + 1, narrow), 7, t))
+    ops.attention_mx4_prompt(case.cache, up(fused), out, n, row_starts=up(np.cumsum([0] + rows).astype(np.int32)),
+                             q_row_stride=wide, out_row_stride=narrow, workspace=ws, **how)
+    got = out.download()
+    assert intact(buf, size) and (got[n] == 7).all() and (got[:, hq * d:] == 7).all()
+    check(got[:n, :hq * d].reshape(q.shape), *attention(case, q, rows, d ** -0.5)[:2], t)
+
+
+def test_captured_calls_of_many_sequences(dev):
+    """More pieces than workgroups, and prompts of one row without row_starts, captured
+    and replayed with other lengths: what the eager calls give."""
+    rng = np.random.default_rng(21)
+    batch, d, hq, hkv = 150, 64, 8, 4
+    case = Case(rng, [1500] * batch, head_dim=d, num_kv_heads=hkv, page_size=32)
+    case.upload()
+    q = up(rng.standard_normal((batch, hq, d)).astype(np.float32))
+    size = max(ops.attention_mx4_workspace(batch, hq, hkv, d), ops.attention_mx4_workspace(batch, hq, hkv, d, batch))
+
+    def step(outs, ws, stream=None):
+        ops.attention_mx4(case.cache, q, outs[0], num_heads=hq, scale=0.1, workspace=ws, stream=stream)
+        ops.attention_mx4_prompt(case.cache, q, outs[1], batch, num_heads=hq, scale=0.1, workspace=ws, stream=stream)
+
+    st, outs, ws = Stream(), [DeviceBuffer.empty((batch, hq, d), np.float32) for _ in "tp"], DeviceBuffer(size)
+    graph = Graph.capture(st, lambda: step(outs, ws, st))
+    for name in ("more pieces than workgroups", "more rows than workgroups", "sequences beyond a wave"):
+        lens = np.minimum(1500, lengths(rng, batch, MANY[name][1])).astype(np.int32)
+        case.lens_dev.upload(lens)
+        synchronize()
+        graph.launch(st)
+        st.synchronize()
+        got = [o.download() for o in outs]
+        again = [DeviceBuffer.empty((batch, hq, d), np.float32) for _ in "tp"]
+        other = DeviceBuffer(size)
+        step(again, other)
+        synchronize()
+        for a, b in zip(again, got):
+            assert np.array_equal(a.download(), b), name
+        # a token is a prompt of one row
+        assert np.linalg.norm(got[0] - got[1]) <= 2e-6 * np.linalg.norm(got[0])
+    graph.destroy()
+    st.destroy()
