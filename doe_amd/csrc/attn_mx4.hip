@@ -227,7 +227,8 @@ __device__ __forceinline__ h8 weights(const TokenArgs &a, State<D> &st, const f3
         float top = logs(0.0f);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float ref = top - kBias > st.m + kLazy ? top - kBias : st.m;
+        float ref = top - kBias > st.m + kLazy ? top - kBias : st.m;
+        ref = ref == INFINITY ? NAN : ref;  // (a score beyond f32: no numbers from here on)
         const float corr = ref == st.m ? 1.0f : __builtin_amdgcn_exp2f(st.m - ref);
         st.m = ref;
         st.l *= corr;

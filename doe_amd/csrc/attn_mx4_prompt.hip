@@ -557,7 +557,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu(D)) void attn_mx4_prompt_kernel
             if (!whole) mask();
             float top = most();
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float ref = top - kBias > m + kLazy ? top - kBias : m;
+            float ref = top - kBias > m + kLazy ? top - kBias : m;
+            ref = ref == INFINITY ? NAN : ref;  // (a score beyond f32: no numbers from here on)
             const float corr = ref == m ? 1.0f : __builtin_amdgcn_exp2f(m - ref);
             m = ref;
             l *= corr;

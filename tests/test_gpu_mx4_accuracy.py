@@ -114,3 +114,21 @@ def test_token_queries_that_are_no_numbers(dev, d, f16):
         q[row, head, dim], bad[row, head] = value, True
     got = token(case, q, f16=f16)
     assert np.array_equal(np.isnan(got), np.repeat(bad[..., None], d, -1))
+
+
+@pytest.mark.parametrize("longest", [50, 3000])
+@pytest.mark.parametrize("form", ["token", "prompt"])
+@pytest.mark.parametrize("d", [64, 160, 512])
+@pytest.mark.parametrize("f16,size,factor", [(False, 1e30, 1e12), (False, 1e30, -1e12), (False, 1e36, 1e7), (False, 1e36, -1e7),
+                                             (True, 1e3, 1e38), (True, 1e3, -1e38)])
+def test_scores_that_overflow_are_no_numbers(dev, tile, form, d, f16, size, factor, longest):  # noqa: F811
+    """Uncapped scores beyond f32, of one sign or the other, give NaN and no zeros."""
+    rng = np.random.default_rng(d)
+    case = Case(rng, [longest, 40, 33], head_dim=d, num_kv_heads=1, page_size=32)
+    case.kc &= 7
+    case.kc[..., 0] = 4
+    case.upload()
+    q = (np.abs(rng.standard_normal((3, 2, d))) * size).astype(np.float16 if f16 else np.float32)
+    q[..., 0] = size
+    got = token(case, q, f16=f16, scale=factor) if form == "token" else prompt(case, q, [1, 1, 1], f16=f16, scale=factor)
+    assert np.isnan(got).all()
