@@ -23,7 +23,7 @@
 // A block's steps overlap with its neighbours': its weights stand beside the next
 // one's scores, its P V beside the next V's way into LDS, so that the matrix and
 // vector units of a SIMD work at once with one or two waves on it.  2048 rows after
-// 8192 positions, 32 / 8 heads of 128 dims, f16: 463 us, 668 TFLOP/s of the 4 D
+// 8192 positions, 32 / 8 heads of 128 dims, f16: 440 us, 704 TFLOP/s of the 4 D
 // operations a pair and position, where a large f16 matrix product reaches 1139; P's two
 // parts make three products of two.  Its matrix units are busy 47 % of the cycles and
 // vector instructions issue in 50: the two waves of a SIMD seldom do both at once.  32 /
