@@ -106,6 +106,15 @@ SIGNATURES: dict[str, list] = {
     "doe_kv_pages_free": [_vp, _vp, _i64, _vp, _vp],
     "doe_kv_pages_compact": [_vp, _vp, _vp, _i64, _vp],
     "doe_kv_pages_copy": [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp],
+    "doe_qkv_rope_append": [_vp, _vp, _i64, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp],
+    "doe_mx4_qkv_rope_append": [_vp, _vp, _i64, _vp, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp],
+    "doe_lora_workspace": [_vp, _i64, C.POINTER(_i64)],
+    "doe_lora_add": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    "doe_beam_select_workspace": [_i64, _i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_beam_select": [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "doe_beam_reorder_rows": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
+    "doe_beam_reorder_pages_workspace": [_i64, _i64, _i64, C.POINTER(_i64)],
+    "doe_beam_reorder_pages": [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp],
     "doe_rmsnorm": [_vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp],
     "doe_rope": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
     "doe_rope_partial": [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp],

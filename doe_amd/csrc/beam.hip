@@ -1,0 +1,486 @@
+// beam.hip -- beam search: the best continuations of a request's beams over the
+// vocabulary (doe_beam_select), and dense states in the order of their parents
+// (doe_beam_reorder_rows; page tables: kv_pages.hip).
+//
+// A candidate (beam, token) scores s_b + x_t - log sum_t' exp x_t', x the logits times
+// the inverse temperature.  Within a row the order is that of the logits, so the first
+// kernel reads them once and leaves, for every wave's part of a row, its `select` best
+// logits and its share of the sum; the second one forms the rows' logarithms in 64 bits
+// and picks among the parts.
+#include "common.h"
+
+#include <math.h>
+#include <algorithm>
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));  // (rows of an odd vocabulary)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxBeams = 64, kMaxSelect = 64;
+constexpr int kWaves = 4;
+constexpr int kList = 256;   // a wave's shortlist
+constexpr int kPick = 1024;  // threads of the second kernel
+constexpr int kPool = 4096;  // its shortlist
+
+struct BeamArgs {
+    const float *logits, *scores;
+    const int32_t *finished;
+    int64_t row_stride;
+    int batch, beams, vocab, select, parts, end_token;  // parts of a row: a wave each
+    float inv_temperature, factor, factor_low;  // factor + factor_low = inv_temperature log2(e)
+    uint64_t *cand;   // [row][part][select]: logit order, ~token; 0: none
+    float *top;       // [row][part]: the part's largest logit (NaN: one is a NaN or infinite)
+    double *sum;      // [row][part]: sum of exp(x - x_top)
+    int32_t *parents, *tokens, *ended;
+    float *best;
+};
+
+// Order of floats as unsigned numbers (no NaN; -0 below 0, as in the comparison of bits).
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t o) {
+    return __uint_as_float(o ^ ((int)o < 0 ? 0x80000000u : 0xffffffffu));
+}
+
+// A beam that offers its tokens: it has a score and has not ended.
+__device__ __forceinline__ bool offers(const BeamArgs &a, int row) {
+    const float s = a.scores[row];
+    return s > -INFINITY && s < INFINITY && !(a.finished && a.finished[row]);
+}
+
+// What lanes of a wave write to LDS before it, its other lanes read behind it: the
+// wave's LDS operations are in order, as long as the compiler leaves them so.
+__device__ __forceinline__ void in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)v, d, 64);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// A wave's part of a row: NV x 256 logits, four side by side a lane, kept in
+// registers.  The `select`-th largest of the lanes' own largest ones is a bound that at
+// least `select` logits reach and few others do (only `select` lanes have any): those go
+// to a list in LDS, and their places in the order are counted.
+template <int NV>
+__global__ __launch_bounds__(64 * kWaves) void beam_parts_kernel(BeamArgs a, int wgs) {
+    __shared__ uint64_t lists[kWaves][kList];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int row = blockIdx.x / wgs, part = (blockIdx.x - row * wgs) * kWaves + wave;
+    if (part >= a.parts || !offers(a, row)) return;  // (its parts are not looked at)
+    const float *x = a.logits + (int64_t)row * a.row_stride;
+    // (parts by place, not by address: equal rows give equal bits)
+    const int first = part * (256 * NV), e0 = first + 4 * lane;
+    f4 v[NV];
+    if (first + 256 * NV <= a.vocab) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = *reinterpret_cast<const f4_any *>(x + e0 + 256 * j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int e = e0 + 256 * j;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][i] = e + i < a.vocab ? x[e + i] : -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+    int at = 0;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            bad = bad || !(v[j][i] < INFINITY);
+            v[j][i] += 0.0f;  // (-0 is 0)
+            if (v[j][i] > top) {
+                top = v[j][i];
+                at = e0 + 256 * j + i;
+            }
+        }
+    const int64_t slot = (int64_t)row * a.parts + part;
+    uint64_t *cand = a.cand + slot * a.select;
+    float most = top;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+    if (__any(bad) || most == -INFINITY) {
+        if (lane == 0) {
+            a.top[slot] = __any(bad) ? NAN : -INFINITY;
+            a.sum[slot] = 0.0;
+        }
+        if (lane < a.select) cand[lane] = 0;
+        return;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float d = v[j][i] - most;
+            sum += __builtin_amdgcn_exp2f(d == -INFINITY ? d : fmaf(d, a.factor, d * a.factor_low));
+        }
+    double all = sum;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+    if (lane == 0) {
+        a.top[slot] = most;
+        a.sum[slot] = all;
+    }
+    const uint64_t mine = top > -INFINITY ? (uint64_t)ordered(top) << 32 | (uint32_t)~at : (uint64_t)lane;
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) above += lane_key(mine, j) > mine ? 1 : 0;
+    const uint64_t bound = lane_key(mine, __builtin_ctzll(__ballot(above == a.select - 1)));
+    const bool any_bound = bound >> 32 != 0;
+    const float low = any_bound ? unordered((uint32_t)(bound >> 32)) : -INFINITY;
+    const int low_at = any_bound ? (int)~(uint32_t)bound : 0;
+    uint64_t *list = lists[wave];
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = e0 + 256 * j + i;
+            const bool in = v[j][i] > low || (v[j][i] == low && low > -INFINITY && e <= low_at);
+            const uint64_t who = __ballot(in);
+            if (who == 0) continue;
+            const int to = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+            if (in && to < kList) list[to] = (uint64_t)ordered(v[j][i]) << 32 | (uint32_t)~e;
+            count += __popcll(who);
+        }
+    if (count <= kList) {
+        in_order();
+        for (int t = lane; t < count; t += 64) {
+            const uint64_t key = list[t];
+            int before = 0;
+            for (int j = 0; j < count; ++j) before += list[j] > key ? 1 : 0;
+            if (before < a.select) cand[before] = key;
+        }
+        if (lane >= count && lane < a.select) cand[lane] = 0;
+        return;
+    }
+    // (rarely: the large ones in few lanes) one after the other
+    uint64_t last = ~0ull;
+    for (int c = 0; c < a.select; ++c) {
+        uint64_t next = 0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t key = v[j][i] > -INFINITY ? (uint64_t)ordered(v[j][i]) << 32 | (uint32_t)~(e0 + 256 * j + i) : 0;
+                if (key < last && key > next) next = key;
+            }
+        last = wave_max(next);
+        if (lane == 0) cand[c] = last;
+    }
+}
+
+// A request's pick: the rows' logarithms, then the same way as above with a thread a
+// part's list instead of a lane its logits.
+__global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
+    __shared__ double base[kMaxBeams], ended_at[kMaxBeams], bounds[kPick / 64], pool[kPool];
+    __shared__ uint64_t pool_at[kPool];  // a candidate's place, see `place`
+    __shared__ int count_;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int request = blockIdx.x, row0 = request * a.beams, C = a.select;
+    const double factor = a.inv_temperature;
+    if (tid == 0) count_ = 0;
+    for (int b = wave; b < a.beams; b += kPick / 64) {
+        const float score = a.scores[row0 + b];
+        const bool ok = score > -INFINITY && score < INFINITY, done = a.finished && a.finished[row0 + b];
+        double start = -INFINITY;
+        if (ok && !done) {
+            const float *top = a.top + (int64_t)(row0 + b) * a.parts;
+            const double *sum = a.sum + (int64_t)(row0 + b) * a.parts;
+            float most = -INFINITY;
+            bool bad = false;
+            for (int p = lane; p < a.parts; p += 64) {
+                bad = bad || top[p] != top[p];
+                most = fmaxf(most, top[p]);
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+            double all = 0.0;
+            if (most > -INFINITY)
+                for (int p = lane; p < a.parts; p += 64)
+                    if (top[p] > -INFINITY) all += sum[p] * exp(((double)top[p] - (double)most) * factor);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+            if (!__any(bad) && most > -INFINITY) start = (double)score - ((double)most * factor + log(all));
+        }
+        if (lane == 0) {
+            base[b] = start;
+            ended_at[b] = ok && done ? (double)score : -INFINITY;
+        }
+    }
+    __syncthreads();
+    const int lists = a.beams * a.parts;
+    const uint64_t *cand = a.cand + (int64_t)row0 * a.parts * C;
+    auto score_of = [&](uint64_t key, int b) { return key ? base[b] + factor * (double)unordered((uint32_t)(key >> 32)) : -INFINITY; };
+    // (the lists of a beam without an offer are not written)
+    auto score_at = [&](int l, int c, uint64_t &key) {
+        const int b = l / a.parts;
+        key = base[b] > -INFINITY ? cand[(int64_t)l * C + c] : 0;
+        return score_of(key, b);
+    };
+    // of equal scores the lower place comes first: beam, then logit from the largest
+    // (scores of a beam may be too near each other for 64 bits), then token
+    auto place = [](int b, uint64_t key) { return (uint64_t)b << 56 | (uint64_t)~(uint32_t)(key >> 32) << 24 | ~(uint32_t)key; };
+    auto end_place = [&](int b) { return (uint64_t)b << 56 | (uint32_t)a.end_token; };
+    constexpr uint64_t kNone = ~0ull;
+    double mine = -INFINITY;
+    for (int l = tid; l < lists; l += kPick) {
+        uint64_t key;
+        mine = fmax(mine, score_at(l, 0, key));
+    }
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) {
+        const double o = __longlong_as_double((long long)lane_key((uint64_t)__double_as_longlong(mine), j));
+        above += o > mine || (o == mine && j < lane) ? 1 : 0;
+    }
+    if (above == C - 1) bounds[wave] = mine;
+    __syncthreads();
+    double bound = bounds[0];
+    for (int w = 1; w < kPick / 64; ++w) bound = fmax(bound, bounds[w]);
+    auto push = [&](double score, uint64_t at) {
+        const int to = atomicAdd(&count_, 1);
+        if (to < kPool) {
+            pool[to] = score;
+            pool_at[to] = at;
+        }
+    };
+    for (int l = tid; l < lists; l += kPick) {
+        const int b = l / a.parts;
+        for (int c = 0; c < C; ++c) {
+            uint64_t key;
+            const double s = score_at(l, c, key);
+            if (key == 0 || s < bound) break;
+            push(s, place(b, key));
+        }
+    }
+    if (tid < a.beams && ended_at[tid] > -INFINITY && ended_at[tid] >= bound) push(ended_at[tid], end_place(tid));
+    __syncthreads();
+    const int count = count_;
+    auto put = [&](int c, double score, uint64_t at) {
+        const int64_t to = (int64_t)request * C + c;
+        const bool none = at == kNone;
+        const int b = none ? 0 : (int)(at >> 56), token = none ? -1 : (int)(at & 0xffffff);
+        a.parents[to] = none ? -1 : row0 + b;
+        a.tokens[to] = token;
+        a.best[to] = (float)score;
+        if (a.ended) a.ended[to] = !none && ((a.finished && a.finished[row0 + b]) || token == a.end_token) ? 1 : 0;
+    };
+    if (count <= kPool) {
+        for (int t = tid; t < count; t += kPick) {
+            const double s = pool[t];
+            const uint64_t at = pool_at[t];
+            int before = 0;
+            for (int j = 0; j < count; ++j) before += pool[j] > s || (pool[j] == s && pool_at[j] < at) ? 1 : 0;
+            if (before < C) put(before, s, at);
+        }
+        if (tid >= count && tid < C) put(tid, -INFINITY, kNone);
+        return;
+    }
+    // (rarely: few full lists among many) one after the other
+    double last = INFINITY;
+    uint64_t last_at = 0;
+    for (int c = 0; c < C; ++c) {
+        double s = -INFINITY;
+        uint64_t at = kNone;
+        auto take = [&](double score, uint64_t where) {
+            const bool behind = score < last || (score == last && where > last_at);
+            if (score > -INFINITY && behind && (score > s || (score == s && where < at))) {
+                s = score;
+                at = where;
+            }
+        };
+        for (int l = tid; l < lists; l += kPick)
+            for (int e = 0; e < C; ++e) {
+                uint64_t key;
+                const double score = score_at(l, e, key);
+                if (key == 0) break;
+                take(score, place(l / a.parts, key));
+            }
+        if (tid < a.beams) take(ended_at[tid], end_place(tid));
+        __syncthreads();  // the last round's places have been read
+        pool[tid] = s;
+        pool_at[tid] = at;
+        __syncthreads();
+        for (int d = kPick / 2; d > 0; d >>= 1) {
+            if (tid < d) {
+                const double o = pool[tid + d];
+                const uint64_t o_at = pool_at[tid + d];
+                if (o > pool[tid] || (o == pool[tid] && o_at < pool_at[tid])) {
+                    pool[tid] = o;
+                    pool_at[tid] = o_at;
+                }
+            }
+            __syncthreads();
+        }
+        last = pool[0];
+        last_at = pool_at[0];
+        if (tid == 0) put(c, last, last_at);
+    }
+}
+
+// Row i of dst = row parents[i] of src in every layer, in pieces of 16 KB.
+template <typename T>
+__global__ __launch_bounds__(256) void beam_rows_kernel(const uint8_t *src, uint8_t *dst, const int32_t *parents, int64_t src_rows,
+                                                        int64_t rows, int64_t row_bytes, int64_t layers, int64_t src_layer,
+                                                        int64_t dst_layer) {
+    constexpr int PIECE = 256 * 4 * (int)sizeof(T);
+    const int64_t pieces = (row_bytes + PIECE - 1) / PIECE, all = rows * layers * pieces;
+    for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
+        const int64_t piece = w % pieces, rest = w / pieces, layer = rest / rows, i = rest - layer * rows;
+        const int64_t parent = parents[i];
+        if (parent < 0 || parent >= src_rows) continue;
+        const int64_t at = piece * PIECE + threadIdx.x * (int)sizeof(T);
+        const uint8_t *s = src + layer * src_layer + parent * row_bytes + at;
+        uint8_t *d = dst + layer * dst_layer + i * row_bytes + at;
+        T v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (at + j * (PIECE / 4) < row_bytes) v[j] = *reinterpret_cast<const T *>(s + j * (PIECE / 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (at + j * (PIECE / 4) < row_bytes) *reinterpret_cast<T *>(d + j * (PIECE / 4)) = v[j];
+    }
+}
+
+// Vectors a lane: long parts where there are rows enough to fill the device.
+int vectors_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)8 << 20 ? 16 : 4; }
+
+struct BeamSizes {
+    int vectors;
+    int64_t parts, cand, top, bytes;
+};
+int beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int64_t select, BeamSizes &z) {
+    DOE_REQUIRE(beams > 0 && beams <= kMaxBeams, DOE_E_UNSUPPORTED, "beams %lld outside 1..%d", (long long)beams, kMaxBeams);
+    DOE_REQUIRE(select > 0 && select <= kMaxSelect, DOE_E_UNSUPPORTED, "select %lld outside 1..%d", (long long)select, kMaxSelect);
+    DOE_REQUIRE(vocab > 0 && vocab <= ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "vocab %lld outside 1..2^24", (long long)vocab);
+    DOE_REQUIRE(batch >= 0 && batch <= 65535, DOE_E_INVALID, "batch %lld outside 0..65535", (long long)batch);
+    const int64_t rows = batch * beams;
+    z.vectors = vectors_of(rows, vocab);
+    z.parts = (vocab + 256 * z.vectors - 1) / (256 * z.vectors);
+    z.cand = rows * z.parts * select * 8;
+    z.top = z.cand + rows * z.parts * 8;
+    z.bytes = std::max<int64_t>(16, z.top + rows * z.parts * 4);
+    return DOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int doe_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t select, int64_t *bytes) {
+    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
+    BeamSizes z;
+    const int rc = beam_sizes(batch, beams, vocab, select, z);
+    if (rc) return rc;
+    *bytes = z.bytes;
+    return DOE_OK;
+}
+
+int doe_beam_select(const float *logits, int64_t row_stride, const float *scores, const int32_t *finished, int64_t batch,
+                    int64_t beams, int64_t vocab, int64_t select, float inv_temperature, int64_t end_token, int32_t *parents,
+                    int32_t *tokens, float *out_scores, int32_t *out_finished, void *workspace, int64_t workspace_bytes,
+                    doe_stream_t stream) {
+    BeamSizes z;
+    int rc = beam_sizes(batch, beams, vocab, select, z);
+    if (rc) return rc;
+    DOE_REQUIRE(row_stride >= vocab, DOE_E_INVALID, "row stride %lld below vocab %lld", (long long)row_stride, (long long)vocab);
+    DOE_REQUIRE(isfinite(inv_temperature) && inv_temperature > 0.0f && isfinite(inv_temperature * 1.4426950408889634f), DOE_E_INVALID,
+                "inv_temperature %g", (double)inv_temperature);
+    DOE_REQUIRE(end_token < vocab && (end_token >= 0 || !finished), DOE_E_INVALID, "end_token %lld of %lld tokens%s", (long long)end_token,
+                (long long)vocab, finished ? ", with finished beams" : "");
+    DOE_REQUIRE(batch == 0 || (logits && scores && parents && tokens && out_scores), DOE_E_INVALID, "null pointer");
+    DOE_REQUIRE(((uintptr_t)logits & 3) == 0, DOE_E_INVALID, "logits must be 4-byte aligned");
+    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bytes, DOE_E_INVALID,
+                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)z.bytes, (long long)workspace_bytes);
+    const int64_t rows = batch * beams, wgs = (z.parts + kWaves - 1) / kWaves;
+    DOE_REQUIRE(rows * wgs < ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %lld logits", (long long)rows, (long long)vocab);
+    if ((rc = doe::require_init())) return rc;
+    if (batch == 0) return DOE_OK;
+    BeamArgs a{};
+    a.logits = logits;
+    a.scores = scores;
+    a.finished = finished;
+    a.row_stride = row_stride;
+    a.batch = (int)batch;
+    a.beams = (int)beams;
+    a.vocab = (int)vocab;
+    a.select = (int)select;
+    a.parts = (int)z.parts;
+    a.end_token = end_token < 0 ? -2 : (int)end_token;  // (-2: no token is)
+    a.inv_temperature = inv_temperature;
+    const double log2e = 1.4426950408889634074, factor = inv_temperature * log2e;
+    a.factor = (float)factor;
+    a.factor_low = (float)(factor - (double)a.factor);
+    a.cand = static_cast<uint64_t *>(workspace);
+    a.sum = reinterpret_cast<double *>(static_cast<uint8_t *>(workspace) + z.cand);
+    a.top = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + z.top);
+    a.parents = parents;
+    a.tokens = tokens;
+    a.best = out_scores;
+    a.ended = out_finished;
+    const hipStream_t st = (hipStream_t)stream;
+    if (z.vectors == 16) hipLaunchKernelGGL(beam_parts_kernel<16>, dim3((unsigned)(rows * wgs)), dim3(64 * kWaves), 0, st, a, (int)wgs);
+    else hipLaunchKernelGGL(beam_parts_kernel<4>, dim3((unsigned)(rows * wgs)), dim3(64 * kWaves), 0, st, a, (int)wgs);
+    DOE_LAUNCH_CHECK("beam_parts_kernel");
+    hipLaunchKernelGGL(beam_pick_kernel, dim3((unsigned)batch), dim3(kPick), 0, st, a);
+    DOE_LAUNCH_CHECK("beam_pick_kernel");
+    return DOE_OK;
+}
+
+int doe_beam_reorder_rows(const void *src, void *dst, const int32_t *parents, int64_t src_rows, int64_t rows, int64_t row_bytes,
+                          int64_t layers, int64_t src_layer_stride, int64_t dst_layer_stride, doe_stream_t stream) {
+    DOE_REQUIRE(src_rows >= 0 && src_rows < ((int64_t)1 << 31) && rows >= 0 && rows < ((int64_t)1 << 31) && layers >= 0 && layers <= 65535,
+                DOE_E_INVALID, "%lld rows of %lld in %lld layers", (long long)rows, (long long)src_rows, (long long)layers);
+    DOE_REQUIRE(row_bytes > 0 && row_bytes % 4 == 0 && row_bytes < ((int64_t)1 << 40), DOE_E_INVALID,
+                "row_bytes %lld is not a positive multiple of 4", (long long)row_bytes);
+    DOE_REQUIRE(std::max(src_rows, rows) <= ((int64_t)1 << 46) / row_bytes, DOE_E_INVALID, "%lld rows of %lld bytes",
+                (long long)std::max(src_rows, rows), (long long)row_bytes);
+    DOE_REQUIRE(layers <= 1 || (src_layer_stride >= src_rows * row_bytes && dst_layer_stride >= rows * row_bytes), DOE_E_INVALID,
+                "layer strides %lld and %lld below the rows' bytes", (long long)src_layer_stride, (long long)dst_layer_stride);
+    DOE_REQUIRE(layers <= 1 || (src_layer_stride % 4 == 0 && dst_layer_stride % 4 == 0 && src_layer_stride < ((int64_t)1 << 46) &&
+                                dst_layer_stride < ((int64_t)1 << 46)),
+                DOE_E_INVALID, "layer strides %lld and %lld", (long long)src_layer_stride, (long long)dst_layer_stride);
+    const bool none = rows == 0 || layers == 0 || src_rows == 0;
+    DOE_REQUIRE(none || (src && dst && parents), DOE_E_INVALID, "null pointer");
+    DOE_REQUIRE((((uintptr_t)src | (uintptr_t)dst) & 3) == 0, DOE_E_INVALID, "src and dst must be 4-byte aligned");
+    const int64_t src_bytes = (layers - 1) * src_layer_stride + src_rows * row_bytes, dst_bytes = (layers - 1) * dst_layer_stride + rows * row_bytes;
+    DOE_REQUIRE(none || (uintptr_t)src + (uintptr_t)src_bytes <= (uintptr_t)dst || (uintptr_t)dst + (uintptr_t)dst_bytes <= (uintptr_t)src,
+                DOE_E_INVALID, "src and dst overlap");
+    const int rc = doe::require_init();
+    if (rc) return rc;
+    if (none) return DOE_OK;
+    const bool wide = row_bytes % 16 == 0 && (((uintptr_t)src | (uintptr_t)dst) & 15) == 0 &&
+                      (layers == 1 || (src_layer_stride % 16 == 0 && dst_layer_stride % 16 == 0));
+    const int64_t piece = 256 * 4 * (wide ? 16 : 4), pieces = (row_bytes + piece - 1) / piece;
+    const int64_t most = (int64_t)1 << 14;
+    const unsigned wgs = (unsigned)(rows > most / layers / pieces ? most : rows * layers * pieces);
+    if (wide)
+        hipLaunchKernelGGL(beam_rows_kernel<u32x4>, dim3(wgs), dim3(256), 0, (hipStream_t)stream, static_cast<const uint8_t *>(src),
+                           static_cast<uint8_t *>(dst), parents, src_rows, rows, row_bytes, layers, src_layer_stride, dst_layer_stride);
+    else
+        hipLaunchKernelGGL(beam_rows_kernel<uint32_t>, dim3(wgs), dim3(256), 0, (hipStream_t)stream, static_cast<const uint8_t *>(src),
+                           static_cast<uint8_t *>(dst), parents, src_rows, rows, row_bytes, layers, src_layer_stride, dst_layer_stride);
+    DOE_LAUNCH_CHECK("beam_rows_kernel");
+    return DOE_OK;
+}
+
+}  // extern "C"

@@ -387,6 +387,133 @@ __global__ __launch_bounds__(kPlan) void pages_copy_plan_kernel(PageArgs a) {
 
 __global__ __launch_bounds__(256) void pages_copy_kernel(PageArgs a) { copy_pages(a, a.plan[0], blockIdx.x, gridDim.x); }
 
+// ---------------------------------------------------------------------------
+// Reordering: slot i becomes what the slot of parents[i] was, all at once.  The plan
+// takes a fresh page for every heir of a partly filled last page but one (the parent's
+// own slot, else the first heir); the wide kernel reads its columns of all rows before
+// it writes any of them.
+constexpr int kReorder = 8192;  // sequences of a call: their marks and a column of their rows fit in LDS
+
+struct ReorderArgs {
+    PageArgs p;        // first: parents; second: the slots (null: 0 .. n - 1); by_seq, taken, pair, need as above
+    int32_t *old_len;  // [n] of the slots before
+    int32_t *heirs;    // [n]
+    int32_t *fresh;    // [n] an heir's own last page, -1: none
+    int columns;       // of a workgroup
+};
+__device__ __forceinline__ int slot_of(const ReorderArgs &a, int i) { return a.p.second ? a.p.second[i] : i; }
+
+__global__ __launch_bounds__(kPlan) void pages_reorder_plan_kernel(ReorderArgs r) {
+    const PageArgs &a = r.p;
+    extern __shared__ int marks[];  // heirs [n], keepers [n]
+    __shared__ int wave_sums[kPlan / 64], sums[kPlan], pages[kPlan];
+    int *heirs = marks, *keeper = marks + a.n;
+    const int tid = threadIdx.x;
+    const uint32_t bits = free_bits(a, 4 * tid);
+    for (int i = tid; i < a.n; i += kPlan) {
+        heirs[i] = 0;
+        keeper[i] = a.n;
+    }
+    if (a.second) mark_all(a.second, a.n, a.max_seqs, a.by_seq);
+    __syncthreads();
+    bool bad = false;
+    for (int i = tid; i < a.n; i += kPlan) {
+        const int s = slot_of(r, i), p = a.first[i];
+        if (s < 0 || s >= a.max_seqs || (a.second && a.by_seq[s] != i) || p >= a.n) {
+            bad = true;
+            continue;
+        }
+        const int len = a.lens[s];
+        bad = bad || len < 0 || len > (int64_t)a.table_stride * a.page_size;
+        r.old_len[i] = len;
+        if (p >= 0) {
+            atomicAdd(&heirs[p], 1);
+            atomicMin(&keeper[p], p == i ? -1 : i);
+        }
+    }
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) {
+            *a.status = -1;
+            a.plan[0] = 0;
+        }
+        return;
+    }
+    // (old_len is read where other threads wrote it: through global memory of this workgroup, behind the barrier)
+    auto own_page = [&](int i) {
+        const int p = a.first[i];
+        if (p < 0 || keeper[p] == (p == i ? -1 : i)) return 0;
+        const int len = r.old_len[p];
+        return len - full_pages(a, len) * a.page_size > 0 ? 1 : 0;
+    };
+    const int want = sum_needs(a, wave_sums, sums, own_page);
+    const int found = take_free(a, want, bits, wave_sums, pages);
+    if (found < want) {
+        if (tid == 0) {
+            *a.status = want - found;
+            a.plan[0] = 0;
+        }
+        return;
+    }
+    for (int i = tid; i < a.n; i += kPlan) {
+        r.heirs[i] = heirs[i];
+        int page = -1;
+        if (own_page(i)) {
+            const int t = (i < kPlan ? sums[i] : a.need[i]) - 1, p = a.first[i];
+            page = taken(a, pages, t);
+            a.pair[2 * t] = a.table[(int64_t)slot_of(r, p) * a.table_stride + full_pages(a, r.old_len[p])];
+            a.pair[2 * t + 1] = page;
+            a.refs[page] = 1;
+        }
+        r.fresh[i] = page;
+    }
+    if (tid == 0) {
+        *a.status = 0;
+        a.plan[0] = want;
+    }
+}
+
+__global__ __launch_bounds__(256) void pages_reorder_kernel(ReorderArgs r) {
+    const PageArgs &a = r.p;
+    extern __shared__ int old[];  // [n][columns]
+    if (*a.status != 0) return;
+    const int C = r.columns, col0 = blockIdx.x * C, cells = a.n * C;
+    if (col0 < a.table_stride) {
+        for (int t = threadIdx.x; t < cells; t += 256) {
+            const int i = t / C, col = col0 + t - i * C;
+            old[t] = col < a.table_stride ? a.table[(int64_t)slot_of(r, i) * a.table_stride + col] : -1;
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < cells; t += 256) {
+            const int i = t / C, c = t - i * C, col = col0 + c;
+            if (col >= a.table_stride) continue;
+            const int s = slot_of(r, i), p = a.first[i];
+            int page = -1;
+            if (p >= 0) {
+                const int len = r.old_len[p], full = full_pages(a, len);
+                if (col < full || (col == full && len > full * a.page_size)) page = old[p * C + c];
+                if (col == full && r.fresh[i] >= 0) page = r.fresh[i];
+                if (col == 0) a.lens[s] = len;
+            } else if (col == 0) {
+                a.lens[s] = 0;
+            }
+            a.table[(int64_t)s * a.table_stride + col] = page;
+            // what slot i held is held by its heirs from here on
+            const int len = r.old_len[i], full = full_pages(a, len), was = old[t], heirs = r.heirs[i];
+            const int more = col < full ? heirs - 1 : (col == full && len > full * a.page_size && heirs == 0 ? -1 : 0);
+            if (more != 0 && was >= 0 && was < a.num_pages) atomicAdd(&a.refs[was], more);
+        }
+    }
+    copy_pages(a, a.plan[0], blockIdx.x, gridDim.x);
+}
+
+int reorder_workspace_ints(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *ints) {
+    DOE_REQUIRE(num_pages > 0 && num_pages < ((int64_t)1 << 30), DOE_E_INVALID, "num_pages %lld", (long long)num_pages);
+    DOE_REQUIRE(max_seqs > 0 && max_seqs <= ((int64_t)1 << 24), DOE_E_INVALID, "max_seqs %lld", (long long)max_seqs);
+    DOE_REQUIRE(n >= 0 && n <= kReorder, DOE_E_UNSUPPORTED, "n %lld outside 0..%d", (long long)n, kReorder);
+    *ints = 16 + num_pages + max_seqs + 6 * n;
+    return DOE_OK;
+}
+
 int workspace_ints(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *ints) {
     DOE_REQUIRE(num_pages > 0 && num_pages < ((int64_t)1 << 30), DOE_E_INVALID, "num_pages %lld", (long long)num_pages);
     DOE_REQUIRE(max_seqs >= 0 && max_seqs <= ((int64_t)1 << 24), DOE_E_INVALID, "max_seqs %lld", (long long)max_seqs);
@@ -559,6 +686,52 @@ int doe_kv_pages_copy(void *pools, int64_t layers, int64_t layer_stride, int64_t
     if (n == 0 || layers == 0) return DOE_OK;
     hipLaunchKernelGGL(pages_copy_kernel, dim3(wide_grid(a, n, 0)), dim3(256), 0, (hipStream_t)stream, a);
     DOE_LAUNCH_CHECK("pages_copy_kernel");
+    return DOE_OK;
+}
+
+int doe_beam_reorder_pages_workspace(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *bytes) {
+    DOE_REQUIRE(bytes, DOE_E_INVALID, "null argument");
+    int64_t ints = 0;
+    const int rc = reorder_workspace_ints(num_pages, max_seqs, n, &ints);
+    if (rc) return rc;
+    *bytes = 4 * ints;
+    return DOE_OK;
+}
+
+int doe_beam_reorder_pages(const doe_kv_pages *pages, const int32_t *seqs, const int32_t *parents, int64_t n, int32_t *status,
+                           void *workspace, int64_t workspace_bytes, doe_stream_t stream) {
+    ReorderArgs r{};
+    PageArgs &a = r.p;
+    int rc = page_args(a, pages, parents, seqs, n, true, status);
+    if (rc) return rc;
+    DOE_REQUIRE(seqs || n <= a.max_seqs, DOE_E_INVALID, "%lld sequences of %d slots", (long long)n, a.max_seqs);
+    if ((rc = pool_checks(a))) return rc;
+    int64_t ints = 0;
+    if ((rc = reorder_workspace_ints(a.num_pages, a.max_seqs, n, &ints))) return rc;
+    DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= 4 * ints, DOE_E_INVALID,
+                "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)(4 * ints), (long long)workspace_bytes);
+    if ((rc = doe::require_init())) return rc;
+    if (n == 0) return doe::fill_bytes_async(status, 0, 4, (hipStream_t)stream);
+    a.plan = static_cast<int32_t *>(workspace);
+    a.by_seq = a.plan + 16;
+    a.taken = a.by_seq + a.max_seqs;
+    a.need = a.taken + a.num_pages;
+    a.pair = a.need + n;
+    r.old_len = a.pair + 2 * n;
+    r.heirs = r.old_len + n;
+    r.fresh = r.heirs + n;
+    const int lds = (int)(8 * n);
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)pages_reorder_plan_kernel,
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 8 * kReorder);
+    DOE_HIP_CHECK(attr_rc);
+    hipLaunchKernelGGL(pages_reorder_plan_kernel, dim3(1), dim3(kPlan), lds, (hipStream_t)stream, r);
+    DOE_LAUNCH_CHECK("pages_reorder_plan_kernel");
+    // a workgroup's cells fit in 32 KB, and the columns spread over the device
+    r.columns = (int)std::max<int64_t>(1, std::min<int64_t>({64, kReorder / n, (a.table_stride + 255) / 256 * 16}));
+    const int64_t chunks = (a.table_stride + r.columns - 1) / r.columns;
+    const unsigned wgs = (unsigned)std::max<int64_t>(chunks, wide_grid(a, n, 0));
+    hipLaunchKernelGGL(pages_reorder_kernel, dim3(wgs), dim3(256), (size_t)n * r.columns * 4, (hipStream_t)stream, r);
+    DOE_LAUNCH_CHECK("pages_reorder_kernel");
     return DOE_OK;
 }
 

@@ -8,8 +8,10 @@
 // comparisons over all codes' borders and their neighbours.  A block with an
 // infinity or a NaN keeps scale byte 255 (codes 0) and reads as NaN throughout.
 #include "mx4_cache.h"
+#include "rope_rows.h"
 
 #include <math.h>
+#include <algorithm>
 
 namespace {
 
@@ -26,7 +28,25 @@ struct RowArgs {
     float *k_out, *v_out;
     const int32_t *row_starts;
     int64_t rows, row_stride;
+    // a rotating call: the workgroups from kv_wgs on take the queries
+    doe::RopeRows r;
+    int kv_wgs, q_rows, q_ways;
 };
+
+// The queries' part of a rotating call; false: this workgroup is one of the cache's.
+__device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_pos) {
+    const int wg = (int)blockIdx.x - a.kv_wgs;
+    if (wg < 0) return false;
+    const int64_t row0 = (int64_t)(wg / a.q_ways) * a.q_rows;
+    const int count = a.rows - row0 < a.q_rows ? (int)(a.rows - row0) : a.q_rows;
+    doe::rotate_queries(a.r, a.c.lens, (int64_t)a.c.table_stride << a.c.page_shift, a.c.batch, a.row_starts, row0, count, head_dim,
+                        wg % a.q_ways, a.q_ways, s_pos);
+    return true;
+}
+__device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own, const float *head, int d, int pos) {
+    const doe::f4 v = doe::rotate_four(a.r, head, d, doe::f4{own.x, own.y, own.z, own.w}, pos);
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
 
 // Bits of the largest magnitude over each 8 lanes, an infinity's or NaN's above
 // all others (as numbers a maximum would drop a NaN).
@@ -66,10 +86,15 @@ struct Place {
 // thread four dims of K and V of a row's head.  10430 rows of 16 heads (f32: 214 MB and 28
 // of codes) are written in 87 us and read in 62 (2.8 and 3.9 TB/s), f16 written in 74: two
 // bytes of K and one of V a store.
-template <bool F16>
+// ROPE: K is rotated on the way, and the queries with it.
+template <bool F16, bool ROPE = false>
 __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
     constexpr int D = 160;
     __shared__ Place place[kRowsPerWg];
+    __shared__ int positions[ROPE ? doe::kRopeRowsPerWg : 1];
+    if constexpr (ROPE) {
+        if (queries(a, D, positions)) return;
+    }
     const int64_t row0 = (int64_t)blockIdx.x * kRowsPerWg;
     if (threadIdx.x < kRowsPerWg) {
         const int64_t row = row0 + threadIdx.x;
@@ -78,6 +103,10 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         if (row < a.rows && doe::mx4_row(a.c, a.row_starts, row, b, pos)) {
             const int page = doe::mx4_page(a.c, b, pos);
             if (page >= 0) p = Place{(int64_t)page * a.c.kv_heads, pos & ((1 << a.c.page_shift) - 1)};
+            if constexpr (ROPE) {
+                if (pos >= a.r.max_positions) p.page = -1;
+                positions[threadIdx.x] = pos;
+            }
         }
         place[threadIdx.x] = p;
     }
@@ -99,6 +128,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         } else {
             k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.k) + at);
             v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.v) + at);
+            if constexpr (ROPE) k = rotated(a, k, static_cast<const float *>(a.k) + at - d, d, positions[r]);
         }
         int ks, vs;
         const uint32_t kc = quantise(k, ks), vc = quantise(v, vs);
@@ -242,11 +272,14 @@ struct Exchange {
     }
 };
 
-template <int D, bool F16>
+template <int D, bool F16, bool ROPE = false>
 __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     using S = Mx4Slab<D>;
     constexpr int C = D / 16;
     __shared__ __align__(16) uint8_t lds[256 * 8];
+    if constexpr (ROPE) {
+        if (queries(a, D, reinterpret_cast<int *>(lds))) return;
+    }
     const Exchange<D> x(lds);
     Four f;
     int head;
@@ -259,6 +292,7 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     for (int i = 0; i < 4; ++i) {
         const int64_t row = f.row0 + i;
         in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && row < a.rows;
+        if constexpr (ROPE) in[i] = in[i] && f.pos0 + i < a.r.max_positions;
         all = all && in[i];
         if (!in[i]) continue;
         const int64_t at = row * a.row_stride + (int64_t)head * D + d;
@@ -272,6 +306,7 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
             const f4 vf = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(static_cast<const float *>(a.v) + at));
             k[i] = make_float4(kf[0], kf[1], kf[2], kf[3]);
             v[i] = make_float4(vf[0], vf[1], vf[2], vf[3]);
+            if constexpr (ROPE) k[i] = rotated(a, k[i], static_cast<const float *>(a.k) + at - d, d, f.pos0 + i);
         }
     }
     uint32_t vc[4] = {};
@@ -372,6 +407,23 @@ void launch_write(bool f16, hipStream_t st, const RowArgs &a) {
         if (f16) hipLaunchKernelGGL((mx4_write_fours_kernel<D, true>), fours_grid<D>(a), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((mx4_write_fours_kernel<D, false>), fours_grid<D>(a), dim3(256), 0, st, a);
     }
+}
+
+// Rotating: the queries' workgroups behind the cache's.
+template <int D>
+int launch_append(hipStream_t st, RowArgs &a) {
+    const dim3 kv = D == 160 ? rows_grid(a) : fours_grid<D>(a);
+    const int64_t q_units = (int64_t)a.r.num_heads * (D / 8);
+    a.q_rows = (int)std::max<int64_t>(1, std::min<int64_t>(doe::kRopeRowsPerWg, a.rows / 2048));
+    a.q_ways = a.q_rows > 1 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(64, (q_units + 255) / 256));
+    a.kv_wgs = (int)kv.x;
+    const unsigned q_wgs = a.r.num_heads ? (unsigned)((a.rows + a.q_rows - 1) / a.q_rows * a.q_ways) : 0;
+    DOE_REQUIRE((int64_t)kv.x + q_wgs < (1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %d and %d heads in one call", (long long)a.rows,
+                a.r.num_heads, a.c.kv_heads);  // (a launch has fewer than 2^32 threads)
+    if constexpr (D == 160) hipLaunchKernelGGL((mx4_write_kernel<false, true>), dim3(kv.x + q_wgs), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((mx4_write_fours_kernel<D, false, true>), dim3(kv.x + q_wgs), dim3(256), 0, st, a);
+    DOE_LAUNCH_CHECK("mx4_write_kernel");
+    return DOE_OK;
 }
 
 template <int D>
@@ -475,6 +527,35 @@ int doe_mx4_kv_write(const doe_mx4_cache *cache, const void *k, const void *v, i
     }
     DOE_LAUNCH_CHECK("mx4_write_kernel");
     return DOE_OK;
+}
+
+int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_t row_stride, void *q_out, int q_f16,
+                            int64_t q_row_stride, int64_t num_heads, const float *freq_cis, int64_t max_positions,
+                            int64_t rotary_dim, int interleaved, const int32_t *row_starts, int64_t rows, doe_stream_t stream) {
+    RowArgs a{};
+    int rc = doe::mx4_view(cache, &a.c);
+    if (rc) return rc;
+    const int64_t d = cache->head_dim;
+    if ((rc = doe::rope_rows_checks(a.r, qkv, row_stride, q_out, q_f16, q_row_stride, num_heads, a.c.kv_heads, d, freq_cis,
+                                    max_positions, rotary_dim, interleaved, row_starts, rows, a.c.batch)))
+        return rc;
+    const float *k = qkv + num_heads * d, *v = k + a.c.kv_heads * d;
+    if ((rc = row_checks(a.c, d, rows, row_stride, row_starts, qkv ? k : nullptr, qkv ? v : nullptr, 4))) return rc;
+    if ((rc = doe::require_init())) return rc;
+    if (rows == 0 || a.c.batch == 0) return DOE_OK;
+    a.k = k;
+    a.v = v;
+    a.row_starts = row_starts;
+    a.rows = rows;
+    a.row_stride = row_stride;
+    const hipStream_t st = (hipStream_t)stream;
+    switch (d) {
+        case 64: return launch_append<64>(st, a);
+        case 128: return launch_append<128>(st, a);
+        case 160: return launch_append<160>(st, a);
+        case 256: return launch_append<256>(st, a);
+        default: return launch_append<512>(st, a);
+    }
 }
 
 int doe_mx4_kv_read(const doe_mx4_cache *cache, float *k, float *v, int64_t row_stride, const int32_t *row_starts,

@@ -916,6 +916,184 @@ def kv_pages_copy(pools: DeviceBuffer, sources: DeviceBuffer, destinations: Devi
               _p(status), _p(workspace), workspace.nbytes, _stream_ptr(stream))
 
 
+class _F16CacheArgs(C.Structure):
+    """doe_f16_cache, field for field."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_pool", "v_pool", "page_table", "kv_lens")] + [
+        (n, C.c_int64) for n in ("num_pages", "page_size", "num_kv_heads", "head_dim", "batch", "table_stride")]
+
+
+class _LoraArgs(C.Structure):
+    """doe_lora, field for field."""
+    _fields_ = [(n, C.c_void_p) for n in ("a", "b", "scales")] + [
+        (n, C.c_int64) for n in ("num_adapters", "rank", "k", "slices")] + [("slice_n", C.c_int64 * 4), ("bf16", C.c_int32)]
+
+
+class F16Cache:
+    """One layer's KV cache in f16 pages ([num_pages][page_size][num_kv_heads]
+    [head_dim] of K and V, the order that ``attention_dispatch`` reads with
+    kv_layout 2), with the page table and lengths of ``batch`` sequences (device
+    int32).  Keeps its buffers alive; build one per layer and use it for every
+    call."""
+
+    def __init__(self, k_pool: DeviceBuffer, v_pool: DeviceBuffer, page_table: DeviceBuffer, kv_lens: DeviceBuffer, *,
+                 num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch: int, table_stride: int):
+        size = num_pages * page_size * num_kv_heads * head_dim * 2
+        _need(k_pool, size, "k_pool")
+        _need(v_pool, size, "v_pool")
+        _need(page_table, batch * table_stride * 4, "page_table")
+        _need(kv_lens, batch * 4, "kv_lens")
+        self.buffers = (k_pool, v_pool, page_table, kv_lens)
+        self.num_kv_heads, self.head_dim, self.batch = num_kv_heads, head_dim, batch
+        self.args = _F16CacheArgs(k_pool.ptr, v_pool.ptr, page_table.ptr, kv_lens.ptr, num_pages, page_size, num_kv_heads,
+                                  head_dim, batch, table_stride)
+
+
+def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: DeviceBuffer | None, rows: int, *,
+                    num_heads: int, freq_cis: DeviceBuffer | None, max_positions: int, rotary_dim: int | None = None,
+                    interleaved: bool = False, q_f16: bool = False, row_starts: DeviceBuffer | None = None,
+                    row_stride: int | None = None, q_row_stride: int | None = None, stream=None) -> None:
+    """``rope`` and cache write of many sequences' rows [q heads | k heads | v
+    heads] (f32) at once: q and k rotated at each row's position, q to ``q_out``
+    (f32 or f16; ``qkv`` itself: in place), k and v into the cache's pages (one row a
+    sequence, or with ``row_starts`` the rows of ragged prompts, the last of a
+    sequence at kv_len - 1).  ``freq_cis`` [max_positions][rotary_dim / 2][2];
+    ``rotary_dim`` None: the whole head."""
+    d, hd = cache.head_dim, num_heads * cache.head_dim
+    width = hd + 2 * cache.num_kv_heads * d
+    stride = width if row_stride is None else row_stride
+    qs = q_row_stride if q_row_stride is not None else (stride if q_out is qkv else hd)
+    rot = d if rotary_dim is None else rotary_dim
+    _mx4_rows(cache, rows, row_starts)
+    if rows:
+        _need(qkv, ((rows - 1) * stride + width) * 4, "qkv")
+        if num_heads:
+            if q_out is None:
+                raise ValueError("no q_out for the rotated queries")
+            _need(q_out, ((rows - 1) * qs + hd) * (2 if q_f16 else 4), "q_out")
+        if rot and max_positions:
+            if freq_cis is None:
+                raise ValueError(f"no freq_cis for a rotary_dim of {rot}")
+            _need(freq_cis, max_positions * rot * 4, "freq_cis")
+    fn = "doe_mx4_qkv_rope_append" if isinstance(cache, Mx4Cache) else "doe_qkv_rope_append"
+    _lib.call(fn, C.byref(cache.args), _p(qkv), stride, _opt(q_out), int(q_f16), qs, num_heads, _opt(freq_cis), max_positions,
+              rot, int(interleaved), _opt(row_starts), rows, _stream_ptr(stream))
+
+
+class Lora:
+    """Low-rank adapters beside a shared projection: ``a`` [num_adapters][slices *
+    rank][k] and ``b`` [num_adapters][n][rank] in f16 (or bf16), ``scales`` (f32)
+    or None.  ``slice_n``: the columns of the projections that share the input (one
+    to four).  Keeps its buffers alive."""
+
+    def __init__(self, a: DeviceBuffer, b: DeviceBuffer, scales: DeviceBuffer | None, *, num_adapters: int, rank: int, k: int,
+                 slice_n, bf16: bool = False):
+        slice_n = [int(n) for n in slice_n]
+        if not 1 <= len(slice_n) <= 4:
+            raise ValueError(f"{len(slice_n)} slices, expected one to four")
+        _need(a, num_adapters * len(slice_n) * rank * k * 2, "a")
+        _need(b, num_adapters * sum(slice_n) * rank * 2, "b")
+        if scales is not None:
+            _need(scales, num_adapters * 4, "scales")
+        self.buffers = (a, b, scales)
+        self.k, self.n = k, sum(slice_n)
+        self.args = _LoraArgs(a.ptr, b.ptr, None if scales is None else scales.ptr, num_adapters, rank, k, len(slice_n),
+                              (C.c_int64 * 4)(*slice_n), int(bf16))
+
+
+def lora_workspace(lora: Lora, rows: int) -> int:
+    """Workspace bytes of ``lora_add`` over ``rows`` rows."""
+    size = C.c_int64()
+    _lib.call("doe_lora_workspace", C.byref(lora.args), rows, C.byref(size))
+    return size.value
+
+
+def lora_add(lora: Lora, adapters: DeviceBuffer, x: DeviceBuffer, y: DeviceBuffer, rows: int, *, workspace: DeviceBuffer,
+             row_starts: DeviceBuffer | None = None, segments: int | None = None, x_row_stride: int | None = None,
+             y_row_stride: int | None = None, stream=None) -> None:
+    """y[r] += scale B (A x[r]) for the adapter of each row (``adapters``, device
+    int32), or with ``row_starts`` of each of ``segments`` runs of rows; an id outside
+    the adapters is none."""
+    xs = lora.k if x_row_stride is None else x_row_stride
+    ys = lora.n if y_row_stride is None else y_row_stride
+    if row_starts is not None and segments is None:
+        raise ValueError("row_starts without the count of segments")
+    count = rows if segments is None else segments
+    _need(adapters, count * 4, "adapters")
+    if row_starts is not None:
+        _need(row_starts, (count + 1) * 4, "row_starts")
+    if rows:
+        _need(x, ((rows - 1) * xs + lora.k) * 4, "x")
+        _need(y, ((rows - 1) * ys + lora.n) * 4, "y")
+    _lib.call("doe_lora_add", C.byref(lora.args), _p(adapters), _opt(row_starts), count, _p(x), xs, _p(y), ys, rows,
+              _p(workspace), workspace.nbytes, _stream_ptr(stream))
+
+
+def beam_select_workspace(batch: int, beams: int, vocab: int, select: int) -> int:
+    """Workspace bytes of ``beam_select``."""
+    size = C.c_int64()
+    _lib.call("doe_beam_select_workspace", batch, beams, vocab, select, C.byref(size))
+    return size.value
+
+
+def beam_select(logits: DeviceBuffer, scores: DeviceBuffer, *, batch: int, beams: int, vocab: int, select: int,
+                parents: DeviceBuffer, tokens: DeviceBuffer, out_scores: DeviceBuffer, workspace: DeviceBuffer,
+                row_stride: int | None = None, inv_temperature: float = 1.0, finished: DeviceBuffer | None = None,
+                end_token: int = -1, out_finished: DeviceBuffer | None = None, stream=None) -> None:
+    """The ``select`` best of each request's beams x vocabulary by score + log
+    softmax(logits * inv_temperature), best first, ties to the lowest beam, then
+    token: ``parents`` (rows of ``logits``), ``tokens``, ``out_scores``; -1 where
+    there are fewer.  A finished beam offers ``end_token`` at its score."""
+    stride = vocab if row_stride is None else row_stride
+    if batch and beams:
+        _need(logits, ((batch * beams - 1) * stride + vocab) * 4, "logits")
+    _need(scores, batch * beams * 4, "scores")
+    if finished is not None:
+        _need(finished, batch * beams * 4, "finished")
+    for buf, role in ((parents, "parents"), (tokens, "tokens"), (out_scores, "out_scores"), (out_finished, "out_finished")):
+        if buf is not None:
+            _need(buf, batch * select * 4, role)
+    _lib.call("doe_beam_select", _p(logits), stride, _p(scores), _opt(finished), batch, beams, vocab, select,
+              inv_temperature, end_token, _p(parents), _p(tokens), _p(out_scores), _opt(out_finished), _p(workspace),
+              workspace.nbytes, _stream_ptr(stream))
+
+
+def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffer, rows: int, *, row_bytes: int,
+                      layers: int = 1, src_rows: int | None = None, src_layer_stride: int | None = None,
+                      dst_layer_stride: int | None = None, stream=None) -> None:
+    """Row i of ``dst`` = row ``parents[i]`` of ``src`` in every layer (strides in
+    bytes); a parent outside the rows leaves its row as it was."""
+    sr = rows if src_rows is None else src_rows
+    ss = sr * row_bytes if src_layer_stride is None else src_layer_stride
+    ds = rows * row_bytes if dst_layer_stride is None else dst_layer_stride
+    if rows and layers:
+        _need(src, (layers - 1) * ss + sr * row_bytes, "src")
+        _need(dst, (layers - 1) * ds + rows * row_bytes, "dst")
+    _need(parents, rows * 4, "parents")
+    _lib.call("doe_beam_reorder_rows", _p(src), _p(dst), _p(parents), sr, rows, row_bytes, layers, ss, ds,
+              _stream_ptr(stream))
+
+
+def beam_reorder_pages_workspace(num_pages: int, max_seqs: int, n: int) -> int:
+    """Workspace bytes of ``beam_reorder_pages``."""
+    size = C.c_int64()
+    _lib.call("doe_beam_reorder_pages_workspace", num_pages, max_seqs, n, C.byref(size))
+    return size.value
+
+
+def beam_reorder_pages(pages: KvPages, parents: DeviceBuffer, n: int, *, status: DeviceBuffer, workspace: DeviceBuffer,
+                       seqs: DeviceBuffer | None = None, stream=None) -> None:
+    """Slot ``seqs[i]`` (None: i) becomes what slot ``seqs[parents[i]]`` was, all at
+    once; a parent below 0 ends it.  Whole pages are shared, a partly filled last
+    one is copied in every layer for all heirs but one.  ``status`` as in the
+    ``kv_pages_`` calls."""
+    _need(parents, n * 4, "parents")
+    if seqs is not None:
+        _need(seqs, n * 4, "seqs")
+    _need(status, 4, "status")
+    _lib.call("doe_beam_reorder_pages", C.byref(pages.args), _opt(seqs), _p(parents), n, _p(status), _p(workspace),
+              workspace.nbytes, _stream_ptr(stream))
+
+
 def tune(key: str, value: int) -> None:
     """Overrides a launch-shape choice (``doe_tune_set``); 0 restores automatic."""
     _lib.call("doe_tune_set", key.encode(), int(value))
@@ -926,6 +1104,9 @@ OPS = {
     "attention_mx4": attention_mx4,
     "attention_mx4_prompt": attention_mx4_prompt,
     "attention_prefill": attention_prefill,
+    "beam_reorder_pages": beam_reorder_pages,
+    "beam_reorder_rows": beam_reorder_rows,
+    "beam_select": beam_select,
     "dequant": dequant_q4k,
     "embed": embed,
     "gelu_gated": gelu_gated,
@@ -936,11 +1117,13 @@ OPS = {
     "kv_pages_free": kv_pages_free,
     "kv_write": kv_write,
     "lm_head": lm_head,
+    "lora_add": lora_add,
     "matmul_q4k": matmul_q4k,
     "matmul_q4k_gemm": matmul_q4k_gemm,
     "matmul_int4g32": matmul_int4g32,
     "mx4_kv_read": mx4_kv_read,
     "mx4_kv_write": mx4_kv_write,
+    "qkv_rope_append": qkv_rope_append,
     "residual": residual,
     "rmsnorm": rmsnorm,
     "rope": rope,

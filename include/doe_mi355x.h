@@ -566,6 +566,108 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
                         float scale, float softcap, int64_t sliding_window, void *workspace, int64_t workspace_bytes,
                         doe_stream_t stream);
 
+/* ---- rows rotated and appended to a paged cache --------------------------------
+ * Rows [num_heads q heads | num_kv_heads k heads | num_kv_heads v heads] of a fused
+ * projection, f32, row_stride elements apart, of any number of sequences
+ * (row_starts, rows, kv_lens as in doe_mx4_kv_write: kv_lens already counts the
+ * rows): each row's q and k heads are rotated at its position, q goes to q_out
+ * (f32, or f16 with q_f16; [num_heads][head_dim], q_row_stride elements apart),
+ * k and v into their pages.  The batched, paged form of doe_qkv_rope_kv_rows and
+ * doe_qkv_rope_half_kv_rows (the prefill steps' rope, rope.wgsl, and the cache
+ * write, run_csl_webgpu_emulator.mjs:615-644), with their arithmetic: pairs
+ * (i, i + rotary_dim / 2) of a head, or (2 i, 2 i + 1) with interleaved, by
+ * freq_cis [max_positions][rotary_dim / 2][2]; dims from rotary_dim on are taken
+ * as they are.
+ * q_out may be the q part of qkv itself (q_out == qkv, f32, the same stride),
+ * otherwise it is apart from qkv.  num_heads 0 appends only.  A row at a position
+ * outside [0, max_positions) has its q unrotated and appends nothing; one whose
+ * page is outside the pool appends nothing; rows of no sequence are left as they
+ * were.  A page that a call writes must not be held by two of its sequences.
+ * rotary_dim is a multiple of 8 (0: no rotation); qkv, q_out and freq_cis are
+ * 16-byte aligned, row strides multiples of 16 bytes.
+ *
+ * The f16 cache: pools [num_pages][page_size][num_kv_heads][head_dim] of K and V,
+ * the order that doe_attention_dispatch reads with kv_layout 2; head_dim a multiple
+ * of 8 up to 1024, any page_size.  page_table and kv_lens as in doe_mx4_cache. */
+typedef struct doe_f16_cache {
+    uint16_t *k_pool, *v_pool;
+    const int32_t *page_table;
+    const int32_t *kv_lens;
+    int64_t num_pages, page_size, num_kv_heads, head_dim, batch, table_stride;
+} doe_f16_cache;
+
+int doe_qkv_rope_append(const doe_f16_cache *cache, const float *qkv, int64_t row_stride, void *q_out, int q_f16,
+                        int64_t q_row_stride, int64_t num_heads, const float *freq_cis, int64_t max_positions,
+                        int64_t rotary_dim, int interleaved, const int32_t *row_starts, int64_t rows,
+                        doe_stream_t stream);
+/* The same into the cache held in 4 bits: the rotated k and the v as
+ * doe_mx4_kv_write holds them. */
+int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_t row_stride, void *q_out, int q_f16,
+                            int64_t q_row_stride, int64_t num_heads, const float *freq_cis, int64_t max_positions,
+                            int64_t rotary_dim, int interleaved, const int32_t *row_starts, int64_t rows,
+                            doe_stream_t stream);
+
+/* ---- low-rank adapters of many requests ----------------------------------------
+ * y[r] += scales[a] B_a (A_a x[r]) beside a shared projection, for the adapter a of
+ * each row's request; no reference counterpart.  x f32 rows of k, x_row_stride
+ * elements apart (16-byte aligned, the stride a multiple of 4); y f32 rows of n,
+ * y_row_stride apart, apart from x: the projection's output.
+ *   a       [num_adapters][slices * rank][k], f16, or bf16 with bf16 != 0
+ *   b       [num_adapters][n][rank], the same type; n = slice_n[0] + ..: the
+ *           projections that share x (q / k / v, gate / up) side by side, the
+ *           columns of slice s taking rows s * rank .. of a
+ *   scales  device f32 [num_adapters], or NULL: 1
+ *   adapters    device int32 [segments]; an id outside [0, num_adapters) is none: its
+ *               rows of y are left as they were
+ *   row_starts  device int32 [segments + 1]: rows [row_starts[s], row_starts[s + 1])
+ *               are segment s's; NULL: rows == segments, a row each.  Rows of no
+ *               segment are left as they were.
+ * f32-accurate (2-3e-7 of float64).  rank a multiple of 8 up to 256, k a multiple of 8
+ * up to 2^20, a and b 16-byte aligned.  The workspace (16-byte aligned,
+ * doe_lora_workspace bytes) is the caller's: calls that may overlap, and captured
+ * graphs that may be replayed side by side, each take their own.  Nothing is kept
+ * in it between calls.  The same bits on every call. */
+typedef struct doe_lora {
+    const void *a;
+    const void *b;
+    const float *scales;
+    int64_t num_adapters, rank, k, slices;
+    int64_t slice_n[4];
+    int32_t bf16;
+} doe_lora;
+
+int doe_lora_workspace(const doe_lora *lora, int64_t rows, int64_t *bytes);
+int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *row_starts, int64_t segments,
+                 const float *x, int64_t x_row_stride, float *y, int64_t y_row_stride, int64_t rows, void *workspace,
+                 int64_t workspace_bytes, doe_stream_t stream);
+
+/* ---- beam search ---------------------------------------------------------------
+ * The `select` best continuations of each request's beams, beside the greedy
+ * doe_argmax; no reference counterpart.  Row r = request * beams + beam of logits
+ * (f32, row_stride elements apart, 4-byte aligned) offers token t at
+ * scores[r] + log softmax(inv_temperature * logits[r])[t]; a logit of -infinity is
+ * no offer.  Where finished (device int32 [batch][beams], or NULL) is not 0 the beam
+ * offers end_token alone, at scores[r].  A beam whose score is not finite offers
+ * nothing, nor does a row with a NaN or +infinity among its logits.
+ * Out, [batch][select], best first, ties to the lowest beam, then token: parents
+ * (the rows; -1 where there are fewer offers), tokens (-1), out_scores (-infinity),
+ * out_finished (may be NULL: 1 where the parent was finished or the token is
+ * end_token).  end_token -1: none (finished is then NULL).  Scores are compared in 64 bits.
+ * beams and select up to 64, vocab up to 2^24.  The workspace (16-byte aligned,
+ * doe_beam_select_workspace bytes) is the caller's, as for doe_lora_add. */
+int doe_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t select, int64_t *bytes);
+int doe_beam_select(const float *logits, int64_t row_stride, const float *scores, const int32_t *finished,
+                    int64_t batch, int64_t beams, int64_t vocab, int64_t select, float inv_temperature,
+                    int64_t end_token, int32_t *parents, int32_t *tokens, float *out_scores, int32_t *out_finished,
+                    void *workspace, int64_t workspace_bytes, doe_stream_t stream);
+/* Dense states (recurrent states, token records) in the order of their parents: row
+ * i of dst = row parents[i] of src in every layer, rows row_bytes (a multiple of 4)
+ * apart, layers the strides apart.  Rows whose parent is outside [0, src_rows) are
+ * left as they were; src and dst are apart from each other. */
+int doe_beam_reorder_rows(const void *src, void *dst, const int32_t *parents, int64_t src_rows, int64_t rows,
+                          int64_t row_bytes, int64_t layers, int64_t src_layer_stride, int64_t dst_layer_stride,
+                          doe_stream_t stream);
+
 /* ---- pages of a KV cache -------------------------------------------------------
  * The bookkeeping of a paged cache on the device, of any page format (the 4-bit
  * cache above, or the f16 pages of doe_attention_dispatch): sequences 0 ..
@@ -612,6 +714,17 @@ int doe_kv_pages_compact(const doe_kv_pages *pages, int32_t *status, void *works
 int doe_kv_pages_copy(void *pools, int64_t layers, int64_t layer_stride, int64_t page_bytes, int64_t num_pages,
                       const int32_t *sources, const int32_t *destinations, int64_t n, int32_t *status, void *workspace,
                       int64_t workspace_bytes, doe_stream_t stream);
+
+/* Sequences in the order of their parents (a step of beam search), all at once: slot
+ * seqs[i] (seqs NULL: i) becomes what slot seqs[parents[i]] was, 0 <= i < n; parents[i]
+ * < 0 ends it.  Whole pages are shared by all heirs of a parent; of a partly filled
+ * last page the heir in the parent's own slot, else the first one, keeps the page and
+ * the others get copies, in pages that were free before the call.  *status as above
+ * (-1: a slot outside [0, max_seqs) or named twice, a parent >= n, a length beyond the
+ * table row).  n up to 8192; the workspace is doe_beam_reorder_pages_workspace bytes. */
+int doe_beam_reorder_pages_workspace(int64_t num_pages, int64_t max_seqs, int64_t n, int64_t *bytes);
+int doe_beam_reorder_pages(const doe_kv_pages *pages, const int32_t *seqs, const int32_t *parents, int64_t n,
+                           int32_t *status, void *workspace, int64_t workspace_bytes, doe_stream_t stream);
 
 /* ---- normalisation, position and elementwise ops ---------------------------
  * RMSNorm per row: out = x * 1/sqrt(mean(x^2) + eps) * (w or 1 + w).
