@@ -10,6 +10,7 @@
 #pragma once
 
 #include "common.h"
+#include "wave.h"
 
 namespace doe {
 
@@ -75,20 +76,6 @@ __device__ __forceinline__ bool mx4_row(const Mx4View &c, const int32_t *row_sta
 __device__ __forceinline__ int mx4_page(const Mx4View &c, int b, int pos) {
     const int page = c.table[(int64_t)b * c.table_stride + (pos >> c.page_shift)];
     return page >= 0 && page < c.num_pages ? page : -1;
-}
-
-// Inclusive sum over the wave's lanes, in registers.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-    v = dpp_add<0x111, 0xf>(v);  // one lane further within sixteen, two, four, eight
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);     // the last lane of a sixteen to the next (rows 1 and 3)
-    return dpp_add<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
 }
 
 // A scale byte as the conversions take it: they look at the exponent field alone,
