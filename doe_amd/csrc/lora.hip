@@ -1,9 +1,12 @@
 // lora.hip -- low-rank adapters of many requests beside a shared projection
 // (doe_lora_add): y[r] += s_a B_a (A_a x[r]) for the adapter a of row r's request.
 //
-// Rows of their own (decode steps): lora_token_kernel, one launch.  A workgroup takes a
-// row and some of its columns, forms the t = A x that they need itself (again in every
-// workgroup of the row: A comes from the caches) and adds B t.
+// Rows of their own (decode steps): lora_token_kernel, in one launch where A is small.  A
+// workgroup takes a row and 1024 of its columns, forms the t = A x that they need itself
+// (again in every workgroup of the row: A comes from the caches) and adds B t; else t is
+// formed by a launch before.  One token beside a projection of 2048 to 2304, rank 16: 4.9
+// us in the kernel, a chain of cold reads (adapter, A and x) and two exchanges; 64 of 48
+// adapters beside q/k/v (19.6 MB): 7.2 us, 2.7 TB/s.
 // Runs of rows (prompts): two launches over tiles of 32 rows of a segment.
 //   * lora_down_tiles_kernel: t^T = A x^T on v_mfma_f32_16x16x32: a lane's x row is the
 //     column of its sums, so that a row's scale is the lane's own.  x is f32: for f16
@@ -12,6 +15,10 @@
 //     that grows; for bf16 ones as three bf16 parts, its 24 bits.
 //   * lora_up_tiles_kernel: y += t B^T on v_mfma_f32_32x32x16, t in parts as above, a
 //     lane a column: rows of y are read and written in runs of 128 bytes.
+// Bound by y's bytes: 4096 rows of twelve segments beside gate and up (2304 to 18432, rank
+// 32, f16: 656 MB) 102 us, 6.4 TB/s with what the last-level cache still holds; 15 of them
+// in the first kernel, 85 to 94 in the second.  2048 rows of four, 5376 to 21504, rank 64, bf16
+// (410 MB): 90 us, 13 and 79, where every tile reads the 2.7 MB of an adapter's B again.
 #include "common.h"
 #include "wave.h"
 
@@ -36,7 +43,7 @@ struct LoraArgs {
     float *y, *t;  // t [split][rows][slices * rank]
     int64_t x_stride, y_stride;
     int segments, rows, num_adapters, rank, k, n, slices;
-    int splits, tiles, columns;  // columns of a workgroup
+    int splits, columns;  // columns of a workgroup
     int slice_end[4], group_end[4];  // columns and workgroups up to a slice's end
 };
 
@@ -68,34 +75,38 @@ __device__ __forceinline__ int adapter_of(const LoraArgs &a, int row) {
     }
     return adapter_at(a, s);
 }
-// Tile `tile` of 32 rows: its adapter (-1: none, or no such tile), first row and rows.
-constexpr int kTile = 32;
-__device__ __forceinline__ int find_tile(const LoraArgs &a, int tile, int &row, int &count) {
+// Tiles of 32 rows.  Segment i has the places from row_starts[i] / 32 + i on, one more than
+// its rows can take at most, so that a place's segment is found by a search in
+// row_starts, 64 ways at a time.  Returns the place's adapter (-1: none, or no rows).
+constexpr int kTile = 32, kShift = 5;
+__device__ __forceinline__ int find_tile(const LoraArgs &a, int place, int &row, int &count) {
     const int lane = threadIdx.x & 63;
     row = count = 0;
-    if (!a.row_starts) {
-        row = tile;
-        count = 1;
-        return tile < a.rows ? adapter_at(a, tile) : -1;
-    }
-    for (int s0 = 0; s0 < a.segments; s0 += 64) {
-        const int s = s0 + lane;
-        const int lo = s < a.segments ? a.row_starts[s] : 0, hi = s < a.segments ? a.row_starts[s + 1] : 0;
-        const int rows = lo < 0 ? 0 : std::max(0, std::min(hi, a.rows) - lo);
-        const int upto = doe::wave_scan((rows + kTile - 1) / kTile);
-        const uint64_t behind = __ballot(upto > tile);
-        if (behind) {
-            const int at = __builtin_ctzll(behind);
-            const int in = tile - (at ? __builtin_amdgcn_readlane(upto, at - 1) : 0);
-            row = __builtin_amdgcn_readlane(lo, at) + in * kTile;
-            count = std::min(kTile, __builtin_amdgcn_readlane(rows, at) - in * kTile);
-            return adapter_at(a, s0 + at);
+    int lo = 0, n = a.segments, start = 0, end = 0;
+    for (;;) {
+        const int step = (n + 63) >> 6, i = lo + lane * step;
+        const bool in = i < lo + n;
+        const int from = in ? a.row_starts[i] : 0, to = in && step == 1 ? a.row_starts[i + 1] : 0;
+        const uint64_t at_or_before = __ballot(in && (from >> kShift) + i <= place);
+        if (at_or_before == 0) return -1;
+        const int at = 63 - __builtin_clzll(at_or_before);
+        if (step == 1) {
+            lo += at;
+            start = __builtin_amdgcn_readlane(from, at);
+            end = __builtin_amdgcn_readlane(to, at);
+            break;
         }
-        tile -= __builtin_amdgcn_readlane(upto, 63);
+        lo += at * step;
+        n = std::min(step, n - at * step);
     }
-    return -1;
+    if (start < 0) return -1;
+    const int64_t first = (int64_t)start + (int64_t)(place - (start >> kShift) - lo) * kTile;
+    const int left = (int)(std::min(end, a.rows) - first);
+    if (left <= 0) return -1;
+    row = (int)first;
+    count = std::min(kTile, left);
+    return adapter_at(a, lo);
 }
-
 template <bool BF16>
 __device__ __forceinline__ void weights8(const u32x4 w, float *f) {
     if constexpr (BF16) {
@@ -155,34 +166,75 @@ __device__ __forceinline__ void token_down(const LoraArgs &a, const uint16_t *w,
     __syncthreads();
 }
 
-// A row's columns from `col` to `end`, a thread each.
+// t of a row, four rows of A a workgroup, its waves every fourth 512 of k.
 template <bool BF16>
-__device__ __forceinline__ void token_up(const LoraArgs &a, int row, int id, const float *t, int col, int end) {
-    const float scale = a.scales ? a.scales[id] : 1.0f;
-    for (int c = col + threadIdx.x; c < end; c += 64 * kTokenWaves) {
-        const uint16_t *b = a.b + ((int64_t)id * a.n + c) * a.rank;
-        float sum = 0.0f;
-        for (int j = 0; j < a.rank; j += 8) {
-            float f[8];
-            weights8<BF16>(*reinterpret_cast<const u32x4 *>(b + j), f);
+__global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
+    __shared__ float part[4][4];
+    const int per_row = a.slices * a.rank, fours = per_row / 4, row = blockIdx.x / fours, j0 = (blockIdx.x - row * fours) * 4;
+    const int id = adapter_of(a, row);
+    if (id < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint16_t *w = a.a + ((int64_t)id * per_row + j0) * a.k;
+    const float *x = a.x + (int64_t)row * a.x_stride;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (int at = wave * 512 + lane * 8; at < a.k; at += 2048) {
+        const f4 x0 = *reinterpret_cast<const f4 *>(x + at), x1 = *reinterpret_cast<const f4 *>(x + at + 4);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(t[j + i], f[i], sum);
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+            weights8<BF16>(*reinterpret_cast<const u32x4 *>(w + (int64_t)j * a.k + at), f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[j] = fmaf(x1[i], f[i + 4], fmaf(x0[i], f[i], sum[j]));
         }
-        float *y = a.y + (int64_t)row * a.y_stride + c;
-        *y = fmaf(scale, sum, *y);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        sum[j] = wave_sum(sum[j]);
+        if (lane == 0) part[j][wave] = sum[j];
+    }
+    __syncthreads();
+    const int j = threadIdx.x;
+    if (j < 4) a.t[(int64_t)row * per_row + j0 + j] = (part[j][0] + part[j][1]) + (part[j][2] + part[j][3]);
 }
 
-template <bool BF16>
+// A thread a column; its B and y are on their way while t is formed (FUSED), or read.
+template <bool BF16, bool FUSED>
 __global__ __launch_bounds__(64 * kTokenWaves) void lora_token_kernel(LoraArgs a) {
     __shared__ __align__(16) float t[kMaxRank];
-    __shared__ float part[kMaxRank][kTokenWaves];
+    __shared__ float part[FUSED ? kMaxRank : 1][kTokenWaves];
     const int groups = a.group_end[3], row = blockIdx.x / groups, id = adapter_of(a, row);
     if (id < 0) return;
     int slice, col, end;
     columns_of(a, blockIdx.x - row * groups, slice, col, end);
-    token_down<BF16>(a, a.a + ((int64_t)id * a.slices + slice) * a.rank * a.k, a.x + (int64_t)row * a.x_stride, t, part);
-    token_up<BF16>(a, row, id, t, col, end);
+    col += threadIdx.x;
+    constexpr int kAhead = 4;  // eights of the rank
+    const uint16_t *b = a.b + ((int64_t)id * a.n + std::min(col, end - 1)) * a.rank;
+    float *y = a.y + (int64_t)row * a.y_stride + std::min(col, end - 1), was = *y;
+    u32x4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = *reinterpret_cast<const u32x4 *>(b + (8 * i < a.rank ? 8 * i : 0));
+    const float scale = a.scales ? a.scales[id] : 1.0f;
+    if constexpr (FUSED) {
+        token_down<BF16>(a, a.a + ((int64_t)id * a.slices + slice) * a.rank * a.k, a.x + (int64_t)row * a.x_stride, t, part);
+    } else {
+        if ((int)threadIdx.x < a.rank) t[threadIdx.x] = a.t[((int64_t)row * a.slices + slice) * a.rank + threadIdx.x];
+        __syncthreads();
+    }
+    if (col >= end) return;
+    float sum = 0.0f;
+    auto add = [&](const u32x4 &w, int j) __attribute__((always_inline)) {
+        float f[8];
+        weights8<BF16>(w, f);
+        const f4 t0 = *reinterpret_cast<const f4 *>(t + j), t1 = *reinterpret_cast<const f4 *>(t + j + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = fmaf(t1[i], f[4 + i], fmaf(t0[i], f[i], sum));
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (8 * i < a.rank) add(ahead[i], 8 * i);
+    for (int j = 8 * kAhead; j < a.rank; j += 8) add(*reinterpret_cast<const u32x4 *>(b + j), j);
+    *y = fmaf(scale, sum, was);
 }
 
 // ---- tiles of 32 rows ----------------------------------------------------------------
@@ -198,98 +250,150 @@ __device__ __forceinline__ f4 mfma16(b8 a, b8 b, f4 c) { return __builtin_amdgcn
 __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(b8 a, b8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-// Eight values in parts whose sum has 22 bits of them (f16) or all (bf16).
+// Eight values, times a power of two, in parts whose sum has 22 bits of them (f16: hi,
+// cut off, and lo of what that leaves) or all 24 (bf16: eight bits a part; `scale`
+// is 1).
 template <bool BF16>
-__device__ __forceinline__ Parts<BF16> split8(const float *f) {
+__device__ __forceinline__ Parts<BF16> split8(const float *f, float scale) {
     Parts<BF16> p;
+    u32x4 u[Parts<BF16>::kCount];
+    float minus = -1.0f;  // (a value, so that g - hi is one instruction that takes hi as f16)
+    __asm__ volatile("" : "+v"(minus));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
+        const float f0 = f[2 * i], f1 = f[2 * i + 1];
         if constexpr (BF16) {
-            const __bf16 b0 = (__bf16)f[i];
-            const float r0 = f[i] - (float)b0;
-            const __bf16 b1 = (__bf16)r0;
-            p.v[0][i] = b0;
-            p.v[1][i] = b1;
-            p.v[2][i] = (__bf16)(r0 - (float)b1);
+            constexpr uint32_t kUpper = 0x07060302u;  // the upper halves of both
+            const float g0 = f0 - __uint_as_float(__float_as_uint(f0) & 0xffff0000u), g1 = f1 - __uint_as_float(__float_as_uint(f1) & 0xffff0000u);
+            const float h0 = g0 - __uint_as_float(__float_as_uint(g0) & 0xffff0000u), h1 = g1 - __uint_as_float(__float_as_uint(g1) & 0xffff0000u);
+            u[0][i] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), kUpper);
+            u[1][i] = __builtin_amdgcn_perm(__float_as_uint(g1), __float_as_uint(g0), kUpper);
+            u[2][i] = __builtin_amdgcn_perm(__float_as_uint(h1), __float_as_uint(h0), kUpper);
         } else {
-            const _Float16 h = (_Float16)f[i];
-            p.v[0][i] = h;
-            p.v[1][i] = (_Float16)(f[i] - (float)h);
+            const float g0 = f0 * scale, g1 = f1 * scale;
+            const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(g0, g1));
+            const h2 lo = {(_Float16)fmaf((float)hi[0], minus, g0), (_Float16)fmaf((float)hi[1], minus, g1)};
+            u[0][i] = __builtin_bit_cast(uint32_t, hi);
+            u[1][i] = __builtin_bit_cast(uint32_t, lo);
         }
     }
+#pragma unroll
+    for (int k = 0; k < Parts<BF16>::kCount; ++k) p.v[k] = __builtin_bit_cast(typename Parts<BF16>::V, u[k]);
     return p;
 }
-// e such that the largest of a row (its bits without the sign) lies in [2^13, 2^14) times
-// 2^-e; 0 for none, infinities and NaN.
-__device__ __forceinline__ int exponent_of(uint32_t top) {
-    return top == 0 || top >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(top)) - 14;
+// e such that the largest magnitude of a row lies in [2^13, 2^14) times 2^-e, held within
+// what 2^-e can be; `none` where there is none, or an infinity.
+__device__ __forceinline__ int exponent_of(float top, int none) {
+    return top > 0.0f && top < __builtin_inff() ? std::max(-112, std::min(112, __builtin_amdgcn_frexp_expf(top) - 14)) : none;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+__device__ __forceinline__ float largest8(const float *f) {
+    float top = fmaxf(fabsf(f[0]), fabsf(f[1]));
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) top = fmaxf(fmaxf(top, fabsf(f[i])), fabsf(f[i + 1]));
+    return top;
 }
 
 constexpr int kDownCols = 64;  // rows of A of a workgroup
 
-// Two steps of 32 of k: a lane's eight values of two x rows and of four rows of A each.
-struct DownRaw {
-    f4 x[2][2][2];  // [step][row tile][half]
-    u32x4 w[2][4];  // [step][column tile]
-};
+// At most N vector-memory operations outstanding.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+    __asm__ volatile("" ::: "memory");
+}
 
-// t^T of a tile and 64 rows of A over this split's share of k: the waves a quarter of it
-// each, added up through LDS.
+// t^T of a tile and 64 rows of A over this split's share of k: the waves take every eighth
+// step of 32 and are added up through LDS.  A step's x (32 rows of 128 bytes) and A (64 of
+// 64) go to the wave's own LDS by direct loads, lanes in the rows' order, two steps under
+// way: read as operands (a lane a row) straight from memory the sixteen lanes that a load
+// takes at once lie in as many lines, four times its time.  16-byte pieces of a row are
+// exchanged by row so that the lanes' reads fall on different banks.
+constexpr int kDownWaves = 8, kStepBytes = 8192;
+constexpr int kDownLds = kDownWaves * 2 * kStepBytes;  // (the sums take half of it at the end)
 template <bool BF16>
-__global__ __launch_bounds__(256, 2) void lora_down_tiles_kernel(LoraArgs a) {
+__global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_tiles_kernel(LoraArgs a) {
     using P = Parts<BF16>;
-    __shared__ f4 sums[4][2][4][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4, per_row = a.slices * a.rank;
     const int col_groups = (per_row + kDownCols - 1) / kDownCols;
-    int rest = blockIdx.x / col_groups, row0, count;
-    const int cols0 = (blockIdx.x - rest * col_groups) * kDownCols, tile = rest / a.splits, split = rest - tile * a.splits;
+    const int rest = blockIdx.x / col_groups, cols0 = (blockIdx.x - rest * col_groups) * kDownCols;
+    const int tile = rest / a.splits, split = rest - tile * a.splits;
+    int row0, count;
     const int id = find_tile(a, tile, row0, count);
     if (id < 0) return;
-    const int steps = (a.k + 31) / 32, parts = 4 * a.splits, part = 4 * split + wave;
-    const int from = (int)((int64_t)steps * part / parts), to = (int)((int64_t)steps * (part + 1) / parts);
-    const float *x[2];
-    const uint16_t *w[4];
+    const int steps = (a.k + 31) / 32, parts = kDownWaves * a.splits, part = kDownWaves * split + wave;
+    const uint8_t *x = reinterpret_cast<const uint8_t *>(a.x + (int64_t)row0 * a.x_stride);
+    const uint8_t *w = reinterpret_cast<const uint8_t *>(a.a + (int64_t)id * per_row * a.k);
+    const uint32_t k4 = 4 * a.k;
+    // this lane's place in the loads: eight rows of x and sixteen of A each
+    uint32_t x_at[4], w_at[4];
+    const uint32_t x_piece = ((lane & 7) ^ (lane >> 4)) * 16, w_piece = ((lane & 3) ^ (lane >> 4)) * 16;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) x[r] = a.x + (int64_t)(row0 + std::min(16 * r + c16, count - 1)) * a.x_stride;
+    for (int i = 0; i < 4; ++i) {
+        x_at[i] = (uint32_t)std::min(8 * i + (lane >> 3), count - 1) * (uint32_t)a.x_stride * 4;
+        w_at[i] = (uint32_t)std::min(cols0 + 16 * i + (lane >> 2), per_row - 1) * (uint32_t)a.k * 2;
+    }
+    uint8_t *mine = lds + wave * 2 * kStepBytes;
+    auto load = [&](int step, int buffer) __attribute__((always_inline)) {
+        // (past the end: k's first values, and weights of zero below)
+        uint8_t *to = mine + buffer * kStepBytes;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) w[c] = a.a + ((int64_t)id * per_row + std::min(cols0 + 16 * c + c16, per_row - 1)) * a.k;
-    auto load = [&](DownRaw &v, int step) __attribute__((always_inline)) {
+        for (int i = 0; i < 4; ++i) {
+            // (rows 8 i .. 8 i + 7: the exchange goes by row / 2)
+            const uint32_t at = 128 * step + (x_piece ^ (64 * (i & 1)));
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(x + (x_at[i] + (at < k4 ? at : 0))),
+                                             (__attribute__((address_space(3))) void *)(to + 1024 * i), 16, 0, 0);
+        }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            // (past the end: k's first values against weights of zero)
-            const bool in = step + s < to && 32 * (step + s) + 8 * g4 < a.k;
-            const int at = in ? 32 * (step + s) + 8 * g4 : 0;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                v.x[s][r][0] = *reinterpret_cast<const f4 *>(x[r] + at);
-                v.x[s][r][1] = *reinterpret_cast<const f4 *>(x[r] + at + 4);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const u32x4 u = *reinterpret_cast<const u32x4 *>(w[c] + at);
-                v.w[s][c] = in ? u : u32x4{0, 0, 0, 0};
-            }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t at = 64 * step + w_piece;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(w + (w_at[i] + (2 * at < k4 ? at : 0))),
+                                             (__attribute__((address_space(3))) void *)(to + 4096 + 1024 * i), 16, 0, 0);
         }
     };
     f4 acc[2][4];
-    int e[2] = {-1000, -1000};  // of the scale of a lane's row
+    constexpr int kUnscaled = -120;
+    int e[2] = {kUnscaled, kUnscaled};  // of the scale of a lane's row
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto add = [&](const DownRaw &v) __attribute__((always_inline)) {
+    load(part, 0);
+    load(part + parts, 1);
+    int buffer = 0;
+#pragma unroll 1
+    for (int step = part; step < steps; step += parts, buffer ^= 1) {
+        wait_vm<8>();  // this step's have landed; the next one's are younger
+        const uint8_t *from = mine + buffer * kStepBytes;
+        f4 raw[2][2];
+        u32x4 wt[4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+            const uint8_t *row = from + (16 * r + c16) * 128;
+            const int turn = c16 >> 1;  // (row / 2) % 8
+            raw[r][0] = *reinterpret_cast<const f4 *>(row + ((2 * g4) ^ turn) * 16);
+            raw[r][1] = *reinterpret_cast<const f4 *>(row + ((2 * g4 + 1) ^ turn) * 16);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) wt[c] = *reinterpret_cast<const u32x4 *>(from + 4096 + (16 * c + c16) * 64 + (g4 ^ (c16 >> 2)) * 16);
+        // (in registers before the next loads overwrite them)
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        load(step + 2 * parts, buffer);
+        const bool in = 128 * step + 32 * g4 < (int)k4;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) wt[c] = in ? wt[c] : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = raw[r][i >> 2][i & 3];
             if constexpr (!BF16) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top = std::max(top, __float_as_uint(v.x[s][r][h][i]) & 0x7fffffffu);
-                int want = top == 0 || top >= 0x7f800000u ? -1000 : exponent_of(top);
+                int want = exponent_of(largest8(f), kUnscaled);
                 if (__any(want > e[r] + 1)) {
                     want = std::max(want, __shfl_xor(want, 16, 64));
                     want = std::max(want, __shfl_xor(want, 32, 64));
@@ -301,27 +405,16 @@ __global__ __launch_bounds__(256, 2) void lora_down_tiles_kernel(LoraArgs a) {
                     e[r] = next;
                 }
             }
+            const P p = split8<BF16>(f, BF16 ? 1.0f : power_of_two(-e[r]));
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float f[8];
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = BF16 ? v.x[s][r][i >> 2][i & 3] : __builtin_amdgcn_ldexpf(v.x[s][r][i >> 2][i & 3], -e[r]);
-                const P p = split8<BF16>(f);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < P::kCount; ++i) acc[r][c] = mfma16(__builtin_bit_cast(typename P::V, v.w[s][c]), p.v[i], acc[r][c]);
-            }
+                for (int i = 0; i < P::kCount; ++i) acc[r][c] = mfma16(__builtin_bit_cast(typename P::V, wt[c]), p.v[i], acc[r][c]);
         }
-    };
-    DownRaw v0, v1;
-    if (from < to) load(v0, from);
-    for (int s = from; s < to; s += 4) {
-        load(v1, s + 2);
-        add(v0);
-        load(v0, s + 4);
-        if (s + 2 < to) add(v1);
     }
+    wait_vm<0>();
+    __syncthreads();  // every wave is done with its buffers
+    f4 *sums = reinterpret_cast<f4 *>(lds);  // [wave][r][c][lane]
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -329,19 +422,23 @@ __global__ __launch_bounds__(256, 2) void lora_down_tiles_kernel(LoraArgs a) {
             if constexpr (!BF16)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[r][c][i] = __builtin_amdgcn_ldexpf(acc[r][c][i], e[r]);
-            sums[wave][r][c][lane] = acc[r][c];
+            sums[((wave * 2 + r) * 4 + c) * 64 + lane] = acc[r][c];
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < 512; i += 256) {
-        const int l = i & 63, c = i >> 6 & 3, r = i >> 8, row = 16 * r + (l & 15), col = cols0 + 16 * c + 4 * (l >> 4);
-        if (row >= count || col >= per_row) continue;
-        const f4 s = (sums[0][r][c][l] + sums[1][r][c][l]) + (sums[2][r][c][l] + sums[3][r][c][l]);
-        *reinterpret_cast<f4 *>(a.t + ((int64_t)split * a.rows + row0 + row) * per_row + col) = s;
-    }
+    static_assert(kDownWaves == 8, "a thread four sums");
+    const int c = wave & 3, r = wave >> 2, row = 16 * r + c16, col = cols0 + 16 * c + 4 * g4;
+    if (row >= count || col >= per_row) return;
+    f4 s = sums[(r * 4 + c) * 64 + lane];
+#pragma unroll
+    for (int v = 1; v < kDownWaves; ++v) s += sums[((v * 2 + r) * 4 + c) * 64 + lane];
+    *reinterpret_cast<f4 *>(a.t + ((int64_t)split * a.rows + row0 + row) * per_row + col) = s;
 }
 
-// y += s t B^T of a tile and a workgroup's columns, 32 of them a wave at a time.  RS: steps
-// of 16 of the rank.
+// y += s t B^T of a tile of 32 rows and a workgroup's columns, 32 of them a wave at a
+// time.  RS: steps of 16 of the rank.  y is read and written past the caches: B, read
+// again for every tile, stays there (four prompts at rank 64: 94 to 80 us).  Tiles of 64
+// rows, which read B half as often, take more registers than there are: 94 to 109 us beside
+// gate and up, 80 to 155 at rank 64.
 template <bool BF16, int RS>
 __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
     using P = Parts<BF16>;
@@ -359,13 +456,12 @@ __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
     __syncthreads();
     {
         // t, its splits added in their order: a thread eight values of a row at a time
-        constexpr int N = (2 * RS + 7) / 8;
-        const int row = tid & 31, per_row = a.slices * a.rank;
-        float f[N][8];
-        uint32_t top = 0;
+        constexpr int kThreads = 256 / kTile, N = (2 * RS + kThreads - 1) / kThreads;  // of a row; units of one
+        const int row = tid % kTile, first = tid / kTile, per_row = a.slices * a.rank;
+        float f[N][8], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = (tid >> 5) + 8 * i;
+            const int u = first + kThreads * i;
             f4 v0 = {0.0f, 0.0f, 0.0f, 0.0f}, v1 = v0;
             if (8 * u < a.rank && row < count) {
                 const float *t = a.t + (int64_t)(row0 + row) * per_row + slice * a.rank + 8 * u;
@@ -376,27 +472,23 @@ __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[i][j] = v0[j], f[i][4 + j] = v1[j];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = std::max(top, __float_as_uint(f[i][j]) & 0x7fffffffu);
+            top = fmaxf(top, largest8(f[i]));
         }
         int e = 0;
         if constexpr (!BF16) {
-            atomicMax(&tops[row], top);
+            atomicMax(&tops[row], __float_as_uint(top));
             __syncthreads();
-            e = exponent_of(tops[row]);
+            e = exponent_of(__uint_as_float(tops[row]), 0);
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = (tid >> 5) + 8 * i;
+            const int u = first + kThreads * i;
             if (u >= 2 * RS) continue;
-            if constexpr (!BF16)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[i][j] = __builtin_amdgcn_ldexpf(f[i][j], -e);
-            const P p = split8<BF16>(f[i]);
+            const P p = split8<BF16>(f[i], power_of_two(-e));
 #pragma unroll
             for (int k = 0; k < P::kCount; ++k) ops[u >> 1][k][(u & 1) * 32 + row] = p.v[k];
         }
-        if (tid < kTile) row_scale[row] = __builtin_amdgcn_ldexpf(scale, e);
+        if (first == 0) row_scale[row] = scale * power_of_two(e);
     }
     __syncthreads();
     float rs[16];
@@ -427,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (mine(r)) v.y[r] = *at(r, col);
+                if (mine(r)) v.y[r] = __builtin_nontemporal_load(at(r, col));
         };
         auto add = [&](Block &v, int c0) __attribute__((always_inline)) {
             const int col = c0 + n32;
@@ -435,20 +527,31 @@ __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
 #pragma unroll
             for (int s = 0; s < RS; ++s)
 #pragma unroll
-                for (int k = 0; k < P::kCount; ++k) acc = mfma32(ops[s][k][lane], __builtin_bit_cast(typename P::V, v.b[s]), acc);
+                for (int k = 0; k < P::kCount; ++k) {
+                    acc = mfma32(ops[s][k][lane], __builtin_bit_cast(typename P::V, v.b[s]), acc);
+                    if (s % 4 == 3 && k == P::kCount - 1) __builtin_amdgcn_sched_barrier(0);  // (t's parts are not read all at once)
+                }
             if (col >= end) return;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (mine(r)) *at(r, col) = fmaf(acc[r], rs[r], v.y[r]);
+                if (mine(r)) __builtin_nontemporal_store(fmaf(acc[r], rs[r], v.y[r]), at(r, col));
         };
-        Block v0 = {}, v1 = {};
         int c = col0 + 32 * wave;
-        if (c < end) load(v0, c);
-        for (; c < end; c += 256) {
-            if (c + 128 < end) load(v1, c + 128);
-            add(v0, c);
-            if (c + 256 < end) load(v0, c + 256);
-            if (c + 128 < end) add(v1, c + 128);
+        Block v0 = {};
+        if constexpr (RS <= 4) {
+            Block v1 = {};
+            if (c < end) load(v0, c);
+            for (; c < end; c += 256) {
+                if (c + 128 < end) load(v1, c + 128);
+                add(v0, c);
+                if (c + 256 < end) load(v0, c + 256);
+                if (c + 128 < end) add(v1, c + 128);
+            }
+        } else {
+            for (; c < end; c += 128) {
+                load(v0, c);
+                add(v0, c);
+            }
         }
     };
     if (count == kTile) work(std::integral_constant<bool, true>());
@@ -491,16 +594,34 @@ int lora_checks(const doe_lora *l, int64_t rows, LoraArgs &a) {
 
 constexpr int kMaxSplits = 8, kCus = 256;
 
-// Whether a call takes tiles: runs of rows long enough to share a tile's weights.
-bool by_tiles(const LoraArgs &a, bool starts, int64_t segments) { return starts && a.rows >= 8 * segments; }
-int64_t tiles_of(const LoraArgs &a, int64_t segments) { return a.rows / kTile + std::min<int64_t>(segments, a.rows); }
-// Splits of k: enough workgroups for the device, two steps of 32 a wave at least.
+// Whether a call takes tiles: where segments have rows to share weights, and what the rows
+// would read of them by themselves is more than the tiles' launches cost.  Rank 16 of 2304
+// to 4096 columns in three slices, rows by themselves against tiles: 64 rows (22 MB) of 32
+// segments 7.3 and 13.3 us, 128 (45 MB) 12.9 and 13.6, 256 (90 MB) 19.8 and 14.6, 512 31.9
+// and 16.7; 32 rows of one segment 6.2 and 12.1; rank 64 of 5376 to 21504, 16 rows of 8
+// (55 MB) 19.5 and 17.7, 64 41.6 and 19.5.
+bool by_tiles(const LoraArgs &a, bool starts, int64_t segments) {
+    const int64_t bytes = 2 * (int64_t)a.rows * a.rank * ((int64_t)a.slices * a.k + a.n);
+    return starts && a.rows >= 2 * segments && bytes > (48 << 20);
+}
+int64_t tiles_of(const LoraArgs &a, int64_t segments) { return a.rows / kTile + segments; }
+// Splits of k: workgroups for the device, two steps of 32 a wave at least.
 int splits_of(const LoraArgs &a, int64_t tiles) {
     const int64_t wgs = tiles * ((a.slices * a.rank + kDownCols - 1) / kDownCols), steps = (a.k + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, 2 * kCus / std::max<int64_t>(1, wgs), steps / 8}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, kCus / std::max<int64_t>(1, wgs), steps / (2 * kDownWaves)}));
 }
 int64_t workspace_of(const LoraArgs &a) {
     return std::max<int64_t>(16, 4 * (int64_t)a.rows * a.slices * a.rank * kMaxSplits);
+}
+
+// Whether a call of rows forms t again in every workgroup that uses it: one launch instead
+// of two, for what a workgroup then reads of A by itself and all of them together.  One
+// launch against two: a token of rank 16, 2048 to 2304 5.0 and 7.0 us, of 5376 to 21504 (172
+// KB a workgroup) 6.4 and 7.0, of rank 64 (688 KB) 14.5 and 9.8; 64 tokens of rank 16, 2304 to
+// 4096 (19 MB) 7.2 and 10.7, 128 (38 MB) 11.6 and 11.2, 200 to 9216 (147 MB) 38.5 and 17.3.
+bool in_one(const LoraArgs &a, int64_t wgs) {
+    const int64_t bytes = 2 * (int64_t)a.rank * a.k;
+    return bytes <= (256 << 10) && wgs * bytes <= (36 << 20);
 }
 
 // Workgroups a slice of `columns` each.
@@ -520,10 +641,8 @@ int fits(const LoraArgs &a, int64_t threads) {
 }
 
 template <bool BF16, int RS>
-int launch_up(const LoraArgs &a, hipStream_t st) {
-    const int64_t wgs = (int64_t)a.tiles * a.group_end[3];
-    const int rc = fits(a, wgs * 256);
-    if (rc) return rc;
+int launch_up(const LoraArgs &a, int64_t segments, hipStream_t st) {
+    const int64_t wgs = tiles_of(a, segments) * a.group_end[3];
     hipLaunchKernelGGL((lora_up_tiles_kernel<BF16, RS>), dim3((unsigned)wgs), dim3(256), 0, st, a);
     DOE_LAUNCH_CHECK("lora_up_tiles_kernel");
     return DOE_OK;
@@ -533,25 +652,35 @@ template <bool BF16>
 int launch(LoraArgs &a, bool starts, int64_t segments, hipStream_t st) {
     int rc;
     if (!by_tiles(a, starts, segments)) {
-        set_columns(a, 1024);
-        const int64_t wgs = (int64_t)a.rows * a.group_end[3];
-        if ((rc = fits(a, wgs * 64 * kTokenWaves))) return rc;
-        hipLaunchKernelGGL(lora_token_kernel<BF16>, dim3((unsigned)wgs), dim3(64 * kTokenWaves), 0, st, a);
+        set_columns(a, 64 * kTokenWaves);
+        const int64_t wgs = (int64_t)a.rows * a.group_end[3], down = (int64_t)a.rows * a.slices * a.rank / 4;
+        if ((rc = fits(a, wgs * 64 * kTokenWaves)) || (rc = fits(a, down * 256))) return rc;
+        if (in_one(a, wgs)) {
+            hipLaunchKernelGGL((lora_token_kernel<BF16, true>), dim3((unsigned)wgs), dim3(64 * kTokenWaves), 0, st, a);
+        } else {
+            hipLaunchKernelGGL(lora_down_rows_kernel<BF16>, dim3((unsigned)down), dim3(256), 0, st, a);
+            DOE_LAUNCH_CHECK("lora_down_rows_kernel");
+            hipLaunchKernelGGL((lora_token_kernel<BF16, false>), dim3((unsigned)wgs), dim3(64 * kTokenWaves), 0, st, a);
+        }
         DOE_LAUNCH_CHECK("lora_token_kernel");
         return DOE_OK;
     }
     const int64_t tiles = tiles_of(a, segments), col_groups = (a.slices * a.rank + kDownCols - 1) / kDownCols;
     a.splits = splits_of(a, tiles);
-    a.tiles = (int)tiles;
     set_columns(a, 512);
-    if ((rc = fits(a, tiles * a.splits * col_groups * 256)) || (rc = fits(a, tiles * a.group_end[3] * 256))) return rc;
-    hipLaunchKernelGGL(lora_down_tiles_kernel<BF16>, dim3((unsigned)(tiles * a.splits * col_groups)), dim3(256), 0, st, a);
+    const int64_t wgs = tiles * a.splits * col_groups;
+    // (both before either runs)
+    if ((rc = fits(a, wgs * 64 * kDownWaves)) || (rc = fits(a, tiles * a.group_end[3] * 256))) return rc;
+    static const hipError_t attr_rc = hipFuncSetAttribute((const void *)lora_down_tiles_kernel<BF16>,
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kDownLds);
+    DOE_HIP_CHECK(attr_rc);
+    hipLaunchKernelGGL(lora_down_tiles_kernel<BF16>, dim3((unsigned)wgs), dim3(64 * kDownWaves), kDownLds, st, a);
     DOE_LAUNCH_CHECK("lora_down_tiles_kernel");
-    if (a.rank <= 16) return launch_up<BF16, 1>(a, st);
-    if (a.rank <= 32) return launch_up<BF16, 2>(a, st);
-    if (a.rank <= 64) return launch_up<BF16, 4>(a, st);
-    if (a.rank <= 128) return launch_up<BF16, 8>(a, st);
-    return launch_up<BF16, 16>(a, st);
+    if (a.rank <= 16) return launch_up<BF16, 1>(a, segments, st);
+    if (a.rank <= 32) return launch_up<BF16, 2>(a, segments, st);
+    if (a.rank <= 64) return launch_up<BF16, 4>(a, segments, st);
+    if (a.rank <= 128) return launch_up<BF16, 8>(a, segments, st);
+    return launch_up<BF16, 16>(a, segments, st);
 }
 
 }  // namespace
@@ -576,7 +705,7 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
     DOE_REQUIRE(segments >= 0 && segments < ((int64_t)1 << 24), DOE_E_INVALID, "segments %lld", (long long)segments);
     DOE_REQUIRE(row_starts || segments == rows, DOE_E_INVALID, "without row_starts a segment is a row (%lld segments, %lld rows)",
                 (long long)segments, (long long)rows);
-    DOE_REQUIRE(x_row_stride >= a.k && x_row_stride % 4 == 0 && x_row_stride < ((int64_t)1 << 32), DOE_E_INVALID,
+    DOE_REQUIRE(x_row_stride >= a.k && x_row_stride % 4 == 0 && x_row_stride < ((int64_t)1 << 24), DOE_E_INVALID,
                 "x_row_stride %lld below k %d, or not a multiple of 4", (long long)x_row_stride, a.k);
     DOE_REQUIRE(y_row_stride >= a.n && y_row_stride < ((int64_t)1 << 26), DOE_E_INVALID, "y_row_stride %lld below the %d columns", (long long)y_row_stride, a.n);
     DOE_REQUIRE(rows == 0 || segments == 0 || (adapters && x && y), DOE_E_INVALID, "null pointer");

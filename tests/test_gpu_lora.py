@@ -129,18 +129,43 @@ def test_ragged_segments(dev, counts, k, slice_n, rank, bf16):
     c.check()
 
 
-@pytest.mark.parametrize("counts", [None, [90, 6]])
+TILES = [
+    # counts, k, slices, rank: enough bytes of weights for tiles of 32 rows
+    ([300, 1, 0, 0, 31, 33, 64, 95], 2304, [1000, 501], 16), ([129, 200], 1032, [260, 3000, 30], 128), ([700], 5000, [2049], 8),
+    ([65, 64, 0, 100], 520, [1096, 40], 256), ([40] * 70, 1000, [333], 24), ([500], 8, [4100, 70, 1, 33], 32), ([1500], 72, [9001], 64),
+]
+
+
+@pytest.mark.parametrize("counts,k,slice_n,rank", TILES)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f16", "bf16"])
+def test_tiles(dev, counts, k, slice_n, rank, bf16):
+    print(f"[lora] {counts[:8]} {k} {slice_n} {rank}", flush=True)
+    assert 2 * sum(counts) * rank * (len(slice_n) * k + sum(slice_n)) > 48 << 20
+    c = Case(k, sum(counts) + 3, k, slice_n, rank, bf16=bf16, counts=counts)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,k,slice_n,rank", [(30, 2304, [9216, 300], 64), (3, 5376, [700], 256), (150, 264, [2000], 128), (200, 2304, [2000, 99], 16)])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f16", "bf16"])
+def test_rows_in_two_launches(dev, rows, k, slice_n, rank, bf16):
+    c = Case(rows, rows, k, slice_n, rank, bf16=bf16)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("counts", [None, [90, 6], [900, 300]])
 def test_strides_and_no_scales(dev, counts):
-    c = Case(7, 96, 264, [37, 64], 16, x_pad=12, y_pad=3, counts=counts, scales=False)
+    c = Case(7, sum(counts or [96]), 2064, [337, 164], 64, x_pad=12, y_pad=3, counts=counts, scales=False)
     c.run()
     got = c.check()
     assert np.array_equal(got[:, c.n:], c.y[:, c.n:])
 
 
-@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("rows", [4, 200, 3000])
 def test_rows_of_widely_different_values(dev, rows):
     """Dims from 1 to 2^20 side by side, and rows of zeros, keep their bits."""
-    c = Case(3, rows, 520, [70], 16, counts=[rows], wide=2.0 ** 20)
+    c = Case(3, rows, 520, [370], 16, counts=[rows], wide=2.0 ** 20)
     c.x[1] = 0
     c.x[2] *= np.float32(2.0 ** 90)
     c.x[3] *= np.float32(2.0 ** -90)
@@ -149,9 +174,9 @@ def test_rows_of_widely_different_values(dev, rows):
     c.check()
 
 
-@pytest.mark.parametrize("rows,bf16", [(3, False), (3, True), (150, False), (150, True)])
+@pytest.mark.parametrize("rows,bf16", [(3, False), (3, True), (150, False), (150, True), (4000, False), (4000, True)])
 def test_infinities_stay_in_their_rows(dev, rows, bf16):
-    c = Case(5, rows, 136, [40], 16, counts=[rows], bf16=bf16)
+    c = Case(5, rows, 136, [440], 16, counts=[rows], bf16=bf16)
     c.x[1, 7], c.x[2, 3] = np.inf, np.nan
     c.bufs["x"] = up(c.x)
     c.run()
@@ -163,11 +188,11 @@ def test_infinities_stay_in_their_rows(dev, rows, bf16):
     assert not np.isfinite(got[1]).any() and np.isnan(got[2]).all()
 
 
-@pytest.mark.parametrize("counts", [None, [100, 30, 70]])
+@pytest.mark.parametrize("counts", [None, [100, 30, 70], [1000, 5, 600]])
 def test_captured_calls_replay(dev, counts):
     """Twice the same bits, captured or not, on a stream of its own and with other ids between replays."""
     s = Stream()
-    c = Case(9, 200, 520, [130, 70], 32, counts=counts)
+    c = Case(9, sum(counts or [200]), 520, [130, 170], 32, counts=counts)
     c.run(s)
     s.synchronize()
     first = c.check()
@@ -191,7 +216,7 @@ def test_captured_calls_replay(dev, counts):
 
 def test_two_calls_at_once_with_workspaces_of_their_own(dev):
     s, t = Stream(), Stream()
-    c, d = Case(1, 300, 1032, [700], 16, counts=[300]), Case(2, 64, 2304, [900], 16)
+    c, d = Case(1, 1300, 1032, [700], 16, counts=[1300]), Case(2, 64, 2304, [900], 16)
     synchronize()
     for _ in range(3):
         c.run(s)
