@@ -29,15 +29,14 @@ struct BeamArgs {
     const int32_t *finished;
     int64_t row_stride;
     int batch, beams, vocab, select, parts, end_token;  // parts of a row: a wave each
-    float inv_temperature, factor, factor_low;  // factor + factor_low = inv_temperature log2(e)
+    float inv_temperature, factor, factor_low;  // factor + factor_low = inv_temperature log2(e), factor_low above 0
     uint64_t *cand;   // [row][part][select]: logit order, ~token; 0: none
-    float *top;       // [row][part]: the part's largest logit (NaN: one is a NaN or infinite)
-    double *sum;      // [row][part]: sum of exp(x - x_top)
+    float2 *stats;    // [row][part]: the largest logit and the sum of their powers over it; 0: none above -infinity
     int32_t *parents, *tokens, *ended;
     float *best;
 };
 
-// Order of floats as unsigned numbers (no NaN; -0 below 0, as in the comparison of bits).
+// Order of floats as unsigned numbers (no NaN).
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __float_as_uint(v);
     return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
@@ -45,11 +44,19 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float unordered(uint32_t o) {
     return __uint_as_float(o ^ ((int)o < 0 ? 0x80000000u : 0xffffffffu));
 }
+__device__ __forceinline__ uint64_t key_of(float v, int token) {
+    return (uint64_t)ordered(v + 0.0f) << 32 | (uint32_t)~token;  // (-0 is 0)
+}
 
 // A beam that offers its tokens: it has a score and has not ended.
 __device__ __forceinline__ bool offers(const BeamArgs &a, int row) {
     const float s = a.scores[row];
     return s > -INFINITY && s < INFINITY && !(a.finished && a.finished[row]);
+}
+
+// exp(inv_temperature d), d at most 0.
+__device__ __forceinline__ float power(const BeamArgs &a, float d) {
+    return __builtin_amdgcn_exp2f(fmaf(d, a.factor, d * a.factor_low));
 }
 
 // What lanes of a wave write to LDS before it, its other lanes read behind it: the
@@ -59,25 +66,51 @@ __device__ __forceinline__ void in_order() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return std::max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(v))));
+    return (uint32_t)__builtin_amdgcn_readlane((int)dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(v)), 63);
 }
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)v, d, 64);
-        v = o > v ? o : v;
+    const uint32_t hi = wave_max((uint32_t)(v >> 32));
+    return (uint64_t)hi << 32 | wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+}
+// A bound that at least `select` (up to 16) of the lanes' values reach and few others: the
+// least of the `select` lanes that are largest but for six bits of their values.
+constexpr int kFew = 16;
+__device__ __forceinline__ float bound_of_few(float v, int select) {
+    uint32_t key = (ordered(v) & ~63u) | (threadIdx.x & 63);
+    bool taken = false;
+    for (int c = 0; c < select; ++c) {
+        const bool most = key == wave_max(key);
+        taken = taken || most;
+        key = most ? 0 : key;
     }
-    return v;
+    return unordered(~wave_max(taken ? ~ordered(v) : 0u));
+}
+// The same of more: bit by bit the largest key that enough values reach, until no more than
+// a quarter too many do.  count(key): how many.
+template <typename F>
+__device__ __forceinline__ float bound_of_many(int select, const F &count) {
+    uint32_t key = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t next = key | 1u << bit;
+        const int n = count(next);
+        if (n < select) continue;
+        key = next;
+        if (n <= select + select / 4) break;
+    }
+    return key > ordered(-INFINITY) ? unordered(key) : -INFINITY;
 }
 
 // A wave's part of a row: NV x 256 logits, four side by side a lane, kept in
-// registers.  The `select`-th largest of the lanes' own largest ones is a bound that at
-// least `select` logits reach and few others do (only `select` lanes have any): those go
-// to a list in LDS, and their places in the order are counted.
+// registers.  Those that reach the bound of the lanes' own largest ones go to a list in
+// LDS, and their places in the order are counted.
 template <int NV>
-__global__ __launch_bounds__(64 * kWaves) void beam_parts_kernel(BeamArgs a, int wgs) {
+__global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kernel(BeamArgs a, int wgs) {
     __shared__ uint64_t lists[kWaves][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int row = blockIdx.x / wgs, part = (blockIdx.x - row * wgs) * kWaves + wave;
@@ -97,82 +130,84 @@ __global__ __launch_bounds__(64 * kWaves) void beam_parts_kernel(BeamArgs a, int
             for (int i = 0; i < 4; ++i) v[j][i] = e + i < a.vocab ? x[e + i] : -INFINITY;
         }
     }
-    float top = -INFINITY;
-    int at = 0;
-    bool bad = false;
+    float most4[NV], most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bad = bad || !(v[j][i] < INFINITY);
-            v[j][i] += 0.0f;  // (-0 is 0)
-            if (v[j][i] > top) {
-                top = v[j][i];
-                at = e0 + 256 * j + i;
-            }
-        }
+    for (int j = 0; j < NV; ++j) {
+        most4[j] = fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3]));
+        most = fmaxf(most, most4[j]);
+    }
     const int64_t slot = (int64_t)row * a.parts + part;
     uint64_t *cand = a.cand + slot * a.select;
-    float most = top;
+    const float top = unordered(wave_max(ordered(most)));
+    // an infinity or a NaN leaves a sum that is no number; -infinity adds 0 (factor_low > 0)
+    f4 sums = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (top > -INFINITY) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
-    if (__any(bad) || most == -INFINITY) {
-        if (lane == 0) {
-            a.top[slot] = __any(bad) ? NAN : -INFINITY;
-            a.sum[slot] = 0.0;
-        }
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[i] += power(a, v[j][i] - top);
+    } else {
+        // (nothing above -infinity: a NaN all the same?)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[i] += v[j][i] == v[j][i] ? 0.0f : v[j][i];
+    }
+    float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if (lane == 0) a.stats[slot] = make_float2(top, sum);
+    if (!(sum > 0.0f)) {
         if (lane < a.select) cand[lane] = 0;
         return;
     }
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
+    float low;
+    if (a.select <= kFew) {
+        low = bound_of_few(most, a.select);
+    } else {
+        // (four values a lane: of one, nearly all would have to be taken)
+        uint32_t key[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float d = v[j][i] - most;
-            sum += __builtin_amdgcn_exp2f(d == -INFINITY ? d : fmaf(d, a.factor, d * a.factor_low));
-        }
-    double all = sum;
+            float m = most4[i * NV / 4];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
-    if (lane == 0) {
-        a.top[slot] = most;
-        a.sum[slot] = all;
+            for (int j = i * NV / 4 + 1; j < (i + 1) * NV / 4; ++j) m = fmaxf(m, most4[j]);
+            key[i] = ordered(fmaxf(m, -INFINITY));
+        }
+        low = bound_of_many(a.select, [&](uint32_t at) __attribute__((always_inline)) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= at));
+            return n;
+        });
     }
-    const uint64_t mine = top > -INFINITY ? (uint64_t)ordered(top) << 32 | (uint32_t)~at : (uint64_t)lane;
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) above += lane_key(mine, j) > mine ? 1 : 0;
-    const uint64_t bound = lane_key(mine, __builtin_ctzll(__ballot(above == a.select - 1)));
-    const bool any_bound = bound >> 32 != 0;
-    const float low = any_bound ? unordered((uint32_t)(bound >> 32)) : -INFINITY;
-    const int low_at = any_bound ? (int)~(uint32_t)bound : 0;
     uint64_t *list = lists[wave];
     int count = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        if (!__any(most4[j] >= low)) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int e = e0 + 256 * j + i;
-            const bool in = v[j][i] > low || (v[j][i] == low && low > -INFINITY && e <= low_at);
+            const bool in = v[j][i] >= low && v[j][i] > -INFINITY;
             const uint64_t who = __ballot(in);
-            if (who == 0) continue;
             const int to = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            if (in && to < kList) list[to] = (uint64_t)ordered(v[j][i]) << 32 | (uint32_t)~e;
+            if (in && to < kList) list[to] = key_of(v[j][i], e0 + 256 * j + i);
             count += __popcll(who);
         }
+    }
     if (count <= kList) {
         in_order();
         for (int t = lane; t < count; t += 64) {
             const uint64_t key = list[t];
             int before = 0;
+#pragma unroll 8
             for (int j = 0; j < count; ++j) before += list[j] > key ? 1 : 0;
             if (before < a.select) cand[before] = key;
         }
         if (lane >= count && lane < a.select) cand[lane] = 0;
         return;
     }
-    // (rarely: the large ones in few lanes) one after the other
+    // (rarely: the large ones in few lanes, or as many equal ones) one after the other
     uint64_t last = ~0ull;
     for (int c = 0; c < a.select; ++c) {
         uint64_t next = 0;
@@ -180,7 +215,7 @@ __global__ __launch_bounds__(64 * kWaves) void beam_parts_kernel(BeamArgs a, int
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint64_t key = v[j][i] > -INFINITY ? (uint64_t)ordered(v[j][i]) << 32 | (uint32_t)~(e0 + 256 * j + i) : 0;
+                const uint64_t key = v[j][i] > -INFINITY ? key_of(v[j][i], e0 + 256 * j + i) : 0;
                 if (key < last && key > next) next = key;
             }
         last = wave_max(next);
@@ -188,38 +223,65 @@ __global__ __launch_bounds__(64 * kWaves) void beam_parts_kernel(BeamArgs a, int
     }
 }
 
+// ln x of a positive number, to 1e-14: x = 2^e m, ln m = 2 (u + u^3 / 3 + ..), u = (m - 1) /
+// (m + 1) within 0.172.
+__device__ __forceinline__ double logarithm(double x) {
+    int e = __builtin_amdgcn_frexp_exp(x);
+    double m = __builtin_amdgcn_frexp_mant(x);  // [0.5, 1)
+    if (m < 0.70710678118654752) {
+        m *= 2.0;
+        --e;
+    }
+    const double u = (m - 1.0) / (m + 1.0), w = u * u;
+    double p = 1.0 / 15.0;
+    p = fma(p, w, 1.0 / 13.0);
+    p = fma(p, w, 1.0 / 11.0);
+    p = fma(p, w, 1.0 / 9.0);
+    p = fma(p, w, 1.0 / 7.0);
+    p = fma(p, w, 1.0 / 5.0);
+    p = fma(p, w, 1.0 / 3.0);
+    return fma((double)e, 0.69314718055994531, 2.0 * fma(u * w, p, u));
+}
+
 // A request's pick: the rows' logarithms, then the same way as above with a thread a
 // part's list instead of a lane its logits.
 __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
-    __shared__ double base[kMaxBeams], ended_at[kMaxBeams], bounds[kPick / 64], pool[kPool];
+    __shared__ double base[kMaxBeams], ended_at[kMaxBeams], pool[kPool];
     __shared__ uint64_t pool_at[kPool];  // a candidate's place, see `place`
-    __shared__ int count_;
+    __shared__ float bounds[kPick / 64];
+    __shared__ int count_, sums[2][kPick / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int request = blockIdx.x, row0 = request * a.beams, C = a.select;
+    const int request = blockIdx.x, row0 = request * a.beams, C = a.select, lists = a.beams * a.parts;
+    const uint64_t *cand = a.cand + (int64_t)row0 * a.parts * C;
     const double factor = a.inv_temperature;
+    // this thread's first list, as far as it is likely to go (a beam without an offer leaves
+    // its lists as they were: not used below)
+    constexpr int kAhead = 4;
+    uint64_t ahead[kAhead];
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) ahead[c] = tid < lists && c < C ? cand[(int64_t)tid * C + c] : 0;
     if (tid == 0) count_ = 0;
     for (int b = wave; b < a.beams; b += kPick / 64) {
         const float score = a.scores[row0 + b];
         const bool ok = score > -INFINITY && score < INFINITY, done = a.finished && a.finished[row0 + b];
         double start = -INFINITY;
         if (ok && !done) {
-            const float *top = a.top + (int64_t)(row0 + b) * a.parts;
-            const double *sum = a.sum + (int64_t)(row0 + b) * a.parts;
+            const float2 *stats = a.stats + (int64_t)(row0 + b) * a.parts;
             float most = -INFINITY;
-            bool bad = false;
-            for (int p = lane; p < a.parts; p += 64) {
-                bad = bad || top[p] != top[p];
-                most = fmaxf(most, top[p]);
-            }
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
             double all = 0.0;
-            if (most > -INFINITY)
-                for (int p = lane; p < a.parts; p += 64)
-                    if (top[p] > -INFINITY) all += sum[p] * exp(((double)top[p] - (double)most) * factor);
+#pragma unroll 2
+            for (int p = lane; p < a.parts; p += 64) {
+                const float2 s = stats[p];
+                if (s.y == 0.0f) continue;
+                const float next = fmaxf(most, s.x);
+                all = (most > -INFINITY ? all * power(a, most - next) : 0.0) + (double)s.y * power(a, s.x - next);
+                most = next;
+            }
+            const float top = unordered(wave_max(ordered(most)));
+            if (most > -INFINITY) all *= power(a, most - top);  // (a NaN stays one)
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
-            if (!__any(bad) && most > -INFINITY) start = (double)score - ((double)most * factor + log(all));
+            if (all > 0.0 && all < INFINITY) start = (double)score - ((double)top * factor + logarithm(all));
         }
         if (lane == 0) {
             base[b] = start;
@@ -227,35 +289,30 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         }
     }
     __syncthreads();
-    const int lists = a.beams * a.parts;
-    const uint64_t *cand = a.cand + (int64_t)row0 * a.parts * C;
-    auto score_of = [&](uint64_t key, int b) { return key ? base[b] + factor * (double)unordered((uint32_t)(key >> 32)) : -INFINITY; };
-    // (the lists of a beam without an offer are not written)
-    auto score_at = [&](int l, int c, uint64_t &key) {
-        const int b = l / a.parts;
-        key = base[b] > -INFINITY ? cand[(int64_t)l * C + c] : 0;
-        return score_of(key, b);
+    auto score_of = [&](uint64_t key, int b) {
+        return key && base[b] > -INFINITY ? base[b] + factor * (double)unordered((uint32_t)(key >> 32)) : -INFINITY;
     };
     // of equal scores the lower place comes first: beam, then logit from the largest
     // (scores of a beam may be too near each other for 64 bits), then token
     auto place = [](int b, uint64_t key) { return (uint64_t)b << 56 | (uint64_t)~(uint32_t)(key >> 32) << 24 | ~(uint32_t)key; };
     auto end_place = [&](int b) { return (uint64_t)b << 56 | (uint32_t)a.end_token; };
     constexpr uint64_t kNone = ~0ull;
-    double mine = -INFINITY;
-    for (int l = tid; l < lists; l += kPick) {
-        uint64_t key;
-        mine = fmax(mine, score_at(l, 0, key));
-    }
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) {
-        const double o = __longlong_as_double((long long)lane_key((uint64_t)__double_as_longlong(mine), j));
-        above += o > mine || (o == mine && j < lane) ? 1 : 0;
-    }
-    if (above == C - 1) bounds[wave] = mine;
-    __syncthreads();
-    double bound = bounds[0];
-    for (int w = 1; w < kPick / 64; ++w) bound = fmax(bound, bounds[w]);
+    auto head_of = [&](int l) { return l == tid ? ahead[0] : cand[(int64_t)l * C]; };
+    // the float at or below a score: a bound of these is below `select` of the scores
+    auto below = [](double score) {
+        const float f = (float)score;
+        return (double)f > score ? unordered(ordered(f) - 1) : f;
+    };
+    int turn = 0;
+    auto block_sum = [&](int n) __attribute__((always_inline)) {  // of the waves' numbers
+        turn ^= 1;
+        if (lane == 0) sums[turn][wave] = n;
+        __syncthreads();
+        n = sums[turn][lane & (kPick / 64 - 1)];
+#pragma unroll
+        for (int d = 1; d < kPick / 64; d <<= 1) n += __shfl_xor(n, d, 64);
+        return __builtin_amdgcn_readfirstlane(n);
+    };
     auto push = [&](double score, uint64_t at) {
         const int to = atomicAdd(&count_, 1);
         if (to < kPool) {
@@ -263,18 +320,89 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             pool_at[to] = at;
         }
     };
-    for (int l = tid; l < lists; l += kPick) {
-        const int b = l / a.parts;
-        for (int c = 0; c < C; ++c) {
-            uint64_t key;
-            const double s = score_at(l, c, key);
-            if (key == 0 || s < bound) break;
-            push(s, place(b, key));
+    // the candidates that reach a bound into the pool; how many
+    auto gather = [&](double bound) {
+        auto offer = [&](uint64_t key, int b) {
+            const double s = score_of(key, b);
+            const bool in = s > -INFINITY && s >= bound;
+            if (in) push(s, place(b, key));
+            return in;
+        };
+        if (lists <= kPick / 4) {  // few lists: a thread an entry, not a list
+            for (int i = tid; i < lists * C; i += kPick) offer(cand[i], i / C / a.parts);
         }
+        for (int l = lists <= kPick / 4 ? lists : tid; l < lists; l += kPick) {
+            const int b = l / a.parts;
+            int c = 0;
+            bool more = true;
+            if (l == tid) {
+#pragma unroll
+                for (; c < kAhead; ++c) more = more && offer(ahead[c], b);
+            }
+            for (; more && c < C; ++c) more = offer(cand[(int64_t)l * C + c], b);
+        }
+        if (tid < a.beams && ended_at[tid] > -INFINITY && ended_at[tid] >= bound) push(ended_at[tid], end_place(tid));
+        __syncthreads();
+        return count_;
+    };
+    auto emptied = [&] {
+        __syncthreads();
+        if (tid == 0) count_ = 0;
+        __syncthreads();
+    };
+    constexpr int kEnough = 4 * kMaxSelect;  // whose order is counted
+    int count = kPool + 1;
+    if (C <= kFew) {
+        double mine = -INFINITY;
+        for (int l = tid; l < lists; l += kPick) mine = fmax(mine, score_of(head_of(l), l / a.parts));
+        const float own = bound_of_few(below(mine), C);
+        if (lane == 0) bounds[wave] = own;
+        __syncthreads();
+        count = gather(unordered(wave_max(ordered(bounds[lane & (kPick / 64 - 1)]))));
     }
-    if (tid < a.beams && ended_at[tid] > -INFINITY && ended_at[tid] >= bound) push(ended_at[tid], end_place(tid));
-    __syncthreads();
-    const int count = count_;
+    if (count > kEnough) {
+        // the lists' best by themselves: no more than `select` lists reach their bound, but for ties
+        constexpr int kHeads = 8;
+        uint32_t key[kHeads];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const int l = tid + i * kPick;
+            key[i] = l < lists ? ordered(below(score_of(head_of(l), l / a.parts))) : 0;
+        }
+        const float own = lists < C ? -INFINITY : bound_of_many(C, [&](uint32_t at) __attribute__((always_inline)) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i) n += __popcll(__ballot(key[i] >= at));
+            for (int l = wave * 64 + lane + kHeads * kPick; l - lane < lists; l += kPick)
+                n += __popcll(__ballot(l < lists && ordered(below(score_of(head_of(l), l / a.parts))) >= at));
+            return block_sum(n);
+        });
+        emptied();
+        count = gather(own);
+    }
+    if (count > kEnough && count <= kPool) {
+        constexpr int kEach = kPool / kPick;
+        double s[kEach];
+        uint64_t at[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const bool in = tid + i * kPick < count;
+            s[i] = in ? pool[tid + i * kPick] : -INFINITY;
+            at[i] = in ? pool_at[tid + i * kPick] : kNone;
+        }
+        const double own = bound_of_many(C, [&](uint32_t key) __attribute__((always_inline)) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) n += __popcll(__ballot(ordered(below(s[i])) >= key));
+            return block_sum(n);
+        });
+        emptied();
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (s[i] > -INFINITY && s[i] >= own) push(s[i], at[i]);
+        __syncthreads();
+        count = count_;
+    }
     auto put = [&](int c, double score, uint64_t at) {
         const int64_t to = (int64_t)request * C + c;
         const bool none = at == kNone;
@@ -285,12 +413,15 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         if (a.ended) a.ended[to] = !none && ((a.finished && a.finished[row0 + b]) || token == a.end_token) ? 1 : 0;
     };
     if (count <= kPool) {
-        for (int t = tid; t < count; t += kPick) {
+        // sixteen threads a candidate
+        for (int t = tid >> 4; t < count; t += kPick / 16) {
             const double s = pool[t];
             const uint64_t at = pool_at[t];
             int before = 0;
-            for (int j = 0; j < count; ++j) before += pool[j] > s || (pool[j] == s && pool_at[j] < at) ? 1 : 0;
-            if (before < C) put(before, s, at);
+            for (int j = tid & 15; j < count; j += 16) before += pool[j] > s || (pool[j] == s && pool_at[j] < at) ? 1 : 0;
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) before += __shfl_xor(before, d, 64);
+            if ((tid & 15) == 0 && before < C) put(before, s, at);
         }
         if (tid >= count && tid < C) put(tid, -INFINITY, kNone);
         return;
@@ -310,9 +441,9 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         };
         for (int l = tid; l < lists; l += kPick)
             for (int e = 0; e < C; ++e) {
-                uint64_t key;
-                const double score = score_at(l, e, key);
-                if (key == 0) break;
+                const uint64_t key = cand[(int64_t)l * C + e];
+                const double score = score_of(key, l / a.parts);
+                if (score == -INFINITY) break;
                 take(score, place(l / a.parts, key));
             }
         if (tid < a.beams) take(ended_at[tid], end_place(tid));
@@ -361,12 +492,13 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const uint8_t *src, uint
     }
 }
 
-// Vectors a lane: long parts where there are rows enough to fill the device.
-int vectors_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)8 << 20 ? 16 : 4; }
+// Vectors a lane: longer parts where there are rows enough to fill the device (128 rows of
+// 248321: 45 us in parts of 1024, 37.5 of 2048, 37.6 of 4096, which spill registers).
+int vectors_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)8 << 20 ? 8 : 4; }
 
 struct BeamSizes {
     int vectors;
-    int64_t parts, cand, top, bytes;
+    int64_t parts, cand, bytes;
 };
 int beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int64_t select, BeamSizes &z) {
     DOE_REQUIRE(beams > 0 && beams <= kMaxBeams, DOE_E_UNSUPPORTED, "beams %lld outside 1..%d", (long long)beams, kMaxBeams);
@@ -377,8 +509,7 @@ int beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int64_t select, Beam
     z.vectors = vectors_of(rows, vocab);
     z.parts = (vocab + 256 * z.vectors - 1) / (256 * z.vectors);
     z.cand = rows * z.parts * select * 8;
-    z.top = z.cand + rows * z.parts * 8;
-    z.bytes = std::max<int64_t>(16, z.top + rows * z.parts * 4);
+    z.bytes = std::max<int64_t>(16, z.cand + rows * z.parts * 8);
     return DOE_OK;
 }
 
@@ -427,18 +558,18 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
     a.parts = (int)z.parts;
     a.end_token = end_token < 0 ? -2 : (int)end_token;  // (-2: no token is)
     a.inv_temperature = inv_temperature;
-    const double log2e = 1.4426950408889634074, factor = inv_temperature * log2e;
+    const double factor = inv_temperature * 1.4426950408889634074;
     a.factor = (float)factor;
+    if ((double)a.factor >= factor) a.factor = nextafterf(a.factor, 0.0f);
     a.factor_low = (float)(factor - (double)a.factor);
     a.cand = static_cast<uint64_t *>(workspace);
-    a.sum = reinterpret_cast<double *>(static_cast<uint8_t *>(workspace) + z.cand);
-    a.top = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + z.top);
+    a.stats = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + z.cand);
     a.parents = parents;
     a.tokens = tokens;
     a.best = out_scores;
     a.ended = out_finished;
     const hipStream_t st = (hipStream_t)stream;
-    if (z.vectors == 16) hipLaunchKernelGGL(beam_parts_kernel<16>, dim3((unsigned)(rows * wgs)), dim3(64 * kWaves), 0, st, a, (int)wgs);
+    if (z.vectors == 8) hipLaunchKernelGGL(beam_parts_kernel<8>, dim3((unsigned)(rows * wgs)), dim3(64 * kWaves), 0, st, a, (int)wgs);
     else hipLaunchKernelGGL(beam_parts_kernel<4>, dim3((unsigned)(rows * wgs)), dim3(64 * kWaves), 0, st, a, (int)wgs);
     DOE_LAUNCH_CHECK("beam_parts_kernel");
     hipLaunchKernelGGL(beam_pick_kernel, dim3((unsigned)batch), dim3(kPick), 0, st, a);

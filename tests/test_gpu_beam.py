@@ -99,7 +99,7 @@ def clear_case(seed, batch, beams, vocab, select, **kw):
 SHAPES = [
     # batch, beams, vocab, select
     (1, 4, 256000, 4), (1, 1, 1, 1), (1, 1, 2, 3), (2, 3, 5, 8), (3, 2, 1023, 4), (1, 5, 1025, 64), (2, 4, 4097, 8), (2, 8, 50257, 16),
-    (9, 8, 151937, 16), (1, 32, 300, 64), (1, 64, 700, 64), (1, 33, 40, 33), (5, 1, 16384, 2), (1, 2, 1000003, 5),
+    (9, 8, 151937, 16), (1, 32, 300, 64), (1, 64, 700, 64), (1, 64, 20000, 64), (2, 40, 140000, 17), (1, 33, 40, 33), (5, 1, 16384, 2), (1, 2, 1000003, 5),
 ]
 
 
