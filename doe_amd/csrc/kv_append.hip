@@ -2,6 +2,12 @@
 // pages of a paged cache (doe_qkv_rope_append).  A page holds page_size positions
 // [num_kv_heads][head_dim], the order that doe_attention_dispatch reads with
 // kv_layout 2.
+//
+// Bound by its bytes: eight prompts of up to 2000 rows, 32 / 8 heads of 128 dims, f16
+// queries (387 MB): 81 us, 4.8 TB/s.  A thread has the same eight values of every row that
+// its workgroup takes, one row at a time (four at once, 112 registers: as fast); rows read
+// past the caches: 85.  One token of 8 / 4 heads of 256: 3 us in the kernel, three dependent
+// reads (length, page, angles) before its stores.
 #include "rope_rows.h"
 
 #include <algorithm>
@@ -19,47 +25,46 @@ struct AppendArgs {
     int num_pages, page_size, kv_heads, head_dim, batch, table_stride, rows_per_wg;
 };
 
-constexpr int kMaxRows = doe::kRopeRowsPerWg;
-
-// A workgroup takes rows_per_wg rows, and gridDim.y of them share a row's units.
 __global__ __launch_bounds__(256) void qkv_rope_append_kernel(AppendArgs a) {
-    __shared__ int s_pos[kMaxRows];
-    __shared__ int64_t s_at[kMaxRows];  // the position's place in the pools, -1: none; -2: no row
+    __shared__ int s_pos[doe::kRopeRowsPerWg];
+    __shared__ int64_t s_at[doe::kRopeRowsPerWg];  // the position's place in the pools, -1: none
     const int64_t row0 = (int64_t)blockIdx.x * a.rows_per_wg;
-    const int rows = (int)std::min<int64_t>(a.rows_per_wg, a.rows - row0);
-    if ((int)threadIdx.x < rows) {
-        int b, pos = -1;
-        int64_t at = -2;
-        if (doe::row_position(a.lens, a.room, a.batch, a.row_starts, row0 + threadIdx.x, b, pos)) {
-            at = -1;
-            if (pos >= 0 && pos < a.r.max_positions) {
-                const int in_table = pos / a.page_size, page = a.table[(int64_t)b * a.table_stride + in_table];
-                if (page >= 0 && page < a.num_pages)
-                    at = ((int64_t)page * a.page_size + (pos - in_table * a.page_size)) * a.kv_heads * a.head_dim;
-            }
+    const int count = (int)std::min<int64_t>(a.rows_per_wg, a.rows - row0);
+    if (threadIdx.x < 64) {
+        int b, pos = doe::kNoRow;
+        int64_t at = -1;
+        if (!doe::rows_positions(a.lens, a.room, a.batch, a.row_starts, row0, count, b, pos)) {
+            pos = doe::kNoRow;
+        } else if (pos >= 0 && pos < a.r.max_positions) {
+            const int in_table = pos / a.page_size, page = a.table[(int64_t)b * a.table_stride + in_table];
+            if (page >= 0 && page < a.num_pages)
+                at = ((int64_t)page * a.page_size + (pos - in_table * a.page_size)) * a.kv_heads * a.head_dim;
         }
-        s_pos[threadIdx.x] = pos;
-        s_at[threadIdx.x] = at;
+        if ((int)threadIdx.x < count) {
+            s_pos[threadIdx.x] = pos;
+            s_at[threadIdx.x] = at;
+        }
     }
     __syncthreads();
-    const int D = a.head_dim, per_head = D / 8, heads = a.r.num_heads + 2 * a.kv_heads, per_row = heads * per_head;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * per_row; i += gridDim.y * 256) {
-        const int r = i / per_row, in_row = i - r * per_row, head = in_row / per_head;
-        const int64_t at = s_at[r], row = row0 + r;
-        const int pos = s_pos[r], kv = head - a.r.num_heads;
-        const bool is_q = kv < 0, is_v = kv >= a.kv_heads;
-        if (at == -2 || (!is_q && at < 0)) continue;
-        doe::RopeUnit u = doe::rope_unit(a.r, in_row - head * per_head);
-        if (is_v) u = {(in_row - head * per_head) * 8, (in_row - head * per_head) * 8 + 4, false};
-        const float *x = a.r.qkv + row * a.r.row_stride + (int64_t)head * D;
-        f4 v0 = *reinterpret_cast<const f4 *>(x + u.at0), v1 = *reinterpret_cast<const f4 *>(x + u.at1);
-        if (!is_v && pos >= 0 && pos < a.r.max_positions) doe::rotate_unit(a.r, u, pos, v0, v1);
+    const int D = a.head_dim, per_head = D / 8;
+    const doe::RopeThread me = doe::rope_thread((a.r.num_heads + 2 * a.kv_heads) * per_head, blockIdx.y);
+    const int head = me.unit / per_head, in_head = me.unit - head * per_head, kv = head - a.r.num_heads;
+    const bool is_q = kv < 0, is_v = kv >= a.kv_heads;
+    const doe::RopeUnit u = is_v ? doe::RopeUnit{8 * in_head, 8 * in_head + 4, false} : doe::rope_unit(a.r, in_head);
+    const bool turns = !is_v && u.at0 < a.r.rotary_dim;
+    _Float16 *pool = is_v ? a.v_pool + (int64_t)(kv - a.kv_heads) * D : a.k_pool + (int64_t)kv * D;
+    for (int i = me.first; i < count; i += me.step) {
+        const int pos = s_pos[i];
+        const int64_t at = s_at[i];
+        if (pos == doe::kNoRow || (!is_q && at < 0)) continue;
+        const f4 *x = reinterpret_cast<const f4 *>(a.r.qkv + (row0 + i) * a.r.row_stride + (int64_t)head * D);
+        f4 v0 = x[u.at0 / 4], v1 = x[u.at1 / 4];
+        if (turns && pos >= 0 && pos < a.r.max_positions) doe::rotate_unit(a.r, u, pos, v0, v1);
         if (is_q) {
-            doe::store_query(a.r, row, head, D, u, v0, v1);
+            doe::store_query<false>(a.r, row0 + i, head, D, u, v0, v1);
         } else {
-            _Float16 *to = (is_v ? a.v_pool + at + (int64_t)(kv - a.kv_heads) * D : a.k_pool + at + (int64_t)kv * D);
-            *reinterpret_cast<h4 *>(to + u.at0) = __builtin_convertvector(v0, h4);
-            *reinterpret_cast<h4 *>(to + u.at1) = __builtin_convertvector(v1, h4);
+            *reinterpret_cast<h4 *>(pool + at + u.at0) = __builtin_convertvector(v0, h4);
+            *reinterpret_cast<h4 *>(pool + at + u.at1) = __builtin_convertvector(v1, h4);
         }
     }
 }
@@ -148,11 +153,12 @@ int doe_qkv_rope_append(const doe_f16_cache *cache, const float *qkv, int64_t ro
     a.head_dim = (int)c.head_dim;
     a.batch = (int)c.batch;
     a.table_stride = (int)c.table_stride;
-    const int64_t per_row = (num_heads + 2 * c.num_kv_heads) * (c.head_dim / 8);
-    a.rows_per_wg = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxRows, rows / 2048));
-    const int64_t ways = a.rows_per_wg > 1 ? 1 : std::min<int64_t>(64, (per_row + 255) / 256);
-    hipLaunchKernelGGL(qkv_rope_append_kernel, dim3((unsigned)((rows + a.rows_per_wg - 1) / a.rows_per_wg), (unsigned)ways), dim3(256),
-                       0, (hipStream_t)stream, a);
+    const doe::RopeShare share = doe::rope_share(rows, (num_heads + 2 * c.num_kv_heads) * (c.head_dim / 8));
+    a.rows_per_wg = share.rows_per_wg;
+    const int64_t wgs = (rows + share.rows_per_wg - 1) / share.rows_per_wg;
+    DOE_REQUIRE(wgs * share.ways < (1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %lld and %lld heads in one call", (long long)rows,
+                (long long)num_heads, (long long)c.num_kv_heads);  // (a launch has fewer than 2^32 threads)
+    hipLaunchKernelGGL(qkv_rope_append_kernel, dim3((unsigned)wgs, (unsigned)share.ways), dim3(256), 0, (hipStream_t)stream, a);
     DOE_LAUNCH_CHECK("qkv_rope_append_kernel");
     return DOE_OK;
 }

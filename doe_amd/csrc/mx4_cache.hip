@@ -33,19 +33,47 @@ struct RowArgs {
     int kv_wgs, q_rows, q_ways;
 };
 
-// The queries' part of a rotating call; false: this workgroup is one of the cache's.
+// The queries' part of a rotating call; false: this workgroup is one of the cache's.  They
+// are read and written past the caches, which the codes alone then fill: 1900 rows of 32 /
+// 16 heads of 256 appended and read back (364 MB) 75 to 67 us, attention behind it as fast.
 __device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_pos) {
     const int wg = (int)blockIdx.x - a.kv_wgs;
     if (wg < 0) return false;
     const int64_t row0 = (int64_t)(wg / a.q_ways) * a.q_rows;
     const int count = a.rows - row0 < a.q_rows ? (int)(a.rows - row0) : a.q_rows;
-    doe::rotate_queries(a.r, a.c.lens, (int64_t)a.c.table_stride << a.c.page_shift, a.c.batch, a.row_starts, row0, count, head_dim,
-                        wg % a.q_ways, a.q_ways, s_pos);
+    doe::rotate_queries<true>(a.r, a.c.lens, (int64_t)a.c.table_stride << a.c.page_shift, a.c.batch, a.row_starts, row0, count, head_dim,
+                        wg % a.q_ways, s_pos);
     return true;
 }
-__device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own, const float *head, int d, int pos) {
-    const doe::f4 v = doe::rotate_four(a.r, head, d, doe::f4{own.x, own.y, own.z, own.w}, pos);
-    return make_float4(v[0], v[1], v[2], v[3]);
+// Dims d .. d + 3 of a head at `head`, of which `own` has been read, rotated.  The other
+// dims of its pairs are another lane's of the head (D / 4 lanes, four dims each): in this
+// wave up to 256 dims, read again from 512.
+template <int D>
+__device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own_, const float *head, int d, int pos) {
+    const doe::RopeRows &r = a.r;
+    const doe::f4 own = {own_.x, own_.y, own_.z, own_.w};
+    doe::f4 out = own;
+    const int half = r.rotary_dim / 2, low = d < half ? d : d - half;
+    const float *freq = r.freq + (int64_t)pos * r.rotary_dim;
+    if (r.interleaved) {
+        if (d < r.rotary_dim) out = doe::rotate_pairs(own, *reinterpret_cast<const doe::f4 *>(freq + d));
+    } else {
+        const int other_d = d < half ? d + half : low;
+        doe::f4 other;
+        if constexpr (D <= 256 && D != 160) {
+            const int lane = (threadIdx.x & 63) + (other_d - d) / 4;  // (past the rotated dims: not used)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) other[i] = __shfl(own[i], lane, 64);
+        } else {
+            other = *reinterpret_cast<const doe::f4 *>(head + (d < r.rotary_dim ? other_d : d));
+        }
+        if (d < r.rotary_dim) {
+            doe::f4 lo = d < half ? own : other, hi = d < half ? other : own;
+            doe::rotate_halves(lo, hi, *reinterpret_cast<const doe::f4 *>(freq + 2 * low), *reinterpret_cast<const doe::f4 *>(freq + 2 * low + 4));
+            out = d < half ? lo : hi;
+        }
+    }
+    return make_float4(out[0], out[1], out[2], out[3]);
 }
 
 // Bits of the largest magnitude over each 8 lanes, an infinity's or NaN's above
@@ -75,6 +103,7 @@ __device__ __forceinline__ uint32_t quantise(const float4 x, int &scale) {
 }
 
 constexpr int kRowsPerWg = 16;
+static_assert(kRowsPerWg >= doe::kRopeRowsPerWg, "positions of a workgroup's rows");
 
 // One row's place, found once for a workgroup's rows.
 struct Place {
@@ -91,7 +120,7 @@ template <bool F16, bool ROPE = false>
 __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
     constexpr int D = 160;
     __shared__ Place place[kRowsPerWg];
-    __shared__ int positions[ROPE ? doe::kRopeRowsPerWg : 1];
+    __shared__ int positions[ROPE ? kRowsPerWg : 1];
     if constexpr (ROPE) {
         if (queries(a, D, positions)) return;
     }
@@ -128,7 +157,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         } else {
             k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.k) + at);
             v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.v) + at);
-            if constexpr (ROPE) k = rotated(a, k, static_cast<const float *>(a.k) + at - d, d, positions[r]);
+            if constexpr (ROPE) k = rotated<D>(a, k, static_cast<const float *>(a.k) + at - d, d, positions[r]);
         }
         int ks, vs;
         const uint32_t kc = quantise(k, ks), vc = quantise(v, vs);
@@ -306,7 +335,7 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
             const f4 vf = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(static_cast<const float *>(a.v) + at));
             k[i] = make_float4(kf[0], kf[1], kf[2], kf[3]);
             v[i] = make_float4(vf[0], vf[1], vf[2], vf[3]);
-            if constexpr (ROPE) k[i] = rotated(a, k[i], static_cast<const float *>(a.k) + at - d, d, f.pos0 + i);
+            if constexpr (ROPE) k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + at - d, d, f.pos0 + i);
         }
     }
     uint32_t vc[4] = {};
@@ -413,9 +442,9 @@ void launch_write(bool f16, hipStream_t st, const RowArgs &a) {
 template <int D>
 int launch_append(hipStream_t st, RowArgs &a) {
     const dim3 kv = D == 160 ? rows_grid(a) : fours_grid<D>(a);
-    const int64_t q_units = (int64_t)a.r.num_heads * (D / 8);
-    a.q_rows = (int)std::max<int64_t>(1, std::min<int64_t>(doe::kRopeRowsPerWg, a.rows / 2048));
-    a.q_ways = a.q_rows > 1 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(64, (q_units + 255) / 256));
+    const doe::RopeShare share = doe::rope_share(a.rows, std::max<int64_t>(1, (int64_t)a.r.num_heads * (D / 8)));
+    a.q_rows = share.rows_per_wg;
+    a.q_ways = share.ways;
     a.kv_wgs = (int)kv.x;
     const unsigned q_wgs = a.r.num_heads ? (unsigned)((a.rows + a.q_rows - 1) / a.q_rows * a.q_ways) : 0;
     DOE_REQUIRE((int64_t)kv.x + q_wgs < (1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %d and %d heads in one call", (long long)a.rows,

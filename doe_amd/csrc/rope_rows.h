@@ -54,9 +54,8 @@ __device__ __forceinline__ RopeUnit rope_unit(const RopeRows &r, int u) {
     const int at = halves ? 4 * u : 8 * u;
     return {at, halves ? at + r.rotary_dim / 2 : at + 4, halves};
 }
-// Rotates a unit; `pos` within the table.
+// Rotates a unit of dims below rotary_dim at a position of the table.
 __device__ __forceinline__ void rotate_unit(const RopeRows &r, const RopeUnit &u, int pos, f4 &v0, f4 &v1) {
-    if (u.at0 >= r.rotary_dim) return;
     const f4 *cs = reinterpret_cast<const f4 *>(r.freq + (int64_t)pos * r.rotary_dim + (u.halves ? 2 * u.at0 : u.at0));
     if (u.halves) {
         rotate_halves(v0, v1, cs[0], cs[1]);
@@ -65,17 +64,29 @@ __device__ __forceinline__ void rotate_unit(const RopeRows &r, const RopeUnit &u
         v1 = rotate_pairs(v1, cs[1]);
     }
 }
+// PAST: past the caches.
+template <bool PAST, typename T>
+__device__ __forceinline__ T load(const T *p) {
+    if constexpr (PAST) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool PAST, typename T>
+__device__ __forceinline__ void store(T *p, T v) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
 // A unit of a query to q_out.
+template <bool PAST>
 __device__ __forceinline__ void store_query(const RopeRows &r, int64_t row, int head, int head_dim, const RopeUnit &u, f4 v0, f4 v1) {
     const int64_t at = row * r.q_stride + (int64_t)head * head_dim;
     if (r.q_f16) {
         _Float16 *q = static_cast<_Float16 *>(r.q_out) + at;
-        *reinterpret_cast<h4 *>(q + u.at0) = __builtin_convertvector(v0, h4);
-        *reinterpret_cast<h4 *>(q + u.at1) = __builtin_convertvector(v1, h4);
+        store<PAST>(reinterpret_cast<h4 *>(q + u.at0), __builtin_convertvector(v0, h4));
+        store<PAST>(reinterpret_cast<h4 *>(q + u.at1), __builtin_convertvector(v1, h4));
     } else {
         float *q = static_cast<float *>(r.q_out) + at;
-        *reinterpret_cast<f4 *>(q + u.at0) = v0;
-        *reinterpret_cast<f4 *>(q + u.at1) = v1;
+        store<PAST>(reinterpret_cast<f4 *>(q + u.at0), v0);
+        store<PAST>(reinterpret_cast<f4 *>(q + u.at1), v1);
     }
 }
 
@@ -108,43 +119,73 @@ __device__ __forceinline__ bool row_position(const int32_t *lens, int64_t room, 
     return true;
 }
 
-// Dims d .. d + 3 of a head at x, of which `own` has been read, rotated.
-__device__ __forceinline__ f4 rotate_four(const RopeRows &r, const float *x, int d, f4 own, int pos) {
-#pragma clang fp contract(off)
-    if (d >= r.rotary_dim) return own;
-    const float *freq = r.freq + (int64_t)pos * r.rotary_dim;
-    if (r.interleaved) return rotate_pairs(own, *reinterpret_cast<const f4 *>(freq + d));
-    const int half = r.rotary_dim / 2, i = d < half ? d : d - half;
-    const f4 other = *reinterpret_cast<const f4 *>(x + (d < half ? d + half : i));
-    f4 lo = d < half ? own : other, hi = d < half ? other : own;
-    rotate_halves(lo, hi, *reinterpret_cast<const f4 *>(freq + 2 * i), *reinterpret_cast<const f4 *>(freq + 2 * i + 4));
-    return d < half ? lo : hi;
+// Sequence and position of rows [row0, row0 + count), count at most 64, a lane of the
+// calling wave each (found: whether it has one).  Up to 64 sequences are looked through at
+// once, a lane each.
+__device__ __forceinline__ bool rows_positions(const int32_t *lens, int64_t room, int batch, const int32_t *row_starts, int64_t row0,
+                                               int count, int &b, int &pos) {
+    const int lane = threadIdx.x & 63;
+    if (!row_starts || batch > 64) return lane < count && row_position(lens, room, batch, row_starts, row0 + lane, b, pos);
+    const int start = lane < batch ? row_starts[lane] : 0, end = lane < batch ? row_starts[lane + 1] : 0;
+    const int held = lane < batch ? held_positions(lens, room, lane) : 0;
+    bool found = false;
+    for (int i = 0; i < count; ++i) {
+        const uint64_t in = __ballot(lane < batch && start <= row0 + i && row0 + i < end);
+        if (in == 0) continue;
+        const int at = 63 - __builtin_clzll(in);
+        const int64_t p = __builtin_amdgcn_readlane(held, at) - ((int64_t)__builtin_amdgcn_readlane(end, at) - (row0 + i));
+        if (lane == i) {
+            found = true;
+            b = at;
+            pos = (int)p;
+        }
+    }
+    return found;
 }
 
-constexpr int kRopeRowsPerWg = 32;
+// The rows of a rotating call over workgroups of 256 threads.  A thread has one unit, of
+// the `units` of a row, in all of its workgroup's rows, so that what it is is found once: a
+// workgroup holds several rows at once, or `ways` of them share a row's units.
+constexpr int kRopeRowsPerWg = 16;
+struct RopeShare {
+    int rows_per_wg, ways;
+};
+inline RopeShare rope_share(int64_t rows, int64_t units) {
+    const int64_t ways = (units + 255) / 256, at_once = units < 256 ? 256 / units : 1;
+    const int64_t per = rows * ways / 16384 > at_once ? rows * ways / 16384 : at_once;  // (some 16384 workgroups)
+    return {(int)(per < kRopeRowsPerWg ? per : kRopeRowsPerWg), (int)ways};
+}
+struct RopeThread {
+    int unit, first, step;  // its unit, first row (past all rows: it has none), and rows from one to the next
+};
+__device__ __forceinline__ RopeThread rope_thread(int units, int way) {
+    if (units >= 256) return {way * 256 + (int)threadIdx.x, way * 256 + (int)threadIdx.x < units ? 0 : kRopeRowsPerWg, 1};
+    const int at_once = 256 / units, first = threadIdx.x / units;
+    return {(int)threadIdx.x - first * units, first < at_once ? first : kRopeRowsPerWg, at_once};
+}
 
-// The queries of rows [row0, row0 + count), count <= kRopeRowsPerWg, by this workgroup
-// of 256 threads: every ways-th 256 of their units from the way-th on.
+// The queries of rows [row0, row0 + count) by a workgroup.
+constexpr int kNoRow = -0x7fffffff;  // the position of a row of no sequence: it is left as it was
+template <bool PAST>
 __device__ __forceinline__ void rotate_queries(const RopeRows &r, const int32_t *lens, int64_t room, int batch,
-                                               const int32_t *row_starts, int64_t row0, int count, int head_dim, int way, int ways,
-                                               int *s_pos) {
-    constexpr int kNone = -0x7fffffff;  // a row of no sequence is left as it was
-    if ((int)threadIdx.x < count) {
-        int b, pos;
-        if (!row_position(lens, room, batch, row_starts, row0 + threadIdx.x, b, pos)) pos = kNone;
-        s_pos[threadIdx.x] = pos;
+                                               const int32_t *row_starts, int64_t row0, int count, int head_dim, int way, int *s_pos) {
+    if (threadIdx.x < 64) {
+        int b, pos = kNoRow;
+        if (!rows_positions(lens, room, batch, row_starts, row0, count, b, pos)) pos = kNoRow;
+        if ((int)threadIdx.x < count) s_pos[threadIdx.x] = pos;
     }
     __syncthreads();
-    const int per_head = head_dim / 8, per_row = r.num_heads * per_head;
-    for (int i = way * 256 + threadIdx.x; i < count * per_row; i += ways * 256) {
-        const int in_block = i / per_row, in_row = i - in_block * per_row, head = in_row / per_head, pos = s_pos[in_block];
-        if (pos == kNone) continue;
-        const int64_t row = row0 + in_block;
-        const RopeUnit u = rope_unit(r, in_row - head * per_head);
-        const float *x = r.qkv + row * r.row_stride + (int64_t)head * head_dim;
-        f4 v0 = *reinterpret_cast<const f4 *>(x + u.at0), v1 = *reinterpret_cast<const f4 *>(x + u.at1);
-        if (pos >= 0 && pos < r.max_positions) rotate_unit(r, u, pos, v0, v1);
-        store_query(r, row, head, head_dim, u, v0, v1);
+    const int per_head = head_dim / 8;
+    const RopeThread me = rope_thread(r.num_heads * per_head, way);
+    const int head = me.unit / per_head;
+    const RopeUnit u = rope_unit(r, me.unit - head * per_head);
+    for (int i = me.first; i < count; i += me.step) {
+        const int pos = s_pos[i];
+        if (pos == kNoRow) continue;
+        const f4 *x = reinterpret_cast<const f4 *>(r.qkv + (row0 + i) * r.row_stride + (int64_t)head * head_dim);
+        f4 v0 = load<PAST>(x + u.at0 / 4), v1 = load<PAST>(x + u.at1 / 4);
+        if (u.at0 < r.rotary_dim && pos >= 0 && pos < r.max_positions) rotate_unit(r, u, pos, v0, v1);
+        store_query<PAST>(r, row0 + i, head, head_dim, u, v0, v1);
     }
 }
 
