@@ -156,6 +156,8 @@ _lib: C.CDLL | None = None
 def load() -> C.CDLL:
     """Loads the library once and declares every signature."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -176,8 +178,7 @@ def load() -> C.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls ``name`` and raises ``DoeError`` on a negative status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != DOE_OK:
-        msg = lib.doe_last_error().decode(errors="replace")
+        msg = load().doe_last_error().decode(errors="replace")
         raise DoeError(name, rc, msg)

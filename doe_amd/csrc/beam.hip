@@ -114,7 +114,11 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
     __shared__ uint64_t lists[kWaves][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int row = blockIdx.x / wgs, part = (blockIdx.x - row * wgs) * kWaves + wave;
-    if (part >= a.parts || !offers(a, row)) return;  // (its parts are not looked at)
+    if (part >= a.parts) return;
+    // (a beam that offers nothing: its parts are not looked at.  Short parts are a small call's,
+    // which reads them all the same rather than wait for the answer)
+    const bool wanted = offers(a, row);
+    if (NV == 8 && !wanted) return;
     const float *x = a.logits + (int64_t)row * a.row_stride;
     // (parts by place, not by address: equal rows give equal bits)
     const int first = part * (256 * NV), e0 = first + 4 * lane;
@@ -130,6 +134,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
             for (int i = 0; i < 4; ++i) v[j][i] = e + i < a.vocab ? x[e + i] : -INFINITY;
         }
     }
+    if (!wanted) return;
     float most4[NV], most = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -262,21 +267,24 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     for (int c = 0; c < kAhead; ++c) ahead[c] = tid < lists && c < C ? cand[(int64_t)tid * C + c] : 0;
     if (tid == 0) count_ = 0;
     for (int b = wave; b < a.beams; b += kPick / 64) {
+        const float2 *stats = a.stats + (int64_t)(row0 + b) * a.parts;
+        float2 first[kAhead];  // (read whether they are used or not)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) first[i] = lane + 64 * i < a.parts ? stats[lane + 64 * i] : make_float2(0.0f, 0.0f);
         const float score = a.scores[row0 + b];
         const bool ok = score > -INFINITY && score < INFINITY, done = a.finished && a.finished[row0 + b];
         double start = -INFINITY;
         if (ok && !done) {
-            const float2 *stats = a.stats + (int64_t)(row0 + b) * a.parts;
             float most = -INFINITY;
             double all = 0.0;
-#pragma unroll 2
-            for (int p = lane; p < a.parts; p += 64) {
-                const float2 s = stats[p];
-                if (s.y == 0.0f) continue;
+            auto add = [&](const float2 &s) {
+                if (s.y == 0.0f) return;
                 const float next = fmaxf(most, s.x);
                 all = (most > -INFINITY ? all * power(a, most - next) : 0.0) + (double)s.y * power(a, s.x - next);
                 most = next;
-            }
+            };
+            for (int i = 0; i < kAhead; ++i) add(first[i]);
+            for (int p = lane + 64 * kAhead; p < a.parts; p += 64) add(stats[p]);
             const float top = unordered(wave_max(ordered(most)));
             if (most > -INFINITY) all *= power(a, most - top);  // (a NaN stays one)
 #pragma unroll

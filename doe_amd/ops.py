@@ -753,6 +753,7 @@ class Mx4Cache:
         self.num_kv_heads, self.head_dim, self.batch = num_kv_heads, head_dim, batch
         self.args = _Mx4CacheArgs(pool.ptr, page_table.ptr, kv_lens.ptr, num_pages, page_size, num_kv_heads, head_dim,
                                   batch, table_stride)
+        self.ref = C.byref(self.args)
 
 
 class KvPages:
@@ -928,6 +929,15 @@ class _LoraArgs(C.Structure):
         (n, C.c_int64) for n in ("num_adapters", "rank", "k", "slices")] + [("slice_n", C.c_int64 * 4), ("bf16", C.c_int32)]
 
 
+def _at(buf: DeviceBuffer | None) -> int | None:
+    """A buffer's address as an argument (ctypes takes the number as a pointer)."""
+    return None if buf is None else buf.ptr
+
+
+def _on(stream):
+    return None if stream is None else _stream_ptr(stream)
+
+
 class F16Cache:
     """One layer's KV cache in f16 pages ([num_pages][page_size][num_kv_heads]
     [head_dim] of K and V, the order that ``attention_dispatch`` reads with
@@ -946,6 +956,7 @@ class F16Cache:
         self.num_kv_heads, self.head_dim, self.batch = num_kv_heads, head_dim, batch
         self.args = _F16CacheArgs(k_pool.ptr, v_pool.ptr, page_table.ptr, kv_lens.ptr, num_pages, page_size, num_kv_heads,
                                   head_dim, batch, table_stride)
+        self.ref = C.byref(self.args)
 
 
 def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: DeviceBuffer | None, rows: int, *,
@@ -975,8 +986,8 @@ def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: Device
                 raise ValueError(f"no freq_cis for a rotary_dim of {rot}")
             _need(freq_cis, max_positions * rot * 4, "freq_cis")
     fn = "doe_mx4_qkv_rope_append" if isinstance(cache, Mx4Cache) else "doe_qkv_rope_append"
-    _lib.call(fn, C.byref(cache.args), _p(qkv), stride, _opt(q_out), int(q_f16), qs, num_heads, _opt(freq_cis), max_positions,
-              rot, int(interleaved), _opt(row_starts), rows, _stream_ptr(stream))
+    _lib.call(fn, cache.ref, qkv.ptr, stride, _at(q_out), int(q_f16), qs, num_heads, _at(freq_cis), max_positions,
+              rot, int(interleaved), _at(row_starts), rows, _on(stream))
 
 
 class Lora:
@@ -998,12 +1009,13 @@ class Lora:
         self.k, self.n = k, sum(slice_n)
         self.args = _LoraArgs(a.ptr, b.ptr, None if scales is None else scales.ptr, num_adapters, rank, k, len(slice_n),
                               (C.c_int64 * 4)(*slice_n), int(bf16))
+        self.ref = C.byref(self.args)
 
 
 def lora_workspace(lora: Lora, rows: int) -> int:
     """Workspace bytes of ``lora_add`` over ``rows`` rows."""
     size = C.c_int64()
-    _lib.call("doe_lora_workspace", C.byref(lora.args), rows, C.byref(size))
+    _lib.call("doe_lora_workspace", lora.ref, rows, C.byref(size))
     return size.value
 
 
@@ -1024,8 +1036,8 @@ def lora_add(lora: Lora, adapters: DeviceBuffer, x: DeviceBuffer, y: DeviceBuffe
     if rows:
         _need(x, ((rows - 1) * xs + lora.k) * 4, "x")
         _need(y, ((rows - 1) * ys + lora.n) * 4, "y")
-    _lib.call("doe_lora_add", C.byref(lora.args), _p(adapters), _opt(row_starts), count, _p(x), xs, _p(y), ys, rows,
-              _p(workspace), workspace.nbytes, _stream_ptr(stream))
+    _lib.call("doe_lora_add", lora.ref, adapters.ptr, _at(row_starts), count, x.ptr, xs, y.ptr, ys, rows,
+              workspace.ptr, workspace.nbytes, _on(stream))
 
 
 def beam_select_workspace(batch: int, beams: int, vocab: int, select: int) -> int:
@@ -1052,9 +1064,9 @@ def beam_select(logits: DeviceBuffer, scores: DeviceBuffer, *, batch: int, beams
     for buf, role in ((parents, "parents"), (tokens, "tokens"), (out_scores, "out_scores"), (out_finished, "out_finished")):
         if buf is not None:
             _need(buf, batch * select * 4, role)
-    _lib.call("doe_beam_select", _p(logits), stride, _p(scores), _opt(finished), batch, beams, vocab, select,
-              inv_temperature, end_token, _p(parents), _p(tokens), _p(out_scores), _opt(out_finished), _p(workspace),
-              workspace.nbytes, _stream_ptr(stream))
+    _lib.call("doe_beam_select", logits.ptr, stride, scores.ptr, _at(finished), batch, beams, vocab, select,
+              inv_temperature, end_token, parents.ptr, tokens.ptr, out_scores.ptr, _at(out_finished), workspace.ptr,
+              workspace.nbytes, _on(stream))
 
 
 def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffer, rows: int, *, row_bytes: int,
@@ -1069,8 +1081,8 @@ def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffe
         _need(src, (layers - 1) * ss + sr * row_bytes, "src")
         _need(dst, (layers - 1) * ds + rows * row_bytes, "dst")
     _need(parents, rows * 4, "parents")
-    _lib.call("doe_beam_reorder_rows", _p(src), _p(dst), _p(parents), sr, rows, row_bytes, layers, ss, ds,
-              _stream_ptr(stream))
+    _lib.call("doe_beam_reorder_rows", src.ptr, dst.ptr, parents.ptr, sr, rows, row_bytes, layers, ss, ds,
+              _on(stream))
 
 
 def beam_reorder_pages_workspace(num_pages: int, max_seqs: int, n: int) -> int:
@@ -1090,8 +1102,8 @@ def beam_reorder_pages(pages: KvPages, parents: DeviceBuffer, n: int, *, status:
     if seqs is not None:
         _need(seqs, n * 4, "seqs")
     _need(status, 4, "status")
-    _lib.call("doe_beam_reorder_pages", C.byref(pages.args), _opt(seqs), _p(parents), n, _p(status), _p(workspace),
-              workspace.nbytes, _stream_ptr(stream))
+    _lib.call("doe_beam_reorder_pages", C.byref(pages.args), _at(seqs), parents.ptr, n, status.ptr, workspace.ptr,
+              workspace.nbytes, _on(stream))
 
 
 def tune(key: str, value: int) -> None:
