@@ -418,7 +418,7 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         a.parents[to] = none ? -1 : row0 + b;
         a.tokens[to] = token;
         a.best[to] = (float)score;
-        if (a.ended) a.ended[to] = !none && ((a.finished && a.finished[row0 + b]) || token == a.end_token) ? 1 : 0;
+        if (a.ended) a.ended[to] = !none && (ended_at[b] > -INFINITY || token == a.end_token) ? 1 : 0;  // (it may be a.finished)
     };
     if (count <= kPool) {
         // sixteen threads a candidate
@@ -548,6 +548,14 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
                 (long long)vocab, finished ? ", with finished beams" : "");
     DOE_REQUIRE(batch == 0 || (logits && scores && parents && tokens && out_scores), DOE_E_INVALID, "null pointer");
     DOE_REQUIRE(((uintptr_t)logits & 3) == 0, DOE_E_INVALID, "logits must be 4-byte aligned");
+    // in place only request by request
+    auto apart = [&](const void *in, const void *out) {
+        const uintptr_t i = (uintptr_t)in, o = (uintptr_t)out;
+        return !in || !out || (i == o && select == beams) || i + (uintptr_t)(4 * batch * beams) <= o || o + (uintptr_t)(4 * batch * select) <= i;
+    };
+    DOE_REQUIRE(apart(scores, out_scores) && apart(finished, out_finished) && apart(scores, out_finished) && apart(finished, out_scores) &&
+                    apart(scores, parents) && apart(scores, tokens) && apart(finished, parents) && apart(finished, tokens),
+                DOE_E_INVALID, "the outputs overlap scores or finished");
     DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bytes, DOE_E_INVALID,
                 "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)z.bytes, (long long)workspace_bytes);
     const int64_t rows = batch * beams, wgs = (z.parts + kWaves - 1) / kWaves;

@@ -720,15 +720,16 @@ int doe_beam_reorder_pages(const doe_kv_pages *pages, const int32_t *seqs, const
     r.old_len = a.pair + 2 * n;
     r.heirs = r.old_len + n;
     r.fresh = r.heirs + n;
+    // a workgroup's cells fit in 32 KB, and the columns spread over the device
+    r.columns = (int)std::max<int64_t>(1, std::min<int64_t>({64, kReorder / n, (a.table_stride + 255) / 256 * 16}));
+    const int64_t chunks = (a.table_stride + r.columns - 1) / r.columns;
+    DOE_REQUIRE(chunks < (1 << 24), DOE_E_UNSUPPORTED, "%lld sequences of up to %d pages", (long long)n, a.table_stride);
     const int lds = (int)(8 * n);
     static const hipError_t attr_rc = hipFuncSetAttribute((const void *)pages_reorder_plan_kernel,
                                                           hipFuncAttributeMaxDynamicSharedMemorySize, 8 * kReorder);
     DOE_HIP_CHECK(attr_rc);
     hipLaunchKernelGGL(pages_reorder_plan_kernel, dim3(1), dim3(kPlan), lds, (hipStream_t)stream, r);
     DOE_LAUNCH_CHECK("pages_reorder_plan_kernel");
-    // a workgroup's cells fit in 32 KB, and the columns spread over the device
-    r.columns = (int)std::max<int64_t>(1, std::min<int64_t>({64, kReorder / n, (a.table_stride + 255) / 256 * 16}));
-    const int64_t chunks = (a.table_stride + r.columns - 1) / r.columns;
     const unsigned wgs = (unsigned)std::max<int64_t>(chunks, wide_grid(a, n, 0));
     hipLaunchKernelGGL(pages_reorder_kernel, dim3(wgs), dim3(256), (size_t)n * r.columns * 4, (hipStream_t)stream, r);
     DOE_LAUNCH_CHECK("pages_reorder_kernel");

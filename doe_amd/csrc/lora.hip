@@ -101,10 +101,10 @@ __device__ __forceinline__ int find_tile(const LoraArgs &a, int place, int &row,
     }
     if (start < 0) return -1;
     const int64_t first = (int64_t)start + (int64_t)(place - (start >> kShift) - lo) * kTile;
-    const int left = (int)(std::min(end, a.rows) - first);
+    const int64_t left = std::min(end, a.rows) - first;
     if (left <= 0) return -1;
     row = (int)first;
-    count = std::min(kTile, left);
+    count = (int)std::min<int64_t>(kTile, left);
     return adapter_at(a, lo);
 }
 template <bool BF16>

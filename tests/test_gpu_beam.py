@@ -207,6 +207,19 @@ def test_captured_select_replays(dev, batch, beams, vocab):
     s.destroy()
 
 
+@pytest.mark.parametrize("batch,beams,vocab", [(3, 4, 5000), (20, 16, 9000)])
+def test_scores_and_flags_in_place(dev, batch, beams, vocab):
+    rng = np.random.default_rng(9)
+    fin = i32(rng.random((batch, beams)) < 0.3)
+    c = clear_case(9, batch, beams, vocab, beams, finished=fin, end=4)
+    c.out[2], c.out[3] = c.bufs["scores"], c.kw["finished"]
+    c.run()
+    got = [o.download().reshape(batch, beams) for o in c.out]
+    want, _ = oracle(c.logits, c.scores, fin, beams, 1.0, 4)
+    assert all(np.array_equal(got[i], want[i]) for i in (0, 1, 3))
+    assert np.all(np.abs(got[2] - want[2]) <= TOL + 2.0 ** -24 * np.abs(want[2]))
+
+
 def test_no_requests_and_no_flags(dev):
     c = clear_case(6, 2, 3, 100, 3)
     p, t, s, _ = c.out

@@ -104,9 +104,22 @@ def test_lora_buffers_are_checked():
         ops.lora_add(lora(), BIG, BIG, Apart(), 5, workspace=BIG, row_starts=BIG)
 
 
+def at(ptr, nbytes=1 << 40):
+    return type("B", (), dict(nbytes=nbytes, ptr=ptr))()
+
+
 def select(**kw):
-    how = dict(batch=2, beams=4, vocab=1000, select=8, parents=BIG, tokens=BIG, out_scores=BIG, workspace=BIG)
-    ops.beam_select(kw.pop("logits", BIG), BIG, **{**how, **kw})
+    how = dict(batch=2, beams=4, vocab=1000, select=8, parents=Apart(), tokens=Apart(), out_scores=Apart(), workspace=BIG)
+    ops.beam_select(kw.pop("logits", BIG), kw.pop("scores", BIG), **{**how, **kw})
+
+
+@pytest.mark.parametrize("how", [
+    dict(out_scores=BIG), dict(out_scores=at(BIG.ptr + 28)), dict(out_scores=at(BIG.ptr - 60)), dict(out_scores=BIG, select=5), dict(parents=BIG),
+    dict(tokens=at(BIG.ptr + 4)), dict(out_scores=at(BIG.ptr + 4), select=4), dict(finished=at(1 << 45), out_finished=at(1 << 45), end_token=1),
+    dict(finished=at(1 << 45), out_finished=at((1 << 45) + 4), end_token=1, select=4), dict(finished=at(1 << 45), out_scores=at((1 << 45) - 8), end_token=1),
+])
+def test_select_in_place(how):
+    refused("overlap scores or finished", select, **how)
 
 
 @pytest.mark.parametrize("message,how", [
