@@ -542,8 +542,9 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
     int rc = beam_sizes(batch, beams, vocab, select, z);
     if (rc) return rc;
     DOE_REQUIRE(row_stride >= vocab, DOE_E_INVALID, "row stride %lld below vocab %lld", (long long)row_stride, (long long)vocab);
-    DOE_REQUIRE(isfinite(inv_temperature) && inv_temperature > 0.0f && isfinite(inv_temperature * 1.4426950408889634f), DOE_E_INVALID,
-                "inv_temperature %g", (double)inv_temperature);
+    // (factor_low, 2^-53 of it at the least, is above 0)
+    DOE_REQUIRE(inv_temperature >= 0x1p-64f && isfinite(inv_temperature * 1.4426950408889634f), DOE_E_INVALID, "inv_temperature %g",
+                (double)inv_temperature);
     DOE_REQUIRE(end_token < vocab && (end_token >= 0 || !finished), DOE_E_INVALID, "end_token %lld of %lld tokens%s", (long long)end_token,
                 (long long)vocab, finished ? ", with finished beams" : "");
     DOE_REQUIRE(batch == 0 || (logits && scores && parents && tokens && out_scores), DOE_E_INVALID, "null pointer");

@@ -622,7 +622,8 @@ int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_
  *   row_starts  device int32 [segments + 1]: rows [row_starts[s], row_starts[s + 1])
  *               are segment s's, in order; NULL: rows == segments, a row each.  Rows
  *               of no segment are left as they were.
- * f32-accurate (2-3e-7 of float64).  rank a multiple of 8 up to 256, k a multiple of 8
+ * f32-accurate (2-3e-7 of float64); a row of x with an infinity or a NaN gives infinities
+ * or NaNs in its own row of y.  rank a multiple of 8 up to 256, k a multiple of 8
  * up to 2^20, a and b 16-byte aligned.  The workspace (16-byte aligned,
  * doe_lora_workspace bytes) is the caller's: calls that may overlap, and captured
  * graphs that may be replayed side by side, each take their own.  Nothing is kept
@@ -652,7 +653,8 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
  * Out, [batch][select], best first, ties to the lowest beam, then token: parents
  * (the rows; -1 where there are fewer offers), tokens (-1), out_scores (-infinity),
  * out_finished (may be NULL: 1 where the parent was finished or the token is
- * end_token).  end_token -1: none (finished is then NULL).  Scores are compared in 64 bits.
+ * end_token).  end_token -1: none (finished is then NULL).  inv_temperature from 2^-64
+ * on.  Scores are compared in 64 bits.
  * With select == beams out_scores may be scores and out_finished finished; otherwise the
  * outputs are apart from both.
  * beams and select up to 64, vocab up to 2^24.  The workspace (16-byte aligned,

@@ -207,6 +207,15 @@ def test_captured_select_replays(dev, batch, beams, vocab):
     s.destroy()
 
 
+@pytest.mark.parametrize("vocab", [900, 30000])
+def test_masked_logits_at_the_least_inverse_temperature(dev, vocab):
+    logits = rows_of(np.random.default_rng(10), 2, 3, vocab)
+    logits[:, :, ::3] = -np.inf
+    c = Case(logits, [[-3.0, -1.0, -2.0], [0.0, -4.0, -1.0]], select=5, factor=2.0 ** -64)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("batch,beams,vocab", [(3, 4, 5000), (20, 16, 9000)])
 def test_scores_and_flags_in_place(dev, batch, beams, vocab):
     rng = np.random.default_rng(9)

@@ -125,7 +125,8 @@ def test_select_in_place(how):
 @pytest.mark.parametrize("message,how", [
     ("beams 65", dict(beams=65)), ("beams 0", dict(beams=0)), ("select 0", dict(select=0)), ("select 65", dict(select=65)),
     ("vocab 0", dict(vocab=0)), ("vocab 16777217", dict(vocab=(1 << 24) + 1)), ("row stride 999", dict(row_stride=999)),
-    ("inv_temperature 0", dict(inv_temperature=0.0)), ("inv_temperature nan", dict(inv_temperature=float("nan"))),
+    ("inv_temperature 0", dict(inv_temperature=0.0)), ("inv_temperature 1e-20", dict(inv_temperature=1e-20)),
+    ("inv_temperature -1", dict(inv_temperature=-1.0)), ("inv_temperature nan", dict(inv_temperature=float("nan"))),
     ("inv_temperature inf", dict(inv_temperature=float("inf"))), ("inv_temperature 3e\\+38", dict(inv_temperature=3e38)),
     ("end_token 1000", dict(end_token=1000)), ("end_token -1", dict(finished=BIG)),
     ("workspace of", dict(workspace=type("S", (), dict(nbytes=16, ptr=16))())),
