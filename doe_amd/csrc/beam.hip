@@ -6,7 +6,9 @@
 // the inverse temperature.  Within a row the order is that of the logits, so the first
 // kernel reads them once and leaves, for every wave's part of a row, its `select` best
 // logits and its share of the sum; the second one forms the rows' logarithms in 64 bits
-// and picks among the parts.
+// and picks among the parts.  Sixteen requests of eight beams, 248321 tokens, the best
+// sixteen (127 MB): 31 us, 25 of them in the first kernel (5 TB/s), 6 in the second; four beams
+// of 256000: 9.1, 4.9 and 4.3, chains of cold reads and barriers.
 #include "common.h"
 
 #include <math.h>
@@ -23,6 +25,7 @@ constexpr int kWaves = 4;
 constexpr int kList = 256;   // a wave's shortlist
 constexpr int kPick = 1024;  // threads of the second kernel
 constexpr int kPool = 4096;  // its shortlist
+constexpr int kAhead = 4;    // entries of a thread's first list that are read at once
 
 struct BeamArgs {
     const float *logits, *scores;
@@ -30,7 +33,8 @@ struct BeamArgs {
     int64_t row_stride;
     int batch, beams, vocab, select, parts, end_token;  // parts of a row: a wave each
     float inv_temperature, factor, factor_low;  // factor + factor_low = inv_temperature log2(e), factor_low above 0
-    uint64_t *cand;   // [row][part][select]: logit order, ~token; 0: none
+    float per_part;   // 1 / parts
+    uint64_t *cand;   // [row][select][part]: logit order, ~token; 0: none
     float2 *stats;    // [row][part]: the largest logit and the sum of their powers over it; 0: none above -infinity
     int32_t *parents, *tokens, *ended;
     float *best;
@@ -78,21 +82,28 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     const uint32_t hi = wave_max((uint32_t)(v >> 32));
     return (uint64_t)hi << 32 | wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
-// A bound that at least `select` (up to 16) of the lanes' values reach and few others: the
-// least of the `select` lanes that are largest but for six bits of their values.
-constexpr int kFew = 16;
-__device__ __forceinline__ float bound_of_few(float v, int select) {
-    uint32_t key = (ordered(v) & ~63u) | (threadIdx.x & 63);
-    bool taken = false;
-    for (int c = 0; c < select; ++c) {
-        const bool most = key == wave_max(key);
-        taken = taken || most;
-        key = most ? 0 : key;
-    }
-    return unordered(~wave_max(taken ? ~ordered(v) : 0u));
+// The value of the lane N before this one in a circle of sixteen.
+template <int N, typename T>
+__device__ __forceinline__ T dpp_turn(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, true));
 }
-// The same of more: bit by bit the largest key that enough values reach, until no more than
-// a quarter too many do.  count(key): how many.
+// The sum over the wave, in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, true);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
+    const uint64_t b = __builtin_bit_cast(uint64_t, dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v)));
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// A bound that at least `select` of some values reach and few others, bit by bit: the largest
+// key that enough of them reach, until no more than a quarter too many do.  count(key): how
+// many.
 template <typename F>
 __device__ __forceinline__ float bound_of_many(int select, const F &count) {
     uint32_t key = 0;
@@ -104,6 +115,24 @@ __device__ __forceinline__ float bound_of_many(int select, const F &count) {
         if (n <= select + select / 4) break;
     }
     return key > ordered(-INFINITY) ? unordered(key) : -INFINITY;
+}
+// The same of the lanes' values, for up to kOne of them.  Up to kFew one lane after the other
+// is taken, the largest but for six bits of its value, and the least of them is the bound:
+// four of a wave 0.5 us less in a call than bit by bit, sixteen 1 us more.
+constexpr int kFew = 8, kOne = 16;
+__device__ __forceinline__ float bound_of_one(float v, int select) {
+    if (select > kFew) {
+        const uint32_t key = ordered(fmaxf(v, -INFINITY));
+        return bound_of_many(select, [&](uint32_t at) __attribute__((always_inline)) { return (int)__popcll(__ballot(key >= at)); });
+    }
+    uint32_t key = (ordered(v) & ~63u) | (threadIdx.x & 63);
+    bool taken = false;
+    for (int c = 0; c < select; ++c) {
+        const bool most = key == wave_max(key);
+        taken = taken || most;
+        key = most ? 0 : key;
+    }
+    return unordered(~wave_max(taken ? ~ordered(v) : 0u));
 }
 
 // A wave's part of a row: NV x 256 logits, four side by side a lane, kept in
@@ -142,7 +171,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
         most = fmaxf(most, most4[j]);
     }
     const int64_t slot = (int64_t)row * a.parts + part;
-    uint64_t *cand = a.cand + slot * a.select;
+    uint64_t *cand = a.cand + (int64_t)row * a.select * a.parts + part;  // (then every parts-th)
     const float top = unordered(wave_max(ordered(most)));
     // an infinity or a NaN leaves a sum that is no number; -infinity adds 0 (factor_low > 0)
     f4 sums = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -163,12 +192,12 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
     if (lane == 0) a.stats[slot] = make_float2(top, sum);
     if (!(sum > 0.0f)) {
-        if (lane < a.select) cand[lane] = 0;
+        if (lane < a.select) cand[(int64_t)lane * a.parts] = 0;
         return;
     }
     float low;
-    if (a.select <= kFew) {
-        low = bound_of_few(most, a.select);
+    if (a.select <= kOne) {
+        low = bound_of_one(most, a.select);
     } else {
         // (four values a lane: of one, nearly all would have to be taken)
         uint32_t key[4];
@@ -207,9 +236,9 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
             int before = 0;
 #pragma unroll 8
             for (int j = 0; j < count; ++j) before += list[j] > key ? 1 : 0;
-            if (before < a.select) cand[before] = key;
+            if (before < a.select) cand[(int64_t)before * a.parts] = key;
         }
-        if (lane >= count && lane < a.select) cand[lane] = 0;
+        if (lane >= count && lane < a.select) cand[(int64_t)lane * a.parts] = 0;
         return;
     }
     // (rarely: the large ones in few lanes, or as many equal ones) one after the other
@@ -224,7 +253,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
                 if (key < last && key > next) next = key;
             }
         last = wave_max(next);
-        if (lane == 0) cand[c] = last;
+        if (lane == 0) cand[(int64_t)c * a.parts] = last;
     }
 }
 
@@ -248,47 +277,60 @@ __device__ __forceinline__ double logarithm(double x) {
     return fma((double)e, 0.69314718055994531, 2.0 * fma(u * w, p, u));
 }
 
-// A request's pick: the rows' logarithms, then the same way as above with a thread a
-// part's list instead of a lane its logits.
+// A request's pick: the rows' logarithms, a bound of the lists' best, the candidates that
+// reach it, and their places in the order.  Entries of a place lie side by side for a beam's
+// parts and are read before it is known which are wanted: sixteen requests of eight 6 us, 10
+// with a list's entries side by side, read in turn, and a bound from the waves' own.
 __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     __shared__ double base[kMaxBeams], ended_at[kMaxBeams], pool[kPool];
     __shared__ uint64_t pool_at[kPool];  // a candidate's place, see `place`
-    __shared__ float bounds[kPick / 64];
+    __shared__ uint64_t ahead[kAhead][kPick];
+    __shared__ float heads[kPick / 64][65], bound_;
+    __shared__ __align__(16) float most[64];
     __shared__ int count_, sums[2][kPick / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int request = blockIdx.x, row0 = request * a.beams, C = a.select, lists = a.beams * a.parts;
     const uint64_t *cand = a.cand + (int64_t)row0 * a.parts * C;
     const double factor = a.inv_temperature;
+    // (l + 1/2 is 2^-15 of an integer's place off it, the product within 2^-16)
+    auto beam_of = [&](int l) __attribute__((always_inline)) { return (int)(((float)l + 0.5f) * a.per_part); };
+    auto entry = [&](int l, int c) __attribute__((always_inline)) {
+        const int b = beam_of(l);
+        return cand[(uint32_t)((b * C + c) * a.parts + (l - b * a.parts))];
+    };
     // this thread's first list, as far as it is likely to go (a beam without an offer leaves
     // its lists as they were: not used below)
-    constexpr int kAhead = 4;
-    uint64_t ahead[kAhead];
+    uint64_t own_list[kAhead];
 #pragma unroll
-    for (int c = 0; c < kAhead; ++c) ahead[c] = tid < lists && c < C ? cand[(int64_t)tid * C + c] : 0;
+    for (int c = 0; c < kAhead; ++c) own_list[c] = entry(std::min(tid, lists - 1), std::min(c, C - 1));
     if (tid == 0) count_ = 0;
     for (int b = wave; b < a.beams; b += kPick / 64) {
         const float2 *stats = a.stats + (int64_t)(row0 + b) * a.parts;
-        float2 first[kAhead];  // (read whether they are used or not)
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) first[i] = lane + 64 * i < a.parts ? stats[lane + 64 * i] : make_float2(0.0f, 0.0f);
         const float score = a.scores[row0 + b];
-        const bool ok = score > -INFINITY && score < INFINITY, done = a.finished && a.finished[row0 + b];
+        const int ended = (a.finished ? a.finished : reinterpret_cast<const int32_t *>(a.scores))[row0 + b];
+        float2 first[kAhead];  // (read whether they are used or not, so that one does not wait for another)
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) first[i] = stats[std::min(lane + 64 * i, a.parts - 1)];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (lane + 64 * i >= a.parts) first[i] = make_float2(-INFINITY, 0.0f);
+        const bool ok = score > -INFINITY && score < INFINITY, done = a.finished && ended;
         double start = -INFINITY;
         if (ok && !done) {
             float most = -INFINITY;
-            double all = 0.0;
-            auto add = [&](const float2 &s) {
-                if (s.y == 0.0f) return;
-                const float next = fmaxf(most, s.x);
-                all = (most > -INFINITY ? all * power(a, most - next) : 0.0) + (double)s.y * power(a, s.x - next);
-                most = next;
-            };
-            for (int i = 0; i < kAhead; ++i) add(first[i]);
-            for (int p = lane + 64 * kAhead; p < a.parts; p += 64) add(stats[p]);
-            const float top = unordered(wave_max(ordered(most)));
-            if (most > -INFINITY) all *= power(a, most - top);  // (a NaN stays one)
 #pragma unroll
-            for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+            for (int i = 0; i < kAhead; ++i) most = fmaxf(most, first[i].x);
+            for (int p = lane + 64 * kAhead; p < a.parts; p += 64) most = fmaxf(most, stats[p].x);
+            const float top = unordered(wave_max(ordered(most)));
+            // (of none above -infinity a NaN, and a NaN stays one)
+            double all = 0.0;
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) all = fma((double)first[i].y, (double)power(a, first[i].x - top), all);
+            for (int p = lane + 64 * kAhead; p < a.parts; p += 64) {
+                const float2 s = stats[p];
+                all = fma((double)s.y, (double)power(a, s.x - top), all);
+            }
+            all = wave_sum(all);
             if (all > 0.0 && all < INFINITY) start = (double)score - ((double)top * factor + logarithm(all));
         }
         if (lane == 0) {
@@ -296,6 +338,8 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             ended_at[b] = ok && done ? (double)score : -INFINITY;
         }
     }
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) ahead[c][tid] = own_list[c];
     __syncthreads();
     auto score_of = [&](uint64_t key, int b) {
         return key && base[b] > -INFINITY ? base[b] + factor * (double)unordered((uint32_t)(key >> 32)) : -INFINITY;
@@ -305,7 +349,7 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     auto place = [](int b, uint64_t key) { return (uint64_t)b << 56 | (uint64_t)~(uint32_t)(key >> 32) << 24 | ~(uint32_t)key; };
     auto end_place = [&](int b) { return (uint64_t)b << 56 | (uint32_t)a.end_token; };
     constexpr uint64_t kNone = ~0ull;
-    auto head_of = [&](int l) { return l == tid ? ahead[0] : cand[(int64_t)l * C]; };
+    auto head_of = [&](int l) { return l == tid ? ahead[0][tid] : entry(l, 0); };
     // the float at or below a score: a bound of these is below `select` of the scores
     auto below = [](double score) {
         const float f = (float)score;
@@ -337,17 +381,13 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             return in;
         };
         if (lists <= kPick / 4) {  // few lists: a thread an entry, not a list
-            for (int i = tid; i < lists * C; i += kPick) offer(cand[i], i / C / a.parts);
+            for (int i = tid; i < lists * C; i += kPick) offer(cand[i], i / (C * a.parts));
         }
         for (int l = lists <= kPick / 4 ? lists : tid; l < lists; l += kPick) {
-            const int b = l / a.parts;
-            int c = 0;
-            bool more = true;
-            if (l == tid) {
-#pragma unroll
-                for (; c < kAhead; ++c) more = more && offer(ahead[c], b);
-            }
-            for (; more && c < C; ++c) more = offer(cand[(int64_t)l * C + c], b);
+            const int b = beam_of(l);
+#pragma unroll 1
+            for (int c = 0; c < C; ++c)
+                if (!offer(l == tid && c < kAhead ? ahead[c][tid] : entry(l, c), b)) break;
         }
         if (tid < a.beams && ended_at[tid] > -INFINITY && ended_at[tid] >= bound) push(ended_at[tid], end_place(tid));
         __syncthreads();
@@ -359,30 +399,51 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         __syncthreads();
     };
     constexpr int kEnough = 4 * kMaxSelect;  // whose order is counted
-    int count = kPool + 1;
-    if (C <= kFew) {
-        double mine = -INFINITY;
-        for (int l = tid; l < lists; l += kPick) mine = fmax(mine, score_of(head_of(l), l / a.parts));
-        const float own = bound_of_few(below(mine), C);
-        if (lane == 0) bounds[wave] = own;
-        __syncthreads();
-        count = gather(unordered(wave_max(ordered(bounds[lane & (kPick / 64 - 1)]))));
+    // a bound: of 64 groups of lists, their best by themselves, the `select`-th best
+    // (equal ones in the groups' order)
+    double mine = -INFINITY;
+    for (int l = tid; l < lists; l += kPick) mine = fmax(mine, score_of(head_of(l), beam_of(l)));
+    heads[wave][lane] = below(mine);
+    __syncthreads();
+    const int group = tid >> 4, sixteenth = tid & 15;
+    {
+        float m = heads[sixteenth][group];
+        m = fmaxf(m, dpp_turn<1>(m));
+        m = fmaxf(m, dpp_turn<2>(m));
+        m = fmaxf(m, dpp_turn<4>(m));
+        m = fmaxf(m, dpp_turn<8>(m));
+        if (sixteenth == 0) most[group] = m;
     }
-    if (count > kEnough) {
+    __syncthreads();
+    {
+        const float m = most[group];
+        const f4 other = *reinterpret_cast<const f4 *>(most + 4 * sixteenth);
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before += other[i] > m || (other[i] == m && 4 * sixteenth + i < group) ? 1 : 0;
+        before += dpp_turn<1>(before);
+        before += dpp_turn<2>(before);
+        before += dpp_turn<4>(before);
+        before += dpp_turn<8>(before);
+        if (sixteenth == 0 && before == C - 1) bound_ = m;
+    }
+    __syncthreads();
+    int count = gather(bound_);
+    if (count > kPool) {
         // the lists' best by themselves: no more than `select` lists reach their bound, but for ties
         constexpr int kHeads = 8;
         uint32_t key[kHeads];
 #pragma unroll
         for (int i = 0; i < kHeads; ++i) {
             const int l = tid + i * kPick;
-            key[i] = l < lists ? ordered(below(score_of(head_of(l), l / a.parts))) : 0;
+            key[i] = l < lists ? ordered(below(score_of(head_of(l), beam_of(l)))) : 0;
         }
         const float own = lists < C ? -INFINITY : bound_of_many(C, [&](uint32_t at) __attribute__((always_inline)) {
             int n = 0;
 #pragma unroll
             for (int i = 0; i < kHeads; ++i) n += __popcll(__ballot(key[i] >= at));
             for (int l = wave * 64 + lane + kHeads * kPick; l - lane < lists; l += kPick)
-                n += __popcll(__ballot(l < lists && ordered(below(score_of(head_of(l), l / a.parts))) >= at));
+                n += __popcll(__ballot(l < lists && ordered(below(score_of(head_of(l), beam_of(l)))) >= at));
             return block_sum(n);
         });
         emptied();
@@ -449,10 +510,10 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         };
         for (int l = tid; l < lists; l += kPick)
             for (int e = 0; e < C; ++e) {
-                const uint64_t key = cand[(int64_t)l * C + e];
-                const double score = score_of(key, l / a.parts);
+                const uint64_t key = entry(l, e);
+                const double score = score_of(key, beam_of(l));
                 if (score == -INFINITY) break;
-                take(score, place(l / a.parts, key));
+                take(score, place(beam_of(l), key));
             }
         if (tid < a.beams) take(ended_at[tid], end_place(tid));
         __syncthreads();  // the last round's places have been read
@@ -579,6 +640,7 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
     a.factor = (float)factor;
     if ((double)a.factor >= factor) a.factor = nextafterf(a.factor, 0.0f);
     a.factor_low = (float)(factor - (double)a.factor);
+    a.per_part = 1.0f / (float)z.parts;
     a.cand = static_cast<uint64_t *>(workspace);
     a.stats = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + z.cand);
     a.parents = parents;
