@@ -743,6 +743,8 @@ class Mx4Cache:
     and lengths of ``batch`` sequences (device int32).  Keeps its buffers
     alive; build one per layer and use it for every call."""
 
+    append = "doe_mx4_qkv_rope_append"
+
     def __init__(self, pool: DeviceBuffer, page_table: DeviceBuffer, kv_lens: DeviceBuffer, *, num_pages: int,
                  page_size: int, num_kv_heads: int, head_dim: int, batch: int, table_stride: int):
         self.page_bytes = _mx4.page_bytes(page_size, num_kv_heads, head_dim)
@@ -929,21 +931,14 @@ class _LoraArgs(C.Structure):
         (n, C.c_int64) for n in ("num_adapters", "rank", "k", "slices")] + [("slice_n", C.c_int64 * 4), ("bf16", C.c_int32)]
 
 
-def _at(buf: DeviceBuffer | None) -> int | None:
-    """A buffer's address as an argument (ctypes takes the number as a pointer)."""
-    return None if buf is None else buf.ptr
-
-
-def _on(stream):
-    return None if stream is None else _stream_ptr(stream)
-
-
 class F16Cache:
     """One layer's KV cache in f16 pages ([num_pages][page_size][num_kv_heads]
     [head_dim] of K and V, the order that ``attention_dispatch`` reads with
     kv_layout 2), with the page table and lengths of ``batch`` sequences (device
     int32).  Keeps its buffers alive; build one per layer and use it for every
     call."""
+
+    append = "doe_qkv_rope_append"
 
     def __init__(self, k_pool: DeviceBuffer, v_pool: DeviceBuffer, page_table: DeviceBuffer, kv_lens: DeviceBuffer, *,
                  num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, batch: int, table_stride: int):
@@ -969,12 +964,14 @@ def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: Device
     sequence, or with ``row_starts`` the rows of ragged prompts, the last of a
     sequence at kv_len - 1).  ``freq_cis`` [max_positions][rotary_dim / 2][2];
     ``rotary_dim`` None: the whole head."""
-    d, hd = cache.head_dim, num_heads * cache.head_dim
+    d = cache.head_dim
+    hd = num_heads * d
     width = hd + 2 * cache.num_kv_heads * d
     stride = width if row_stride is None else row_stride
     qs = q_row_stride if q_row_stride is not None else (stride if q_out is qkv else hd)
     rot = d if rotary_dim is None else rotary_dim
-    _mx4_rows(cache, rows, row_starts)
+    if row_starts is not None or rows != cache.batch:
+        _mx4_rows(cache, rows, row_starts)
     if rows:
         _need(qkv, ((rows - 1) * stride + width) * 4, "qkv")
         if num_heads:
@@ -985,9 +982,9 @@ def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: Device
             if freq_cis is None:
                 raise ValueError(f"no freq_cis for a rotary_dim of {rot}")
             _need(freq_cis, max_positions * rot * 4, "freq_cis")
-    fn = "doe_mx4_qkv_rope_append" if isinstance(cache, Mx4Cache) else "doe_qkv_rope_append"
-    _lib.call(fn, cache.ref, qkv.ptr, stride, _at(q_out), int(q_f16), qs, num_heads, _at(freq_cis), max_positions,
-              rot, int(interleaved), _at(row_starts), rows, _on(stream))
+    _lib.call(cache.append, cache.ref, qkv.ptr, stride, None if q_out is None else q_out.ptr, 1 if q_f16 else 0, qs, num_heads,
+              None if freq_cis is None else freq_cis.ptr, max_positions, rot, 1 if interleaved else 0,
+              None if row_starts is None else row_starts.ptr, rows, None if stream is None else _stream_ptr(stream))
 
 
 class Lora:
@@ -1036,8 +1033,8 @@ def lora_add(lora: Lora, adapters: DeviceBuffer, x: DeviceBuffer, y: DeviceBuffe
     if rows:
         _need(x, ((rows - 1) * xs + lora.k) * 4, "x")
         _need(y, ((rows - 1) * ys + lora.n) * 4, "y")
-    _lib.call("doe_lora_add", lora.ref, adapters.ptr, _at(row_starts), count, x.ptr, xs, y.ptr, ys, rows,
-              workspace.ptr, workspace.nbytes, _on(stream))
+    _lib.call("doe_lora_add", lora.ref, adapters.ptr, None if row_starts is None else row_starts.ptr, count, x.ptr, xs, y.ptr, ys,
+              rows, workspace.ptr, workspace.nbytes, None if stream is None else _stream_ptr(stream))
 
 
 def beam_select_workspace(batch: int, beams: int, vocab: int, select: int) -> int:
@@ -1061,12 +1058,16 @@ def beam_select(logits: DeviceBuffer, scores: DeviceBuffer, *, batch: int, beams
     _need(scores, batch * beams * 4, "scores")
     if finished is not None:
         _need(finished, batch * beams * 4, "finished")
-    for buf, role in ((parents, "parents"), (tokens, "tokens"), (out_scores, "out_scores"), (out_finished, "out_finished")):
-        if buf is not None:
-            _need(buf, batch * select * 4, role)
-    _lib.call("doe_beam_select", logits.ptr, stride, scores.ptr, _at(finished), batch, beams, vocab, select,
-              inv_temperature, end_token, parents.ptr, tokens.ptr, out_scores.ptr, _at(out_finished), workspace.ptr,
-              workspace.nbytes, _on(stream))
+    size = batch * select * 4
+    _need(parents, size, "parents")
+    _need(tokens, size, "tokens")
+    _need(out_scores, size, "out_scores")
+    if out_finished is not None:
+        _need(out_finished, size, "out_finished")
+    _lib.call("doe_beam_select", logits.ptr, stride, scores.ptr, None if finished is None else finished.ptr, batch, beams, vocab,
+              select, inv_temperature, end_token, parents.ptr, tokens.ptr, out_scores.ptr,
+              None if out_finished is None else out_finished.ptr, workspace.ptr, workspace.nbytes,
+              None if stream is None else _stream_ptr(stream))
 
 
 def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffer, rows: int, *, row_bytes: int,
@@ -1082,7 +1083,7 @@ def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffe
         _need(dst, (layers - 1) * ds + rows * row_bytes, "dst")
     _need(parents, rows * 4, "parents")
     _lib.call("doe_beam_reorder_rows", src.ptr, dst.ptr, parents.ptr, sr, rows, row_bytes, layers, ss, ds,
-              _on(stream))
+              None if stream is None else _stream_ptr(stream))
 
 
 def beam_reorder_pages_workspace(num_pages: int, max_seqs: int, n: int) -> int:
@@ -1102,8 +1103,8 @@ def beam_reorder_pages(pages: KvPages, parents: DeviceBuffer, n: int, *, status:
     if seqs is not None:
         _need(seqs, n * 4, "seqs")
     _need(status, 4, "status")
-    _lib.call("doe_beam_reorder_pages", C.byref(pages.args), _at(seqs), parents.ptr, n, status.ptr, workspace.ptr,
-              workspace.nbytes, _on(stream))
+    _lib.call("doe_beam_reorder_pages", C.byref(pages.args), None if seqs is None else seqs.ptr, parents.ptr, n, status.ptr,
+              workspace.ptr, workspace.nbytes, None if stream is None else _stream_ptr(stream))
 
 
 def tune(key: str, value: int) -> None:
