@@ -4,9 +4,9 @@
 // Rows of their own (decode steps): lora_token_kernel, in one launch where A is small.  A
 // workgroup takes a row and 1024 of its columns, forms the t = A x that they need itself
 // (again in every workgroup of the row: A comes from the caches) and adds B t; else t is
-// formed by a launch before.  One token beside a projection of 2048 to 2304, rank 16: 4.9
+// formed by a launch before.  One token beside a projection of 2048 to 2304, rank 16: 4.3
 // us in the kernel, a chain of cold reads (adapter, A and x) and two exchanges; 64 of 48
-// adapters beside q/k/v (19.6 MB): 7.2 us, 2.7 TB/s.
+// adapters beside q/k/v (19.6 MB): 6.8 us, 2.9 TB/s.
 // Runs of rows (prompts): two launches over tiles of 32 rows of a segment.
 //   * lora_down_tiles_kernel: t^T = A x^T on v_mfma_f32_16x16x32: a lane's x row is the
 //     column of its sums, so that a row's scale is the lane's own.  x is f32: for f16
@@ -170,6 +170,45 @@ __device__ __forceinline__ void token_down(const LoraArgs &a, const uint16_t *w,
     __syncthreads();
 }
 
+// This wave's part of four rows of A, k apart, times x: every `ways`-th 512 of k.  Two of
+// them are on their way at once, whole (lanes past k take the first values, times 0): a
+// load that a lane's condition guards is waited for by itself (a token of rank 64, 5376 to
+// 21504: 9.4 to 8.9 us; in lora_token_kernel, whose waves have one or two, no gain).
+template <bool BF16>
+__device__ __forceinline__ void four_dots(const uint16_t *rows, const float *x, int k, int way, int ways, float *sum) {
+    const int units = (k + 511) / 512, mine = (threadIdx.x & 63) * 8;
+    struct Unit {
+        f4 x0, x1;
+        u32x4 w[4];
+    };
+    auto load = [&](Unit &v, int u) __attribute__((always_inline)) {
+        const int at = u * 512 + mine, from = at < k ? at : 0;
+        v.x0 = *reinterpret_cast<const f4 *>(x + from);
+        v.x1 = *reinterpret_cast<const f4 *>(x + from + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.w[j] = *reinterpret_cast<const u32x4 *>(rows + (int64_t)j * k + from);
+    };
+    auto add = [&](const Unit &v, int u) __attribute__((always_inline)) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = u * 512 + mine < k ? (i < 4 ? v.x0[i & 3] : v.x1[i & 3]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+            weights8<BF16>(v.w[j], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[j] = fmaf(y[i], f[i], sum[j]);
+        }
+    };
+    for (int u = way; u < units; u += 2 * ways) {
+        Unit v0, v1;
+        load(v0, u);
+        if (u + ways < units) load(v1, u + ways);
+        add(v0, u);
+        if (u + ways < units) add(v1, u + ways);
+    }
+}
+
 // t of a row, four rows of A a workgroup, its waves every fourth 512 of k.
 template <bool BF16>
 __global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
@@ -177,21 +216,9 @@ __global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
     const int per_row = a.slices * a.rank, fours = per_row / 4, row = blockIdx.x / fours, j0 = (blockIdx.x - row * fours) * 4;
     const int id = adapter_of(a, row);
     if (id < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint16_t *w = a.a + ((int64_t)id * per_row + j0) * a.k;
-    const float *x = a.x + (int64_t)row * a.x_stride;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-    for (int at = wave * 512 + lane * 8; at < a.k; at += 2048) {
-        const f4 x0 = *reinterpret_cast<const f4 *>(x + at), x1 = *reinterpret_cast<const f4 *>(x + at + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f[8];
-            weights8<BF16>(*reinterpret_cast<const u32x4 *>(w + (int64_t)j * a.k + at), f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[j] = fmaf(x1[i], f[i + 4], fmaf(x0[i], f[i], sum[j]));
-        }
-    }
+    four_dots<BF16>(a.a + ((int64_t)id * per_row + j0) * a.k, a.x + (int64_t)row * a.x_stride, a.k, wave, 4, sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         sum[j] = wave_sum(sum[j]);
@@ -442,7 +469,7 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void lora_down_tiles_kernel(Lor
 // time.  RS: steps of 16 of the rank.  y is read and written past the caches: B, read
 // again for every tile, stays there (four prompts at rank 64: 94 to 80 us).  Tiles of 64
 // rows, which read B half as often, take more registers than there are: 94 to 109 us beside
-// gate and up, 80 to 155 at rank 64.
+// gate and up, 80 to 155 at rank 64; as two halves one after the other 104 and 82.
 template <bool BF16, int RS>
 __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
     using P = Parts<BF16>;
