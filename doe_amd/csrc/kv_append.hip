@@ -4,10 +4,11 @@
 // kv_layout 2.
 //
 // Bound by its bytes: eight prompts of up to 2000 rows, 32 / 8 heads of 128 dims, f16
-// queries (387 MB): 81 us, 4.8 TB/s.  A thread has the same eight values of every row that
-// its workgroup takes, one row at a time (four at once, 112 registers: as fast); rows read
-// past the caches: 85.  One token of 8 / 4 heads of 256: 3 us in the kernel, three dependent
-// reads (length, page, angles) before its stores.
+// queries (387 MB): 76 us, 5.1 TB/s.  A thread has the same eight values of every row that
+// its workgroup takes; a row is read before its position is known, and the next one while it
+// turns (without: 81; 16384 workgroups instead of 8192: 78, 4096: 81).  One token of 8 / 4
+// heads of 256: 2.7 us in the kernel, three dependent reads (length, page, angles) before its
+// stores.
 #include "rope_rows.h"
 
 #include <algorithm>
@@ -30,6 +31,21 @@ __global__ __launch_bounds__(256) void qkv_rope_append_kernel(AppendArgs a) {
     __shared__ int64_t s_at[doe::kRopeRowsPerWg];  // the position's place in the pools, -1: none
     const int64_t row0 = (int64_t)blockIdx.x * a.rows_per_wg;
     const int count = (int)std::min<int64_t>(a.rows_per_wg, a.rows - row0);
+    const int D = a.head_dim, per_head = D / 8;
+    const doe::RopeThread me = doe::rope_thread((a.r.num_heads + 2 * a.kv_heads) * per_head, blockIdx.y);
+    const int head = me.unit / per_head, in_head = me.unit - head * per_head, kv = head - a.r.num_heads;
+    const bool is_q = kv < 0, is_v = kv >= a.kv_heads;
+    const doe::RopeUnit u = is_v ? doe::RopeUnit{8 * in_head, 8 * in_head + 4, false} : doe::rope_unit(a.r, in_head);
+    const bool turns = !is_v && u.at0 < a.r.rotary_dim;
+    _Float16 *pool = is_v ? a.v_pool + (int64_t)(kv - a.kv_heads) * D : a.k_pool + (int64_t)kv * D;
+    const float *x = a.r.qkv + row0 * a.r.row_stride + (int64_t)head * D;
+    // (a row's values are on their way before its position is known, the next one's while it turns)
+    f4 next0 = {}, next1 = {};
+    auto read = [&](int i) __attribute__((always_inline)) {
+        next0 = *reinterpret_cast<const f4 *>(x + i * a.r.row_stride + u.at0);
+        next1 = *reinterpret_cast<const f4 *>(x + i * a.r.row_stride + u.at1);
+    };
+    if (me.first < count) read(me.first);
     if (threadIdx.x < 64) {
         int b, pos = doe::kNoRow;
         int64_t at = -1;
@@ -46,19 +62,12 @@ __global__ __launch_bounds__(256) void qkv_rope_append_kernel(AppendArgs a) {
         }
     }
     __syncthreads();
-    const int D = a.head_dim, per_head = D / 8;
-    const doe::RopeThread me = doe::rope_thread((a.r.num_heads + 2 * a.kv_heads) * per_head, blockIdx.y);
-    const int head = me.unit / per_head, in_head = me.unit - head * per_head, kv = head - a.r.num_heads;
-    const bool is_q = kv < 0, is_v = kv >= a.kv_heads;
-    const doe::RopeUnit u = is_v ? doe::RopeUnit{8 * in_head, 8 * in_head + 4, false} : doe::rope_unit(a.r, in_head);
-    const bool turns = !is_v && u.at0 < a.r.rotary_dim;
-    _Float16 *pool = is_v ? a.v_pool + (int64_t)(kv - a.kv_heads) * D : a.k_pool + (int64_t)kv * D;
     for (int i = me.first; i < count; i += me.step) {
         const int pos = s_pos[i];
         const int64_t at = s_at[i];
+        f4 v0 = next0, v1 = next1;
+        if (i + me.step < count) read(i + me.step);
         if (pos == doe::kNoRow || (!is_q && at < 0)) continue;
-        const f4 *x = reinterpret_cast<const f4 *>(a.r.qkv + (row0 + i) * a.r.row_stride + (int64_t)head * D);
-        f4 v0 = x[u.at0 / 4], v1 = x[u.at1 / 4];
         if (turns && pos >= 0 && pos < a.r.max_positions) doe::rotate_unit(a.r, u, pos, v0, v1);
         if (is_q) {
             doe::store_query<false>(a.r, row0 + i, head, D, u, v0, v1);

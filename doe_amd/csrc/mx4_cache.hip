@@ -35,7 +35,7 @@ struct RowArgs {
 
 // The queries' part of a rotating call; false: this workgroup is one of the cache's.  They
 // are read and written past the caches, which the codes alone then fill: 1900 rows of 32 /
-// 16 heads of 256 appended and read back (364 MB) 75 to 67 us, attention behind it as fast.
+// 16 heads of 256 appended and read back (364 MB) 75 to 66 us, attention behind it as fast.
 __device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_pos) {
     const int wg = (int)blockIdx.x - a.kv_wgs;
     if (wg < 0) return false;
@@ -45,20 +45,32 @@ __device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_p
                         wg % a.q_ways, s_pos);
     return true;
 }
+// The angles that dims d .. d + 3 of a head turn by at a position (of a rotated head whole,
+// else its first two); where they do not turn, whatever lies at K's first row.
+struct Angles {
+    doe::f4 first, second;
+};
+__device__ __forceinline__ Angles angles_of(const RowArgs &a, int d, int pos) {
+    const doe::RopeRows &r = a.r;
+    const int half = r.rotary_dim / 2;
+    const float *at = d < r.rotary_dim && pos < r.max_positions
+                          ? r.freq + (int64_t)pos * r.rotary_dim + (r.interleaved ? d : 2 * (d < half ? d : d - half))
+                          : static_cast<const float *>(a.k);
+    return {*reinterpret_cast<const doe::f4 *>(at), *reinterpret_cast<const doe::f4 *>(at + (d < r.rotary_dim && !r.interleaved ? 4 : 0))};
+}
 // Dims d .. d + 3 of a head at `head`, of which `own` has been read, rotated.  The other
 // dims of its pairs are another lane's of the head (D / 4 lanes, four dims each): in this
 // wave up to 256 dims, read again from 512.
 template <int D>
-__device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own_, const float *head, int d, int pos) {
+__device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own_, const float *head, int d, const Angles &t) {
     const doe::RopeRows &r = a.r;
     const doe::f4 own = {own_.x, own_.y, own_.z, own_.w};
     doe::f4 out = own;
-    const int half = r.rotary_dim / 2, low = d < half ? d : d - half;
-    const float *freq = r.freq + (int64_t)pos * r.rotary_dim;
+    const int half = r.rotary_dim / 2;
     if (r.interleaved) {
-        if (d < r.rotary_dim) out = doe::rotate_pairs(own, *reinterpret_cast<const doe::f4 *>(freq + d));
+        if (d < r.rotary_dim) out = doe::rotate_pairs(own, t.first);
     } else {
-        const int other_d = d < half ? d + half : low;
+        const int other_d = d < half ? d + half : d - half;
         doe::f4 other;
         if constexpr (D <= 256 && D != 160) {
             const int lane = (threadIdx.x & 63) + (other_d - d) / 4;  // (past the rotated dims: not used)
@@ -69,7 +81,7 @@ __device__ __forceinline__ float4 rotated(const RowArgs &a, const float4 own_, c
         }
         if (d < r.rotary_dim) {
             doe::f4 lo = d < half ? own : other, hi = d < half ? other : own;
-            doe::rotate_halves(lo, hi, *reinterpret_cast<const doe::f4 *>(freq + 2 * low), *reinterpret_cast<const doe::f4 *>(freq + 2 * low + 4));
+            doe::rotate_halves(lo, hi, t.first, t.second);
             out = d < half ? lo : hi;
         }
     }
@@ -157,7 +169,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         } else {
             k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.k) + at);
             v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.v) + at);
-            if constexpr (ROPE) k = rotated<D>(a, k, static_cast<const float *>(a.k) + at - d, d, positions[r]);
+            if constexpr (ROPE) k = rotated<D>(a, k, static_cast<const float *>(a.k) + at - d, d, angles_of(a, d, positions[r]));
         }
         int ks, vs;
         const uint32_t kc = quantise(k, ks), vc = quantise(v, vs);
@@ -240,24 +252,54 @@ template <int D>
 __device__ __forceinline__ bool find_four(const RowArgs &a, Four &f, int &head) {
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 4), place = unit / a.c.kv_heads;
     head = (int)(unit - place * a.c.kv_heads);
-    int b = 0;
-    int64_t at = place, n = 1, four = 0;
+    int b = 0, at = 0, len = 0;
+    int64_t n = 0;
     if (a.row_starts) {
-        int hi = a.c.batch;  // the last b whose places begin at or before this one
-        while (hi - b > 1) {
-            const int mid = (b + hi) >> 1;
-            if ((a.row_starts[mid] >> 2) + 2 * (int64_t)mid <= place) b = mid;
-            else hi = mid;
+        // the last sequence whose places begin at or before this one: a lane a sequence of 64,
+        // read once where there are no more, and a wave's units find theirs among them (forty
+        // prompts of twenty rows appended and read back: 11.8 to 8.7 us from a search by each)
+        constexpr int LANES = D / 4 < 64 ? D / 4 : 64;
+        const int lane = threadIdx.x & 63;
+        int from, to, held, lo = 0, left = a.c.batch;
+        auto read = [&]() __attribute__((always_inline)) {
+            const bool in = lane < left;
+            from = in ? a.row_starts[lo + lane] : 0;
+            to = in ? a.row_starts[lo + lane + 1] : 0;
+            held = in ? doe::mx4_len(a.c, lo + lane) : 0;
+        };
+        if (left <= 64) read();
+        for (int u = 0; u < 64 / LANES; ++u) {
+            const int mine = __builtin_amdgcn_readlane((int)place, u * LANES);
+            if (a.c.batch > 64) {
+                lo = 0;
+                left = a.c.batch;
+                while (left > 64) {  // 64 ways at a time
+                    const int step = (left + 63) >> 6, i = lo + lane * step;
+                    const uint64_t before = __ballot(i < lo + left && (a.row_starts[i] >> 2) + 2 * i <= mine);
+                    const int last = before ? 63 - __builtin_clzll(before) : 0;
+                    lo += last * step;
+                    left = std::min(step, left - last * step);
+                }
+                read();
+            }
+            const uint64_t before = __ballot(lane < left && (from >> 2) + 2 * (lo + lane) <= mine);
+            if (before == 0) continue;  // (n stays 0)
+            const int last = 63 - __builtin_clzll(before);
+            if (lane / LANES == u) {
+                b = lo + last;
+                at = __builtin_amdgcn_readlane(from, last);
+                n = (int64_t)__builtin_amdgcn_readlane(to, last) - at;
+                len = __builtin_amdgcn_readlane(held, last);
+            }
         }
-        at = a.row_starts[b];
-        n = a.row_starts[b + 1] - at;
-        four = place - (at >> 2) - 2 * (int64_t)b;
     } else {
         if (place >= a.c.batch) return false;
-        b = (int)place;
+        b = at = (int)place;
+        n = 1;
+        len = doe::mx4_len(a.c, b);
     }
+    int64_t four = a.row_starts ? place - (at >> 2) - 2 * (int64_t)b : 0;
     if (at < 0 || n <= 0 || four < 0) return false;
-    const int len = doe::mx4_len(a.c, b);
     f.from = (int)(len - n);
     f.last = len - 1;
     four += f.from >> 2;
@@ -317,14 +359,16 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     uint8_t *slab = a.c.pool + ((int64_t)f.page * a.c.kv_heads + head) * S::bytes(shift);
     bool in[4], all = true;
     float4 k[4] = {}, v[4] = {};
+    Angles angles[ROPE ? 4 : 1] = {};
+    // (all of a unit's reads before the first of them is used, rows that it lacks included:
+    // a read that a condition guards is waited for by itself)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = f.row0 + i;
         in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && row < a.rows;
         if constexpr (ROPE) in[i] = in[i] && f.pos0 + i < a.r.max_positions;
         all = all && in[i];
-        if (!in[i]) continue;
-        const int64_t at = row * a.row_stride + (int64_t)head * D + d;
+        const int64_t at = std::max<int64_t>(0, std::min(row, a.rows - 1)) * a.row_stride + (int64_t)head * D + d;
         if constexpr (F16) {
             const h4 kh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.k) + at));
             const h4 vh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.v) + at));
@@ -335,8 +379,13 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
             const f4 vf = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(static_cast<const float *>(a.v) + at));
             k[i] = make_float4(kf[0], kf[1], kf[2], kf[3]);
             v[i] = make_float4(vf[0], vf[1], vf[2], vf[3]);
-            if constexpr (ROPE) k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + at - d, d, f.pos0 + i);
+            if constexpr (ROPE) angles[i] = angles_of(a, d, f.pos0 + i);
         }
+    }
+    if constexpr (ROPE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + (f.row0 + i) * a.row_stride + (int64_t)head * D, d, angles[i]);
     }
     uint32_t vc[4] = {};
     int vs[4] = {};

@@ -57,11 +57,12 @@ __device__ __forceinline__ RopeUnit rope_unit(const RopeRows &r, int u) {
 // Rotates a unit of dims below rotary_dim at a position of the table.
 __device__ __forceinline__ void rotate_unit(const RopeRows &r, const RopeUnit &u, int pos, f4 &v0, f4 &v1) {
     const f4 *cs = reinterpret_cast<const f4 *>(r.freq + (int64_t)pos * r.rotary_dim + (u.halves ? 2 * u.at0 : u.at0));
+    const f4 cs0 = cs[0], cs1 = cs[1];
     if (u.halves) {
-        rotate_halves(v0, v1, cs[0], cs[1]);
+        rotate_halves(v0, v1, cs0, cs1);
     } else {
-        v0 = rotate_pairs(v0, cs[0]);
-        v1 = rotate_pairs(v1, cs[1]);
+        v0 = rotate_pairs(v0, cs0);
+        v1 = rotate_pairs(v1, cs1);
     }
 }
 // PAST: past the caches.
@@ -152,7 +153,7 @@ struct RopeShare {
 };
 inline RopeShare rope_share(int64_t rows, int64_t units) {
     const int64_t ways = (units + 255) / 256, at_once = units < 256 ? 256 / units : 1;
-    const int64_t per = rows * ways / 16384 > at_once ? rows * ways / 16384 : at_once;  // (some 16384 workgroups)
+    const int64_t per = rows * ways / 8192 > at_once ? rows * ways / 8192 : at_once;  // (some 8192 workgroups)
     return {(int)(per < kRopeRowsPerWg ? per : kRopeRowsPerWg), (int)ways};
 }
 struct RopeThread {
@@ -169,23 +170,31 @@ constexpr int kNoRow = -0x7fffffff;  // the position of a row of no sequence: it
 template <bool PAST>
 __device__ __forceinline__ void rotate_queries(const RopeRows &r, const int32_t *lens, int64_t room, int batch,
                                                const int32_t *row_starts, int64_t row0, int count, int head_dim, int way, int *s_pos) {
+    const int per_head = head_dim / 8;
+    const RopeThread me = rope_thread(r.num_heads * per_head, way);
+    const int head = me.unit / per_head;
+    const RopeUnit u = rope_unit(r, me.unit - head * per_head);
+    const float *x = r.qkv + row0 * r.row_stride + (int64_t)head * head_dim;
+    // (a row's values are on their way before its position is known, the next one's while it turns)
+    f4 v0 = {}, v1 = {};
+    auto read = [&](int i) __attribute__((always_inline)) {
+        v0 = load<PAST>(reinterpret_cast<const f4 *>(x + i * r.row_stride + u.at0));
+        v1 = load<PAST>(reinterpret_cast<const f4 *>(x + i * r.row_stride + u.at1));
+    };
+    if (me.first < count) read(me.first);
     if (threadIdx.x < 64) {
         int b, pos = kNoRow;
         if (!rows_positions(lens, room, batch, row_starts, row0, count, b, pos)) pos = kNoRow;
         if ((int)threadIdx.x < count) s_pos[threadIdx.x] = pos;
     }
     __syncthreads();
-    const int per_head = head_dim / 8;
-    const RopeThread me = rope_thread(r.num_heads * per_head, way);
-    const int head = me.unit / per_head;
-    const RopeUnit u = rope_unit(r, me.unit - head * per_head);
     for (int i = me.first; i < count; i += me.step) {
         const int pos = s_pos[i];
+        f4 w0 = v0, w1 = v1;
+        if (i + me.step < count) read(i + me.step);
         if (pos == kNoRow) continue;
-        const f4 *x = reinterpret_cast<const f4 *>(r.qkv + (row0 + i) * r.row_stride + (int64_t)head * head_dim);
-        f4 v0 = load<PAST>(x + u.at0 / 4), v1 = load<PAST>(x + u.at1 / 4);
-        if (u.at0 < r.rotary_dim && pos >= 0 && pos < r.max_positions) rotate_unit(r, u, pos, v0, v1);
-        store_query<PAST>(r, row0 + i, head, head_dim, u, v0, v1);
+        if (u.at0 < r.rotary_dim && pos >= 0 && pos < r.max_positions) rotate_unit(r, u, pos, w0, w1);
+        store_query<PAST>(r, row0 + i, head, head_dim, u, w0, w1);
     }
 }
 

@@ -241,3 +241,29 @@ def test_captured_with_growing_sequences(dev, mx4_cache):
         c.check()
     g.destroy()
     s.destroy()
+
+
+@pytest.mark.parametrize("batch,d", [(65, 64), (130, 256), (200, 512), (4200, 128)])
+def test_more_sequences_than_lanes(dev, batch, d):
+    """The same pages and rows as by calls of fifty sequences each."""
+    rng = np.random.default_rng(batch)
+    counts = rng.integers(0, 6, batch)
+    counts[[0, 40, batch - 1]] = 0
+    c = Case(batch, list(counts + rng.integers(0, 40, batch)), list(counts), hq=1, hkv=1, d=d, ps=32, mx4_cache=True, lead=3)
+    c.run()
+    got = c.dpools[0].download()
+    assert not np.array_equal(got, c.pool)
+    kr, vr = (up(np.zeros((c.rows, d), np.float32)) for _ in "kv")
+    ops.mx4_kv_read(c.cache, kr, vr, c.rows, row_starts=c.row_starts)
+    pool = up(c.pool)
+    ks, vs = (up(np.zeros((c.rows, d), np.float32)) for _ in "kv")
+    for b in range(0, batch, 50):
+        n = min(50, batch - b)
+        how = dict(c.how, batch=n)
+        part = ops.Mx4Cache(pool, c.dtable.view(4 * b * c.stride, 4 * n * c.stride), c.dlens.view(4 * b, 4 * n), **how)
+        starts = c.row_starts.view(4 * b, 4 * (n + 1))
+        ops.qkv_rope_append(part, c.dqkv, None if not c.hq else c.dq, c.rows, num_heads=c.hq, freq_cis=up(c.freq),
+                            max_positions=c.positions, row_starts=starts, row_stride=c.qkv.shape[1], q_row_stride=c.q.shape[1])
+        ops.mx4_kv_read(part, ks, vs, c.rows, row_starts=starts)
+    assert np.array_equal(got, pool.download())
+    assert np.array_equal(kr.download(), ks.download()) and np.array_equal(vr.download(), vs.download())
