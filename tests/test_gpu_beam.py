@@ -160,6 +160,27 @@ def test_large_logits_side_by_side(dev, vocab, select):
     c.check(clear=False)
 
 
+def test_more_lists_than_threads_and_pool(dev):
+    """64 beams: lists whose places fall together hold low logits only; all logits equal;
+    more than 8192 lists."""
+    rng = np.random.default_rng(11)
+    scores = -0.01 * np.arange(64, dtype=np.float32)[None]
+    vocab = 20000
+    logits = rows_of(rng, 1, 64, vocab)
+    parts = -(-vocab // 1024)
+    for b in range(64):
+        for p in range(parts):
+            if (b * parts + p) % 64 == 5:
+                logits[0, b, 1024 * p:1024 * (p + 1)] -= 50
+    for x in (logits, np.full((1, 64, vocab), 2.5, np.float32)):
+        c = Case(x, scores, select=64)
+        c.run()
+        c.check(clear=False)
+    c = clear_case(12, 1, 64, 300001, 20)
+    c.run()
+    c.check()
+
+
 def test_rows_that_offer_nothing(dev):
     rng = np.random.default_rng(3)
     logits = rows_of(rng, 6, 4, 3000)
@@ -281,7 +302,10 @@ class Host(PagesHost):
         n = len(parents)
         seqs = list(range(n)) if seqs is None else list(seqs)
         table, lens = self.table.copy(), self.lens.copy()
-        heirs = {p: [i for i in range(n) if parents[i] == p] for p in range(n)}
+        heirs = {p: [] for p in range(n)}
+        for i, p in enumerate(parents):
+            if p >= 0:
+                heirs[p].append(i)
         keeps = {p: p if p in h else h[0] for p, h in heirs.items() if h}
         part = lambda p: bool(lens[seqs[p]] % self.ps)  # noqa: E731
         mine = [i for i in range(n) if parents[i] >= 0 and part(parents[i]) and keeps[parents[i]] != i]
@@ -318,12 +342,14 @@ class Host(PagesHost):
 
 
 @pytest.mark.parametrize("seqs,stride,pages,ps,page_bytes", [(1, 2, 4, 16, 48), (4, 8, 60, 16, 48), (12, 40, 700, 32, 16400), (96, 31, 4000, 64, 64),
-                                                             (1500, 6, 12000, 16, 16), (300, 300, 60000, 8, 16)])
+                                                             (1500, 6, 12000, 16, 16), (300, 300, 60000, 8, 16),
+                                                             (8192, 3, 30000, 16, 16)])
 def test_reorder_pages(dev, seqs, stride, pages, ps, page_bytes):
     rng = np.random.default_rng(seqs)
     print(f"[reorder] {seqs} {stride} {pages} {ps}", flush=True)
     lens = rng.integers(0, (stride - 1) * ps + 1, seqs) // (2 if seqs > 100 else 1)
     h = Host(rng, seqs, stride, pages, ps, lens, page_bytes=page_bytes)
+    ws = DeviceBuffer(ops.kv_pages_workspace(pages, seqs, seqs))
     for turn in range(3):
         parents = rng.integers(-1 if turn else 0, seqs, seqs)
         if turn == 1:
@@ -332,7 +358,7 @@ def test_reorder_pages(dev, seqs, stride, pages, ps, page_bytes):
         h.same(h.reorder(parents))
         # and on from there: sequences grow by a position each
         add = (h.lens < stride * ps).astype(np.int32)
-        ops.kv_pages_extend(h.pages, up(i32(np.arange(seqs))), up(add), seqs, status=h.status, workspace=h.ws)
+        ops.kv_pages_extend(h.pages, up(i32(np.arange(seqs))), up(add), seqs, status=h.status, workspace=ws)
         h.same(h.extend(range(seqs), add))
 
 

@@ -133,6 +133,7 @@ TILES = [
     # counts, k, slices, rank: enough bytes of weights for tiles of 32 rows
     ([300, 1, 0, 0, 31, 33, 64, 95], 2304, [1000, 501], 16), ([129, 200], 1032, [260, 3000, 30], 128), ([700], 5000, [2049], 8),
     ([65, 64, 0, 100], 520, [1096, 40], 256), ([40] * 70, 1000, [333], 24), ([500], 8, [4100, 70, 1, 33], 32), ([1500], 72, [9001], 64),
+    (list(np.random.default_rng(0).integers(0, 6, 4300)), 512, [500], 8),
 ]
 
 
