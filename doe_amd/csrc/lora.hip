@@ -737,8 +737,9 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
     DOE_REQUIRE(row_starts || segments == rows, DOE_E_INVALID, "without row_starts a segment is a row (%lld segments, %lld rows)",
                 (long long)segments, (long long)rows);
     DOE_REQUIRE(x_row_stride >= a.k && x_row_stride % 4 == 0 && x_row_stride < ((int64_t)1 << 24), DOE_E_INVALID,
-                "x_row_stride %lld below k %d, or not a multiple of 4", (long long)x_row_stride, a.k);
-    DOE_REQUIRE(y_row_stride >= a.n && y_row_stride < ((int64_t)1 << 26), DOE_E_INVALID, "y_row_stride %lld below the %d columns", (long long)y_row_stride, a.n);
+                "x_row_stride %lld outside k %d .. 2^24, or not a multiple of 4", (long long)x_row_stride, a.k);
+    DOE_REQUIRE(y_row_stride >= a.n && y_row_stride < ((int64_t)1 << 26), DOE_E_INVALID,
+                "y_row_stride %lld outside the %d columns .. 2^26", (long long)y_row_stride, a.n);
     DOE_REQUIRE(rows == 0 || segments == 0 || (adapters && x && y), DOE_E_INVALID, "null pointer");
     DOE_REQUIRE(((uintptr_t)x & 15) == 0 && ((uintptr_t)y & 3) == 0, DOE_E_INVALID, "x must be 16-byte, y 4-byte aligned");
     const uintptr_t from = (uintptr_t)x, to = (uintptr_t)y;

@@ -250,6 +250,18 @@ def test_scores_and_flags_in_place(dev, batch, beams, vocab):
     assert np.all(np.abs(got[2] - want[2]) <= TOL + 2.0 ** -24 * np.abs(want[2]))
 
 
+def test_rows_past_four_gigabytes(dev):
+    c = clear_case(13, 2, 3, 20000, 8)
+    stride = (1 << 28) + 1
+    far = DeviceBuffer(4 * (5 * stride + 20000))
+    for r in range(6):
+        far.view(4 * r * stride, 80000, np.float32, (20000,)).upload(c.logits.reshape(6, -1)[r])
+    c.bufs["logits"], c.kw["row_stride"] = far, stride
+    c.run()
+    c.check()
+    far.free()
+
+
 def test_no_requests_and_no_flags(dev):
     c = clear_case(6, 2, 3, 100, 3)
     p, t, s, _ = c.out
@@ -290,6 +302,20 @@ def test_reorder_rows_of_unaligned_buffers_and_none(dev):
     ops.beam_reorder_rows(src, dst, up(i32([0])), 0, row_bytes=64)
     ops.beam_reorder_rows(src, dst, up(i32([0])), 1, row_bytes=64, layers=0)
     assert np.array_equal(dst.download(), want)
+
+
+def test_reordered_rows_past_four_gigabytes(dev):
+    """Rows of 1 MiB - 4 in layers 2.5 GiB apart."""
+    row, stride = (1 << 20) - 4, 5 << 29
+    src, dst = DeviceBuffer(2 * stride + 3 * row), DeviceBuffer(2 * stride + 3 * row)
+    rng = np.random.default_rng(1)
+    rows = [rng.integers(0, 256, (3, row)).astype(np.uint8) for _ in range(3)]
+    for i, r in enumerate(rows):
+        src.view(i * stride, 3 * row, np.uint8, r.shape).upload(r)
+    ops.beam_reorder_rows(src, dst, up(i32([2, 0, 2])), 3, row_bytes=row, layers=3, src_layer_stride=stride, dst_layer_stride=stride)
+    for i, r in enumerate(rows):
+        assert np.array_equal(dst.view(i * stride, 3 * row, np.uint8, r.shape).download(), r[[2, 0, 2]])
+    src.free(), dst.free()
 
 
 # ---- pages -------------------------------------------------------------------------

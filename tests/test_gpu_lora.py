@@ -252,3 +252,22 @@ def test_beside_a_quantized_projection(dev):
     base = c.bufs["y"].download()
     c.run()
     c.check(base)
+
+
+@pytest.mark.parametrize("counts", [None, [30], [1100]])
+def test_rows_of_y_past_four_gigabytes(dev, counts):
+    """The same sums as beside each other, 5 MB and more from row to row."""
+    rows = sum(counts or [30])
+    c = Case(11, rows, 1024, [3000], 24, counts=counts)
+    c.run()
+    near = c.bufs["y"].download()
+    stride = ((5 << 30) // 4 + (rows - 2)) // (rows - 1)
+    far = DeviceBuffer(4 * ((rows - 1) * stride + c.n))
+    assert far.nbytes > 5 << 30
+    parts = [far.view(4 * r * stride, 4 * c.n, np.float32, (c.n,)) for r in range(rows)]
+    for part, y in zip(parts, c.y):
+        part.upload(y)
+    c.bufs["y"], c.how["y_row_stride"] = far, stride
+    c.run()
+    assert all(np.array_equal(part.download(), row) for part, row in zip(parts, near))
+    far.free()

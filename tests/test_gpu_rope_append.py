@@ -267,3 +267,25 @@ def test_more_sequences_than_lanes(dev, batch, d):
         ops.mx4_kv_read(part, ks, vs, c.rows, row_starts=starts)
     assert np.array_equal(got, pool.download())
     assert np.array_equal(kr.download(), ks.download()) and np.array_equal(vr.download(), vs.download())
+
+
+def test_pages_past_four_gigabytes(dev):
+    """The last pages of pools of 5 GiB each."""
+    ps, hkv, d = 64, 4, 128
+    page_bytes = 2 * ps * hkv * d
+    pages = (5 << 30) // page_bytes
+    pools = [DeviceBuffer(pages * page_bytes) for _ in "kv"]
+    last = [p.view((pages - 3) * page_bytes, 3 * page_bytes, np.float16, (3, ps, hkv, d)) for p in pools]
+    c = Case(6, [70, 20], [70, 2], hq=2, hkv=hkv, d=d, ps=ps, spare=0)
+    assert c.num_pages == 3
+    for small, far in zip(c.dpools, last):
+        far.upload(small.download())
+    c.run()
+    c.check()
+    how = dict(c.how, num_pages=pages)
+    c.cache = ops.F16Cache(*pools, up(np.where(c.table < 0, -1, c.table + np.int32(pages - 3))), c.dlens, **how)
+    c.run()
+    for small, far in zip(c.dpools, last):
+        assert np.array_equal(small.download(), far.download())
+    for p in pools:
+        p.free()

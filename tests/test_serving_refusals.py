@@ -85,7 +85,8 @@ def lora(**kw):
     ("slice_n\\[1\\] 0", dict(slice_n=[8, 0]), {}), ("num_adapters 0", dict(num_adapters=0), {}),
     ("16-byte aligned", dict(b=Odd()), {}),
     ("x_row_stride 60", {}, dict(x_row_stride=60)), ("x_row_stride 66", {}, dict(x_row_stride=66)),
-    ("y_row_stride 63", {}, dict(y_row_stride=63)),
+    ("y_row_stride 63", {}, dict(y_row_stride=63)), ("y_row_stride 67108864", {}, dict(y_row_stride=1 << 26)),
+    ("x_row_stride 16777216", {}, dict(x_row_stride=1 << 24)),
     ("4 segments, 5 rows", {}, dict(segments=4)),
     ("workspace of", {}, dict(workspace=type("S", (), dict(nbytes=16, ptr=16))())),
     ("x must be 16-byte", {}, dict(x=Odd())),
