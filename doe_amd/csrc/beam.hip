@@ -11,6 +11,7 @@
 // of 256000: 9.1, 4.9 and 4.3, chains of cold reads and barriers.
 #include "common.h"
 
+#include <float.h>
 #include <math.h>
 #include <algorithm>
 
@@ -25,6 +26,7 @@ constexpr int kWaves = 4;
 constexpr int kList = 256;   // a wave's shortlist
 constexpr int kPick = 1024;  // threads of the second kernel
 constexpr int kPool = 4096;  // its shortlist
+constexpr int kMost = 128;   // groups of candidates
 constexpr int kAhead = 4;    // entries of a thread's first list that are read at once
 
 struct BeamArgs {
@@ -82,10 +84,9 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     const uint32_t hi = wave_max((uint32_t)(v >> 32));
     return (uint64_t)hi << 32 | wave_max((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
-// The value of the lane N before this one in a circle of sixteen.
-template <int N, typename T>
-__device__ __forceinline__ T dpp_turn(T v) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, true));
+template <int CTRL>
+__device__ __forceinline__ int dpp_take(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
 }
 // The sum over the wave, in every lane.
 template <int CTRL, int ROWS>
@@ -280,14 +281,17 @@ __device__ __forceinline__ double logarithm(double x) {
 // A request's pick: the rows' logarithms, a bound of the lists' best, the candidates that
 // reach it, and their places in the order.  Entries of a place lie side by side for a beam's
 // parts and are read before it is known which are wanted: sixteen requests of eight 6 us, 10
-// with a list's entries side by side, read in turn, and a bound from the waves' own.
+// with a list's entries side by side, read in turn, and a bound from the waves' own.  A list
+// that goes on is read by a wave: eight requests of 32 beams of 32000, the best 64, of which
+// few lists hold most, 10.7 us, 42 by the thread that found it.
 __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     __shared__ double base[kMaxBeams], ended_at[kMaxBeams], pool[kPool];
     __shared__ uint64_t pool_at[kPool];  // a candidate's place, see `place`
     __shared__ uint64_t ahead[kAhead][kPick];
-    __shared__ float heads[kPick / 64][65], bound_;
-    __shared__ __align__(16) float most[64];
-    __shared__ int count_, sums[2][kPick / 64];
+    __shared__ float bound_;
+    __shared__ __align__(16) uint32_t most[kMost];  // of a group, as a number in their order; 0: none
+    __shared__ int deep[kPick];  // lists that go on
+    __shared__ int count_, deep_, sums[2][kPick / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int request = blockIdx.x, row0 = request * a.beams, C = a.select, lists = a.beams * a.parts;
     const uint64_t *cand = a.cand + (int64_t)row0 * a.parts * C;
@@ -303,7 +307,8 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     uint64_t own_list[kAhead];
 #pragma unroll
     for (int c = 0; c < kAhead; ++c) own_list[c] = entry(std::min(tid, lists - 1), std::min(c, C - 1));
-    if (tid == 0) count_ = 0;
+    if (tid == 0) count_ = deep_ = 0;
+    if (tid < kMost) most[tid] = 0;
     for (int b = wave; b < a.beams; b += kPick / 64) {
         const float2 *stats = a.stats + (int64_t)(row0 + b) * a.parts;
         const float score = a.scores[row0 + b];
@@ -372,6 +377,7 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             pool_at[to] = at;
         }
     };
+    const bool few = lists <= kPick / 4;
     // the candidates that reach a bound into the pool; how many
     auto gather = [&](double bound) {
         auto offer = [&](uint64_t key, int b) {
@@ -380,14 +386,26 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             if (in) push(s, place(b, key));
             return in;
         };
-        if (lists <= kPick / 4) {  // few lists: a thread an entry, not a list
+        if (few) {  // a thread an entry, not a list
             for (int i = tid; i < lists * C; i += kPick) offer(cand[i], i / (C * a.parts));
         }
-        for (int l = lists <= kPick / 4 ? lists : tid; l < lists; l += kPick) {
-            const int b = beam_of(l);
+        for (int l = few ? lists : tid; l < lists; l += kPick) {
+            const int b = beam_of(l), known = l == tid ? std::min(C, kAhead) : 0;
+            bool more = known || score_of(entry(l, 0), b) >= std::max<double>(bound, -FLT_MAX);
 #pragma unroll 1
-            for (int c = 0; c < C; ++c)
-                if (!offer(l == tid && c < kAhead ? ahead[c][tid] : entry(l, c), b)) break;
+            for (int c = 0; more && c < known; ++c) more = offer(ahead[c][tid], b);
+            if (!more || known == C) continue;
+            const int to = atomicAdd(&deep_, 1);
+            if (to < kPick) deep[to] = l;
+            else for (int c = known; more && c < C; ++c) more = offer(entry(l, c), b);
+        }
+        if (!few && (C > kAhead || lists > kPick)) {
+            // the rest of such a list at once, by a wave
+            __syncthreads();
+            for (int q = wave; q < std::min(deep_, kPick); q += kPick / 64) {
+                const int l = deep[q], c = lane + (l < kPick ? kAhead : 0);
+                if (c < C) offer(entry(l, c), beam_of(l));
+            }
         }
         if (tid < a.beams && ended_at[tid] > -INFINITY && ended_at[tid] >= bound) push(ended_at[tid], end_place(tid));
         __syncthreads();
@@ -395,40 +413,50 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
     };
     auto emptied = [&] {
         __syncthreads();
-        if (tid == 0) count_ = 0;
+        if (tid == 0) count_ = deep_ = 0;
+        if (tid < kMost) most[tid] = 0;
         __syncthreads();
     };
     constexpr int kEnough = 4 * kMaxSelect;  // whose order is counted
-    // a bound: of 64 groups of lists, their best by themselves, the `select`-th best
-    // (equal ones in the groups' order)
-    double mine = -INFINITY;
-    for (int l = tid; l < lists; l += kPick) mine = fmax(mine, score_of(head_of(l), beam_of(l)));
-    heads[wave][lane] = below(mine);
-    __syncthreads();
-    const int group = tid >> 4, sixteenth = tid & 15;
-    {
-        float m = heads[sixteenth][group];
-        m = fmaxf(m, dpp_turn<1>(m));
-        m = fmaxf(m, dpp_turn<2>(m));
-        m = fmaxf(m, dpp_turn<4>(m));
-        m = fmaxf(m, dpp_turn<8>(m));
-        if (sixteenth == 0) most[group] = m;
-    }
-    __syncthreads();
-    {
-        const float m = most[group];
-        const f4 other = *reinterpret_cast<const f4 *>(most + 4 * sixteenth);
+    // A bound: of 64 groups of candidates (128 if nearly all of 64 were to be taken) the
+    // `select`-th best by themselves, equal ones in the groups' order.  `most` has been
+    // cleared; give(offer): the candidates, by a number that finds their group.
+    const int bits = C > 48 ? 7 : 6, sharers = kPick >> bits;
+    auto group_bound = [&](const auto &give) __attribute__((always_inline)) {
+        give([&](int i, double score) __attribute__((always_inline)) {
+            if (score > -INFINITY) atomicMax(&most[(uint32_t)i * 0x9e3779b1u >> (32 - bits)], ordered(below(score)));
+        });
+        __syncthreads();
+        // (sixteen or eight threads a group)
+        const int group = tid / sharers, mine = tid & (sharers - 1);
+        const uint32_t m = most[group];
         int before = 0;
+        for (int i = 4 * mine; i < 1 << bits; i += 4 * sharers) {
+            const u32x4 other = *reinterpret_cast<const u32x4 *>(most + i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) before += other[i] > m || (other[i] == m && 4 * sixteenth + i < group) ? 1 : 0;
-        before += dpp_turn<1>(before);
-        before += dpp_turn<2>(before);
-        before += dpp_turn<4>(before);
-        before += dpp_turn<8>(before);
-        if (sixteenth == 0 && before == C - 1) bound_ = m;
-    }
-    __syncthreads();
-    int count = gather(bound_);
+            for (int e = 0; e < 4; ++e) before += other[e] > m || (other[e] == m && i + e < group) ? 1 : 0;
+        }
+        before += dpp_take<0xB1>(before);  // the neighbour, the other pair, the other four, the other eight
+        before += dpp_take<0x4E>(before);
+        before += dpp_take<0x141>(before);
+        if (sharers == 16) before += dpp_take<0x140>(before);
+        if (mine == 0 && before == C - 1) bound_ = m ? unordered(m) : -INFINITY;
+        __syncthreads();
+        return bound_;
+    };
+    const float bound = group_bound([&](const auto &offer) __attribute__((always_inline)) {
+        if (few) {
+            for (int i = tid; i < lists * C; i += kPick) offer(i, score_of(cand[i], i / (C * a.parts)));
+            return;
+        }
+        for (int l = tid; l < lists; l += kPick) offer(l, score_of(head_of(l), beam_of(l)));
+        // (few lists may hold most of many)
+        if (C > kOne && tid < lists) {
+#pragma unroll 1
+            for (int c = 1; c < kAhead; ++c) offer(c * kPick + tid, score_of(ahead[c][tid], beam_of(tid)));
+        }
+    });
+    int count = gather(bound);
     if (count > kPool) {
         // the lists' best by themselves: no more than `select` lists reach their bound, but for ties
         constexpr int kHeads = 8;
@@ -459,13 +487,11 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
             s[i] = in ? pool[tid + i * kPick] : -INFINITY;
             at[i] = in ? pool_at[tid + i * kPick] : kNone;
         }
-        const double own = bound_of_many(C, [&](uint32_t key) __attribute__((always_inline)) {
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) n += __popcll(__ballot(ordered(below(s[i])) >= key));
-            return block_sum(n);
-        });
         emptied();
+        const float own = group_bound([&](const auto &offer) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) offer(tid + i * kPick, s[i]);
+        });
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             if (s[i] > -INFINITY && s[i] >= own) push(s[i], at[i]);
