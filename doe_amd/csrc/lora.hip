@@ -496,6 +496,8 @@ __global__ __launch_bounds__(256, 2) void lora_up_tiles_kernel(LoraArgs a) {
             f4 v0 = {0.0f, 0.0f, 0.0f, 0.0f}, v1 = v0;
             if (8 * u < a.rank && row < count) {
                 const float *t = a.t + (int64_t)(row0 + row) * per_row + slice * a.rank + 8 * u;
+                // (four splits' reads at once; from rank 33 on that costs registers and 2 us of 89)
+#pragma unroll(RS <= 2 ? 4 : 1)
                 for (int z = 0; z < a.splits; ++z, t += (int64_t)a.rows * per_row) {
                     v0 += *reinterpret_cast<const f4 *>(t);
                     v1 += *reinterpret_cast<const f4 *>(t + 4);
@@ -625,15 +627,26 @@ int lora_checks(const doe_lora *l, int64_t rows, LoraArgs &a) {
 
 constexpr int kMaxSplits = 8, kCus = 256;
 
+// Workgroups a slice of `columns` each.
+void set_columns(LoraArgs &a, int columns) {
+    a.columns = columns;
+    int groups = 0;
+    for (int s = 0; s < 4; ++s) {
+        const int begin = s ? a.slice_end[s - 1] : 0;
+        groups += (a.slice_end[s] - begin + columns - 1) / columns;
+        a.group_end[s] = groups;
+    }
+}
 // Whether a call takes tiles: where segments have rows to share weights, and what the rows
-// would read of them by themselves is more than the tiles' launches cost.  Rank 16 of 2304
-// to 4096 columns in three slices, rows by themselves against tiles: 64 rows (22 MB) of 32
-// segments 7.3 and 13.3 us, 128 (45 MB) 12.9 and 13.6, 256 (90 MB) 19.8 and 14.6, 512 31.9
-// and 16.7; 32 rows of one segment 6.2 and 12.1; rank 64 of 5376 to 21504, 16 rows of 8
-// (55 MB) 19.5 and 17.7, 64 41.6 and 19.5.
+// would read of them by themselves, or their workgroups, cost more than the tiles'
+// launches.  Rows by themselves against tiles, rank 16 of 2304 to 4096 columns in three
+// slices: 64 rows (22 MB) of 32 segments 7.3 and 13.3 us, 128 (45 MB) 12.9 and 13.6, 256 (90
+// MB) 19.8 and 14.6, 512 31.9 and 16.7; rank 64 of 5376 to 21504, 16 rows of 8 (55 MB) 19.5
+// and 17.7, 64 41.6 and 19.5; rank 8 of 1024 to 300, 600 rows (600 workgroups) 10.0 and 10.6;
+// rank 32 of 256 to 62 in three slices, 638 rows (1914) 26.9 and 10.2.
 bool by_tiles(const LoraArgs &a, bool starts, int64_t segments) {
     const int64_t bytes = 2 * (int64_t)a.rows * a.rank * ((int64_t)a.slices * a.k + a.n);
-    return starts && a.rows >= 2 * segments && bytes > (48 << 20);
+    return starts && a.rows >= 2 * segments && (bytes > (48 << 20) || (int64_t)a.rows * a.group_end[3] > 640);
 }
 int64_t tiles_of(const LoraArgs &a, int64_t segments) { return a.rows / kTile + segments; }
 // Splits of k: workgroups for the device, two steps of 32 a wave at least.
@@ -655,16 +668,6 @@ bool in_one(const LoraArgs &a, int64_t wgs) {
     return bytes <= (256 << 10) && wgs * bytes <= (36 << 20);
 }
 
-// Workgroups a slice of `columns` each.
-void set_columns(LoraArgs &a, int columns) {
-    a.columns = columns;
-    int groups = 0;
-    for (int s = 0; s < 4; ++s) {
-        const int begin = s ? a.slice_end[s - 1] : 0;
-        groups += (a.slice_end[s] - begin + columns - 1) / columns;
-        a.group_end[s] = groups;
-    }
-}
 // A launch has fewer than 2^32 threads.
 int fits(const LoraArgs &a, int64_t threads) {
     DOE_REQUIRE(threads < ((int64_t)1 << 32), DOE_E_UNSUPPORTED, "%d rows of %d columns in one call", a.rows, a.n);
@@ -682,8 +685,8 @@ int launch_up(const LoraArgs &a, int64_t segments, hipStream_t st) {
 template <bool BF16>
 int launch(LoraArgs &a, bool starts, int64_t segments, hipStream_t st) {
     int rc;
+    set_columns(a, 64 * kTokenWaves);
     if (!by_tiles(a, starts, segments)) {
-        set_columns(a, 64 * kTokenWaves);
         const int64_t wgs = (int64_t)a.rows * a.group_end[3], down = (int64_t)a.rows * a.slices * a.rank / 4;
         if ((rc = fits(a, wgs * 64 * kTokenWaves)) || (rc = fits(a, down * 256))) return rc;
         if (in_one(a, wgs)) {
@@ -698,7 +701,12 @@ int launch(LoraArgs &a, bool starts, int64_t segments, hipStream_t st) {
     }
     const int64_t tiles = tiles_of(a, segments), col_groups = (a.slices * a.rank + kDownCols - 1) / kDownCols;
     a.splits = splits_of(a, tiles);
-    set_columns(a, 512);
+    // 512 columns a workgroup, fewer where that leaves the device short of them (150 rows of four,
+    // 512 columns: 13.8 to 10.7 us; 27 of five, 8577: 19.8 to 16.4)
+    for (int columns = 512; columns >= 128; columns /= 2) {
+        set_columns(a, columns);
+        if (tiles * a.group_end[3] >= 2 * kCus) break;
+    }
     const int64_t wgs = tiles * a.splits * col_groups;
     // (both before either runs)
     if ((rc = fits(a, wgs * 64 * kDownWaves)) || (rc = fits(a, tiles * a.group_end[3] * 256))) return rc;

@@ -135,6 +135,8 @@ TILES = [
     ([65, 64, 0, 100], 520, [1096, 40], 256), ([40] * 70, 1000, [333], 24), ([500], 8, [4100, 70, 1, 33], 32), ([1500], 72, [9001], 64),
     (list(np.random.default_rng(0).integers(0, 6, 4300)), 512, [500], 8),
 ]
+# ... or workgroups
+TILES_OF_FEW_BYTES = [([500, 145], 64, [33], 8), ([60, 0, 91, 100], 136, [1, 1030, 7], 24), ([350], 72, [1025], 16)]
 
 
 @pytest.mark.parametrize("counts,k,slice_n,rank", TILES)
@@ -142,6 +144,15 @@ TILES = [
 def test_tiles(dev, counts, k, slice_n, rank, bf16):
     print(f"[lora] {counts[:8]} {k} {slice_n} {rank}", flush=True)
     assert 2 * sum(counts) * rank * (len(slice_n) * k + sum(slice_n)) > 48 << 20
+    c = Case(k, sum(counts) + 3, k, slice_n, rank, bf16=bf16, counts=counts)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("counts,k,slice_n,rank", TILES_OF_FEW_BYTES)
+@pytest.mark.parametrize("bf16", [False, True], ids=["f16", "bf16"])
+def test_tiles_of_few_bytes(dev, counts, k, slice_n, rank, bf16):
+    assert sum(counts) * sum(-(-n // 1024) for n in slice_n) > 640
     c = Case(k, sum(counts) + 3, k, slice_n, rank, bf16=bf16, counts=counts)
     c.run()
     c.check()
