@@ -121,26 +121,37 @@ __device__ __forceinline__ bool row_position(const int32_t *lens, int64_t room, 
 }
 
 // Sequence and position of rows [row0, row0 + count), count at most 64, a lane of the
-// calling wave each (found: whether it has one).  Up to 64 sequences are looked through at
-// once, a lane each.
+// calling wave each (found: whether it has one).  The 64 sequences from the first row's on
+// are looked through at once, a lane each; rows behind those search for theirs.
 __device__ __forceinline__ bool rows_positions(const int32_t *lens, int64_t room, int batch, const int32_t *row_starts, int64_t row0,
                                                int count, int &b, int &pos) {
     const int lane = threadIdx.x & 63;
-    if (!row_starts || batch > 64) return lane < count && row_position(lens, room, batch, row_starts, row0 + lane, b, pos);
-    const int start = lane < batch ? row_starts[lane] : 0, end = lane < batch ? row_starts[lane + 1] : 0;
-    const int held = lane < batch ? held_positions(lens, room, lane) : 0;
+    if (!row_starts) return lane < count && row_position(lens, room, batch, row_starts, row0 + lane, b, pos);
+    int first = 0;
+    for (int left = batch; left > 64;) {  // 64 ways at a time
+        const int step = (left + 63) >> 6, at = first + lane * step;
+        const uint64_t before = __ballot(at < first + left && row_starts[at] <= row0);
+        const int last = before ? 63 - __builtin_clzll(before) : 0;
+        first += last * step;
+        left = left - last * step < step ? left - last * step : step;
+    }
+    const int n = batch - first < 64 ? batch - first : 64;
+    const int start = lane < n ? row_starts[first + lane] : 0, end = lane < n ? row_starts[first + lane + 1] : 0;
+    const int held = lane < n ? held_positions(lens, room, first + lane) : 0;
     bool found = false;
     for (int i = 0; i < count; ++i) {
-        const uint64_t in = __ballot(lane < batch && start <= row0 + i && row0 + i < end);
+        const uint64_t in = __ballot(lane < n && start <= row0 + i && row0 + i < end);
         if (in == 0) continue;
         const int at = 63 - __builtin_clzll(in);
         const int64_t p = __builtin_amdgcn_readlane(held, at) - ((int64_t)__builtin_amdgcn_readlane(end, at) - (row0 + i));
         if (lane == i) {
             found = true;
-            b = at;
+            b = first + at;
             pos = (int)p;
         }
     }
+    if (first + n < batch && lane < count && !found && row0 + lane >= __builtin_amdgcn_readlane(end, n - 1))
+        found = row_position(lens, room, batch, row_starts, row0 + lane, b, pos);
     return found;
 }
 

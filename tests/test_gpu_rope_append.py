@@ -289,3 +289,14 @@ def test_pages_past_four_gigabytes(dev):
         assert np.array_equal(small.download(), far.download())
     for p in pools:
         p.free()
+
+
+@pytest.mark.parametrize("counts", ["few", "mostly none"])
+@pytest.mark.parametrize("batch", [65, 300, 4500])
+def test_many_sequences_to_f16_pages(dev, batch, counts):
+    rng = np.random.default_rng(batch)
+    counts = rng.integers(0, 4, batch) if counts == "few" else (rng.random(batch) < 0.01).astype(int)
+    counts[-1] = 2
+    c = Case(batch, list(counts + rng.integers(0, 40, batch)), list(counts), hq=2, hkv=1, d=16, ps=16, lead=5)
+    c.run()
+    c.check()
