@@ -4,11 +4,10 @@
 // kv_layout 2.
 //
 // Bound by its bytes: eight prompts of up to 2000 rows, 32 / 8 heads of 128 dims, f16
-// queries (387 MB): 76 us, 5.1 TB/s.  A thread has the same eight values of every row that
+// queries (387 MB): 75 us, 5.1 TB/s.  A thread has the same eight values of every row that
 // its workgroup takes; a row is read before its position is known, and the next one while it
-// turns (without: 81; 16384 workgroups instead of 8192: 78, 4096: 81).  One token of 8 / 4
-// heads of 256: 2.7 us in the kernel, three dependent reads (length, page, angles) before its
-// stores.
+// turns (without: 81; the next one's angles with it: no change).  One token of 8 / 4 heads of
+// 256: 2.7 us in the kernel, three dependent reads (length, page, angles) before its stores.
 #include "rope_rows.h"
 
 #include <algorithm>

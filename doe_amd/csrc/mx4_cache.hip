@@ -35,7 +35,7 @@ struct RowArgs {
 
 // The queries' part of a rotating call; false: this workgroup is one of the cache's.  They
 // are read and written past the caches, which the codes alone then fill: 1900 rows of 32 /
-// 16 heads of 256 appended and read back (364 MB) 75 to 66 us, attention behind it as fast.
+// 16 heads of 256 appended and read back (364 MB) 75 to 64 us, attention behind it as fast.
 __device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_pos) {
     const int wg = (int)blockIdx.x - a.kv_wgs;
     if (wg < 0) return false;

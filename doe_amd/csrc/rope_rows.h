@@ -157,14 +157,17 @@ __device__ __forceinline__ bool rows_positions(const int32_t *lens, int64_t room
 
 // The rows of a rotating call over workgroups of 256 threads.  A thread has one unit, of
 // the `units` of a row, in all of its workgroup's rows, so that what it is is found once: a
-// workgroup holds several rows at once, or `ways` of them share a row's units.
+// workgroup holds several rows at once, or `ways` of them share a row's units; twice as many
+// rows, the second read while the first turns, where 2048 workgroups are left (77 prompts of up
+// to 405 rows to f16 pages: 42 us with one row a workgroup, 35 with two, 34.8 with three; eight
+// of up to 2000 in three ways 78, 75.4 and 76).
 constexpr int kRopeRowsPerWg = 16;
 struct RopeShare {
     int rows_per_wg, ways;
 };
 inline RopeShare rope_share(int64_t rows, int64_t units) {
     const int64_t ways = (units + 255) / 256, at_once = units < 256 ? 256 / units : 1;
-    const int64_t per = rows * ways / 8192 > at_once ? rows * ways / 8192 : at_once;  // (some 8192 workgroups)
+    const int64_t per = rows * ways >= 2 * 2048 * at_once ? 2 * at_once : at_once;
     return {(int)(per < kRopeRowsPerWg ? per : kRopeRowsPerWg), (int)ways};
 }
 struct RopeThread {
