@@ -343,6 +343,10 @@ struct Exchange {
     }
 };
 
+// The row that is read for a row of a unit, which the call may not have.
+__device__ __forceinline__ int64_t held_row(const RowArgs &a, int64_t row) {
+    return std::max<int64_t>(0, std::min(row, a.rows - 1));
+}
 template <int D, bool F16, bool ROPE = false>
 __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     using S = Mx4Slab<D>;
@@ -368,7 +372,7 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
         in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && row < a.rows;
         if constexpr (ROPE) in[i] = in[i] && f.pos0 + i < a.r.max_positions;
         all = all && in[i];
-        const int64_t at = std::max<int64_t>(0, std::min(row, a.rows - 1)) * a.row_stride + (int64_t)head * D + d;
+        const int64_t at = held_row(a, row) * a.row_stride + (int64_t)head * D + d;
         if constexpr (F16) {
             const h4 kh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.k) + at));
             const h4 vh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.v) + at));
@@ -385,7 +389,7 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     if constexpr (ROPE) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + (f.row0 + i) * a.row_stride + (int64_t)head * D, d, angles[i]);
+            k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + held_row(a, f.row0 + i) * a.row_stride + (int64_t)head * D, d, angles[i]);
     }
     uint32_t vc[4] = {};
     int vs[4] = {};

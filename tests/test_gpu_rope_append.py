@@ -300,3 +300,18 @@ def test_many_sequences_to_f16_pages(dev, batch, counts):
     c = Case(batch, list(counts + rng.integers(0, 40, batch)), list(counts), hq=2, hkv=1, d=16, ps=16, lead=5)
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "pairs"])
+@pytest.mark.parametrize("rot", [168, 512])
+def test_units_that_begin_before_and_end_behind_the_rows(dev, rot, interleaved):
+    """Heads of 512 dims, whose pairs are read again: positions 4 n + 1 to 4 n + 3 first and 4 n
+    to 4 n + 2 last, in rows that fill their buffer."""
+    for past, counts in ((1, [244, 6, 1]), (3, [2, 7, 90]), (2, [1])):
+        c = Case(past, [past + 4 * i + n for i, n in enumerate(counts)], counts, hq=8, hkv=1, d=512, ps=32, rot=rot, interleaved=interleaved,
+                 q_f16=True, mx4_cache=True)
+        c.rows = sum(counts)
+        c.qkv, c.q = c.qkv[:c.rows].copy(), c.q[:c.rows].copy()
+        c.dqkv, c.dq = up(c.qkv), up(c.q)
+        c.run()
+        c.check()
