@@ -7,7 +7,7 @@
 // kernel reads them once and leaves, for every wave's part of a row, its `select` best
 // logits and its share of the sum; the second one forms the rows' logarithms in 64 bits
 // and picks among the parts.  Sixteen requests of eight beams, 248321 tokens, the best
-// sixteen (127 MB): 31 us, 25 of them in the first kernel (5 TB/s), 6 in the second; four beams
+// sixteen (127 MB): 30.7 us, 25 of them in the first kernel (5 TB/s), 6 in the second; four beams
 // of 256000: 9.1, 4.9 and 4.3, chains of cold reads and barriers.
 #include "common.h"
 
@@ -88,13 +88,21 @@ template <int CTRL>
 __device__ __forceinline__ int dpp_take(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
 }
-// The sum over the wave, in every lane.
+// The sum over the wave, the same in every lane.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, true);
     return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v))), 63));
 }
 __device__ __forceinline__ double wave_sum(double v) {
     v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
@@ -188,9 +196,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
 #pragma unroll
             for (int i = 0; i < 4; ++i) sums[i] += v[j][i] == v[j][i] ? 0.0f : v[j][i];
     }
-    float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    const float sum = wave_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
     if (lane == 0) a.stats[slot] = make_float2(top, sum);
     if (!(sum > 0.0f)) {
         if (lane < a.select) cand[(int64_t)lane * a.parts] = 0;
