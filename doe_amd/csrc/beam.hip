@@ -594,8 +594,12 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const uint8_t *src, uint
 }
 
 // Vectors a lane: longer parts where there are rows enough to fill the device (128 rows of
-// 248321: 45 us in parts of 1024, 37.5 of 2048, 37.6 of 4096, which spill registers).
-int vectors_of(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)8 << 20 ? 8 : 4; }
+// 248321: 45 us in parts of 1024, 37.5 of 2048, 37.6 of 4096, which spill registers), and
+// sooner where a part's list is what costs (256 rows of 32000, the best 64: 35.4 and 25.9 us;
+// 80 of 60000, 40: 19.2 and 18.4; 84 of 17880, 21: 13.4 and 15.5).
+int vectors_of(int64_t rows, int64_t vocab, int64_t select) {
+    return rows * vocab >= (int64_t)(select > kOne ? 2 : 8) << 20 ? 8 : 4;
+}
 
 struct BeamSizes {
     int vectors;
@@ -607,7 +611,7 @@ int beam_sizes(int64_t batch, int64_t beams, int64_t vocab, int64_t select, Beam
     DOE_REQUIRE(vocab > 0 && vocab <= ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "vocab %lld outside 1..2^24", (long long)vocab);
     DOE_REQUIRE(batch >= 0 && batch <= 65535, DOE_E_INVALID, "batch %lld outside 0..65535", (long long)batch);
     const int64_t rows = batch * beams;
-    z.vectors = vectors_of(rows, vocab);
+    z.vectors = vectors_of(rows, vocab, select);
     z.parts = (vocab + 256 * z.vectors - 1) / (256 * z.vectors);
     z.cand = rows * z.parts * select * 8;
     z.bytes = std::max<int64_t>(16, z.cand + rows * z.parts * 8);
