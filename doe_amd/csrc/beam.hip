@@ -7,9 +7,11 @@
 // kernel reads them once and leaves, for every wave's part of a row, its `select` best
 // logits and its share of the sum; the second one forms the rows' logarithms in 64 bits
 // and picks among the parts.  Sixteen requests of eight beams, 248321 tokens, the best
-// sixteen (127 MB): 30.7 us, 25 of them in the first kernel (5 TB/s), 6 in the second; four beams
-// of 256000: 9.1, 4.9 and 4.3, chains of cold reads and barriers.
+// sixteen (127 MB): 27.9 us, 23.5 of them in the first kernel (5.4 TB/s; 18.6 without its
+// lists), 6 in the second; four beams of 256000: 8.5, 4.2 and 4.3, chains of cold reads and
+// barriers.
 #include "common.h"
+#include "wave.h"
 
 #include <float.h>
 #include <math.h>
@@ -112,11 +114,10 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 // A bound that at least `select` of some values reach and few others, bit by bit: the largest
 // key that enough of them reach, until no more than a quarter too many do.  count(key): how
-// many.
+// many; all reach `key`, which is 0 from `bit` on.
 template <typename F>
-__device__ __forceinline__ float bound_of_many(int select, const F &count) {
-    uint32_t key = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+__device__ __forceinline__ float bound_of_many(int select, const F &count, uint32_t key = 0, int bit = 31) {
+    for (; bit >= 0; --bit) {
         const uint32_t next = key | 1u << bit;
         const int n = count(next);
         if (n < select) continue;
@@ -132,7 +133,11 @@ constexpr int kFew = 8, kOne = 16;
 __device__ __forceinline__ float bound_of_one(float v, int select) {
     if (select > kFew) {
         const uint32_t key = ordered(fmaxf(v, -INFINITY));
-        return bound_of_many(select, [&](uint32_t at) __attribute__((always_inline)) { return (int)__popcll(__ballot(key >= at)); });
+        // (from the first bit on in which they differ)
+        const uint32_t most = wave_max(key), differ = most ^ ~wave_max(~key);
+        const int bit = 31 - __builtin_clz(differ | 1);
+        return bound_of_many(select, [&](uint32_t at) __attribute__((always_inline)) { return (int)__popcll(__ballot(key >= at)); },
+                             most & ~((2u << bit) - 1), bit);
     }
     uint32_t key = (ordered(v) & ~63u) | (threadIdx.x & 63);
     bool taken = false;
@@ -142,6 +147,19 @@ __device__ __forceinline__ float bound_of_one(float v, int select) {
         key = most ? 0 : key;
     }
     return unordered(~wave_max(taken ? ~ordered(v) : 0u));
+}
+
+// Value e of a lane's, found by halves (they are registers).
+template <int NV>
+__device__ __forceinline__ float value_of(const f4 (&v)[NV], int e) {
+    float s[2 * NV];
+#pragma unroll
+    for (int k = 0; k < 2 * NV; ++k) s[k] = e & 1 ? v[k / 2][k % 2 * 2 + 1] : v[k / 2][k % 2 * 2];
+#pragma unroll
+    for (int n = NV, bit = 2; n > 0; n /= 2, bit *= 2)
+#pragma unroll
+        for (int k = 0; k < n; ++k) s[k] = e & bit ? s[2 * k + 1] : s[2 * k];
+    return s[0];
 }
 
 // A wave's part of a row: NV x 256 logits, four side by side a lane, kept in
@@ -163,7 +181,12 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
     f4 v[NV];
     if (first + 256 * NV <= a.vocab) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = *reinterpret_cast<const f4_any *>(x + e0 + 256 * j);
+        for (int j = 0; j < NV; ++j) {
+            // (many logits past the caches: 30.8 to 30.2 us for 127 MB; few: 9.0 to 9.3)
+            const f4_any *at = reinterpret_cast<const f4_any *>(x + e0 + 256 * j);
+            if constexpr (NV == 8) v[j] = __builtin_nontemporal_load(at);
+            else v[j] = *at;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -222,21 +245,23 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
             return n;
         });
     }
+    // those that reach it: a bit each, and their places by a sum over the lanes (a ballot for every
+    // value: 30.2 to 27.9 us for 127 MB)
     uint64_t *list = lists[wave];
-    int count = 0;
+    const float least = fmaxf(low, -FLT_MAX);
+    uint32_t hits = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        if (!__any(most4[j] >= low)) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = v[j][i] >= low && v[j][i] > -INFINITY;
-            const uint64_t who = __ballot(in);
-            const int to = count + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-            if (in && to < kList) list[to] = key_of(v[j][i], e0 + 256 * j + i);
-            count += __popcll(who);
-        }
-    }
+    for (int e = 4 * NV - 1; e >= 0; --e) hits = 2 * hits + (v[e / 4][e % 4] >= least ? 1 : 0);
+    const int upto = doe::wave_scan(__popc(hits)), count = __builtin_amdgcn_readlane(upto, 63);
     if (count <= kList) {
+        int to = upto - __popc(hits);
+        while (__any(hits)) {
+            if (hits) {
+                const int e = __builtin_ctz(hits);
+                list[to++] = key_of(value_of(v, e), e0 + 256 * (e >> 2) + (e & 3));
+                hits &= hits - 1;
+            }
+        }
         in_order();
         for (int t = lane; t < count; t += 64) {
             const uint64_t key = list[t];
