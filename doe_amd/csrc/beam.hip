@@ -266,7 +266,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
         for (int t = lane; t < count; t += 64) {
             const uint64_t key = list[t];
             int before = 0;
-#pragma unroll 8
+#pragma unroll 4
             for (int j = 0; j < count; ++j) before += list[j] > key ? 1 : 0;
             if (before < a.select) cand[(int64_t)before * a.parts] = key;
         }
