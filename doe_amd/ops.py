@@ -1027,12 +1027,13 @@ def lora_add(lora: Lora, adapters: DeviceBuffer, x: DeviceBuffer, y: DeviceBuffe
     if row_starts is not None and segments is None:
         raise ValueError("row_starts without the count of segments")
     count = rows if segments is None else segments
-    _need(adapters, count * 4, "adapters")
     if row_starts is not None:
         _need(row_starts, (count + 1) * 4, "row_starts")
-    if rows:
-        _need(x, ((rows - 1) * xs + lora.k) * 4, "x")
-        _need(y, ((rows - 1) * ys + lora.n) * 4, "y")
+    x_size, y_size = (((rows - 1) * xs + lora.k) * 4, ((rows - 1) * ys + lora.n) * 4) if rows else (0, 0)
+    if adapters.nbytes < count * 4 or x.nbytes < x_size or y.nbytes < y_size:
+        _need(adapters, count * 4, "adapters")
+        _need(x, x_size, "x")
+        _need(y, y_size, "y")
     _lib.call("doe_lora_add", lora.ref, adapters.ptr, None if row_starts is None else row_starts.ptr, count, x.ptr, xs, y.ptr, ys,
               rows, workspace.ptr, workspace.nbytes, None if stream is None else _stream_ptr(stream))
 
@@ -1078,10 +1079,11 @@ def beam_reorder_rows(src: DeviceBuffer, dst: DeviceBuffer, parents: DeviceBuffe
     sr = rows if src_rows is None else src_rows
     ss = sr * row_bytes if src_layer_stride is None else src_layer_stride
     ds = rows * row_bytes if dst_layer_stride is None else dst_layer_stride
-    if rows and layers:
-        _need(src, (layers - 1) * ss + sr * row_bytes, "src")
-        _need(dst, (layers - 1) * ds + rows * row_bytes, "dst")
-    _need(parents, rows * 4, "parents")
+    src_size, dst_size = ((layers - 1) * ss + sr * row_bytes, (layers - 1) * ds + rows * row_bytes) if rows and layers else (0, 0)
+    if src.nbytes < src_size or dst.nbytes < dst_size or parents.nbytes < rows * 4:
+        _need(src, src_size, "src")
+        _need(dst, dst_size, "dst")
+        _need(parents, rows * 4, "parents")
     _lib.call("doe_beam_reorder_rows", src.ptr, dst.ptr, parents.ptr, sr, rows, row_bytes, layers, ss, ds,
               None if stream is None else _stream_ptr(stream))
 
