@@ -650,12 +650,20 @@ bool by_tiles(const LoraArgs &a, bool starts, int64_t segments) {
 }
 int64_t tiles_of(const LoraArgs &a, int64_t segments) { return a.rows / kTile + segments; }
 // Splits of k: workgroups for the device, two steps of 32 a wave at least.
-int splits_of(const LoraArgs &a, int64_t tiles) {
-    const int64_t wgs = tiles * ((a.slices * a.rank + kDownCols - 1) / kDownCols), steps = (a.k + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplits, kCus / std::max<int64_t>(1, wgs), steps / (2 * kDownWaves)}));
+int64_t most_splits(const LoraArgs &a) {
+    return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (a.k + 31) / 32 / (2 * kDownWaves)));
 }
+int splits_of(const LoraArgs &a, int64_t tiles) {
+    const int64_t wgs = tiles * ((a.slices * a.rank + kDownCols - 1) / kDownCols);
+    return (int)std::max<int64_t>(1, std::min(most_splits(a), kCus / wgs));
+}
+// Copies of t for any count of segments, and for any fewer rows: rows times splits_of, of
+// which a call has more than one only where tiles x column groups (of rows / 32 at the
+// least) leave CUs over.
 int64_t workspace_of(const LoraArgs &a) {
-    return std::max<int64_t>(16, 4 * (int64_t)a.rows * a.slices * a.rank * kMaxSplits);
+    const int64_t per_row = (int64_t)a.slices * a.rank, groups = (per_row + kDownCols - 1) / kDownCols;
+    const int64_t split_rows = std::min<int64_t>(a.rows * most_splits(a), kCus * kTile / groups);
+    return std::max<int64_t>(16, 4 * per_row * std::max<int64_t>(a.rows, split_rows));
 }
 
 // Whether a call of rows forms t again in every workgroup that uses it: one launch instead

@@ -1010,7 +1010,7 @@ class Lora:
 
 
 def lora_workspace(lora: Lora, rows: int) -> int:
-    """Workspace bytes of ``lora_add`` over ``rows`` rows."""
+    """Workspace bytes of ``lora_add`` over up to ``rows`` rows."""
     size = C.c_int64()
     _lib.call("doe_lora_workspace", lora.ref, rows, C.byref(size))
     return size.value

@@ -625,9 +625,9 @@ int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_
  * f32-accurate (2-3e-7 of float64); a row of x with an infinity or a NaN gives infinities
  * or NaNs in its own row of y.  rank a multiple of 8 up to 256, k a multiple of 8
  * up to 2^20, a and b 16-byte aligned.  The workspace (16-byte aligned,
- * doe_lora_workspace bytes) is the caller's: calls that may overlap, and captured
- * graphs that may be replayed side by side, each take their own.  Nothing is kept
- * in it between calls.  The same bits on every call. */
+ * doe_lora_workspace bytes, which serve any fewer rows too) is the caller's: calls
+ * that may overlap, and captured graphs that may be replayed side by side, each take
+ * their own.  Nothing is kept in it between calls.  The same bits on every call. */
 typedef struct doe_lora {
     const void *a;
     const void *b;
