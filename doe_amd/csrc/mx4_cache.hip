@@ -343,10 +343,6 @@ struct Exchange {
     }
 };
 
-// The row that is read for a row of a unit, which the call may not have.
-__device__ __forceinline__ int64_t held_row(const RowArgs &a, int64_t row) {
-    return std::max<int64_t>(0, std::min(row, a.rows - 1));
-}
 template <int D, bool F16, bool ROPE = false>
 __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     using S = Mx4Slab<D>;
@@ -361,18 +357,15 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
     if (!find_four<D>(a, f, head) || f.page < 0) return;  // (all lanes of a unit)
     const int shift = a.c.page_shift, x0 = f.pos0 & ((1 << shift) - 1), d = threadIdx.x % (D / 4) * 4;
     uint8_t *slab = a.c.pool + ((int64_t)f.page * a.c.kv_heads + head) * S::bytes(shift);
-    bool in[4], all = true;
-    float4 k[4] = {}, v[4] = {};
+    float4 k[4], v[4];
     Angles angles[ROPE ? 4 : 1] = {};
-    // (all of a unit's reads before the first of them is used, rows that it lacks included:
-    // a read that a condition guards is waited for by itself)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = f.row0 + i;
-        in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && row < a.rows;
-        if constexpr (ROPE) in[i] = in[i] && f.pos0 + i < a.r.max_positions;
-        all = all && in[i];
-        const int64_t at = held_row(a, row) * a.row_stride + (int64_t)head * D + d;
+    // the row of position i; where the unit has none there, of the nearest that it has
+    auto held = [&](int i) __attribute__((always_inline)) { return std::max(f.from - f.pos0, std::min(i, f.last - f.pos0)); };
+    auto row_at = [&](int i) __attribute__((always_inline)) {
+        return std::max<int64_t>(0, std::min<int64_t>(f.row0 + held(i), a.rows - 1)) * a.row_stride + (int64_t)head * D;
+    };
+    auto read = [&](int i) __attribute__((always_inline)) {
+        const int64_t at = row_at(i) + d;
         if constexpr (F16) {
             const h4 kh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.k) + at));
             const h4 vh = __builtin_nontemporal_load(reinterpret_cast<const h4 *>(static_cast<const _Float16 *>(a.v) + at));
@@ -383,37 +376,61 @@ __global__ __launch_bounds__(256) void mx4_write_fours_kernel(RowArgs a) {
             const f4 vf = __builtin_nontemporal_load(reinterpret_cast<const f4 *>(static_cast<const float *>(a.v) + at));
             k[i] = make_float4(kf[0], kf[1], kf[2], kf[3]);
             v[i] = make_float4(vf[0], vf[1], vf[2], vf[3]);
-            if constexpr (ROPE) angles[i] = angles_of(a, d, f.pos0 + i);
+            if constexpr (ROPE) angles[i] = angles_of(a, d, f.pos0 + held(i));
         }
+    };
+    auto turn = [&](int i) __attribute__((always_inline)) {
+        if constexpr (ROPE) k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + row_at(i), d, angles[i]);
+    };
+    auto put_k = [&](int at, const float4 &row) __attribute__((always_inline)) {
+        int ks;
+        const uint32_t kc = quantise(row, ks);
+        *reinterpret_cast<uint16_t *>(slab + S::k_code(at) + d / 2) = (uint16_t)kc;
+        if ((d & 31) == 0) slab[S::k_scale(shift, at) + d / 32] = (uint8_t)ks;
+    };
+    auto put_v = [&](int at, uint32_t vc, int vs) __attribute__((always_inline)) {
+        *reinterpret_cast<uint16_t *>(slab + S::v_code(shift, at, d / C) + d % C / 2) = (uint16_t)vc;
+        if ((d & 31) == 0) slab[S::v_scale(shift, at, d / 32)] = (uint8_t)vs;
+    };
+    if (!a.row_starts) {
+        // one row a unit (4096 of 8 heads of 512: 42 us, 72 as a unit of four that lacks three)
+        const int i = held(0);
+        if (ROPE && f.pos0 + i >= a.r.max_positions) return;
+        read(0);
+        turn(0);
+        put_k(x0 + i, k[0]);
+        int vs;
+        const uint32_t vc = quantise(v[0], vs);
+        put_v(x0 + i, vc, vs);
+        return;
     }
-    if constexpr (ROPE) {
+    // (all of a unit's reads before the first of them is used, and for the positions that it lacks
+    // a row that it has: a read that a condition guards is waited for by itself)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            k[i] = rotated<D>(a, k[i], static_cast<const float *>(a.k) + held_row(a, f.row0 + i) * a.row_stride + (int64_t)head * D, d, angles[i]);
-    }
+    for (int i = 0; i < 4; ++i) read(i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) turn(i);
+    bool in[4], all = true;
     uint32_t vc[4] = {};
     int vs[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        in[i] = f.pos0 + i >= f.from && f.pos0 + i <= f.last && f.row0 + i < a.rows;
+        if constexpr (ROPE) in[i] = in[i] && f.pos0 + i < a.r.max_positions;
+        all = all && in[i];
         if (!in[i]) continue;
-        int ks;
-        const uint32_t kc = quantise(k[i], ks);
+        put_k(x0 + i, k[i]);
         vc[i] = quantise(v[i], vs[i]);
-        *reinterpret_cast<uint16_t *>(slab + S::k_code(x0 + i) + d / 2) = (uint16_t)kc;
-        if ((d & 31) == 0) slab[S::k_scale(shift, x0 + i) + d / 32] = (uint8_t)ks;
     }
-    uint8_t *vsat = slab + S::v_scale(shift, x0, d / 32);
     if (all) {
         const uint64_t w = x.to_page(vc);
         *reinterpret_cast<uint64_t *>(slab + S::v_code(shift, x0, d / C) + d % C * 2) = w;
-        if ((d & 31) == 0) *reinterpret_cast<uint32_t *>(vsat) = vs[0] | vs[1] << 8 | vs[2] << 16 | (uint32_t)vs[3] << 24;
+        if ((d & 31) == 0)
+            *reinterpret_cast<uint32_t *>(slab + S::v_scale(shift, x0, d / 32)) = vs[0] | vs[1] << 8 | vs[2] << 16 | (uint32_t)vs[3] << 24;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (!in[i]) continue;
-            *reinterpret_cast<uint16_t *>(slab + S::v_code(shift, x0 + i, d / C) + d % C / 2) = (uint16_t)vc[i];
-            if ((d & 31) == 0) vsat[i] = (uint8_t)vs[i];
-        }
+        for (int i = 0; i < 4; ++i)
+            if (in[i]) put_v(x0 + i, vc[i], vs[i]);
     }
 }
 
