@@ -256,8 +256,9 @@ __device__ __forceinline__ bool find_four(const RowArgs &a, Four &f, int &head) 
     int64_t n = 0;
     if (a.row_starts) {
         // the last sequence whose places begin at or before this one: a lane a sequence of 64,
-        // read once where there are no more, and a wave's units find theirs among them (forty
-        // prompts of twenty rows appended and read back: 11.8 to 8.7 us from a search by each)
+        // read once for a wave's units (forty prompts of twenty rows appended and read back: 11.8
+        // to 8.7 us from a search by each; 4000 of up to two, 64 dims: 12.0 to 8.9 written and 9.1
+        // to 7.4 read from a search by each unit in turn)
         constexpr int LANES = D / 4 < 64 ? D / 4 : 64;
         const int lane = threadIdx.x & 63;
         int from, to, held, lo = 0, left = a.c.batch;
@@ -267,22 +268,26 @@ __device__ __forceinline__ bool find_four(const RowArgs &a, Four &f, int &head) 
             to = in ? a.row_starts[lo + lane + 1] : 0;
             held = in ? doe::mx4_len(a.c, lo + lane) : 0;
         };
+        auto begun = [&](int mine) __attribute__((always_inline)) { return __ballot(lane < left && (from >> 2) + 2 * (lo + lane) <= mine); };
         if (left <= 64) read();
         for (int u = 0; u < 64 / LANES; ++u) {
             const int mine = __builtin_amdgcn_readlane((int)place, u * LANES);
-            if (a.c.batch > 64) {
+            uint64_t before = u || a.c.batch <= 64 ? begun(mine) : 0;
+            // (of more sequences the 64 from the first unit's on, and further ones where all of
+            // these begin before a unit)
+            if (a.c.batch > 64 && (u == 0 || (before >> (left - 1) && lo + left < a.c.batch))) {
                 lo = 0;
-                left = a.c.batch;
-                while (left > 64) {  // 64 ways at a time
-                    const int step = (left + 63) >> 6, i = lo + lane * step;
-                    const uint64_t before = __ballot(i < lo + left && (a.row_starts[i] >> 2) + 2 * i <= mine);
-                    const int last = before ? 63 - __builtin_clzll(before) : 0;
+                for (int all = a.c.batch; all > 64;) {  // 64 ways at a time
+                    const int step = (all + 63) >> 6, i = lo + lane * step;
+                    const uint64_t at_or_before = __ballot(i < lo + all && (a.row_starts[i] >> 2) + 2 * i <= mine);
+                    const int last = at_or_before ? 63 - __builtin_clzll(at_or_before) : 0;
                     lo += last * step;
-                    left = std::min(step, left - last * step);
+                    all = std::min(step, all - last * step);
                 }
+                left = std::min(64, a.c.batch - lo);
                 read();
+                before = begun(mine);
             }
-            const uint64_t before = __ballot(lane < left && (from >> 2) + 2 * (lo + lane) <= mine);
             if (before == 0) continue;  // (n stays 0)
             const int last = 63 - __builtin_clzll(before);
             if (lane / LANES == u) {
