@@ -671,16 +671,21 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
                 (long long)vocab, finished ? ", with finished beams" : "");
     DOE_REQUIRE(batch == 0 || (logits && scores && parents && tokens && out_scores), DOE_E_INVALID, "null pointer");
     DOE_REQUIRE(((uintptr_t)logits & 3) == 0, DOE_E_INVALID, "logits must be 4-byte aligned");
-    // in place only request by request
-    auto apart = [&](const void *in, const void *out) {
-        const uintptr_t i = (uintptr_t)in, o = (uintptr_t)out;
-        return !in || !out || (i == o && select == beams) || i + (uintptr_t)(4 * batch * beams) <= o || o + (uintptr_t)(4 * batch * select) <= i;
+    const int64_t in_bytes = 4 * batch * beams, out_bytes = 4 * batch * select;
+    auto apart = [](const void *p, int64_t p_bytes, const void *q, int64_t q_bytes) {
+        return !p || !q || (uintptr_t)p + (uintptr_t)p_bytes <= (uintptr_t)q || (uintptr_t)q + (uintptr_t)q_bytes <= (uintptr_t)p;
     };
-    DOE_REQUIRE(apart(scores, out_scores) && apart(finished, out_finished) && apart(scores, out_finished) && apart(finished, out_scores) &&
-                    apart(scores, parents) && apart(scores, tokens) && apart(finished, parents) && apart(finished, tokens),
-                DOE_E_INVALID, "the outputs overlap scores or finished");
+    // in place only request by request, scores over scores and flags over flags
+    const void *const outs[4] = {parents, tokens, out_scores, out_finished};
+    for (int o = 0; o < 4; ++o)
+        DOE_REQUIRE((apart(scores, in_bytes, outs[o], out_bytes) || (o == 2 && out_scores == scores && select == beams)) &&
+                        (apart(finished, in_bytes, outs[o], out_bytes) || (o == 3 && out_finished == finished && select == beams)),
+                    DOE_E_INVALID, "the outputs overlap scores or finished");
     DOE_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= z.bytes, DOE_E_INVALID,
                 "a 16-byte aligned workspace of %lld bytes is needed (got %lld)", (long long)z.bytes, (long long)workspace_bytes);
+    for (int o = 1; o < 4; ++o)
+        for (int p = 0; p < o; ++p)
+            DOE_REQUIRE(apart(outs[p], out_bytes, outs[o], out_bytes), DOE_E_INVALID, "the outputs overlap each other");
     const int64_t rows = batch * beams, wgs = (z.parts + kWaves - 1) / kWaves;
     DOE_REQUIRE(rows * wgs < ((int64_t)1 << 24), DOE_E_UNSUPPORTED, "%lld rows of %lld logits", (long long)rows, (long long)vocab);
     if ((rc = doe::require_init())) return rc;

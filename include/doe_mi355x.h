@@ -656,7 +656,7 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
  * end_token).  end_token -1: none (finished is then NULL).  inv_temperature from 2^-64
  * on.  Scores are compared in 64 bits.
  * With select == beams out_scores may be scores and out_finished finished; otherwise the
- * outputs are apart from both.
+ * outputs are apart from both, and always from each other.
  * beams and select up to 64, vocab up to 2^24.  The workspace (16-byte aligned,
  * doe_beam_select_workspace bytes) is the caller's, as for doe_lora_add. */
 int doe_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t select, int64_t *bytes);
