@@ -422,7 +422,8 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         }
         for (int l = few ? lists : tid; l < lists; l += kPick) {
             const int b = beam_of(l), known = l == tid ? std::min(C, kAhead) : 0;
-            bool more = known || score_of(entry(l, 0), b) >= std::max<double>(bound, -FLT_MAX);
+            const double head = known ? 0.0 : score_of(entry(l, 0), b);
+            bool more = known || (head > -INFINITY && head >= bound);
 #pragma unroll 1
             for (int c = 0; more && c < known; ++c) more = offer(ahead[c][tid], b);
             if (!more || known == C) continue;
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
         const int b = none ? 0 : (int)(at >> 56), token = none ? -1 : (int)(at & 0xffffff);
         a.parents[to] = none ? -1 : row0 + b;
         a.tokens[to] = token;
-        a.best[to] = (float)score;
+        a.best[to] = none ? -INFINITY : (float)std::max<double>(score, -FLT_MAX);  // (masked by the lowest logit, at 1 / T above 1)
         if (a.ended) a.ended[to] = !none && (ended_at[b] > -INFINITY || token == a.end_token) ? 1 : 0;  // (it may be a.finished)
     };
     if (count <= kPool) {

@@ -654,7 +654,8 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
  * (the rows; -1 where there are fewer offers), tokens (-1), out_scores (-infinity),
  * out_finished (may be NULL: 1 where the parent was finished or the token is
  * end_token).  end_token -1: none (finished is then NULL).  inv_temperature from 2^-64
- * on.  Scores are compared in 64 bits.
+ * on.  Scores are compared in 64 bits; one below the lowest f32 (a logit of that value,
+ * inv_temperature above 1) is held at it in out_scores.
  * With select == beams out_scores may be scores and out_finished finished; otherwise the
  * outputs are apart from both, and always from each other.
  * beams and select up to 64, vocab up to 2^24.  The workspace (16-byte aligned,
