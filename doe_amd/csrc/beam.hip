@@ -35,7 +35,7 @@ struct BeamArgs {
     const float *logits, *scores;
     const int32_t *finished;
     int64_t row_stride;
-    int batch, beams, vocab, select, parts, end_token;  // parts of a row: a wave each
+    int beams, vocab, select, parts, end_token;  // parts of a row: a wave each
     float inv_temperature, factor, factor_low;  // factor + factor_low = inv_temperature log2(e), factor_low above 0
     float per_part;   // 1 / parts
     uint64_t *cand;   // [row][select][part]: logit order, ~token; 0: none
@@ -89,28 +89,6 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 template <int CTRL>
 __device__ __forceinline__ int dpp_take(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
-}
-// The sum over the wave, the same in every lane.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_add(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, true);
-    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, ROWS, 0xf, true));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v))), 63));
-}
-__device__ __forceinline__ double wave_sum(double v) {
-    v = dpp_add<0x118, 0xf>(dpp_add<0x114, 0xf>(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v))));
-    const uint64_t b = __builtin_bit_cast(uint64_t, dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v)));
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // A bound that at least `select` of some values reach and few others, bit by bit: the largest
 // key that enough of them reach, until no more than a quarter too many do.  count(key): how
@@ -219,7 +197,7 @@ __global__ __launch_bounds__(64 * kWaves, NV == 8 ? 4 : 8) void beam_parts_kerne
 #pragma unroll
             for (int i = 0; i < 4; ++i) sums[i] += v[j][i] == v[j][i] ? 0.0f : v[j][i];
     }
-    const float sum = wave_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
+    const float sum = doe::wave_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
     if (lane == 0) a.stats[slot] = make_float2(top, sum);
     if (!(sum > 0.0f)) {
         if (lane < a.select) cand[(int64_t)lane * a.parts] = 0;
@@ -366,7 +344,7 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(BeamArgs a) {
                 const float2 s = stats[p];
                 all = fma((double)s.y, (double)power(a, s.x - top), all);
             }
-            all = wave_sum(all);
+            all = doe::wave_sum(all);
             if (all > 0.0 && all < INFINITY) start = (double)score - ((double)top * factor + logarithm(all));
         }
         if (lane == 0) {
@@ -696,7 +674,6 @@ int doe_beam_select(const float *logits, int64_t row_stride, const float *scores
     a.scores = scores;
     a.finished = finished;
     a.row_stride = row_stride;
-    a.batch = (int)batch;
     a.beams = (int)beams;
     a.vocab = (int)vocab;
     a.select = (int)select;

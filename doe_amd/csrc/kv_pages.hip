@@ -15,6 +15,7 @@
 // and the long tables are a second, wide kernel that reads the plan.  A call
 // that cannot be done whole (status not 0) changes nothing.
 #include "common.h"
+#include "wave.h"
 
 #include <algorithm>
 
@@ -35,27 +36,15 @@ struct PageArgs {
     int32_t *plan, *by_seq, *by_page, *need, *taken, *pair;
 };
 
-// Inclusive sums over the lanes of a wave, in registers.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int scan16(int v) {  // of each sixteen
-    v = dpp_add<0x111, 0xf>(v);
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    return dpp_add<0x118, 0xf>(v);
-}
 // Inclusive sum over the workgroup; `total` the last thread's.
 __device__ __forceinline__ int scan(int v, int *wave_sums, int &total) {
     static_assert(kPlan == 1024, "sixteen waves");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    v = dpp_add<0x142, 0xa>(scan16(v));
-    v = dpp_add<0x143, 0xc>(v);
+    v = doe::wave_scan(v);
     __syncthreads();  // the last call's sums have been read
     if (lane == 63) wave_sums[wave] = v;
     __syncthreads();
-    const int upto = scan16(wave_sums[lane & 15]);
+    const int upto = doe::scan16(wave_sums[lane & 15]);
     total = __builtin_amdgcn_readlane(upto, 15);
     return v + (wave ? __builtin_amdgcn_readlane(upto, wave - 1) : 0);
 }

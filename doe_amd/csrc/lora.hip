@@ -121,16 +121,6 @@ __device__ __forceinline__ void weights8(const u32x4 w, float *f) {
         for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
     }
 }
-// The sum over the wave, in lane 63.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    v = dpp_add<0x140, 0xf>(dpp_add<0x141, 0xf>(dpp_add<0x4E, 0xf>(dpp_add<0xB1, 0xf>(v))));
-    return dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v));
-}
-
 // t[j] = A_j . x for the `rank` rows of A at `w`, into LDS: a wave four of them and a part
 // of k, parts added in their order.
 constexpr int kTokenWaves = 16, kMaxRank = 256;
@@ -157,7 +147,7 @@ __device__ __forceinline__ void token_down(const LoraArgs &a, const uint16_t *w,
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            sum[j] = wave_sum(sum[j]);
+            sum[j] = doe::wave_sum(sum[j]);
             if (lane == 63) part[j0 + j][way] = sum[j];
         }
     }
@@ -221,7 +211,7 @@ __global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
     four_dots<BF16>(a.a + ((int64_t)id * per_row + j0) * a.k, a.x + (int64_t)row * a.x_stride, a.k, wave, 4, sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        sum[j] = wave_sum(sum[j]);
+        sum[j] = doe::wave_sum(sum[j]);
         if (lane == 63) part[j][wave] = sum[j];
     }
     __syncthreads();
