@@ -405,9 +405,9 @@ __device__ __forceinline__ int slot_of(const ReorderArgs &a, int i) { return a.p
 constexpr int kWhole = -0x7fffffff;  // in place of a last page: there is none but whole ones
 __global__ __launch_bounds__(kPlan) void pages_reorder_plan_kernel(ReorderArgs r) {
     const PageArgs &a = r.p;
-    extern __shared__ int marks[];  // of each slot: heirs, keeper, its length and last page before
+    extern __shared__ int marks[];  // of each slot: heirs, keeper, its last page before
     __shared__ int wave_sums[kPlan / 64], sums[kPlan], pages[kPlan];
-    int *heirs = marks, *keeper = marks + a.n, *lens = marks + 2 * a.n, *last = marks + 3 * a.n;
+    int *heirs = marks, *keeper = marks + a.n, *last = marks + 2 * a.n;
     const int tid = threadIdx.x;
     const uint32_t bits = free_bits(a, 4 * tid);
     for (int i = tid; i < a.n; i += kPlan) {
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(kPlan) void pages_reorder_plan_kernel(ReorderArgs r
             continue;
         }
         bad = bad || len < 0 || len > (int64_t)a.table_stride * a.page_size;
-        lens[i] = r.old_len[i] = len;
+        r.old_len[i] = len;
         last[i] = len > full * a.page_size ? page : kWhole;
         if (p >= 0) {
             atomicAdd(&heirs[p], 1);
@@ -723,9 +723,9 @@ int doe_beam_reorder_pages(const doe_kv_pages *pages, const int32_t *seqs, const
     r.columns = (int)std::max<int64_t>(1, std::min<int64_t>({64, kReorder / n, (a.table_stride + 255) / 256 * 16}));
     const int64_t chunks = (a.table_stride + r.columns - 1) / r.columns;
     DOE_REQUIRE(chunks < (1 << 24), DOE_E_UNSUPPORTED, "%lld sequences of up to %d pages", (long long)n, a.table_stride);
-    const int lds = (int)(16 * n);
+    const int lds = (int)(12 * n);
     static const hipError_t attr_rc = hipFuncSetAttribute((const void *)pages_reorder_plan_kernel,
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 16 * kReorder);
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 12 * kReorder);
     DOE_HIP_CHECK(attr_rc);
     hipLaunchKernelGGL(pages_reorder_plan_kernel, dim3(1), dim3(kPlan), lds, (hipStream_t)stream, r);
     DOE_LAUNCH_CHECK("pages_reorder_plan_kernel");
