@@ -9,7 +9,7 @@
 // of a block are one run and no byte is shared between positions.
 #pragma once
 
-#include "common.h"
+#include "ragged.h"
 #include "wave.h"
 
 namespace doe {
@@ -41,36 +41,8 @@ struct Mx4Slab {
 };
 
 // Positions of sequence b that the cache can hold and has in use.
-__device__ __forceinline__ int mx4_len(const Mx4View &c, int b) {
-    const int64_t room = (int64_t)c.table_stride << c.page_shift;
-    const int n = c.lens[b];
-    return n < 0 ? 0 : (n > room ? (int)room : n);
-}
-
-// The sequence b and position of row `row` of a call (row_starts null: row b of
-// sequence b); false where it has none: rows before and behind the
-// sequences', positions before 0.
-__device__ __forceinline__ bool mx4_row(const Mx4View &c, const int32_t *row_starts, int64_t row, int &b, int &pos) {
-    int lo = 0;
-    int64_t first = row, next = row + 1;
-    if (row_starts) {
-        int hi = c.batch;  // the last b with row_starts[b] <= row
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (row_starts[mid] <= row) lo = mid;
-            else hi = mid;
-        }
-        first = row_starts[lo];
-        next = row_starts[lo + 1];
-        if (row < first || row >= next) return false;
-    } else {
-        lo = (int)row;
-    }
-    b = lo;
-    const int64_t p = (int64_t)mx4_len(c, b) - (next - first) + (row - first);
-    pos = (int)p;
-    return p >= 0;
-}
+__device__ __forceinline__ int64_t mx4_room(const Mx4View &c) { return (int64_t)c.table_stride << c.page_shift; }
+__device__ __forceinline__ int mx4_len(const Mx4View &c, int b) { return held_positions(c.lens, mx4_room(c), b); }
 
 // The page of position pos of sequence b; -1 where the table names none of the pool.
 __device__ __forceinline__ int mx4_page(const Mx4View &c, int b, int pos) {

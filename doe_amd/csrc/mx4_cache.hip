@@ -41,7 +41,7 @@ __device__ __forceinline__ bool queries(const RowArgs &a, int head_dim, int *s_p
     if (wg < 0) return false;
     const int64_t row0 = (int64_t)(wg / a.q_ways) * a.q_rows;
     const int count = a.rows - row0 < a.q_rows ? (int)(a.rows - row0) : a.q_rows;
-    doe::rotate_queries<true>(a.r, a.c.lens, (int64_t)a.c.table_stride << a.c.page_shift, a.c.batch, a.row_starts, row0, count, head_dim,
+    doe::rotate_queries<true>(a.r, a.c.lens, doe::mx4_room(a.c), a.c.batch, a.row_starts, row0, count, head_dim,
                         wg % a.q_ways, s_pos);
     return true;
 }
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void mx4_write_kernel(RowArgs a) {
         const int64_t row = row0 + threadIdx.x;
         Place p{-1, 0};
         int b, pos;
-        if (row < a.rows && doe::mx4_row(a.c, a.row_starts, row, b, pos)) {
+        if (row < a.rows && doe::row_position(a.c.lens, doe::mx4_room(a.c), a.c.batch, a.row_starts, row, b, pos) && pos >= 0) {
             const int page = doe::mx4_page(a.c, b, pos);
             if (page >= 0) p = Place{(int64_t)page * a.c.kv_heads, pos & ((1 << a.c.page_shift) - 1)};
             if constexpr (ROPE) {
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(RowArgs a) {
         const int64_t row = row0 + threadIdx.x;
         Place p{-1, 0};
         int b, pos;
-        if (row < a.rows && doe::mx4_row(a.c, a.row_starts, row, b, pos)) {
+        if (row < a.rows && doe::row_position(a.c.lens, doe::mx4_room(a.c), a.c.batch, a.row_starts, row, b, pos) && pos >= 0) {
             const int page = doe::mx4_page(a.c, b, pos);
             if (page >= 0) p = Place{(int64_t)page * a.c.kv_heads, pos & ((1 << a.c.page_shift) - 1)};
         }
