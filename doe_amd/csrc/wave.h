@@ -36,20 +36,20 @@ __device__ __forceinline__ int wave_scan(int v) {
     return dpp_add<0x143, 0xc>(v);       // lane 31 to rows 2 and 3
 }
 
-// The sum over the wave, the same in every lane (float, double).
-__device__ __forceinline__ float last_lane(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
-}
-__device__ __forceinline__ double last_lane(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
+// The sum over the wave (float, double), in lane 63, and in every lane.
 template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
+__device__ __forceinline__ T wave_sum_last(T v) {
     v = dpp_add<0x4E, 0xf>(dpp_add<0xB1, 0xf>(v));    // the neighbour, the other pair
     v = dpp_add<0x140, 0xf>(dpp_add<0x141, 0xf>(v));  // the other four, the other eight
-    return last_lane(dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v)));
+    return dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(wave_sum_last(v)), 63));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, wave_sum_last(v));
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
 }  // namespace doe
