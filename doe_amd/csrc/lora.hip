@@ -738,8 +738,11 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
                 "y_row_stride %lld outside the %d columns .. 2^26", (long long)y_row_stride, a.n);
     DOE_REQUIRE(rows == 0 || segments == 0 || (adapters && x && y), DOE_E_INVALID, "null pointer");
     DOE_REQUIRE(((uintptr_t)x & 15) == 0 && ((uintptr_t)y & 3) == 0, DOE_E_INVALID, "x must be 16-byte, y 4-byte aligned");
-    const uintptr_t from = (uintptr_t)x, to = (uintptr_t)y;
-    DOE_REQUIRE(rows == 0 || from + (uintptr_t)(((rows - 1) * x_row_stride + a.k) * 4) <= to ||
+    // whole, or column by column within rows of the same stride
+    const uintptr_t from = (uintptr_t)x, to = (uintptr_t)y, row = 4 * (uintptr_t)x_row_stride;
+    const uintptr_t behind = to >= from ? (to - from) % row : (row - (from - to) % row) % row;  // of x's row to y's
+    const bool columns = x_row_stride == y_row_stride && behind >= 4 * (uintptr_t)a.k && behind + 4 * (uintptr_t)a.n <= row;
+    DOE_REQUIRE(rows == 0 || columns || from + (uintptr_t)(((rows - 1) * x_row_stride + a.k) * 4) <= to ||
                     to + (uintptr_t)(((rows - 1) * y_row_stride + a.n) * 4) <= from,
                 DOE_E_INVALID, "x and y are apart from each other");
     const int64_t need = workspace_of(a);

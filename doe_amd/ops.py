@@ -1021,7 +1021,7 @@ def lora_add(lora: Lora, adapters: DeviceBuffer, x: DeviceBuffer, y: DeviceBuffe
              y_row_stride: int | None = None, stream=None) -> None:
     """y[r] += scale B (A x[r]) for the adapter of each row (``adapters``, device
     int32), or with ``row_starts`` of each of ``segments`` runs of rows; an id outside
-    the adapters is none."""
+    the adapters is none.  ``y`` may be other columns of the rows of ``x``."""
     xs = lora.k if x_row_stride is None else x_row_stride
     ys = lora.n if y_row_stride is None else y_row_stride
     if row_starts is not None and segments is None:

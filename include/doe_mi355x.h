@@ -611,7 +611,8 @@ int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_
  * y[r] += scales[a] B_a (A_a x[r]) beside a shared projection, for the adapter a of
  * each row's request; no reference counterpart.  x f32 rows of k, x_row_stride
  * elements apart (16-byte aligned, the stride a multiple of 4 below 2^24); y f32 rows
- * of n, y_row_stride (below 2^26) apart, apart from x: the projection's output.
+ * of n, y_row_stride (below 2^26) apart: the projection's output.  y is apart from x,
+ * or other columns of the same rows (equal strides, no column in both).
  *   a       [num_adapters][slices * rank][k], f16, or bf16 with bf16 != 0
  *   b       [num_adapters][n][rank], the same type; n = slice_n[0] + ..: the
  *           projections that share x (q / k / v, gate / up) side by side, the
