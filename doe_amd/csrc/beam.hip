@@ -8,8 +8,9 @@
 // logits and its share of the sum; the second one forms the rows' logarithms in 64 bits
 // and picks among the parts.  Sixteen requests of eight beams, 248321 tokens, the best
 // sixteen (127 MB): 27.9 us, 23.5 of them in the first kernel (5.4 TB/s; 18.6 without its
-// lists), 6 in the second; four beams of 256000: 8.5, 4.2 and 4.3, chains of cold reads and
-// barriers.
+// lists), 6 in the second; four beams of 256000: 8.5, 4.0 and 4.4, chains of cold reads and
+// barriers.  Powers and a part's sum of up to 2048 of them are f32 (their rounding is within
+// 2^-18 of the logarithm, half a step of an f32 score from 2^6 on); from there on 64 bits.
 #include "common.h"
 #include "wave.h"
 

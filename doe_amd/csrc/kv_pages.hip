@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(PageArgs a) { copy_page
 // takes a fresh page for every heir of a partly filled last page but one (the parent's
 // own slot, else the first heir); the wide kernel reads its columns of all rows before
 // it writes any of them.  Twelve requests of eight beams, 26 last pages of 52 layers (177
-// MB): 36 us, 4.9 TB/s, behind 4.6 of the plan; three of four 4.3 and 3.7.
+// MB): 33 us, 5.3 TB/s, behind 4.8 of the plan; three of four 4.2 and 3.7.
 constexpr int kReorder = 8192;  // sequences of a call: their marks and a column of their rows fit in LDS
 
 struct ReorderArgs {

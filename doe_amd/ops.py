@@ -990,7 +990,7 @@ def qkv_rope_append(cache: F16Cache | Mx4Cache, qkv: DeviceBuffer, q_out: Device
 class Lora:
     """Low-rank adapters beside a shared projection: ``a`` [num_adapters][slices *
     rank][k] and ``b`` [num_adapters][n][rank] in f16 (or bf16), ``scales`` (f32)
-    or None.  ``slice_n``: the columns of the projections that share the input (one
+    or None; a rank that is no multiple of 8 padded with zeros.  ``slice_n``: the columns of the projections that share the input (one
     to four).  Keeps its buffers alive."""
 
     def __init__(self, a: DeviceBuffer, b: DeviceBuffer, scales: DeviceBuffer | None, *, num_adapters: int, rank: int, k: int,

@@ -587,8 +587,10 @@ int doe_attn_mx4_prompt(const doe_mx4_cache *cache, const void *q, int q_f16, in
  * 16-byte aligned, row strides multiples of 16 bytes.
  *
  * The f16 cache: pools [num_pages][page_size][num_kv_heads][head_dim] of K and V,
- * the order that doe_attention_dispatch reads with kv_layout 2; head_dim a multiple
- * of 8 up to 1024, any page_size.  page_table and kv_lens as in doe_mx4_cache. */
+ * the order that doe_attention_dispatch reads with kv_layout 2, one sequence a call: its
+ * row of page_table, its length and its f32 queries, at the head dims of that call.
+ * Queries in f16 are what the 4-bit cache's attention takes.  head_dim a multiple of 8
+ * up to 1024, any page_size.  page_table and kv_lens as in doe_mx4_cache. */
 typedef struct doe_f16_cache {
     uint16_t *k_pool, *v_pool;
     const int32_t *page_table;
@@ -623,9 +625,14 @@ int doe_mx4_qkv_rope_append(const doe_mx4_cache *cache, const float *qkv, int64_
  *   row_starts  device int32 [segments + 1]: rows [row_starts[s], row_starts[s + 1])
  *               are segment s's, in order; NULL: rows == segments, a row each.  Rows
  *               of no segment are left as they were.
- * f32-accurate (2-3e-7 of float64); a row of x with an infinity or a NaN gives infinities
- * or NaNs in its own row of y.  rank a multiple of 8 up to 256, k a multiple of 8
- * up to 2^20, a and b 16-byte aligned.  The workspace (16-byte aligned,
+ * Sums are f32 (y within 2-3e-7 of float64).  Single rows, and segments of few, multiply x
+ * and t = A x as they are.  Longer segments go in tiles (which by the call's sizes), and
+ * hold both in f16 parts with f16 adapters: 22 of a value's 24 bits, fewer from 2^-16 of
+ * its row's largest downward and none below 2^-38 of it (nor of 2^-98, where the largest
+ * is less); with bf16 adapters in three bf16 parts, all 24.  A row of x with an infinity
+ * or a NaN gives infinities or NaNs in its own row of y.  rank a multiple of 8 up to 256
+ * (smaller ones with rows of zeros in a and columns of zeros in b), k a multiple of 8 up to
+ * 2^20, a and b 16-byte aligned.  The workspace (16-byte aligned,
  * doe_lora_workspace bytes, which serve any fewer rows too) is the caller's: calls
  * that may overlap, and captured graphs that may be replayed side by side, each take
  * their own.  Nothing is kept in it between calls.  The same bits on every call. */
@@ -655,7 +662,10 @@ int doe_lora_add(const doe_lora *lora, const int32_t *adapters, const int32_t *r
  * (the rows; -1 where there are fewer offers), tokens (-1), out_scores (-infinity),
  * out_finished (may be NULL: 1 where the parent was finished or the token is
  * end_token).  end_token -1: none (finished is then NULL).  inv_temperature from 2^-64
- * on.  Scores are compared in 64 bits; one below the lowest f32 (a logit of that value,
+ * on.  A row's logarithm is within 2^-18: powers and sums of up to 2048 logits are f32,
+ * those sums are joined in 64 bits.  Scores are compared in 64 bits, so offers of one
+ * beam are in the order of its logits; two beams' that lie within the logarithms' error may
+ * change places.  A score below the lowest f32 (a logit of that value,
  * inv_temperature above 1) is held at it in out_scores.
  * With select == beams out_scores may be scores and out_finished finished; otherwise the
  * outputs are apart from both, and always from each other.
