@@ -121,48 +121,6 @@ __device__ __forceinline__ void weights8(const u32x4 w, float *f) {
         for (int i = 0; i < 8; ++i) f[i] = (float)h[i];
     }
 }
-// Four rows of A, k apart, times x: this wave's 512s of k, `from`, from + step .. below
-// `to`.  AHEAD of them are on their way at once, whole (lanes past k take the first
-// values, times 0): a load that a lane's condition guards is waited for by itself.  Two
-// at once: a token of rank 64, 5376 to 21504, 9.4 to 8.9 us; in lora_token_kernel, whose
-// waves have one or two, 6.6 to 6.8.
-template <bool BF16, int AHEAD>
-__device__ __forceinline__ void four_dots(const uint16_t *rows, const float *x, int k, int from, int to, int step, float *sum) {
-    const int mine = (threadIdx.x & 63) * 8;
-    struct Unit {
-        f4 x0, x1;
-        u32x4 w[4];
-    };
-    auto load = [&](Unit &v, int u) __attribute__((always_inline)) {
-        const int at = u * 512 + mine, first = at < k ? at : 0;
-        v.x0 = *reinterpret_cast<const f4 *>(x + first);
-        v.x1 = *reinterpret_cast<const f4 *>(x + first + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v.w[j] = *reinterpret_cast<const u32x4 *>(rows + (int64_t)j * k + first);
-    };
-    auto add = [&](const Unit &v, int u) __attribute__((always_inline)) {
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = u * 512 + mine < k ? (i < 4 ? v.x0[i & 3] : v.x1[i & 3]) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f[8];
-            weights8<BF16>(v.w[j], f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[j] = fmaf(y[i], f[i], sum[j]);
-        }
-    };
-    for (int u = from; u < to; u += AHEAD * step) {
-        Unit v[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (i == 0 || u + i * step < to) load(v[i], u + i * step);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (i == 0 || u + i * step < to) add(v[i], u + i * step);
-    }
-}
-
 // t[j] = A_j . x for the `rank` rows of A at `w`, into LDS: a wave four of them and a part
 // of k, parts added in their order.
 constexpr int kTokenWaves = 16, kMaxRank = 256;
@@ -173,7 +131,20 @@ __device__ __forceinline__ void token_down(const LoraArgs &a, const uint16_t *w,
     const int way = wave % ways, units = (a.k + 511) / 512, per = (units + ways - 1) / ways;
     for (int j0 = 4 * (wave / ways); j0 < a.rank; j0 += 4 * (kTokenWaves / ways)) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        four_dots<BF16, 1>(w + (int64_t)j0 * a.k, x, a.k, way * per, std::min(units, (way + 1) * per), 1, sum);
+        const uint16_t *rows = w + (int64_t)j0 * a.k;
+#pragma unroll 2
+        for (int u = way * per; u < std::min(units, (way + 1) * per); ++u) {
+            const int at = u * 512 + lane * 8;
+            if (at >= a.k) continue;
+            const f4 x0 = *reinterpret_cast<const f4 *>(x + at), x1 = *reinterpret_cast<const f4 *>(x + at + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[8];
+                weights8<BF16>(*reinterpret_cast<const u32x4 *>(rows + (int64_t)j * a.k + at), f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[j] = fmaf(x1[i], f[i + 4], fmaf(x0[i], f[i], sum[j]));
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             sum[j] = doe::wave_sum_last(sum[j]);
@@ -189,6 +160,47 @@ __device__ __forceinline__ void token_down(const LoraArgs &a, const uint16_t *w,
     __syncthreads();
 }
 
+// This wave's part of four rows of A, k apart, times x: every `ways`-th 512 of k.  Two of
+// them are on their way at once, whole (lanes past k take the first values, times 0): a
+// load that a lane's condition guards is waited for by itself (a token of rank 64, 5376 to
+// 21504: 9.4 to 8.9 us).  token_down, whose waves have one or two and whose lanes past k
+// load nothing, is a form of its own: by this one 64 tokens of 2304 take 6.36 for 6.28 us,
+// four of 16000 6.57 for 6.41, 214 of 232 26.3 for 25.8.
+template <bool BF16>
+__device__ __forceinline__ void four_dots(const uint16_t *rows, const float *x, int k, int way, int ways, float *sum) {
+    const int units = (k + 511) / 512, mine = (threadIdx.x & 63) * 8;
+    struct Unit {
+        f4 x0, x1;
+        u32x4 w[4];
+    };
+    auto load = [&](Unit &v, int u) __attribute__((always_inline)) {
+        const int at = u * 512 + mine, from = at < k ? at : 0;
+        v.x0 = *reinterpret_cast<const f4 *>(x + from);
+        v.x1 = *reinterpret_cast<const f4 *>(x + from + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.w[j] = *reinterpret_cast<const u32x4 *>(rows + (int64_t)j * k + from);
+    };
+    auto add = [&](const Unit &v, int u) __attribute__((always_inline)) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = u * 512 + mine < k ? (i < 4 ? v.x0[i & 3] : v.x1[i & 3]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+            weights8<BF16>(v.w[j], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[j] = fmaf(y[i], f[i], sum[j]);
+        }
+    };
+    for (int u = way; u < units; u += 2 * ways) {
+        Unit v0, v1;
+        load(v0, u);
+        if (u + ways < units) load(v1, u + ways);
+        add(v0, u);
+        if (u + ways < units) add(v1, u + ways);
+    }
+}
+
 // t of a row, four rows of A a workgroup, its waves every fourth 512 of k.
 template <bool BF16>
 __global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
@@ -198,7 +210,7 @@ __global__ __launch_bounds__(256) void lora_down_rows_kernel(LoraArgs a) {
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    four_dots<BF16, 2>(a.a + ((int64_t)id * per_row + j0) * a.k, a.x + (int64_t)row * a.x_stride, a.k, wave, (a.k + 511) / 512, 4, sum);
+    four_dots<BF16>(a.a + ((int64_t)id * per_row + j0) * a.k, a.x + (int64_t)row * a.x_stride, a.k, wave, 4, sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         sum[j] = doe::wave_sum_last(sum[j]);
